@@ -25,8 +25,9 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 ARCH = "gfx950"
 
 HIP_SOURCES = ["prefill_fwd.hip", "prefill_rows64.hip", "prefill_f32.hip", "prefill_wide.hip", "prefill_wide512.hip", "prefill_fp8.hip", "decode_splitkv.hip", "decode_stream.hip", "lse_merge.hip", "fp8_quant.hip", "kv_append.hip",
+               "kv_append_fp8.hip", "decode_fp8.hip", "attn_weights.hip", "kv_evict.hip",
                "dtattn_abi.cpp"]
-HOST_SOURCES = ["host/sdpa_op.cc", "host/bindings.cc"]
+HOST_SOURCES = ["host/sdpa_op.cc", "host/cache_ops.cc", "host/bindings.cc"]
 
 HIPCC_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-mcode-object-version=5",

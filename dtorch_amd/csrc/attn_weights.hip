@@ -1,0 +1,267 @@
+// Accumulated attention weights: weights[b, hk, j] += sum over the query heads h of hk and the queries i that see key j
+// of exp(scale * q[b, h, i] . k[b, hk, j] - lse[b, h, i]), lse being what the attention returned.
+//
+// No counterpart in the reference, which keeps no KV cache (python/dtorch/test/modules/llama.py:126-156); the weights are
+// what dtattn_kv_evict chooses by.
+//
+// One query per sequence (decode) is bound by HBM: the keys are read once.  A prompt is bound by its products and
+// exponentials.  Both keep a wave's keys in registers as MFMA operands (64 keys: four tiles of 16) and pass the queries
+// by in sets of 16 (query, head) columns, so that the sum over queries stays in registers too and no two waves add
+// to one weight: the result does not depend on timing.
+#include <type_traits>
+
+#include "fp8_cache.hpp"
+
+namespace dtattn {
+
+struct WeightParams {
+    float* w;
+    const char* q;
+    const char* k;
+    const float* ks;
+    const float* lse;
+    const int32_t* lengths;  // may be NULL
+    int64_t w_b, w_h;
+    int64_t q_b, q_h, q_s;  // elements
+    int64_t k_b, k_h, k_s;
+    int64_t ks_b, ks_h, lse_b, lse_h;
+    int64_t q_offset;
+    int32_t B, Hkv, group, L, S, d, block_shift;
+    float c;  // scale * log2(e)
+    uint32_t q_and, q_xor;
+};
+
+namespace {
+
+constexpr int kTiles = 4;  // key tiles of 16 per wave
+
+// How a wave holds one tile's 16 keys (A operand: lane & 15 is the key) and one set's 16 queries (B operand), and their product.
+// 16-bit and 8-bit keys: 16x16x32 MFMAs on 16-bit operands; codes are exact there, and fp32 queries over codes are
+// three bf16 parts.
+template <typename TQ, typename TK, int D>
+struct Operands {
+    typedef typename std::conditional<std::is_same<TQ, f16_t>::value, f16_t, bf16_t>::type E;
+    typedef typename Elem<E>::vec8 V8;
+    static constexpr bool codes = sizeof(TK) == 1;
+    static constexpr int parts = std::is_same<TQ, float>::value ? 3 : 1;
+    static constexpr int steps = D / 32;
+    struct Keys { V8 v[steps]; };
+    struct Queries { V8 v[parts][steps]; };
+    // first head dim of the 8 of step s: chunks of 16 bytes of keys
+    static __device__ __forceinline__ int dim(int g4, int s) { return codes ? 64 * (s >> 1) + 16 * g4 + 8 * (s & 1) : 32 * s + 8 * g4; }
+    // row: the key's first element; past: the row lies past the last key
+    static __device__ __forceinline__ void keys(Keys& f, const TK* row, int g4, int d, bool past) {
+#pragma unroll
+        for (int s = 0; s < steps; s += codes ? 2 : 1) {
+            const int x = dim(g4, s);
+            const u32x4 w = x < d && !past ? ld16_nt(row + x) : u32x4{0u, 0u, 0u, 0u};
+            if constexpr (codes) f.v[s] = codes_to_vec8<E>(w.x, w.y), f.v[s + 1] = codes_to_vec8<E>(w.z, w.w);
+            else f.v[s] = __builtin_bit_cast(V8, w);
+        }
+    }
+    static __device__ __forceinline__ void queries(Queries& f, const TQ* row, int g4, int d, bool past, uint32_t q_and, uint32_t q_xor) {
+#pragma unroll
+        for (int s = 0; s < steps; ++s) {
+            const int x = dim(g4, s);
+            Chunk<TQ> w = {};
+            if (x < d && !past) w = load_chunk<TQ, false>(row + x);
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(w.v) / sizeof(w.v[0])); ++i) w.v[i] = x < d && !past ? q_bits(w.v[i], q_and, q_xor) : w.v[i];
+            if constexpr (parts == 1) {
+                f.v[0][s] = __builtin_bit_cast(V8, w.v[0]);
+            } else {
+                float y[8];
+                unpack_chunk<TQ>(w, y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    bf16_t t[3];
+                    split3(y[e], t);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) f.v[i][s][e] = t[i];
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ f32x4 product(const Keys& k, const Queries& q) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < steps; ++s)
+#pragma unroll
+            for (int i = 0; i < parts; ++i) a = mfma16(k.v[s], q.v[i][s], a);
+        return a;
+    }
+};
+// fp32 keys: the fp32 matrix cores
+template <int D>
+struct Operands<float, float, D> {
+    static constexpr int steps = D / 16;
+    struct Keys { f32x4 v[steps]; };
+    struct Queries { f32x4 v[steps]; };
+    static __device__ __forceinline__ void keys(Keys& f, const float* row, int g4, int d, bool past) {
+#pragma unroll
+        for (int s = 0; s < steps; ++s) {
+            const int x = 16 * s + 4 * g4;
+            f.v[s] = x < d && !past ? __builtin_bit_cast(f32x4, ld16_nt(row + x)) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    static __device__ __forceinline__ void queries(Queries& f, const float* row, int g4, int d, bool past, uint32_t q_and, uint32_t q_xor) {
+#pragma unroll
+        for (int s = 0; s < steps; ++s) {
+            const int x = 16 * s + 4 * g4;
+            f.v[s] = x < d && !past ? __builtin_bit_cast(f32x4, q_bits(ld16(row + x), q_and, q_xor)) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    static __device__ __forceinline__ f32x4 product(const Keys& k, const Queries& q) {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < steps; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.v[s][e], q.v[s][e], a, 0, 0, 0);
+        return a;
+    }
+};
+
+}  // namespace
+
+// Grid: (64-key chunks / 4, kv heads, sequences); one chunk per wave.  Column c of a set is (query, head) number 16 * set + c,
+// query-major: query c / group, head c % group.
+template <typename TQ, typename TK, int D, bool CAUSAL>
+__global__ void __launch_bounds__(256) attn_weights_kernel(const WeightParams p) {
+    typedef Operands<TQ, TK, D> Op;
+    const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
+    const int64_t b = blockIdx.z;
+    const int hk = blockIdx.y;
+    const int k0 = ((int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 16 * kTiles;
+    const int n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
+    if (k0 >= n) return;
+    const TK* kb = reinterpret_cast<const TK*>(p.k) + b * p.k_b + hk * p.k_h;
+    const TQ* qb = reinterpret_cast<const TQ*>(p.q) + b * p.q_b + (int64_t)hk * p.group * p.q_h;
+    const float* lb = p.lse + b * p.lse_b + (int64_t)hk * p.group * p.lse_h;
+    typename Op::Keys kf[kTiles];
+    float c[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        const int key = k0 + 16 * t + col;
+        Op::keys(kf[t], kb + (int64_t)min(key, n - 1) * p.k_s, g4, p.d, key >= n);
+        c[t] = p.c;
+        if constexpr (sizeof(TK) == 1) c[t] *= p.ks[b * p.ks_b + hk * p.ks_h + (min(k0 + 16 * t, n - 1) >> p.block_shift)];
+    }
+    const int64_t N = (int64_t)p.L * p.group;
+    // the first column that sees the chunk's first key, and the end of those that are not padding
+    int64_t first = 0, last = N;
+    if constexpr (CAUSAL) {
+        first = max((int64_t)k0 - p.q_offset, (int64_t)0) * p.group;
+        if (p.lengths != nullptr) last = min(N, max(n - p.q_offset, (int64_t)0) * p.group);
+    }
+    float sum[kTiles][4] = {};
+    for (int64_t n0 = first; n0 < last; n0 += 16) {
+        const int64_t at = n0 + col;
+        const int64_t i = min(at, last - 1) / p.group;
+        const int h = (int)(min(at, last - 1) - i * p.group);
+        const float lse = lb[h * p.lse_h + i];
+        // columns past the end, and rows that see no key: a query of zeros at a weight of 0
+        const bool none = at >= last || lse == kNegInf;
+        typename Op::Queries qf;
+        Op::queries(qf, qb + h * p.q_h + i * p.q_s, g4, p.d, none, p.q_and, p.q_xor);
+        const float nl = none ? kNegInf : -lse * kLog2e;
+        const int64_t sees = i + p.q_offset;  // the last key of this column
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const f32x4 s = Op::product(kf[t], qf);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x = fast_exp2(__builtin_fmaf(s[e], c[t], nl));
+                if constexpr (CAUSAL) x = k0 + 16 * t + 4 * g4 + e <= sees ? x : 0.f;
+                sum[t][e] += x;
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        float v = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float s = group_sum<16>(sum[t][e]);
+            v = col == e ? s : v;
+        }
+        const int key = k0 + 16 * t + 4 * g4 + col;
+        if (col < 4 && key < n) p.w[b * p.w_b + hk * p.w_h + key] += v;
+    }
+}
+
+template <typename TQ, typename TK, int D>
+static int launch_weights(const WeightParams& p, bool causal, hipStream_t stream) {
+    const dim3 grid((unsigned)((p.S + 64 * kTiles - 1) / (64 * kTiles)), (unsigned)p.Hkv, (unsigned)p.B);
+    if (causal) hipLaunchKernelGGL((attn_weights_kernel<TQ, TK, D, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attn_weights_kernel<TQ, TK, D, false>), grid, dim3(256), 0, stream, p);
+    return check_launch("attn_weights_kernel");
+}
+
+template <typename TQ, typename TK>
+static int dispatch_weights(const WeightParams& p, bool causal, hipStream_t stream) {
+    return p.d <= 64 ? launch_weights<TQ, TK, 64>(p, causal, stream) : launch_weights<TQ, TK, 128>(p, causal, stream);
+}
+
+}  // namespace dtattn
+
+using namespace dtattn;
+
+extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stream_) {
+    const char* who = "attention_weights";
+    if (a == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: args is NULL", who);
+    if (a->B < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->L < 0 || a->S < 0 || a->D <= 0)
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
+    if (a->Hq % a->Hkv != 0) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: Hq is not a multiple of Hkv", who);
+    if (a->q_dtype != DTATTN_BF16 && a->q_dtype != DTATTN_FP16 && a->q_dtype != DTATTN_FP32)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: query dtype %d not supported (bf16, fp16, fp32)", who, a->q_dtype);
+    const bool codes = a->k_dtype == DTATTN_FP8_E4M3FN;
+    if (!codes && a->k_dtype != a->q_dtype)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: keys are of the query's dtype or e4m3fn codes, not %d", who, a->k_dtype);
+    const int64_t qe = a->q_dtype == DTATTN_FP32 ? 4 : 2, ke = codes ? 1 : qe;
+    if (a->D > 128 || (a->D * ke) % 16 != 0)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: head dim %lld not supported (rows of a multiple of 16 bytes, up to 128)", who, (long long)a->D);
+    if (a->S > (1 << 29) || a->L > (1 << 29) || a->B > 65535 || a->Hkv > 65535)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
+    const int64_t most = (int64_t)1 << 40;
+    if (a->q_offset > most || a->q_offset < -most) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: q_offset out of range", who);
+    ScalePlan sp;
+    const int st = plan_scale(a->scale, a->D, a->q_dtype == DTATTN_FP32 ? kSign32 : kSign16, &sp);
+    if (st != DTATTN_OK) return st;
+    WeightParams p = {};
+    if (codes) {
+        if (a->block < 16 || a->block > 256 || (a->block & (a->block - 1)) != 0 || a->S % a->block != 0)
+            return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: block %d must be a power of two from 16 to 256 that divides S", who, a->block);
+        p.block_shift = __builtin_ctz((unsigned)a->block);
+    }
+    if (a->B == 0 || a->S == 0 || a->L == 0) return DTATTN_OK;
+    if (a->weights == nullptr || a->q == nullptr || a->k == nullptr || a->lse == nullptr || (codes && a->k_scale == nullptr))
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    for (int i = 0; i < 3; ++i)
+        if ((a->q_stride[i] * qe) % 16 != 0 || (a->k_stride[i] * ke) % 16 != 0)
+            return fail(DTATTN_ERR_UNSUPPORTED, "%s: strides must be multiples of 16 bytes", who);
+    if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k)) & 15u)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: query and keys must be 16-byte aligned", who);
+    p.w = a->weights;
+    p.q = reinterpret_cast<const char*>(a->q), p.k = reinterpret_cast<const char*>(a->k);
+    p.ks = a->k_scale, p.lse = a->lse, p.lengths = a->lengths;
+    p.w_b = a->w_stride[0], p.w_h = a->w_stride[1];
+    p.q_b = a->q_stride[0], p.q_h = a->q_stride[1], p.q_s = a->q_stride[2];
+    p.k_b = a->k_stride[0], p.k_h = a->k_stride[1], p.k_s = a->k_stride[2];
+    p.ks_b = a->k_scale_stride[0], p.ks_h = a->k_scale_stride[1];
+    p.lse_b = a->lse_stride[0], p.lse_h = a->lse_stride[1];
+    p.q_offset = a->q_offset;
+    p.B = (int32_t)a->B, p.Hkv = (int32_t)a->Hkv, p.group = (int32_t)(a->Hq / a->Hkv);
+    p.L = (int32_t)a->L, p.S = (int32_t)a->S, p.d = (int32_t)a->D;
+    p.c = sp.scale * kLog2e;
+    p.q_and = sp.q_and, p.q_xor = sp.q_xor;
+    const bool causal = a->causal != 0;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    if (codes) {
+        if (a->q_dtype == DTATTN_BF16) return dispatch_weights<bf16_t, uint8_t>(p, causal, stream);
+        if (a->q_dtype == DTATTN_FP16) return dispatch_weights<f16_t, uint8_t>(p, causal, stream);
+        return dispatch_weights<float, uint8_t>(p, causal, stream);
+    }
+    if (a->q_dtype == DTATTN_BF16) return dispatch_weights<bf16_t, bf16_t>(p, causal, stream);
+    if (a->q_dtype == DTATTN_FP16) return dispatch_weights<f16_t, f16_t>(p, causal, stream);
+    return dispatch_weights<float, float>(p, causal, stream);
+}

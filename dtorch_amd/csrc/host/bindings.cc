@@ -4,6 +4,7 @@
 // DTorch Kernel would call.
 #include <torch/extension.h>
 
+#include "cache_ops.h"
 #include "dtattn.h"
 #include "sdpa_op.h"
 
@@ -172,6 +173,73 @@ PYBIND11_MODULE(_dtattn_host, m) {
     py::class_<Fp8QuantizeOp>(m, "Fp8QuantizeOp")
         .def(py::init<>())
         .def("compute", [](const Fp8QuantizeOp& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
+
+    // The 8-bit KV cache and the bounded one.
+    auto a8 = py::class_<KvCacheAppendFp8Param>(m, "KvCacheAppendFp8Param").def(py::init<>());
+    BindSerialisation<KvCacheAppendFp8Param>(a8);
+    auto a8p = py::class_<KvCacheAppendFp8PagedParam>(m, "KvCacheAppendFp8PagedParam").def(py::init<>());
+    BindSerialisation<KvCacheAppendFp8PagedParam>(a8p);
+    auto d8 = py::class_<SdpaDecodeFp8Param>(m, "SdpaDecodeFp8Param")
+                  .def(py::init<>())
+                  .def(py::init<std::optional<double>>(), py::arg("scale"))
+                  .def_readwrite("scale", &SdpaDecodeFp8Param::scale);
+    BindSerialisation<SdpaDecodeFp8Param>(d8);
+    auto d8p = py::class_<SdpaDecodeFp8PagedParam, SdpaDecodeFp8Param>(m, "SdpaDecodeFp8PagedParam")
+                   .def(py::init<>())
+                   .def(py::init<std::optional<double>>(), py::arg("scale"));
+    BindSerialisation<SdpaDecodeFp8PagedParam>(d8p);
+    auto wp = py::class_<AttentionWeightsParam>(m, "AttentionWeightsParam")
+                  .def(py::init<>())
+                  .def(py::init<std::optional<double>, bool, int64_t>(), py::arg("scale"), py::arg("is_causal") = false,
+                       py::arg("q_offset") = 0)
+                  .def_readwrite("scale", &AttentionWeightsParam::scale)
+                  .def_readwrite("is_causal", &AttentionWeightsParam::isCausal)
+                  .def_readwrite("q_offset", &AttentionWeightsParam::qOffset);
+    BindSerialisation<AttentionWeightsParam>(wp);
+    auto ep = py::class_<KvCacheEvictParam>(m, "KvCacheEvictParam")
+                  .def(py::init<>())
+                  .def(py::init<int64_t, int64_t, int64_t>(), py::arg("keep"), py::arg("recent"), py::arg("block") = 0)
+                  .def_readwrite("keep", &KvCacheEvictParam::keep)
+                  .def_readwrite("recent", &KvCacheEvictParam::recent)
+                  .def_readwrite("block", &KvCacheEvictParam::block);
+    BindSerialisation<KvCacheEvictParam>(ep);
+
+    py::class_<KvCacheAppendFp8Op>(m, "KvCacheAppendFp8Op")
+        .def(py::init<>())
+        .def("compute", [](const KvCacheAppendFp8Op& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
+    py::class_<KvCacheAppendFp8PagedOp>(m, "KvCacheAppendFp8PagedOp")
+        .def(py::init<>())
+        .def("compute", [](const KvCacheAppendFp8PagedOp& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
+    py::class_<SdpaDecodeFp8Op>(m, "SdpaDecodeFp8Op")
+        .def(py::init<SdpaDecodeFp8Param>(), py::arg("param"))
+        .def(py::init([](std::optional<double> s) { return SdpaDecodeFp8Op(SdpaDecodeFp8Param(s)); }), py::arg("scale") = std::nullopt)
+        .def_property_readonly("param", &SdpaDecodeFp8Op::Param)
+        .def("compute", [](const SdpaDecodeFp8Op& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
+    py::class_<SdpaDecodeFp8PagedOp>(m, "SdpaDecodeFp8PagedOp")
+        .def(py::init<SdpaDecodeFp8PagedParam>(), py::arg("param"))
+        .def(py::init([](std::optional<double> s) { return SdpaDecodeFp8PagedOp(SdpaDecodeFp8PagedParam(s)); }), py::arg("scale") = std::nullopt)
+        .def_property_readonly("param", &SdpaDecodeFp8PagedOp::Param)
+        .def("compute", [](const SdpaDecodeFp8PagedOp& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
+    py::class_<AttentionWeightsOp>(m, "AttentionWeightsOp")
+        .def(py::init<AttentionWeightsParam>(), py::arg("param"))
+        .def_property_readonly("param", &AttentionWeightsOp::Param)
+        .def("compute", [](const AttentionWeightsOp& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
+    py::class_<KvCacheEvictOp>(m, "KvCacheEvictOp")
+        .def(py::init<KvCacheEvictParam>(), py::arg("param"))
+        .def_property_readonly("param", &KvCacheEvictOp::Param)
+        .def("compute", [](const KvCacheEvictOp& op, const std::vector<std::optional<at::Tensor>>& in) {
             return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
         });
 

@@ -1,0 +1,249 @@
+// Quantised KV-cache append: new keys and values as e4m3fn codes with one power-of-two scale per block of tokens.
+//
+// No counterpart in the reference, which keeps no KV cache (python/dtorch/test/modules/llama.py:126-156).  With
+// amax = max |x| over the finite new values of a block, the block needs s = 2^k, the smallest power of two with
+// amax <= 448 s; code = e4m3_rne(x / s).  A floating code loses nothing by a power of two (its relative precision does not
+// depend on the scale, only the range below the block's maximum does, and that is 2^-9 at the least), and a block that
+// grows over several appends then re-encodes its older rows by an exact shift instead of rounding them again each time.
+//
+// HBM-bound: one wave per (sequence, kv head, K or V, touched block).  It holds the block's new rows in registers
+// (up to 16 chunks of 8 elements per lane: 64 tokens of 128 elements), so that they are read once; larger
+// blocks read them twice, the second time from L2.  Few items per sequence (a decode step) run as one workgroup per
+// sequence, which also advances the length; with more a second launch on the same stream does.
+#include "fp8_cache.hpp"
+
+namespace dtattn {
+
+struct Append8Params {
+    const char* src[2];  // new K, new V
+    char* dst[2];        // codes: cache base, or page pool base
+    float* scale[2];
+    const int32_t* block_table;  // paged only
+    int32_t* lengths;
+    int64_t n_b[2], n_h[2], n_s[2];  // byte strides of the new tokens
+    int64_t d_b[2], d_h[2], d_s[2];  // byte strides of the codes: (batch | page), head, row
+    int64_t s_b[2], s_h[2];          // element strides of the scales
+    int64_t bt_s, items;
+    int32_t Hkv, n_new, cpr;  // cpr: chunks of 8 elements per token row
+    int32_t nblk;             // most blocks that a sequence's new tokens touch
+    int32_t capacity, page_shift, num_pages, block_shift;
+};
+
+namespace {
+
+constexpr int kHeld = 16;     // chunks of 8 elements that a lane holds: 64 rows of 128
+constexpr int kHeldStep = 4;  // in the step kernel, whose items are up to 16 rows
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+
+// The smallest power of two s >= 2^-126 with m <= 448 s; 1 for m = 0.  m = f 2^e with 1 <= f < 2: 448 = 1.75 * 2^8.
+__device__ __forceinline__ float scale_for(float m) {
+    if (m == 0.f) return 1.f;
+    const uint32_t bits = __builtin_bit_cast(uint32_t, m);
+    const int k = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);  // biased by 127
+    return __builtin_bit_cast(float, (uint32_t)max(k, 1) << 23);
+}
+
+__device__ __forceinline__ uint32_t codes4(const float* x) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+}
+
+// 8 values times `inv` as codes, NaN for values that are not finite (their product with inv may be).
+__device__ __forceinline__ u32x2 encode8(const float* x, float inv) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = finite(x[e]) ? x[e] * inv : __builtin_nanf("");
+    return u32x2{codes4(y), codes4(y + 4)};
+}
+
+// 4 codes times `f`, rounded to codes again.
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float f) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    const float y[4] = {a[0] * f, a[1] * f, b[0] * f, b[1] * f};
+    return codes4(y);
+}
+
+// One wave's item: block i of those that the new tokens of (b, h) touch, of K (kv = 0) or V.
+template <typename T, bool PAGED, int HELD>
+__device__ __forceinline__ void append8_item(const Append8Params& p, int64_t b, int h, int kv, int i, int length) {
+    const int lane = threadIdx.x & 63;
+    const int start = max(length, 0);
+    if (start >= p.capacity) return;
+    const int t0 = ((start >> p.block_shift) + i) << p.block_shift;
+    const int first = max(start, t0);
+    const int stop = min((int)min((int64_t)start + p.n_new, (int64_t)p.capacity), t0 + (1 << p.block_shift));
+    if (first >= stop) return;
+    int64_t slot = b;
+    int row0 = t0;
+    if constexpr (PAGED) {
+        const int page = p.block_table[b * p.bt_s + (t0 >> p.page_shift)];
+        if (page < 0 || page >= p.num_pages) return;  // not a page of the pool: the tokens are dropped
+        slot = page;
+        row0 = t0 & ((1 << p.page_shift) - 1);
+    }
+    char* dst = p.dst[kv] + slot * p.d_b[kv] + h * p.d_h[kv] + row0 * p.d_s[kv];  // the block's first row
+    float* sp = p.scale[kv] + slot * p.s_b[kv] + h * p.s_h[kv] + (row0 >> p.block_shift);
+    const char* src = p.src[kv] + b * p.n_b[kv] + h * p.n_h[kv] + (int64_t)(first - start) * p.n_s[kv];
+    const int total = (stop - first) * p.cpr;
+    const float old = first > t0 ? *sp : 0.f;
+
+    Chunk<T> raw[HELD];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+            const int idx = min(base + 64 * k + lane, total - 1);
+            if (base + 64 * k < total)
+                raw[k] = load_chunk<T, false>(reinterpret_cast<const T*>(src + (idx / p.cpr) * p.n_s[kv]) + (idx % p.cpr) * 8);
+        }
+    };
+    float m = 0.f;
+    for (int base = 0; base < total; base += 64 * HELD) {
+        load(base);
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+            if (base + 64 * k >= total) break;
+            float x[8];
+            unpack_chunk<T>(raw[k], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, finite(x[e]) ? fabsf(x[e]) : 0.f);
+        }
+    }
+    m = wave_max(m);
+    float s = scale_for(m);
+    if (first > t0) {
+        s = fmaxf(old, s);
+        if (s != old) {  // the block's older rows at its new scale
+            const float f = old / s;
+            const int cells = (first - t0) * p.cpr;
+            for (int idx = lane; idx < cells; idx += 64) {
+                u32x2* at = reinterpret_cast<u32x2*>(dst + (idx / p.cpr) * p.d_s[kv] + (idx % p.cpr) * 8);
+                const u32x2 w = *at;
+                *at = u32x2{recode4(w.x, f), recode4(w.y, f)};
+            }
+        }
+    }
+    if (lane == 0) *sp = s;
+    const float inv = 1.f / s;
+    const int64_t skip = (int64_t)(first - t0) * p.d_s[kv];
+    for (int base = 0; base < total; base += 64 * HELD) {
+        if (total > 64 * HELD) load(base);
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+            const int idx = base + 64 * k + lane;
+            if (base + 64 * k >= total) break;
+            float x[8];
+            unpack_chunk<T>(raw[k], x);
+            const u32x2 w = encode8(x, inv);
+            if (idx < total) *reinterpret_cast<u32x2*>(dst + skip + (idx / p.cpr) * p.d_s[kv] + (idx % p.cpr) * 8) = w;
+        }
+    }
+}
+
+}  // namespace
+
+template <typename T, bool PAGED>
+__global__ void __launch_bounds__(256) kv_append_fp8_kernel(const Append8Params p) {
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= p.items) return;
+    const int64_t bh = item / (2 * p.nblk), b = bh / p.Hkv;
+    const int r = (int)(item % (2 * p.nblk));
+    append8_item<T, PAGED, kHeld>(p, b, (int)(bh % p.Hkv), r & 1, r >> 1, p.lengths[b]);
+}
+
+// One sequence per workgroup, and its length.
+template <typename T, bool PAGED>
+__global__ void __launch_bounds__(1024) kv_append_fp8_step_kernel(const Append8Params p) {
+    const int64_t b = blockIdx.x;
+    const int length = p.lengths[b];
+    const int per = 2 * p.nblk, items = p.Hkv * per;
+    for (int it = threadIdx.x >> 6; it < items; it += blockDim.x >> 6)
+        append8_item<T, PAGED, kHeldStep>(p, b, it / per, (it % per) & 1, (it % per) >> 1, length);
+    __syncthreads();  // every thread has read the length
+    if (threadIdx.x == 0) p.lengths[b] = (int)min((int64_t)max(length, 0) + p.n_new, (int64_t)p.capacity);
+}
+
+__global__ void __launch_bounds__(256) kv_lengths_fp8_kernel(int32_t* lengths, int64_t B, int32_t n_new, int32_t capacity) {
+    const int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (b < B) lengths[b] = (int)min((int64_t)max(lengths[b], 0) + n_new, (int64_t)capacity);
+}
+
+template <typename T, bool PAGED>
+static int launch_append8(const Append8Params& p, int64_t B, hipStream_t stream) {
+    const int64_t per_seq = p.items / B;
+    if (p.n_new > 0 && per_seq <= 64 && p.n_new <= 64 * kHeldStep / 16 && B <= 0x7fffffff) {
+        const unsigned waves = (unsigned)(per_seq < 16 ? per_seq : 16);
+        hipLaunchKernelGGL((kv_append_fp8_step_kernel<T, PAGED>), dim3((unsigned)B), dim3(64 * waves), 0, stream, p);
+        return check_launch("kv_append_fp8_step_kernel");
+    }
+    const int64_t blocks = (p.items + 3) / 4;
+    if (blocks > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "kv_append_fp8: grid too large");
+    if (p.n_new > 0) {
+        hipLaunchKernelGGL((kv_append_fp8_kernel<T, PAGED>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        const int st = check_launch("kv_append_fp8_kernel");
+        if (st != DTATTN_OK) return st;
+    }
+    hipLaunchKernelGGL(kv_lengths_fp8_kernel, dim3((unsigned)((B + 255) / 256)), dim3(256), 0, stream, p.lengths, B, p.n_new, p.capacity);
+    return check_launch("kv_lengths_fp8_kernel");
+}
+
+}  // namespace dtattn
+
+using namespace dtattn;
+
+extern "C" int dtattn_kv_append_fp8(const dtattn_kv_append_fp8_args* a, void* stream_) {
+    const char* who = "kv_append_fp8";
+    if (a == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: args is NULL", who);
+    if (a->B < 0 || a->Hkv <= 0 || a->n_new < 0 || a->D <= 0 || a->Hkv > (1 << 20))
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
+    Append8Params p = {};
+    Fp8Cache c;
+    int st = fp8_cache_checks(a, a->block_table != nullptr, who, &c);
+    if (st != DTATTN_OK) return st;
+    if (a->dtype != DTATTN_BF16 && a->dtype != DTATTN_FP16 && a->dtype != DTATTN_FP32)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: dtype %d not supported (bf16, fp16, fp32)", who, a->dtype);
+    if (a->n_new > 0x3fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many new tokens", who);
+    if (a->B == 0) return DTATTN_OK;
+    if (a->lengths == nullptr || (a->n_new > 0 && (a->k_new == nullptr || a->v_new == nullptr)))
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    const int64_t esz = a->dtype == DTATTN_FP32 ? 4 : 2;
+    for (int i = 0; i < 3; ++i)
+        if ((a->k_new_stride[i] * esz) % 16 != 0 || (a->v_new_stride[i] * esz) % 16 != 0)
+            return fail(DTATTN_ERR_UNSUPPORTED, "%s: strides of the new tokens must be multiples of 16 bytes", who);
+    if ((reinterpret_cast<uintptr_t>(a->k_new) | reinterpret_cast<uintptr_t>(a->v_new)) & 15u)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: new tokens must be 16-byte aligned", who);
+    const void* src[2] = {a->k_new, a->v_new};
+    void* dst[2] = {a->k_cache, a->v_cache};
+    float* scale[2] = {a->k_scale, a->v_scale};
+    const int64_t* ns[2] = {a->k_new_stride, a->v_new_stride};
+    const int64_t* ds[2] = {a->k_stride, a->v_stride};
+    const int64_t* ss[2] = {a->k_scale_stride, a->v_scale_stride};
+    for (int i = 0; i < 2; ++i) {
+        p.src[i] = reinterpret_cast<const char*>(src[i]);
+        p.dst[i] = reinterpret_cast<char*>(dst[i]);
+        p.scale[i] = scale[i];
+        p.n_b[i] = ns[i][0] * esz, p.n_h[i] = ns[i][1] * esz, p.n_s[i] = ns[i][2] * esz;
+        p.d_b[i] = ds[i][0], p.d_h[i] = ds[i][1], p.d_s[i] = ds[i][2];
+        p.s_b[i] = ss[i][0], p.s_h[i] = ss[i][1];
+    }
+    p.block_table = a->block_table;
+    p.bt_s = a->block_table_stride;
+    p.lengths = a->lengths;
+    p.Hkv = (int32_t)a->Hkv;
+    p.n_new = (int32_t)a->n_new;
+    p.cpr = (int32_t)(a->D / 8);
+    p.capacity = c.capacity;
+    p.page_shift = c.page_shift;
+    p.num_pages = c.num_pages;
+    p.block_shift = c.block_shift;
+    // the first new token may be the last row of its block
+    p.nblk = a->n_new == 0 ? 0 : (int32_t)((a->block - 1 + a->n_new - 1) / a->block + 1);
+    p.items = a->B * a->Hkv * 2 * p.nblk;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const bool paged = a->block_table != nullptr;
+    switch (a->dtype) {
+        case DTATTN_BF16: return paged ? launch_append8<bf16_t, true>(p, a->B, stream) : launch_append8<bf16_t, false>(p, a->B, stream);
+        case DTATTN_FP16: return paged ? launch_append8<f16_t, true>(p, a->B, stream) : launch_append8<f16_t, false>(p, a->B, stream);
+        default: return paged ? launch_append8<float, true>(p, a->B, stream) : launch_append8<float, false>(p, a->B, stream);
+    }
+}

@@ -7,7 +7,9 @@ launches the gfx950 kernels through the dtattn C ABI on the current HIP stream.
 
 New entry points (no reference counterpart, see the host operators):
 ``scaled_dot_product_attention_with_lse``, ``decode_attention``, ``lse_merge``,
-``ring_attention_step`` and ``quantize_fp8_per_head``.
+``ring_attention_step`` and ``quantize_fp8_per_head``; over an 8-bit KV cache ``kv_cache_append_fp8`` and
+``decode_attention_fp8`` (and their paged forms); to bound a cache ``attention_weight_accumulate`` and
+``kv_cache_evict``.
 """
 from __future__ import annotations
 
@@ -152,6 +154,83 @@ def kv_cache_append_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_ta
     """kv_cache_append for the paged cache of decode_attention_paged; the block table must already name
     the pages of the positions being written."""
     _h.KvCacheAppendPagedOp().compute([k_pages, v_pages, block_table, lengths, k_new, v_new])
+
+
+def kv_cache_append_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                        lengths: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
+    """kv_cache_append into an 8-bit cache, in place: e4m3fn codes with one scale per block of tokens and kv head.
+
+    k_cache / v_cache float8_e4m3fn [B, Hkv, S_max, D]; k_scale / v_scale fp32 [B, Hkv, S_max / block] (the block,
+    a power of two from 16 to 256, follows from the shapes); k_new / v_new bf16, fp16 or fp32 [B, Hkv, n_new, D].
+    A value is code * scale.  A block's scale is the smallest power of two that holds its largest value within
+    +-448; a block that outgrows its scale re-encodes its older tokens (exact, subnormal codes apart).  NaN and
+    infinite inputs become NaN codes and leave the scale to the others.
+    """
+    _h.KvCacheAppendFp8Op().compute([k_cache, v_cache, k_scale, v_scale, lengths, k_new, v_new])
+
+
+def kv_cache_append_fp8_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                              block_table: torch.Tensor, lengths: torch.Tensor, k_new: torch.Tensor,
+                              v_new: torch.Tensor) -> None:
+    """kv_cache_append_fp8 into a paged cache: pools float8_e4m3fn [num_pages, Hkv, page_size, D], scales fp32
+    [num_pages, Hkv, page_size / block]; block table and dropped tokens as for kv_cache_append_paged."""
+    _h.KvCacheAppendFp8PagedOp().compute([k_pages, v_pages, k_scale, v_scale, block_table, lengths, k_new, v_new])
+
+
+def decode_attention_fp8(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, lengths: torch.Tensor,
+                         scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """decode_attention over an 8-bit cache (kv_cache_append_fp8), any positive scales.
+
+    query bf16, fp16 or fp32 [B, Hq, 1, D], D a multiple of 16 up to 128.  Returns (O [B, Hq, 1, D] in the query's
+    type, LSE [B, Hq] fp32).
+    """
+    o, lse = _h.SdpaDecodeFp8Op(None if scale is None else float(scale)).compute(
+        [query, k_cache, v_cache, k_scale, v_scale, lengths])
+    return o, lse
+
+
+def decode_attention_fp8_paged(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                               k_scale: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor,
+                               lengths: torch.Tensor,
+                               scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """decode_attention_fp8 over a paged 8-bit cache (kv_cache_append_fp8_paged)."""
+    o, lse = _h.SdpaDecodeFp8PagedOp(None if scale is None else float(scale)).compute(
+        [query, k_pages, v_pages, k_scale, v_scale, block_table, lengths])
+    return o, lse
+
+
+def attention_weight_accumulate(weights: torch.Tensor, query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor,
+                                lengths: Optional[torch.Tensor] = None, is_causal: bool = False, q_offset: int = 0,
+                                scale: Optional[float] = None,
+                                key_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Add the attention weight that each key has received to ``weights`` (fp32 [B, Hkv, S]), in place.
+
+    weights[b, hk, j] += sum over the query heads of hk and the queries i that see key j of
+    exp(scale q_i . k_j - lse_i).  query [B, Hq, L, D] with the LSE [B, Hq, L] of its attention over the same keys (for
+    one query also [B, Hq], as decode_attention returns it); key [B, Hkv, S, D] of the query's dtype, or float8_e4m3fn
+    codes with key_scale [B, Hkv, S / block].  Key j is visible to query i iff j < lengths[b] (S without lengths) and,
+    when causal, j <= i + q_offset; with causal and lengths, queries at or past lengths[b] are padding and add nothing.
+    Weights at or past lengths[b] are left as they are.  Returns ``weights``.
+    """
+    param = _h.AttentionWeightsParam(None if scale is None else float(scale), bool(is_causal), int(q_offset))
+    return _h.AttentionWeightsOp(param).compute([weights, query, key, lse, lengths, key_scale])[0]
+
+
+def kv_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, weights: torch.Tensor,
+                   keep: int, recent: int, block: Optional[int] = None, k_scale: Optional[torch.Tensor] = None,
+                   v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Shrink each sequence of a padded cache to ``keep`` tokens by accumulated attention weight, in place.
+
+    Every kv head keeps its last ``recent`` tokens and, of the others, those with the largest ``weights`` (fp32
+    [B, Hkv, S_max], as attention_weight_accumulate sums them; of equal ones the first), in units of ``block`` tokens:
+    1 by default, the tokens of a scale for an 8-bit cache with k_scale and v_scale.  What stays moves to the front in
+    its order, its weights and scales with it; weights behind are zeroed and ``lengths`` shrinks.  A sequence of no
+    more than keep / block blocks is left alone.  ``keep`` and ``recent`` are multiples of ``block``.  Returns the
+    indices of the blocks that stayed, int32 [B, Hkv, keep / block], -1 past them.
+    """
+    param = _h.KvCacheEvictParam(int(keep), int(recent), 0 if block is None else int(block))
+    return _h.KvCacheEvictOp(param).compute([k_cache, v_cache, lengths, weights, k_scale, v_scale])[0]
 
 
 def lse_merge(outs: Sequence[torch.Tensor], lses: Sequence[torch.Tensor],

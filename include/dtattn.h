@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define DTATTN_ABI_VERSION 11
+#define DTATTN_ABI_VERSION 12
 
 /* Softmax scale fields (ABI version 8): NaN selects 1/sqrt(D) (computed in double and rounded once to
  * float, as libtorch computes its default, from ABI version 10); any finite value is used as given,
@@ -289,6 +289,153 @@ typedef struct {
 } dtattn_kv_append_paged_args;
 
 int dtattn_kv_append_paged(const dtattn_kv_append_paged_args* args, void* stream);
+
+/* ---- KV cache in 8 bits (ABI version 12) -----------------------------------------------------------
+ *
+ * No counterpart in the reference, which keeps no KV cache (python/dtorch/test/modules/llama.py:126-156).
+ * Keys and values are held as OCP e4m3fn codes, with one fp32 scale for each block of `block` consecutive
+ * tokens of a kv head, separately for K and V: value = code * scale.  `block` is a power of two from 16 to
+ * 256.  In a padded cache block i of sequence b holds tokens [i * block, (i + 1) * block) and its scale is
+ * k_scale[b, h, i]; S_max is a multiple of `block`.  In a paged cache a page holds page_size / block whole
+ * blocks and the scale of the block that row r of a page lies in is k_scale[page, h, r / block].  Scales
+ * have a stride of 1 between the blocks of a head.  Head dims D: multiples of 16 up to 128; code strides
+ * are multiples of 16 bytes, a row stride is at least D, and code pointers are 16-byte aligned.
+ */
+
+/* Quantised append: the new tokens' keys and values as codes into the cache.
+ *
+ * Positions, capacity, unassigned pages and the lengths' advance are those of dtattn_kv_append[_paged].
+ * With amax the largest |x| over the finite new values of a block (of K or of V), the block needs the scale
+ * 2^k, the smallest power of two with amax <= 448 * 2^k and k >= -126 (1 when amax is 0).  A block whose
+ * first row is among the new tokens takes that scale.  A block that already holds tokens keeps the larger
+ * of its scale and the needed one; when that is a new scale, its r older rows become
+ * e4m3fn_rne(code * (old / new)), which is exact for the powers of two that this call writes, subnormal
+ * codes apart.  New codes are e4m3fn_rne(x * (1 / scale)); NaN and infinities become NaN codes.  Rows past
+ * the written ones are left as they were. */
+typedef struct {
+    const void* k_new;     /* [B, Hkv, n_new, D], `dtype` (any strides that are multiples of 16 bytes, D stride 1) */
+    const void* v_new;
+    void* k_cache;         /* codes [B, Hkv, S_max, D], or a page pool [num_pages, Hkv, page_size, D] */
+    void* v_cache;
+    float* k_scale;        /* [B, Hkv, S_max / block], or [num_pages, Hkv, page_size / block] */
+    float* v_scale;
+    const int32_t* block_table; /* paged: [B, max_pages] device int32; NULL: padded cache */
+    int32_t* lengths;      /* [B] device int32, read and then advanced */
+    int64_t B, Hkv, n_new, D;
+    int64_t S_max;         /* padded: capacity */
+    int64_t num_pages, page_size, max_pages; /* paged: page_size a power of two >= 16 */
+    int64_t k_new_stride[3]; /* B, H, token (elements) */
+    int64_t v_new_stride[3];
+    int64_t k_stride[3];     /* (B | page), H, row (bytes) */
+    int64_t v_stride[3];
+    int64_t k_scale_stride[2]; /* (B | page), H (elements) */
+    int64_t v_scale_stride[2];
+    int64_t block_table_stride;
+    int32_t block;
+    int32_t dtype;           /* of the new tokens: BF16, FP16 or FP32 */
+} dtattn_kv_append_fp8_args;
+
+int dtattn_kv_append_fp8(const dtattn_kv_append_fp8_args* args, void* stream);
+
+/* Single-token attention over such a cache: dtattn_decode_splitkv's arithmetic with K = code * k_scale and
+ * V = code * v_scale, any positive finite scales.  Scores, softmax statistics and accumulators are fp32; codes enter the products
+ * exactly.  With 16-bit queries P is rounded to their type for the second product, as in the 16-bit decode; with FP32
+ * queries both products carry fp32 operands (three bf16 parts of each).  Rows at or past lengths[b] are never read; page ids are
+ * clamped into the pool. */
+typedef struct {
+    const void* q;           /* [B, Hq, 1, D], 16-byte aligned, strides multiples of 16 bytes */
+    const void* k_cache;     /* codes, as above */
+    const void* v_cache;
+    const float* k_scale;
+    const float* v_scale;
+    const int32_t* block_table; /* NULL: padded cache */
+    const int32_t* lengths;  /* [B] device int32; clamped to [0, capacity]; 0 gives O = 0, LSE = -inf */
+    void* o;                 /* [B, Hq, 1, D], dtype of q, 16-byte aligned, strides multiples of 16 bytes */
+    float* lse;              /* [B, Hq] fp32; may be NULL */
+    int64_t B, Hq, Hkv, D;
+    int64_t S_max;
+    int64_t num_pages, page_size, max_pages;
+    int64_t q_stride[2];     /* B, H (elements) */
+    int64_t k_stride[3];     /* (B | page), H, row (bytes) */
+    int64_t v_stride[3];
+    int64_t k_scale_stride[2];
+    int64_t v_scale_stride[2];
+    int64_t o_stride[2];     /* B, H (elements) */
+    int64_t lse_stride[1];   /* B (H stride is 1) */
+    int64_t block_table_stride;
+    int32_t block;
+    int32_t dtype;           /* of q and o: BF16, FP16 or FP32 */
+    float scale;             /* NaN means 1/sqrt(D) */
+    void* workspace;         /* >= dtattn_decode_fp8_workspace_size(args, stream) bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} dtattn_decode_fp8_args;
+
+/* Workspace of a call on `stream`'s device; reads the sizes of `args` only. */
+size_t dtattn_decode_fp8_workspace_size(const dtattn_decode_fp8_args* args, void* stream);
+int dtattn_decode_fp8(const dtattn_decode_fp8_args* args, void* stream);
+
+/* ---- a bounded KV cache (ABI version 12) -------------------------------------------------------------
+ *
+ * Accumulated attention weights: for every kv head and key,
+ *   weights[b, hk, j] += sum over the query heads h of hk and the queries i that see key j of
+ *                        exp(scale * q[b, h, i] . k[b, hk, j] - lse[b, h, i])
+ * where lse is what the attention over the same keys returned.  Key j is visible to query i iff
+ * j < n = lengths[b] (S without lengths) and, when causal, j <= i + q_offset; with causal and lengths a query at
+ * i + q_offset >= n is padding and adds nothing.  A row whose lse is -inf (it sees no key) adds nothing.
+ * Sums are fp32 in an order that depends on the sizes alone.  Only weights[b, hk, j < n] are touched. */
+typedef struct {
+    float* weights;          /* [B, Hkv, S], key stride 1 */
+    const void* q;           /* [B, Hq, L, D] */
+    const void* k;           /* [B, Hkv, S, D], `k_dtype`; codes take k_scale */
+    const float* k_scale;    /* FP8 keys: [B, Hkv, S / block] */
+    const float* lse;        /* [B, Hq, L] fp32, query stride 1 */
+    const int32_t* lengths;  /* [B] device int32, clamped to [0, S]; may be NULL */
+    int64_t B, Hq, Hkv, L, S, D;
+    int64_t w_stride[2];     /* B, H */
+    int64_t q_stride[3];     /* B, H, L (elements) */
+    int64_t k_stride[3];     /* B, H, S (elements) */
+    int64_t k_scale_stride[2];
+    int64_t lse_stride[2];   /* B, H */
+    int64_t q_offset;
+    int32_t causal;
+    int32_t block;           /* FP8 keys: tokens per scale */
+    int32_t q_dtype;         /* BF16, FP16 or FP32 */
+    int32_t k_dtype;         /* q_dtype or FP8_E4M3FN */
+    float scale;             /* NaN means 1/sqrt(D) */
+} dtattn_weights_args;
+
+int dtattn_attention_weights(const dtattn_weights_args* args, void* stream);
+
+/* Eviction by accumulated weight.  A kv head of a sequence of n = lengths[b] tokens (clamped to [0, S_max]) is
+ * ceil(n / block) blocks of `block` tokens, the last one of n's remainder.  With more than keep / block of them, the last
+ * recent / block stay, and of the others the keep / block - recent / block with the largest weight: the sum of the block's
+ * weights in 64 bits rounded to fp32, NaN as -inf, of equal ones the lowest index.  The rows of the blocks that stay move
+ * to the front in their order, with their weights and (8-bit caches) their scales; the weights behind them up to n become
+ * 0, and lengths[b] becomes keep - block + the tokens of the last block.  Rows behind are left as they were.  A sequence
+ * of no more than keep / block blocks is left alone.  kept[b, h, i] is the index of the i-th block that stayed, -1 past
+ * them.  1 <= block <= recent <= keep, both multiples of block, block a power of two up to 256; with codes, block is a multiple of
+ * scale_block.  K and V rows are `row_bytes` bytes, a multiple of 16, at strides that are multiples of 16 bytes. */
+typedef struct {
+    void* k_cache;           /* [B, Hkv, S_max, row] */
+    void* v_cache;
+    float* k_scale;          /* NULL, or [B, Hkv, S_max / scale_block] */
+    float* v_scale;
+    float* weights;          /* [B, Hkv, S_max], key stride 1 */
+    int32_t* lengths;        /* [B] device int32, read and then updated */
+    int32_t* kept;           /* [B, Hkv, keep / block] contiguous */
+    int64_t B, Hkv, S_max, keep, recent, block, scale_block;
+    int64_t row_bytes;
+    int64_t k_stride[3];     /* B, H, row (bytes) */
+    int64_t v_stride[3];
+    int64_t k_scale_stride[2];
+    int64_t v_scale_stride[2];
+    int64_t w_stride[2];     /* B, H */
+    void* workspace;         /* >= dtattn_kv_evict_workspace_size(args) bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} dtattn_kv_evict_args;
+
+size_t dtattn_kv_evict_workspace_size(const dtattn_kv_evict_args* args);
+int dtattn_kv_evict(const dtattn_kv_evict_args* args, void* stream);
 
 /* LSE merge of n partial attention blocks over the same queries.
  *
