@@ -8,8 +8,10 @@
 // exponentials.  Both keep a wave's keys in registers as MFMA operands (64 keys: four tiles of 16) and pass the queries
 // by in sets of 16 (query, head) columns, so that the sum over queries stays in registers too and no two waves add
 // to one weight: the result does not depend on timing.
+#include <algorithm>
 #include <type_traits>
 
+#include "decode_params.hpp"
 #include "fp8_cache.hpp"
 
 namespace dtattn {
@@ -29,6 +31,9 @@ struct WeightParams {
     int32_t B, Hkv, group, L, S, d, block_shift;
     float c;  // scale * log2(e)
     uint32_t q_and, q_xor;
+    float* part;               // prompts whose columns several workgroups share: [parts, B * Hkv, S]
+    int32_t parts, part_tiles; // and the column tiles of each
+    int32_t key_blocks;
 };
 
 namespace {
@@ -189,8 +194,302 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(const WeightParams p)
     }
 }
 
+// ---- prompts --------------------------------------------------------------------------------------------------
+
+namespace {
+
+constexpr int kCols = 32;  // columns of a tile: 32x32 products
+
+// 16-bit and 8-bit keys are one operand; fp32 ones are three bf16 parts (8 bits each, exact), of whose nine products with the
+// query's parts the six largest count: what is left out is below 2^-23 of |q| |k|, an fp32 sum's own rounding.
+template <typename TQ, typename TK>
+struct PromptTypes {
+    typedef typename std::conditional<std::is_same<TQ, f16_t>::value, f16_t, bf16_t>::type E;
+    typedef typename Elem<E>::vec8 V8;
+    static constexpr int qparts = std::is_same<TQ, float>::value ? 3 : 1;
+    static constexpr int kparts = std::is_same<TK, float>::value ? 3 : 1;
+    static constexpr int tiles = kparts == 3 ? 1 : 2;  // of 32 keys per wave
+    static constexpr int keys = 4 * 32 * tiles;        // per workgroup
+};
+
+// Elements x .. x + 7 of a row of d (a multiple of 16 bytes), zeros past its end.
+template <typename T>
+__device__ __forceinline__ Chunk<T> load8(const T* row, int x, int d) {
+    Chunk<T> w = {};
+    if (x < d) w.v[0] = ld16(row + x);
+    if constexpr (sizeof(T) == 4) if (x + 4 < d) w.v[1] = ld16(row + x + 4);
+    return w;
+}
+
+// 8 elements as the bf16 parts or the one operand that they are.
+template <typename T, typename V8, int PARTS>
+__device__ __forceinline__ void to_parts(const Chunk<T>& w, V8* out) {
+    if constexpr (PARTS == 1) {
+        out[0] = __builtin_bit_cast(V8, w.v[0]);
+    } else {
+        float y[8];
+        unpack_chunk<T>(w, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            bf16_t t[3];
+            split3(y[e], t);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) out[i][e] = t[i];
+        }
+    }
+}
+
+// (query, head) of a column, columns query-major, stepping by kCols.
+struct Column {
+    int64_t i;
+    int h;
+    __device__ __forceinline__ Column(int64_t n, int group) : i(n / group), h((int)(n - n / group * group)) {}
+    __device__ __forceinline__ void step(int di, int dh, int group) {
+        i += di;
+        h += dh;
+        if (h >= group) h -= group, ++i;
+    }
+};
+
+}  // namespace
+
+// A workgroup of four waves holds 256 keys (128 in fp32) as operands and passes column tiles by, which its threads stage
+// through LDS one tile ahead.  A column is a lane, so its lse is one register and the sums over columns are one
+// add per score; lanes meet once, at the end.  Per wave and tile of 16-bit operands 16 MFMAs against 32 exponentials and 64 other
+// VALU instructions.
+template <typename TQ, typename TK, int D, bool CAUSAL>
+__global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const WeightParams p) {
+    typedef PromptTypes<TQ, TK> Types;
+    typedef typename Types::E E;
+    typedef typename Types::V8 V8;
+    constexpr int QP = Types::qparts, KP = Types::kparts, KT = Types::tiles, KS = D / 16, DC = D / 8;
+    constexpr int PER = kCols * DC / 256;  // chunks of 8 elements that a thread stages
+    __shared__ __attribute__((aligned(16))) V8 stage[2][QP][kCols * DC];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    // workgroup -> (key block, part of the columns, slice); slices go round the XCDs, whose L2 then holds their queries
+    const int slices = p.B * p.Hkv;
+    const int slice = blockIdx.x % slices;
+    const int rest = blockIdx.x / slices;
+    const int part = rest % p.parts, kblock = rest / p.parts;
+    const int64_t b = slice / p.Hkv;
+    const int hk = slice % p.Hkv;
+    const int n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
+    const int kwg = kblock * Types::keys;
+    if (kwg >= n) return;
+    const int64_t N = (int64_t)p.L * p.group;
+    int64_t first = 0, last = N;  // the block's columns
+    if constexpr (CAUSAL) {
+        first = min(max((int64_t)kwg - p.q_offset, (int64_t)0) * p.group, N);
+        if (p.lengths != nullptr) last = min(N, max(n - p.q_offset, (int64_t)0) * p.group);
+    }
+    const int64_t t0 = max(first / kCols, (int64_t)part * p.part_tiles);
+    const int64_t t1 = min((last + kCols - 1) / kCols, (int64_t)(part + 1) * p.part_tiles);
+    if (t0 >= t1) return;  // the sum knows
+    const int k0 = kwg + __builtin_amdgcn_readfirstlane(tid >> 6) * 32 * KT;
+
+    const TK* kb = reinterpret_cast<const TK*>(p.k) + b * p.k_b + hk * p.k_h;
+    V8 kf[KT][KP][KS];
+    float c[KT][2];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const TK* row = kb + (int64_t)min(k0 + 32 * t + col, n - 1) * p.k_s;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int x = 16 * s + 8 * half;
+            if constexpr (sizeof(TK) == 1) {
+                const u32x2 w = x < p.d ? *reinterpret_cast<const u32x2*>(row + x) : u32x2{0u, 0u};
+                kf[t][0][s] = codes_to_vec8<E>(w.x, w.y);
+            } else {
+                const Chunk<TK> w = load8(row, x, p.d);
+                V8 o[KP];
+                to_parts<TK, V8, KP>(w, o);
+#pragma unroll
+                for (int i = 0; i < KP; ++i) kf[t][i][s] = o[i];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            c[t][u] = p.c;
+            if constexpr (sizeof(TK) == 1) c[t][u] *= p.ks[b * p.ks_b + hk * p.ks_h + (min(k0 + 32 * t + 16 * u, n - 1) >> p.block_shift)];
+        }
+    }
+
+    const TQ* qb = reinterpret_cast<const TQ*>(p.q) + b * p.q_b + (int64_t)hk * p.group * p.q_h;
+    const float* lb = p.lse + b * p.lse_b + (int64_t)hk * p.group * p.lse_h;
+    const int di = kCols / p.group, dh = kCols % p.group;
+    // chunk x of row r of a tile lies at x ^ swz(r): 16 rows read one chunk each without a conflict
+    auto swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+    Column own(t0 * kCols + col, p.group);  // this lane's column
+    int64_t left = last - t0 * kCols;       // columns from the tile on
+    const int r0 = tid / DC, x0 = tid % DC;  // rows r0 + k * 256 / DC of a tile
+    Column src0(t0 * kCols + r0, p.group), src1(t0 * kCols + r0 + 256 / DC, p.group);
+    Chunk<TQ> raw[PER];
+    float lse;
+    auto load = [&]() {  // the tile that src0, src1 and own stand at, and on to the next
+        int64_t at[2] = {src0.i * p.q_s + src0.h * p.q_h, src1.i * p.q_s + src1.h * p.q_h};
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const bool ok = r0 + k * (256 / DC) < left;
+            raw[k] = load8(qb + (ok ? at[k] : 0), 8 * x0, ok ? p.d : 0);
+        }
+        lse = col < left ? lb[own.h * p.lse_h + own.i] : kNegInf;
+        left -= kCols;
+        src0.step(di, dh, p.group);
+        src1.step(di, dh, p.group);
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int r = r0 + k * (256 / DC);
+            Chunk<TQ> w = raw[k];
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(w.v) / sizeof(w.v[0])); ++i) w.v[i] = q_bits(w.v[i], p.q_and, p.q_xor);
+            V8 o[QP];
+            to_parts<TQ, V8, QP>(w, o);
+#pragma unroll
+            for (int i = 0; i < QP; ++i) stage[buf][i][r * DC + (x0 ^ swz(r))] = o[i];
+        }
+    };
+
+    float sum[KT][16] = {};
+    load();
+    for (int64_t t = t0; t < t1; ++t) {
+        const int buf = (int)(t - t0) & 1;
+        put(buf);
+        const bool none = lse == kNegInf;
+        const float nl = -lse * kLog2e;
+        int lim = 32 * KT - 1;  // the last of the wave's keys that this column sees
+        if constexpr (CAUSAL) lim = (int)min(max(own.i + p.q_offset - k0, (int64_t)-1), (int64_t)(32 * KT - 1));
+        if (none) lim = -1;
+        own.step(di, dh, p.group);
+        if (t + 1 < t1) load();
+        lds_barrier();
+        // buffers alternate, and this barrier has every wave past its reads of the other one's last tile
+        if (k0 < n && __ballot(lim >= 0) != 0) {
+            f32x16 s[KT] = {};
+#pragma unroll
+            for (int x = 0; x < KS; ++x) {
+                V8 qf[QP];
+#pragma unroll
+                for (int i = 0; i < QP; ++i) qf[i] = stage[buf][i][col * DC + ((2 * x + half) ^ swz(col))];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < KP; ++i)
+#pragma unroll
+                        for (int j = 0; j < QP && i + j < 3; ++j) s[kt] = Elem<E>::mfma32(kf[kt][i][x], qf[j], s[kt]);
+            }
+            if (__ballot(lim < 32 * KT - 1) == 0) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[kt][i] += fast_exp2(__builtin_fmaf(s[kt][i], c[kt][i >> 3], nl));
+            } else {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = fast_exp2(__builtin_fmaf(s[kt][i], c[kt][i >> 3], nl));
+                        sum[kt][i] += 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3) <= lim ? x : 0.f;
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float s = group_sum<32>(sum[kt][i]);
+            v = col == i ? s : v;
+        }
+        const int key = k0 + 32 * kt + 8 * (col >> 2) + 4 * half + (col & 3);
+        if (col < 16 && key < n) {
+            if (p.parts == 1) p.w[b * p.w_b + hk * p.w_h + key] += v;
+            else p.part[((int64_t)part * slices + slice) * p.S + key] = v;
+        }
+    }
+}
+
+// Adds the parts of a key in their order: those whose workgroup had columns.
+template <bool CAUSAL>
+__global__ void __launch_bounds__(256) attn_weights_sum_kernel(const WeightParams p, int keys) {
+    const int key = blockIdx.x * 256 + threadIdx.x;
+    const int slices = p.B * p.Hkv, slice = blockIdx.y;
+    const int64_t b = slice / p.Hkv;
+    const int hk = slice % p.Hkv;
+    const int n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
+    if (key >= n) return;
+    const int64_t N = (int64_t)p.L * p.group;
+    int64_t first = 0, last = N;
+    if constexpr (CAUSAL) {
+        first = min(max((int64_t)(key / keys * keys) - p.q_offset, (int64_t)0) * p.group, N);
+        if (p.lengths != nullptr) last = min(N, max(n - p.q_offset, (int64_t)0) * p.group);
+    }
+    const int64_t t0 = first / kCols, t1 = (last + kCols - 1) / kCols;
+    if (t0 >= t1) return;
+    const int x0 = (int)(t0 / p.part_tiles), x1 = (int)((t1 - 1) / p.part_tiles);
+    float v = 0.f;
+    for (int x = x0; x <= x1; ++x) v += p.part[((int64_t)x * slices + slice) * p.S + key];
+    p.w[b * p.w_b + hk * p.w_h + key] += v;
+}
+
+namespace {
+
+// Parts that a prompt's columns are cut in, so that the workgroups (two fit a CU) go round a few times.
+struct PromptPlan {
+    int64_t key_blocks, parts, part_tiles;
+    size_t bytes;
+};
+
+PromptPlan prompt_plan(const dtattn_weights_args* a, int keys, int cus) {
+    PromptPlan r;
+    r.key_blocks = (a->S + keys - 1) / keys;
+    const int64_t group = a->Hq / a->Hkv, slices = a->B * a->Hkv;
+    const int64_t tiles = (a->L * group + kCols - 1) / kCols;
+    double work = (double)r.key_blocks * (double)tiles;
+    if (a->causal != 0) {  // key block k sees the columns from key k * keys - q_offset on
+        work = 0;
+        const int64_t step = std::max<int64_t>(1, r.key_blocks / 256);  // sampled
+        for (int64_t k = 0; k < r.key_blocks; k += step) {
+            const int64_t from = std::min<int64_t>(std::max<int64_t>(k * keys - a->q_offset, 0), a->L);
+            work += (double)step * (double)((a->L - from) * group) / kCols;
+        }
+    }
+    work *= (double)slices;
+    r.part_tiles = std::max<int64_t>(8, (int64_t)(work / (2.0 * cus * 3)) + 1);
+    r.part_tiles = std::min(r.part_tiles, tiles);
+    r.parts = (tiles + r.part_tiles - 1) / r.part_tiles;
+    r.bytes = r.parts > 1 ? (((size_t)r.parts * slices * a->S * sizeof(float) + 255) & ~(size_t)255) : 0;
+    return r;
+}
+
+// One set of 16 columns is the token form's; it reads the keys once and is done.
+bool is_prompt(const dtattn_weights_args* a) { return a->L * (a->Hq / a->Hkv) > 64; }
+
+int prompt_keys(const dtattn_weights_args* a) { return a->k_dtype == DTATTN_FP32 ? PromptTypes<float, float>::keys : PromptTypes<bf16_t, bf16_t>::keys; }
+
+}  // namespace
+
 template <typename TQ, typename TK, int D>
-static int launch_weights(const WeightParams& p, bool causal, hipStream_t stream) {
+static int launch_prompt(WeightParams p, bool causal, const PromptPlan& plan, hipStream_t stream) {
+    const int64_t slices = (int64_t)p.B * p.Hkv;
+    p.parts = (int32_t)plan.parts, p.part_tiles = (int32_t)plan.part_tiles, p.key_blocks = (int32_t)plan.key_blocks;
+    const dim3 grid((unsigned)(slices * plan.parts * plan.key_blocks));
+    if (causal) hipLaunchKernelGGL((attn_weights_prompt_kernel<TQ, TK, D, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attn_weights_prompt_kernel<TQ, TK, D, false>), grid, dim3(256), 0, stream, p);
+    const int st = check_launch("attn_weights_prompt_kernel");
+    if (st != DTATTN_OK || plan.parts == 1) return st;
+    const dim3 sums((unsigned)((p.S + 255) / 256), (unsigned)slices);
+    const int keys = PromptTypes<TQ, TK>::keys;
+    if (causal) hipLaunchKernelGGL(attn_weights_sum_kernel<true>, sums, dim3(256), 0, stream, p, keys);
+    else hipLaunchKernelGGL(attn_weights_sum_kernel<false>, sums, dim3(256), 0, stream, p, keys);
+    return check_launch("attn_weights_sum_kernel");
+}
+
+template <typename TQ, typename TK, int D>
+static int launch_weights(const WeightParams& p, bool causal, const PromptPlan* plan, hipStream_t stream) {
+    if (plan != nullptr) return launch_prompt<TQ, TK, D>(p, causal, *plan, stream);
     const dim3 grid((unsigned)((p.S + 64 * kTiles - 1) / (64 * kTiles)), (unsigned)p.Hkv, (unsigned)p.B);
     if (causal) hipLaunchKernelGGL((attn_weights_kernel<TQ, TK, D, true>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((attn_weights_kernel<TQ, TK, D, false>), grid, dim3(256), 0, stream, p);
@@ -198,13 +497,19 @@ static int launch_weights(const WeightParams& p, bool causal, hipStream_t stream
 }
 
 template <typename TQ, typename TK>
-static int dispatch_weights(const WeightParams& p, bool causal, hipStream_t stream) {
-    return p.d <= 64 ? launch_weights<TQ, TK, 64>(p, causal, stream) : launch_weights<TQ, TK, 128>(p, causal, stream);
+static int dispatch_weights(const WeightParams& p, bool causal, const PromptPlan* plan, hipStream_t stream) {
+    return p.d <= 64 ? launch_weights<TQ, TK, 64>(p, causal, plan, stream) : launch_weights<TQ, TK, 128>(p, causal, plan, stream);
 }
 
 }  // namespace dtattn
 
 using namespace dtattn;
+
+extern "C" size_t dtattn_attention_weights_workspace_size(const dtattn_weights_args* a, void* stream) {
+    if (a == nullptr || a->B <= 0 || a->Hkv <= 0 || a->Hq < a->Hkv || a->L <= 0 || a->S <= 0 || !is_prompt(a)) return 0;
+    const int cus = stream_cus(reinterpret_cast<hipStream_t>(stream));
+    return prompt_plan(a, prompt_keys(a), cus > 0 ? cus : 256).bytes;
+}
 
 extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stream_) {
     const char* who = "attention_weights";
@@ -220,7 +525,7 @@ extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stre
     const int64_t qe = a->q_dtype == DTATTN_FP32 ? 4 : 2, ke = codes ? 1 : qe;
     if (a->D > 128 || (a->D * ke) % 16 != 0)
         return fail(DTATTN_ERR_UNSUPPORTED, "%s: head dim %lld not supported (rows of a multiple of 16 bytes, up to 128)", who, (long long)a->D);
-    if (a->S > (1 << 29) || a->L > (1 << 29) || a->B > 65535 || a->Hkv > 65535)
+    if (a->S > (1 << 29) || a->L > (1 << 29) || a->B > 65535 || a->Hkv > 65535 || a->B * a->Hkv > 65535)
         return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
     const int64_t most = (int64_t)1 << 40;
     if (a->q_offset > most || a->q_offset < -most) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: q_offset out of range", who);
@@ -256,12 +561,25 @@ extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stre
     p.q_and = sp.q_and, p.q_xor = sp.q_xor;
     const bool causal = a->causal != 0;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-    if (codes) {
-        if (a->q_dtype == DTATTN_BF16) return dispatch_weights<bf16_t, uint8_t>(p, causal, stream);
-        if (a->q_dtype == DTATTN_FP16) return dispatch_weights<f16_t, uint8_t>(p, causal, stream);
-        return dispatch_weights<float, uint8_t>(p, causal, stream);
+    PromptPlan prompt;
+    const PromptPlan* plan = nullptr;
+    if (is_prompt(a)) {
+        const int cus = stream_cus(stream);
+        if (cus <= 0) return fail(DTATTN_ERR_DEVICE, "%s: cannot tell the stream's device", who);
+        prompt = prompt_plan(a, prompt_keys(a), cus);
+        if (prompt.key_blocks * prompt.parts * a->B * a->Hkv > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
+        if (prompt.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < prompt.bytes))
+            return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, prompt.bytes, a->workspace_bytes);
+        if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(DTATTN_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+        p.part = reinterpret_cast<float*>(a->workspace);
+        plan = &prompt;
     }
-    if (a->q_dtype == DTATTN_BF16) return dispatch_weights<bf16_t, bf16_t>(p, causal, stream);
-    if (a->q_dtype == DTATTN_FP16) return dispatch_weights<f16_t, f16_t>(p, causal, stream);
-    return dispatch_weights<float, float>(p, causal, stream);
+    if (codes) {
+        if (a->q_dtype == DTATTN_BF16) return dispatch_weights<bf16_t, uint8_t>(p, causal, plan, stream);
+        if (a->q_dtype == DTATTN_FP16) return dispatch_weights<f16_t, uint8_t>(p, causal, plan, stream);
+        return dispatch_weights<float, uint8_t>(p, causal, plan, stream);
+    }
+    if (a->q_dtype == DTATTN_BF16) return dispatch_weights<bf16_t, bf16_t>(p, causal, plan, stream);
+    if (a->q_dtype == DTATTN_FP16) return dispatch_weights<f16_t, f16_t>(p, causal, plan, stream);
+    return dispatch_weights<float, float>(p, causal, plan, stream);
 }

@@ -226,7 +226,15 @@ void AttentionWeightsOp::Compute(const TorchTensorOptArray& in, TorchTensorArray
     a.q_dtype = DtypeCode(st);
     a.k_dtype = DtypeCode(k.scalar_type());
     a.scale = s;
-    Check(dtattn_attention_weights(&a, CurrentStream(w)), "dtattn_attention_weights");
+    void* stream = CurrentStream(w);
+    const size_t ws = dtattn_attention_weights_workspace_size(&a, stream);
+    at::Tensor wst;
+    if (ws > 0) {
+        wst = at::empty({(int64_t)ws}, w.options().dtype(at::kByte));
+        a.workspace = wst.data_ptr();
+        a.workspace_bytes = ws;
+    }
+    Check(dtattn_attention_weights(&a, stream), "dtattn_attention_weights");
     outputs.push_back(w);
 }
 

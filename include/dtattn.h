@@ -402,8 +402,12 @@ typedef struct {
     int32_t q_dtype;         /* BF16, FP16 or FP32 */
     int32_t k_dtype;         /* q_dtype or FP8_E4M3FN */
     float scale;             /* NaN means 1/sqrt(D) */
+    void* workspace;         /* >= dtattn_attention_weights_workspace_size(args, stream) bytes (it may be 0), 256-byte aligned */
+    size_t workspace_bytes;
 } dtattn_weights_args;
 
+/* Workspace of a call on `stream`'s device; reads the sizes, types and `causal` / `q_offset` of `args` only. */
+size_t dtattn_attention_weights_workspace_size(const dtattn_weights_args* args, void* stream);
 int dtattn_attention_weights(const dtattn_weights_args* args, void* stream);
 
 /* Eviction by accumulated weight.  A kv head of a sequence of n = lengths[b] tokens (clamped to [0, S_max]) is

@@ -92,8 +92,11 @@ def test_one_query(dtype, codes, Hq, Hkv, D):
 @pytest.mark.parametrize("L,S,Hq,Hkv,D,causal,q_offset,lengths", [
     (1, 1, 2, 2, 64, True, 0, None), (50, 50, 4, 2, 128, True, 0, None), (50, 50, 6, 2, 64, True, 0, [50, 33, 0]), (130, 130, 3, 3, 48, True, 0, [1, 130, 64]),
     (33, 200, 8, 2, 128, True, 167, [200, 180, 190]), (40, 100, 4, 1, 64, False, 0, None), (40, 100, 4, 1, 64, False, 0, [7, 100, 64]),
-    (30, 90, 5, 1, 128, True, -10, None), (20, 64, 2, 1, 64, True, 500, None), (257, 257, 4, 4, 128, True, 0, None)])
+    (30, 90, 5, 1, 128, True, -10, None), (20, 64, 2, 1, 64, True, 500, None), (257, 257, 4, 4, 128, True, 0, None), (100, 300, 2, 2, 20, True, 200, [300, 250, 1]),
+    (90, 60, 12, 4, 8, False, 0, [60, 33, 0]), (600, 600, 14, 2, 64, True, 0, [600, 599, 257])])
 def test_prompt(dtype, L, S, Hq, Hkv, D, causal, q_offset, lengths):
+    if D == 20 and dtype != torch.float32:
+        D = 24  # rows of 16-bit elements are a multiple of 8
     rng = np.random.default_rng(L * 100 + S)
     _check_weights(rng, 3, Hq, Hkv, L, S, D, dtype, lengths=lengths, causal=causal, q_offset=q_offset)
 
