@@ -16,8 +16,12 @@
 // bf16, so three MFMAs give the fp32 product.
 //
 // All (kv head, sequence, 32-token unit) triples are laid end to end by a prefix sum of the lengths and cut in equal
-// shares, one per wave.  What a share cuts (its first and its last sequence) goes to a record per head, which
-// decode_fp8_merge_kernel merges by LSE; sequences inside one share are written directly.
+// shares, one per workgroup, whose four waves take its units in turn and meet in LDS where a sequence ends.  What a share cuts (its
+// first and its last sequence) goes to a record per head, which decode_fp8_merge_kernel merges by LSE; sequences inside
+// one share are written directly.  The keys of the next unit are loaded when this one's scores are done, its values when P V
+// is.  Waves that stream shares of their own (four times the streams and records) take 14.3 us where this takes 12.8 (1x4000),
+// and 106 where this takes 104 (64 of 512 to 8192); more waves per CU only slow the memory down (16: 234 instead of 150 us for
+// 16 of 20000 to 32768).
 #include <algorithm>
 #include <cmath>
 
@@ -45,35 +49,44 @@ struct Decode8Params {
     int64_t o_b, o_h, lse_b, bt_s;
     int32_t B, Hq, Hkv, group, nsub;  // nsub: 16-head column sets of a kv head's query heads
     int32_t capacity, page_shift, num_pages, block_shift;
-    int32_t d, shares;
+    int32_t d, shares;  // shares: at most so many
     float c;  // scale * log2(e)
     uint32_t q_and, q_xor;
 };
 
 namespace {
 
-constexpr int kUnit8 = 32;  // tokens per step: two tiles of 16
+constexpr int kTiles8 = 2;             // tiles of 16 tokens per step of a wave
+constexpr int kUnit8 = 16 * kTiles8;
+constexpr int kWaves8 = 4;             // waves of a workgroup, which take the units of its share in turn
+// Shares per CU, and units that a share has at least.  us, 1x4000 / 64 sequences of 512 to 8192 in 16-token pages / 16 of
+// 20000 to 32768 (8 kv heads of 128): one share per CU 14.4 / 128 / 165, two 12.8 / 104 / 144, three 14.6 / 103 / 147; two units
+// at least 15.6 / 104 / 144, eight 15.8 / 105 / 144.
+constexpr int kSharesPerCu = 2;
+constexpr int kShareLeast = kWaves8;
 
-__device__ __forceinline__ int units8(const Decode8Params& p, int64_t b) {
-    return (min(max(p.lengths[b], 0), p.capacity) + kUnit8 - 1) / kUnit8;
+__device__ __forceinline__ int tokens8(const Decode8Params& p, int64_t b) { return min(max(p.lengths[b], 0), p.capacity); }
+__device__ __forceinline__ int units8(const Decode8Params& p, int64_t b) { return (tokens8(p, b) + kUnit8 - 1) / kUnit8; }
+
+// Inclusive prefix sum over the wave's lanes, by DPP: within rows of 16, then the last lanes of rows to those behind.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
 }
-
-// Inclusive prefix sum over the wave's lanes.
 __device__ __forceinline__ int scan64(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
-    return v;
+    v = dpp_add<0x111, 0xf>(v);  // row_shr:1
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    return dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
 
 // V units in `n` shares of V / n or one more (all the longer ones first); the host keeps V below 2^31.
 struct Shares8 {
     int n, q, rem;
     __device__ __forceinline__ Shares8(int V, int most) {
-        n = min(most, max(1, V));
+        n = min(most, max(1, V / kShareLeast));
         q = V / n;
         rem = V - q * n;
     }
@@ -117,52 +130,79 @@ __device__ __forceinline__ void operands(const float* x, typename Elem<typename 
 __device__ __forceinline__ float colmax(float x) { return max_across_groups<16>(x); }
 __device__ __forceinline__ float colsum(float x) { return sum_across_groups<16>(x); }
 
-template <int D>
-struct Stage8 {
-    u32x4 k[2][D / 64];
-    uint32_t v[8][D / 64];
-    float ks[2], vs[2];
-};
+// Bits of 4 bytes of 8 tokens (two tiles' rows 4 g4 .. 4 g4 + 3) as operands of 4 dims: bytes paired by token, then two dims of
+// one pair per conversion.
+template <typename E>
+__device__ __forceinline__ void transpose4x8(const uint32_t (&v)[8], typename Elem<E>::vec8 (&out)[4]) {
+    uint32_t w[4][4];  // [dim][token pair]
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const uint32_t lo = __builtin_amdgcn_perm(v[2 * t + 1], v[2 * t], 0x05010400u);
+        const uint32_t hi = __builtin_amdgcn_perm(v[2 * t + 1], v[2 * t], 0x07030602u);
+        w[0][t] = codes_to_pair<E, false>(lo), w[1][t] = codes_to_pair<E, true>(lo);
+        w[2][t] = codes_to_pair<E, false>(hi), w[3][t] = codes_to_pair<E, true>(hi);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = __builtin_bit_cast(typename Elem<E>::vec8, u32x4{w[j][0], w[j][1], w[j][2], w[j][3]});
+}
 
 }  // namespace
 
-template <typename T, int D, bool PAGED>
-__global__ void __launch_bounds__(64, 2) decode_fp8_kernel(const Decode8Params p) {
+// PAGES: 0, a padded cache; 1, pages of a whole unit or more; 2, smaller pages.
+template <typename T, int D, int PAGES>
+__global__ void __launch_bounds__(64 * kWaves8, kSharesPerCu) decode_fp8_kernel(const Decode8Params p) {
     typedef typename Q8<T>::E E;
     typedef typename Elem<E>::vec8 V8;
+    constexpr int NT = kTiles8;
     constexpr int NP = Q8<T>::parts, DH = D / 64, DPL = D / 16;  // DPL: V bytes (dims) per lane and token
-    const int lane = threadIdx.x;
+    constexpr int NR = PAGES == 2 ? NT : 1;                      // buffer resources of a unit
+    constexpr int RP = D + 4;  // floats per row of red_o: rows 16 bytes apart in the banks
+    __shared__ __attribute__((aligned(16))) float red_o[kWaves8][16][RP];
+    __shared__ float red_m[kWaves8][16], red_l[kWaves8][16], red_e[kWaves8][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g4 = lane >> 4;
 
-    const int own0 = lane < p.B ? units8(p, lane) : 0;
+    // units of all sequences (the first 64 are kept: their prefix finds the share's start)
+    const int len0 = lane < p.B ? tokens8(p, lane) : 0;
+    const int own0 = (len0 + kUnit8 - 1) / kUnit8;
     const int pre0 = scan64(own0);
-    int U = __shfl(pre0, 63, 64);
-    for (int j0 = 64; j0 < p.B; j0 += 64) U += __shfl(scan64(j0 + lane < p.B ? units8(p, j0 + lane) : 0), 63, 64);
-    U = __builtin_amdgcn_readfirstlane(U);
+    int U = __builtin_amdgcn_readlane(pre0, 63);
+    for (int j0 = 64; j0 < p.B; j0 += 64) U += __builtin_amdgcn_readlane(scan64(j0 + lane < p.B ? units8(p, j0 + lane) : 0), 63);
     if (U == 0) return;
     const Shares8 sh(U * p.Hkv * p.nsub, p.shares);
     const int r = blockIdx.x;
     if (r >= sh.n) return;
-    const int u0 = sh.start(r), n = sh.start(r + 1) - u0;  // first unit and units of this wave
+    const int u0 = sh.start(r), n = sh.start(r + 1) - u0;  // first unit and units of this workgroup
 
-    struct At {
-        int slot, b, tok, L;  // slot: kv head * nsub + column set
-        bool first;           // the unit starts a segment
-        int page[2];          // PAGED: of its two tiles
-    };
     typedef const __attribute__((address_space(4))) int32_t cint32;
     typedef const __attribute__((address_space(4))) float cfloat;
     cint32* const lengths = (cint32*)p.lengths;
     cint32* const table = (cint32*)p.block_table;
-    cfloat* const kscale = (cfloat*)p.ks;
-    cfloat* const vscale = (cfloat*)p.vs;
     auto length = [&](int b) { return min(max(lengths[b], 0), p.capacity); };
+    // Where a unit lies (cur: of the workgroup's segment; nx: the next that this wave loads).  Lengths, page ids and scales are scalar loads, which leave the vector loads in flight alone.
+    struct At {
+        int slot, hk, b, tok, L;  // slot: kv head * nsub + column set
+        const uint8_t* k;         // PAGES 0: first rows
+        const uint8_t* v;
+        cfloat* ks;               // PAGES 0: scales of the head
+        cfloat* vs;
+        int page[NR];             // PAGES 1, 2
+    };
     // a tile past the sequence's end stands for its last token: no row of it is read
     auto tile_token = [&](const At& a, int tt) { return min(a.tok + 16 * tt, a.L - 1); };
+    auto enter = [&](At& a) {  // a segment
+        a.hk = p.nsub == 1 ? a.slot : a.slot / p.nsub;
+        if constexpr (PAGES == 0) {
+            a.k = p.k + a.b * p.k_b + a.hk * p.k_h + a.tok * p.k_s;
+            a.v = p.v + a.b * p.v_b + a.hk * p.v_h + a.tok * p.v_s;
+            a.ks = (cfloat*)p.ks + a.b * p.ks_b + a.hk * p.ks_h;
+            a.vs = (cfloat*)p.vs + a.b * p.vs_b + a.hk * p.vs_h;
+        }
+    };
     auto pages = [&](At& a) {
-        if constexpr (PAGED) {
+        if constexpr (PAGES != 0) {
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt) a.page[tt] = table[a.b * p.bt_s + (tile_token(a, tt) >> p.page_shift)];
+            for (int i = 0; i < NR; ++i) a.page[i] = table[a.b * p.bt_s + (tile_token(a, i) >> p.page_shift)];
         }
     };
     At at;
@@ -170,247 +210,300 @@ __global__ void __launch_bounds__(64, 2) decode_fp8_kernel(const Decode8Params p
     int x = u0 - at.slot * U;
     at.b = 0;
     for (int j0 = 0;; j0 += 64) {
-        const int own = j0 == 0 ? own0 : j0 + lane < p.B ? units8(p, j0 + lane) : 0;
+        const int len = j0 == 0 ? len0 : j0 + lane < p.B ? tokens8(p, j0 + lane) : 0;
+        const int own = (len + kUnit8 - 1) / kUnit8;
         const int s = j0 == 0 ? pre0 : scan64(own);
         const uint64_t hit = __ballot(s > x);  // sequences ending past x
         if (hit != 0) {
             const int l = __builtin_ctzll(hit);
-            at.b = __builtin_amdgcn_readfirstlane(j0 + l);
-            x -= __builtin_amdgcn_readfirstlane(__shfl(s - own, l, 64));
+            at.b = j0 + l;
+            at.L = __builtin_amdgcn_readlane(len, l);
+            x -= __builtin_amdgcn_readlane(s - own, l);
             break;
         }
-        x -= __builtin_amdgcn_readfirstlane(__shfl(s, 63, 64));
+        x -= __builtin_amdgcn_readlane(s, 63);
     }
     at.tok = x * kUnit8;
-    at.L = length(at.b);
-    at.first = true;
-    pages(at);
-    auto next = [&](At a) {
-        a.tok += kUnit8;
-        a.first = false;
-        if (a.tok >= a.L) {
-            a.tok = 0;
-            a.first = true;
-            do {  // a unit follows, so a sequence with tokens does
-                if (++a.b == p.B) a.b = 0, ++a.slot;
-                a.L = length(a.b);
-            } while (a.L == 0);
+    auto advance = [&](At& a, int units) {
+        a.tok += units * kUnit8;
+        if (a.tok < a.L) {
+            if constexpr (PAGES == 0) {
+                a.k += units * kUnit8 * p.k_s;
+                a.v += units * kUnit8 * p.v_s;
+            }
+            return;
         }
-        pages(a);
-        return a;
+        do {  // a unit follows, so a sequence with tokens does
+            a.tok -= (a.L + kUnit8 - 1) & -kUnit8;
+            if (++a.b == p.B) a.b = 0, ++a.slot;
+            a.L = length(a.b);
+        } while (a.tok >= a.L);
+        enter(a);
     };
 
-    // byte offsets of this lane's loads in a tile of 16 rows; chunks past the real head dim lie past any tile
+    // byte offsets of this lane's loads from a unit's (PAGES 2: a tile's) first row; chunks past the real head dim lie past any
     const uint32_t kp = (uint32_t)p.k_s, vp = (uint32_t)p.v_s;
-    uint32_t koff[DH];
+    uint32_t koff[DH], voff[4];
 #pragma unroll
-    for (int h = 0; h < DH; ++h) koff[h] = 64 * h + 16 * g4 < p.d ? (uint32_t)col * kp + (uint32_t)(64 * h + 16 * g4) : 0xfffffff0u;
-    uint32_t voff[4];
+    for (int h = 0; h < DH; ++h) koff[h] = 64 * h + 16 * g4 < p.d ? (uint32_t)col * kp + (uint32_t)(64 * h + 16 * g4) : 0xc0000000u;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) voff[e] = DPL * col < p.d ? (uint32_t)(4 * g4 + e) * vp + (uint32_t)(DPL * col) : 0xfffffff0u;
+    for (int e = 0; e < 4; ++e) voff[e] = DPL * col < p.d ? (uint32_t)(4 * g4 + e) * vp + (uint32_t)(DPL * col) : 0xc0000000u;
 
-    auto load = [&](Stage8<D>& st, const At& a) {
-        const int hk = a.slot / p.nsub;
+    u32x4 kr[NT][DH];
+    uint32_t vr[NT / 2][DH][8];  // by pairs of tiles
+    float ks[NT], vs[NT];
+    // rows of a resource that hold tokens: of the unit, or of tile i
+    auto rows_of = [&](const At& a, int i) { return min(max(a.L - a.tok - (NR > 1 ? 16 * i : 0), 0), NR > 1 ? 16 : kUnit8); };
+    auto slot_of = [&](const At& a, int i) { return (int64_t)min(max(a.page[i], 0), p.num_pages - 1); };
+    auto row_of = [&](const At& a, int i) { return (tile_token(a, i) & ((1 << p.page_shift) - 1)) & ~15; };
+    auto load_k = [&](const At& a) {
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            const int tok = tile_token(a, tt), rows = min(max(a.L - a.tok - 16 * tt, 0), 16);
-            int64_t slot = a.b;
-            int row = tok;
-            if constexpr (PAGED) {
-                slot = min(max(a.page[tt], 0), p.num_pages - 1);
-                row = tok & ((1 << p.page_shift) - 1);
-            }
-            const int blk = row >> p.block_shift;
-            row &= ~15;  // the tile's first row (tiles past the end read nothing)
-            const auto krs = make_rsrc(p.k + slot * p.k_b + hk * p.k_h + row * p.k_s, rows > 0 ? (uint32_t)(rows - 1) * kp + (uint32_t)p.d : 0u);
-            const auto vrs = make_rsrc(p.v + slot * p.v_b + hk * p.v_h + row * p.v_s, rows > 0 ? (uint32_t)(rows - 1) * vp + (uint32_t)p.d : 0u);
+        for (int i = 0; i < NR; ++i) {
+            const int rows = rows_of(a, i);
+            const uint8_t* base;
+            if constexpr (PAGES == 0) base = a.k;
+            else base = p.k + slot_of(a, i) * p.k_b + a.hk * p.k_h + row_of(a, i) * p.k_s;
+            const auto rs = make_rsrc(base, rows > 0 ? (uint32_t)(rows - 1) * kp + (uint32_t)p.d : 0u);
 #pragma unroll
-            for (int h = 0; h < DH; ++h) st.k[tt][h] = buf_ld16_nt(krs, koff[h]);
+            for (int tt = NR > 1 ? i : 0; tt < (NR > 1 ? i + 1 : NT); ++tt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if constexpr (D == 128) {
-                    const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vrs, voff[e], 0, 2));
-                    st.v[4 * tt + e][0] = w.x, st.v[4 * tt + e][DH - 1] = w.y;
-                } else {
-                    st.v[4 * tt + e][0] = __builtin_amdgcn_raw_buffer_load_b32(vrs, voff[e], 0, 2);
+                for (int h = 0; h < DH; ++h) kr[tt][h] = buf_ld16_nt(rs, koff[h] + (NR > 1 ? 0u : 16u * tt * kp));
+        }
+    };
+    auto load_v = [&](const At& a) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int rows = rows_of(a, i);
+            const uint8_t* base;
+            if constexpr (PAGES == 0) base = a.v;
+            else base = p.v + slot_of(a, i) * p.v_b + a.hk * p.v_h + row_of(a, i) * p.v_s;
+            const auto rs = make_rsrc(base, rows > 0 ? (uint32_t)(rows - 1) * vp + (uint32_t)p.d : 0u);
+#pragma unroll
+            for (int tt = NR > 1 ? i : 0; tt < (NR > 1 ? i + 1 : NT); ++tt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t off = voff[e] + (NR > 1 ? 0u : 16u * tt * vp);
+                    if constexpr (D == 128) {
+                        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 2));
+                        vr[tt / 2][0][4 * (tt & 1) + e] = w.x, vr[tt / 2][DH - 1][4 * (tt & 1) + e] = w.y;
+                    } else {
+                        vr[tt / 2][0][4 * (tt & 1) + e] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 2);
+                    }
                 }
+        }
+    };
+    auto load_scales = [&](const At& a) {
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+            if constexpr (PAGES == 0) {
+                const int blk = tile_token(a, tt) >> p.block_shift;
+                ks[tt] = a.ks[blk];
+                vs[tt] = a.vs[blk];
+            } else {
+                const int64_t slot = slot_of(a, NR > 1 ? tt : 0);
+                const int blk = (tile_token(a, tt) & ((1 << p.page_shift) - 1)) >> p.block_shift;
+                ks[tt] = ((cfloat*)p.ks)[slot * p.ks_b + a.hk * p.ks_h + blk];
+                vs[tt] = ((cfloat*)p.vs)[slot * p.vs_b + a.hk * p.vs_h + blk];
             }
-            st.ks[tt] = kscale[slot * p.ks_b + hk * p.ks_h + blk];
-            st.vs[tt] = vscale[slot * p.vs_b + hk * p.vs_h + blk];
         }
     };
 
-    float ML = kNegInf, l = 0.f;            // running max of the scores, and the row sum on that base
-    float ER = kNegInf, eb = kNegInf;       // running max of score + log2(v scale), and the accumulators' base
+    float ML = kNegInf, l = 0.f;       // running max of the scores, and the row sum on that base
+    float ER = kNegInf, eb = kNegInf;  // running max of score + log2(v scale), and the accumulators' base
     f32x4 acc[DPL];
     V8 qf[NP][2 * DH];
-    int start = 0;          // the segment's first token
-    bool cut_first = true;  // the segment is the share's first
-
-    auto compute = [&](const Stage8<D>& st, const At& cur, int s) {
-        const int hk = cur.slot / p.nsub, sub = cur.slot - hk * p.nsub;
-        const int heads = min(p.group - 16 * sub, 16);
-        const int hq = hk * p.group + 16 * sub + col;  // this lane's query head, where col < heads
-        if (cur.first || s == 0) {
-            const T* qp = reinterpret_cast<const T*>(p.q) + cur.b * p.q_b + (hk * p.group + 16 * sub + min(col, heads - 1)) * p.q_h;
+    At cur = at, nx = at;
+    cur.hk = p.nsub == 1 ? cur.slot : cur.slot / p.nsub;
+    if (wave < n) {
+        enter(nx);
+        if (wave > 0) advance(nx, wave);
+        pages(nx);
+        load_k(nx);
+        load_v(nx);
+        load_scales(nx);
+    }
+    int s = wave;  // this wave's next unit of the share
+    for (int u = 0; u < n;) {
+      const int m = min((cur.L - cur.tok + kUnit8 - 1) / kUnit8, n - u);  // units of the segment
+      const int hk = cur.hk, b = cur.b, sub = cur.slot - hk * p.nsub;
+      const int heads = min(p.group - 16 * sub, 16);
+      ML = ER = eb = kNegInf;
+      l = 0.f;
 #pragma unroll
-            for (int k = 0; k < 2 * DH; ++k) {
-                const int dim = 64 * (k >> 1) + 16 * g4 + 8 * (k & 1);
-                Chunk<T> w = load_chunk<T, false>(qp + (dim < p.d ? dim : 0));
-                float f[8];
+      for (int j = 0; j < DPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (s < u + m) {
+        const T* qp = reinterpret_cast<const T*>(p.q) + b * p.q_b + (hk * p.group + 16 * sub + min(col, heads - 1)) * p.q_h;
 #pragma unroll
-                for (int i = 0; i < (int)(sizeof(w.v) / sizeof(w.v[0])); ++i) w.v[i] = dim < p.d ? q_bits(w.v[i], p.q_and, p.q_xor) : u32x4{0u, 0u, 0u, 0u};
-                if constexpr (NP == 1) {
-                    qf[0][k] = __builtin_bit_cast(V8, w.v[0]);
-                } else {
-                    unpack_chunk<T>(w, f);
-                    V8 t[NP];
-                    operands<T>(f, t);
+        for (int k = 0; k < 2 * DH; ++k) {
+            const int dim = 64 * (k >> 1) + 16 * g4 + 8 * (k & 1);
+            Chunk<T> w = load_chunk<T, false>(qp + (dim < p.d ? dim : 0));
+            float f[8];
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) qf[i][k] = t[i];
-                }
+            for (int i = 0; i < (int)(sizeof(w.v) / sizeof(w.v[0])); ++i) w.v[i] = dim < p.d ? q_bits(w.v[i], p.q_and, p.q_xor) : u32x4{0u, 0u, 0u, 0u};
+            if constexpr (NP == 1) {
+                qf[0][k] = __builtin_bit_cast(V8, w.v[0]);
+            } else {
+                unpack_chunk<T>(w, f);
+                V8 t[NP];
+                operands<T>(f, t);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) qf[i][k] = t[i];
             }
-            ML = ER = eb = kNegInf;
-            l = 0.f;
-#pragma unroll
-            for (int j = 0; j < DPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            start = cur.tok;
-            cut_first = s == 0;
         }
-        const int left = cur.L - cur.tok;
-        f32x4 sc[2];
-        float lv[2], tm[2];
+      }
+      for (; s < u + m; s += kWaves8) {
+        const int left = cur.L - cur.tok - (s - u) * kUnit8;
+        const bool more = s + kWaves8 < n;
+        if (more) {
+            advance(nx, kWaves8);
+            pages(nx);
+        }
+        f32x4 sc[NT];
+        float tm[NT], lv[NT];
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
+        for (int tt = 0; tt < NT; ++tt) {
             f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < 2 * DH; ++k) {
-                const u32x4 w = st.k[tt][k >> 1];
+                const u32x4 w = kr[tt][k >> 1];
                 const V8 kf = k & 1 ? codes_to_vec8<E>(w.z, w.w) : codes_to_vec8<E>(w.x, w.y);
 #pragma unroll
                 for (int i = 0; i < NP; ++i) a = mfma16(kf, qf[i][k], a);
             }
-            const float c = p.c * st.ks[tt];
-            lv[tt] = __log2f(st.vs[tt]);
-            tm[tt] = kNegInf;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sc[tt][i] = 16 * tt + 4 * g4 + i < left ? a[i] * c : kNegInf;
-                tm[tt] = fmaxf(tm[tt], sc[tt][i]);
-            }
-            tm[tt] = colmax(tm[tt]);
+            sc[tt] = a * (p.c * ks[tt]);
+            lv[tt] = __log2f(vs[tt]);
         }
+        if (more) load_k(nx);  // the keys are used up
+        if (left < kUnit8) {
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (16 * tt + 4 * g4 + i >= left) sc[tt][i] = kNegInf;
+        }
+        if (more) load_scales(nx);
         // The row sum is on the running max of the scores.  P is on a base of its own, E, where the exponents of a tile's
         // scores and of its V scale add up, so the product of P and codes needs no scaling.  E is the unit's own largest
         // value, so that the largest P is a power of two and rounds exactly, but at most 2^24 below the running one, which
         // keeps alpha and the accumulators finite.  That power is 1, and in fp16 2^15: its subnormals then begin 2^-29
         // below the largest P and not 2^-14, and a small P next to it keeps its precision.
-        const float Mn = fmaxf(ML, fmaxf(tm[0], tm[1]));
+        float Mn = ML, e0 = kNegInf;
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+            tm[tt] = fmaxf(fmaxf(sc[tt][0], sc[tt][1]), fmaxf(sc[tt][2], sc[tt][3]));
+            Mn = fmaxf(Mn, tm[tt]);
+            e0 = fmaxf(e0, tm[tt] + lv[tt]);
+        }
+        Mn = colmax(Mn);
+        e0 = colmax(e0);
         const float Mb = Mn == kNegInf ? 0.f : Mn;
-        const float e0 = fmaxf(tm[0] + lv[0], tm[1] + lv[1]);
         ER = fmaxf(ER, e0);
         const float en = fmaxf(e0, ER - 24.f) - (__is_same(E, f16_t) ? 15.f : 0.f);
         const float base = en == kNegInf ? 0.f : en;
         const float alpha = fast_exp2(eb - base);
         eb = en;
         float us = 0.f;
-        float pf[8];
+        V8 pk[NT / 2][NP];
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            const float pb = base - lv[tt];
+        for (int tp = 0; tp < NT / 2; ++tp) {
+            float pf[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                us += fast_exp2(sc[tt][i] - Mb);
-                pf[4 * tt + i] = fast_exp2(sc[tt][i] - pb);
+            for (int i = 0; i < 8; ++i) {
+                const int tt = 2 * tp + (i >> 2);
+                us += fast_exp2(sc[tt][i & 3] - Mb);
+                pf[i] = fast_exp2(sc[tt][i & 3] - (base - lv[tt]));
             }
+            operands<T>(pf, pk[tp]);
         }
         l = __builtin_fmaf(l, fast_exp2(ML - Mb), us);
         ML = Mn;
-        V8 pk[NP];
-        operands<T>(pf, pk);
 #pragma unroll
-        for (int h = 0; h < DH; ++h) {
-            // four dims of eight tokens: bytes paired by token, then two dims of one pair per conversion
-            uint32_t w[4][4];  // [dim][token pair]
+        for (int j = 0; j < DPL; ++j) acc[j] *= alpha;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const uint32_t lo = __builtin_amdgcn_perm(st.v[2 * t + 1][h], st.v[2 * t][h], 0x05010400u);
-                const uint32_t hi = __builtin_amdgcn_perm(st.v[2 * t + 1][h], st.v[2 * t][h], 0x07030602u);
-                w[0][t] = codes_to_pair<E, false>(lo), w[1][t] = codes_to_pair<E, true>(lo);
-                w[2][t] = codes_to_pair<E, false>(hi), w[3][t] = codes_to_pair<E, true>(hi);
+        for (int tp = 0; tp < NT / 2; ++tp)
+#pragma unroll
+            for (int h = 0; h < DH; ++h) {
+                V8 vf[4];
+                transpose4x8<E>(vr[tp][h], vf);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) acc[4 * h + j] = mfma16(vf[j], pk[tp][i], acc[4 * h + j]);
             }
+        if (more) load_v(nx);
+      }
+      // the waves meet: each leaves its accumulators and their bases
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const V8 vf = __builtin_bit_cast(V8, u32x4{w[j][0], w[j][1], w[j][2], w[j][3]});
-                f32x4 a = acc[4 * h + j] * alpha;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int i = 0; i < NP; ++i) a = mfma16(vf, pk[i], a);
-                acc[4 * h + j] = a;
+        for (int j = 0; j < DPL; j += 4)
+            *reinterpret_cast<f32x4*>(&red_o[wave][col][DPL * (4 * g4 + i) + j]) = f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+      const float lw = colsum(l);
+      if (g4 == 0) red_m[wave][col] = ML, red_l[wave][col] = lw, red_e[wave][col] = eb;
+      lds_barrier();
+      const int g = tid >> 4;  // a head, and DPL of its dims
+      if (g < heads) {
+        float M = kNegInf, X = kNegInf;
+#pragma unroll
+        for (int w = 0; w < kWaves8; ++w) M = fmaxf(M, red_m[w][g]), X = fmaxf(X, red_e[w][g]);
+        float lt = 0.f, o[DPL] = {};
+#pragma unroll
+        for (int w = 0; w < kWaves8; ++w) {
+            const float mw = red_m[w][g], ew = red_e[w][g];
+            lt += (mw == kNegInf ? 0.f : fast_exp2(mw - M)) * red_l[w][g];
+            const float f = ew == kNegInf ? 0.f : fast_exp2(ew - X);
+#pragma unroll
+            for (int j = 0; j < DPL; j += 4) {
+                const f32x4 a = *reinterpret_cast<const f32x4*>(&red_o[w][g][DPL * (tid & 15) + j]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[j + i] = __builtin_fmaf(a[i], f, o[j + i]);
             }
         }
-        const bool ends = left <= kUnit8;  // the sequence's last unit
-        if (ends || s + 1 == n) {
-            const float lt = colsum(l);
-            if (col < heads) {
-                const float lse = __builtin_fmaf(ML, kLn2, __log2f(lt) * kLn2);
-                const bool whole = ends && start == 0;
-                // every score -inf: a record of O = 0 at the LSE of -inf, which drops it in the merge; the output itself is 0 / 0
-                const float f = lt == 0.f && !whole ? 0.f : fast_exp2(eb - ML) / lt;
-                const int rec = 2 * r + (cut_first ? 0 : 1);
+        const int hq = hk * p.group + 16 * sub + g, dim = DPL * (tid & 15);
+        const float lse = __builtin_fmaf(M, kLn2, __log2f(lt) * kLn2);
+        const bool whole = cur.tok == 0 && u + m <= n && m * kUnit8 >= cur.L;
+        // every score -inf: a record of O = 0 at the LSE of -inf, which drops it in the merge; the output itself is 0 / 0
+        const float f = lt == 0.f && !whole ? 0.f : fast_exp2(X - M) / lt;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int dim = DPL * (4 * g4 + i);
-                    float o[DPL];
+        for (int j = 0; j < DPL; ++j) o[j] *= f;
+        if (whole) {
+            T* op = reinterpret_cast<T*>(p.o) + b * p.o_b + hq * p.o_h + dim;
+            if (dim < p.d) {
 #pragma unroll
-                    for (int j = 0; j < DPL; ++j) o[j] = acc[j][i] * f;
-                    if (whole) {
-                        T* op = reinterpret_cast<T*>(p.o) + cur.b * p.o_b + hq * p.o_h + dim;
-                        if (dim < p.d) {
-#pragma unroll
-                            for (int j = 0; j < DPL; j += 4) {
-                                if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
-                                else *reinterpret_cast<u32x2*>(op + j) = u32x2{pack2<T>(o[j], o[j + 1]), pack2<T>(o[j + 2], o[j + 3])};
-                            }
-                        }
-                    } else {
-                        float* op = p.part_o + ((int64_t)rec * 16 + col) * D + dim;
-#pragma unroll
-                        for (int j = 0; j < DPL; j += 4) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
-                    }
+                for (int j = 0; j < DPL; j += 4) {
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
+                    else *reinterpret_cast<u32x2*>(op + j) = u32x2{pack2<T>(o[j], o[j + 1]), pack2<T>(o[j + 2], o[j + 3])};
                 }
-                if (g4 == 0) {
-                    if (!whole) p.part_lse[rec * 16 + col] = lse;
-                    else if (p.lse != nullptr) p.lse[cur.b * p.lse_b + hq] = lse;
-                }
             }
+            if (p.lse != nullptr && (tid & 15) == 0) p.lse[b * p.lse_b + hq] = lse;
+        } else {
+            const int rec = 2 * r + (u == 0 ? 0 : 1);
+            float* op = p.part_o + ((int64_t)rec * 16 + g) * D + dim;
+#pragma unroll
+            for (int j = 0; j < DPL; j += 4) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
+            if ((tid & 15) == 0) p.part_lse[rec * 16 + g] = lse;
         }
-    };
-
-    // two stages in registers: while one is computed the other is in flight
-    Stage8<D> s0, s1;
-    At a0 = at, a1 = at;
-    load(s0, a0);
-    for (int s = 0; s < n; s += 2) {
-        if (s + 1 < n) {
-            a1 = next(a0);
-            load(s1, a1);
-        }
-        compute(s0, a0, s);
-        if (s + 1 >= n) break;
-        if (s + 2 < n) {
-            a0 = next(a1);
-            load(s0, a0);
-        }
-        compute(s1, a1, s + 1);
+      }
+      u += m;
+      if (u < n) {
+        lds_barrier();  // every wave has read the others' before they write again
+        cur.tok = 0;
+        do {  // a unit follows, so a sequence with tokens does
+            if (++cur.b == p.B) cur.b = 0, ++cur.slot;
+            cur.L = length(cur.b);
+        } while (cur.L == 0);
+        cur.hk = p.nsub == 1 ? cur.slot : cur.slot / p.nsub;
+      }
     }
 }
 
-// Merges the records of the shares that cut a sequence, one (b, query head) per wave.
-template <typename T, int D>
+// Merges the records of the shares that cut a sequence: one (b, query head) per W waves.
+template <typename T, int D, int W>
 __global__ void __launch_bounds__(256) decode_fp8_merge_kernel(const Decode8Params p) {
     constexpr int DL = D / 64;  // dims per lane
-    const int lane = threadIdx.x & 63;
-    const int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ float red[W > 1 ? W : 1][D];
+    const int lane = threadIdx.x & 63, wave = W > 1 ? threadIdx.x >> 6 : 0;
+    const int64_t pair = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (pair >= (int64_t)p.B * p.Hq) return;
     const int b = (int)(pair / p.Hq), hq = (int)(pair % p.Hq), hk = hq / p.group, g = hq - hk * p.group;
     int U = 0, before = 0, own = 0;
@@ -421,10 +514,11 @@ __global__ void __launch_bounds__(256) decode_fp8_merge_kernel(const Decode8Para
             own = __shfl(u, b - j0, 64);
             before = U + __shfl(s, b - j0, 64) - own;
         }
-        U += __shfl(s, 63, 64);
+        U += __builtin_amdgcn_readlane(s, 63);
     }
     T* op = reinterpret_cast<T*>(p.o) + b * p.o_b + hq * p.o_h;
     if (own == 0) {  // empty sequence: O = 0, LSE = -inf
+        if (wave > 0) return;
 #pragma unroll
         for (int e = 0; e < DL; ++e)
             if (DL * lane + e < p.d) op[DL * lane + e] = Elem<T>::from_f32(0.f);
@@ -447,21 +541,31 @@ __global__ void __launch_bounds__(256) decode_fp8_merge_kernel(const Decode8Para
     const float inv = 1.f / sum;
     float acc[DL] = {};
     constexpr int MB = 8;  // records in flight
-    for (int j0 = 0; j0 < ns; j0 += MB) {
+    for (int j0 = wave; j0 < ns; j0 += W * MB) {
         float lw[MB], v[MB][DL];
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
-            const int64_t q = rec(min(j0 + j, ns - 1));
+            const int64_t q = rec(min(j0 + W * j, ns - 1));
             lw[j] = p.part_lse[q];
 #pragma unroll
             for (int e = 0; e < DL; ++e) v[j][e] = p.part_o[q * D + DL * lane + e];
         }
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
-            const float w = j0 + j < ns ? __expf(lw[j] - mx) * inv : 0.f;
+            const float w = j0 + W * j < ns ? __expf(lw[j] - mx) * inv : 0.f;
 #pragma unroll
             for (int e = 0; e < DL; ++e) acc[e] = __builtin_fmaf(w, v[j][e], acc[e]);
         }
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int e = 0; e < DL; ++e) red[wave][DL * lane + e] = acc[e];
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w)
+#pragma unroll
+            for (int e = 0; e < DL; ++e) acc[e] += red[w][DL * lane + e];
     }
 #pragma unroll
     for (int e = 0; e < DL; ++e)
@@ -476,13 +580,13 @@ struct Plan8 {
     size_t bytes;
 };
 
-// Shares: eight waves per CU, and no more than there can be units.
+// Shares: no more than there can be units for.
 Plan8 plan8(const dtattn_decode_fp8_args* a, int64_t capacity, int cus) {
     Plan8 r;
     r.kernel_d = a->D <= 64 ? 64 : 128;
     r.nsub = (int32_t)((a->Hq / a->Hkv + 15) / 16);
     const int64_t units = a->B * a->Hkv * r.nsub * ((capacity + kUnit8 - 1) / kUnit8);
-    r.shares = (int32_t)std::max<int64_t>(1, std::min<int64_t>(8 * (int64_t)cus, units));
+    r.shares = (int32_t)std::max<int64_t>(1, std::min<int64_t>(kSharesPerCu * (int64_t)cus, units / kShareLeast));
     const size_t records = (size_t)2 * r.shares * 16;
     r.bytes = (records * (r.kernel_d + 1) * sizeof(float) + 255) & ~(size_t)255;
     return r;
@@ -492,14 +596,16 @@ int64_t capacity_of(const dtattn_decode_fp8_args* a) { return a->block_table != 
 
 template <typename T, int D>
 int launch8(const Decode8Params& p, hipStream_t stream) {
-    if (p.block_table != nullptr)
-        hipLaunchKernelGGL((decode_fp8_kernel<T, D, true>), dim3((unsigned)p.shares), dim3(64), 0, stream, p);
-    else
-        hipLaunchKernelGGL((decode_fp8_kernel<T, D, false>), dim3((unsigned)p.shares), dim3(64), 0, stream, p);
+    const dim3 grid((unsigned)p.shares);
+    if (p.block_table == nullptr) hipLaunchKernelGGL((decode_fp8_kernel<T, D, 0>), grid, dim3(64 * kWaves8), 0, stream, p);
+    else if ((1 << p.page_shift) >= kUnit8) hipLaunchKernelGGL((decode_fp8_kernel<T, D, 1>), grid, dim3(64 * kWaves8), 0, stream, p);
+    else hipLaunchKernelGGL((decode_fp8_kernel<T, D, 2>), grid, dim3(64 * kWaves8), 0, stream, p);
     const int st = check_launch("decode_fp8_kernel");
     if (st != DTATTN_OK) return st;
     const int64_t pairs = (int64_t)p.B * p.Hq;
-    hipLaunchKernelGGL((decode_fp8_merge_kernel<T, D>), dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, stream, p);
+    // few pairs are cut into many records each
+    if (pairs <= 512) hipLaunchKernelGGL((decode_fp8_merge_kernel<T, D, 4>), dim3((unsigned)pairs), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((decode_fp8_merge_kernel<T, D, 1>), dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, stream, p);
     return check_launch("decode_fp8_merge_kernel");
 }
 
