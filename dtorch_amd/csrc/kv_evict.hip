@@ -3,13 +3,15 @@
 // No counterpart in the reference, which keeps no KV cache (python/dtorch/test/modules/llama.py:126-156).
 //
 // kv_evict_select_kernel: one workgroup per (sequence, kv head) finds the weight of the last block that stays by a radix
-// select over the blocks' weights (as unsigned numbers in their order, 8 bits a round), takes of the blocks at that
-// weight the first ones, and writes the list of blocks that stay, in order.
-// kv_evict_move_kernel: one workgroup per (sequence, kv head, K / V / weights and scales) moves rows to the front in
-// place.  Row i of the result comes from a row at or past i, so a tile of rows may be written as soon as the tile itself
-// has been read: what a write covers belongs to rows already read.
+// select over the blocks' weights (as unsigned numbers in their order; 11, 11 and 10 bits a round), takes of the blocks at that
+// weight the first ones, and writes the list of blocks that stay, in order.  Up to 16384 candidates are held in registers.
+// kv_evict_move_kernel: moves rows to the front in place.  Row i of the result comes from a row at or past i, so a tile
+// of rows may be written as soon as the tile itself has been read: what a write covers belongs to rows already read.  A workgroup
+// has the next tile's loads in flight while it writes one, and that tile's list entries before them.  Few heads share a row's chunks
+// among several workgroups, all on one XCD, whose L2 puts the lines together again.  Bound by HBM.
 #include <algorithm>
 
+#include "decode_params.hpp"
 #include "dtattn_common.hpp"
 
 namespace dtattn {
@@ -20,12 +22,13 @@ struct EvictParams {
     float* w;
     int32_t* lengths;
     int32_t* kept;
-    uint32_t* order;  // [B, Hkv, S_max / block]: candidates' weights in unsigned order
+    uint32_t* order;  // [B, Hkv, S_max / block]: candidates' weights in unsigned order (where registers do not hold them)
+    int2* plan;       // [B, Hkv]: tokens before, and after (equal: nothing moves)
     int64_t kv_b[2], kv_h[2], kv_s[2];  // bytes
     int64_t s_b[2], s_h[2], w_b, w_h;
     int32_t B, Hkv, S_max, keep, recent;  // keep and recent in blocks
     int32_t block_shift, scale_shift;     // tokens per block; scale blocks per block
-    int32_t chunks;                       // 16-byte chunks per row
+    int32_t chunks, width, groups;        // 16-byte chunks per row, of which a workgroup moves `width`, `groups` of them a row
     int32_t blocks_max;                   // ceil(S_max / block)
 };
 
@@ -73,8 +76,11 @@ __device__ __forceinline__ int tokens_of(const EvictParams& p, int64_t b) { retu
 
 }  // namespace
 
+// The candidates' weights: PER per thread in registers (candidate tid + kSelect * k), or PER = 0 in memory.
+template <int PER>
 __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictParams p) {
-    __shared__ int hist[256];
+    constexpr int BINS = 2048;
+    __shared__ int hist[BINS];
     __shared__ int waves[kSelect / 64];
     __shared__ int found[2];
     const int tid = threadIdx.x;
@@ -83,6 +89,8 @@ __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictPar
     const int n = tokens_of(p, b);
     const int blocks = (n + (1 << p.block_shift) - 1) >> p.block_shift;
     int32_t* kept = p.kept + bh * p.keep;
+    const int left = blocks <= p.keep ? n : ((p.keep - 1) << p.block_shift) + n - ((blocks - 1) << p.block_shift);
+    if (tid == 0) p.plan[bh] = make_int2(n, left);
     if (blocks <= p.keep) {
         for (int i = tid; i < p.keep; i += kSelect) kept[i] = i < blocks ? i : -1;
         return;
@@ -91,96 +99,151 @@ __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictPar
     int need = p.keep - p.recent;        // of which so many stay; fewer than cand
     uint32_t* order = p.order + bh * p.blocks_max;
     const float* w = p.w + b * p.w_b + h * p.w_h;
-    for (int i = tid; i < cand; i += kSelect) {
-        float m;
-        if (p.block_shift == 0) {
-            m = w[i];
-        } else {
-            double s = 0.;
-            const float* x = w + ((int64_t)i << p.block_shift);
-            for (int j = 0; j < (1 << p.block_shift); ++j) s += (double)x[j];
-            m = (float)s;
-        }
-        order[i] = ordered(m);
+    auto weight = [&](int i) {
+        if (p.block_shift == 0) return ordered(w[i]);
+        double s = 0.;
+        const float* x = w + ((int64_t)i << p.block_shift);
+        for (int j = 0; j < (1 << p.block_shift); ++j) s += (double)x[j];
+        return ordered((float)s);
+    };
+    uint32_t mine[PER > 0 ? PER : 1];
+    if constexpr (PER > 0) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) mine[k] = tid + k * kSelect < cand ? weight(tid + k * kSelect) : 0u;
+    } else {
+        for (int i = tid; i < cand; i += kSelect) order[i] = weight(i);
+        __syncthreads();
     }
-    __syncthreads();
-    // The need-th largest, 8 bits a round: `prefix` holds the bits found so far, and `need` how many stay of those that share them
+    // f(candidate, its weight) for this thread's candidates
+    auto each = [&](auto f) {
+        if constexpr (PER > 0) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (tid + k * kSelect < cand) f(tid + k * kSelect, mine[k]);
+        } else {
+            for (int i = tid; i < cand; i += kSelect) f(i, order[i]);
+        }
+    };
+    // The need-th largest, some bits a round: `prefix` holds the bits found so far, and `need` how many stay of those that share them
     uint32_t prefix = 0, mask = 0;
     if (need > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+        for (int round = 0; round < 3; ++round) {
+            const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bins = round < 2 ? 2048 : 1024;
+            for (int i = tid; i < BINS; i += kSelect) hist[i] = 0;
             __syncthreads();
-            for (int i = tid; i < cand; i += kSelect) {
-                const uint32_t u = order[i];
-                if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255u], 1);
-            }
+            each([&](int, uint32_t u) {
+                if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & (bins - 1)], 1);
+            });
             __syncthreads();
-            const int mine = tid < 256 ? hist[255 - tid] : 0;  // from the largest down
+            // two bins a thread, from the largest down
+            const int hi = hist[BINS - 1 - 2 * tid], lo = hist[BINS - 2 - 2 * tid];
             int total;
-            const int before = scan_all(mine, waves, total);
-            if (tid < 256 && before < need && before + mine >= need) {
-                found[0] = 255 - tid;
-                found[1] = need - before;
+            const int before = scan_all(hi + lo, waves, total);
+            if (before < need && before + hi + lo >= need) {
+                const bool upper = before + hi >= need;
+                found[0] = BINS - 1 - 2 * tid - (upper ? 0 : 1);
+                found[1] = need - before - (upper ? 0 : hi);
             }
             __syncthreads();
             prefix |= (uint32_t)found[0] << shift;
-            mask |= 255u << shift;
+            mask |= (uint32_t)(bins - 1) << shift;
             need = found[1];
             __syncthreads();
         }
     } else {
         prefix = 0xffffffffu;  // above every weight
     }
-    // those above stay, and the first `need` of those at it; a thread takes a run of candidates
-    const int run = (cand + kSelect - 1) / kSelect;
-    const int i0 = min(tid * run, cand), i1 = min(i0 + run, cand);
-    int above = 0, at = 0;
-    for (int i = i0; i < i1; ++i) {
-        above += order[i] > prefix;
-        at += order[i] == prefix;
-    }
-    int total;
-    const int at0 = scan_all(at, waves, total);
-    const int mine = above + min(max(need - at0, 0), at);
-    int out = scan_all(mine, waves, total);
-    int left = need - at0;
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t u = order[i];
-        const bool stays = u > prefix || (u == prefix && left-- > 0);
-        if (stays) kept[out++] = i;
+    // those above stay, and the first `need` of those at it: one row of kSelect candidates after another
+    int out = 0, seen = 0;  // kept, and met at the prefix, in the rows before
+    const int rows = (cand + kSelect - 1) / kSelect;
+    auto row = [&](int k, uint32_t u) {
+        const int i = tid + k * kSelect;
+        const bool above = i < cand && u > prefix, at = i < cand && u == prefix;
+        int total;
+        const int before = scan_all(((int)above << 16) + (int)at, waves, total);
+        const int at_before = seen + (before & 0xffff);
+        // of those before me in this row: all above, and those at it that stay
+        const int stay_at = min(max(need - seen, 0), before & 0xffff);
+        if (above || (at && at_before < need)) kept[out + (before >> 16) + stay_at] = i;
+        out += (total >> 16) + min(max(need - seen, 0), total & 0xffff);
+        seen += total & 0xffff;
+    };
+    if constexpr (PER > 0) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (k < rows) row(k, mine[k]);
+    } else {
+        for (int k = 0; k < rows; ++k) row(k, tid + k * kSelect < cand ? order[tid + k * kSelect] : 0u);
     }
     for (int i = tid; i < p.recent; i += kSelect) kept[p.keep - p.recent + i] = cand + i;
 }
 
+// A workgroup per (sequence, kv head, K or V, group of chunks), eight of them in a row on different XCDs; blockIdx.y = 1: the
+// weights and scales of a (sequence, kv head).
 __global__ void __launch_bounds__(1024) kv_evict_move_kernel(const EvictParams p) {
     const int tid = threadIdx.x;
-    const int64_t bh = blockIdx.x, b = bh / p.Hkv;
-    const int h = (int)(bh % p.Hkv), what = blockIdx.y;
-    const int n = tokens_of(p, b);
-    const int blocks = (n + (1 << p.block_shift) - 1) >> p.block_shift;
-    if (blocks <= p.keep) return;
+    const int64_t heads = (int64_t)p.B * p.Hkv;
+    int64_t item = blockIdx.x;
+    int group = 0;
+    if (blockIdx.y == 0) {
+        const int64_t lot = item / (8 * p.groups);  // eight items' groups
+        group = (int)(item / 8 % p.groups);
+        item = lot * 8 + item % 8;
+        if (item >= 2 * heads) return;
+    } else if (item >= heads) {
+        return;
+    }
+    const int what = blockIdx.y == 0 ? (int)(item & 1) : 2;
+    const int64_t bh = blockIdx.y == 0 ? item >> 1 : item, b = bh / p.Hkv;
+    const int h = (int)(bh % p.Hkv);
+    const int2 plan = p.plan[bh];
+    const int n = plan.x, left = plan.y;
+    if (what == 2 && h == 0 && tid == 0 && left < n) p.lengths[b] = left;
+    if (left == n) return;
     const int32_t* kept = p.kept + bh * p.keep;
-    const int left = ((p.keep - 1) << p.block_shift) + n - ((blocks - 1) << p.block_shift);  // tokens that stay
     const int inner = (1 << p.block_shift) - 1;
     auto source = [&](int row) { return (kept[row >> p.block_shift] << p.block_shift) + (row & inner); };
     if (what < 2) {
-        constexpr int PER = 4;  // chunks per thread and tile
-        char* base = p.kv[what] + b * p.kv_b[what] + h * p.kv_h[what];
+        constexpr int PER = 4;  // rows per thread and tile
         const int64_t pitch = p.kv_s[what];
-        const int64_t cells = (int64_t)left * p.chunks;
-        for (int64_t c0 = 0; c0 < cells; c0 += 1024 * PER) {
-            u32x4 v[PER];
+        const int c = tid % p.width, step = 1024 / p.width;  // this thread's chunk, and rows that the threads cover at once
+        const int chunk = group * p.width + c;
+        const bool works = tid < step * p.width && chunk < p.chunks;
+        char* base = p.kv[what] + b * p.kv_b[what] + h * p.kv_h[what] + chunk * 16;
+        const int first = works ? tid / p.width : left;  // row of the first pass
+        const int tile = PER * step;
+        u32x4 v[2][PER];
+        int src[PER];
+        auto look = [&](int r0) {  // where the rows of the tile at r0 come from
+#pragma unroll
+            for (int k = 0; k < PER; ++k) src[k] = source(min(first + r0 + k * step, left - 1));
+        };
+        auto load = [&](u32x4* x) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (works) x[k] = ld16_nt(base + src[k] * pitch);
+        };
+        auto store = [&](u32x4* x, int r0) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k) asm volatile("" : "+v"(x[k]));  // the tile has been read
+            lds_barrier();                                              // by every wave
 #pragma unroll
             for (int k = 0; k < PER; ++k) {
-                const int64_t c = c0 + k * 1024 + tid;
-                if (c < cells) v[k] = ld16(base + source((int)(c / p.chunks)) * pitch + (c % p.chunks) * 16);
+                const int r = first + r0 + k * step;
+                if (r < left) st16(base + r * pitch, x[k]);
             }
-            read_all();
-#pragma unroll
-            for (int k = 0; k < PER; ++k) {
-                const int64_t c = c0 + k * 1024 + tid;
-                if (c < cells) st16(base + (c / p.chunks) * pitch + (c % p.chunks) * 16, v[k]);
-            }
+        };
+        look(0);
+        load(v[0]);
+        look(tile);
+        for (int r0 = 0; r0 < left; r0 += 2 * tile) {
+            if (r0 + tile < left) load(v[1]);
+            look(r0 + 2 * tile);
+            store(v[0], r0);
+            if (r0 + tile >= left) break;
+            if (r0 + 2 * tile < left) load(v[0]);
+            look(r0 + 3 * tile);
+            store(v[1], r0 + tile);
         }
         return;
     }
@@ -211,17 +274,19 @@ __global__ void __launch_bounds__(1024) kv_evict_move_kernel(const EvictParams p
     }
 }
 
-__global__ void __launch_bounds__(256) kv_evict_lengths_kernel(const EvictParams p) {
-    const int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (b >= p.B) return;
-    const int n = tokens_of(p, b);
-    const int blocks = (n + (1 << p.block_shift) - 1) >> p.block_shift;
-    if (blocks > p.keep) p.lengths[b] = ((p.keep - 1) << p.block_shift) + n - ((blocks - 1) << p.block_shift);
-}
+struct EvictSpace {
+    size_t plan, order;  // bytes
+};
 
-static size_t evict_workspace(const dtattn_kv_evict_args* a) {
+constexpr int kHeldRows = 16;  // candidates a thread holds
+
+static EvictSpace evict_workspace(const dtattn_kv_evict_args* a) {
     const int64_t blocks = (a->S_max + a->block - 1) / a->block;
-    return ((size_t)a->B * a->Hkv * blocks * sizeof(uint32_t) + 255) & ~(size_t)255;
+    const size_t heads = (size_t)a->B * a->Hkv;
+    EvictSpace r;
+    r.plan = (heads * sizeof(int2) + 255) & ~(size_t)255;
+    r.order = blocks > kHeldRows * kSelect ? ((heads * blocks * sizeof(uint32_t) + 255) & ~(size_t)255) : 0;
+    return r;
 }
 
 }  // namespace dtattn
@@ -230,7 +295,8 @@ using namespace dtattn;
 
 extern "C" size_t dtattn_kv_evict_workspace_size(const dtattn_kv_evict_args* a) {
     if (a == nullptr || a->B <= 0 || a->Hkv <= 0 || a->S_max <= 0 || a->block <= 0) return 0;
-    return evict_workspace(a);
+    const EvictSpace r = evict_workspace(a);
+    return r.plan + r.order;
 }
 
 extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
@@ -260,7 +326,8 @@ extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     if (a->k_cache == nullptr || a->v_cache == nullptr || a->weights == nullptr || a->lengths == nullptr || a->kept == nullptr)
         return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
     if (a->B * a->Hkv > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
-    const size_t need = evict_workspace(a);
+    const EvictSpace space = evict_workspace(a);
+    const size_t need = space.plan + space.order;
     if (a->workspace == nullptr || a->workspace_bytes < need)
         return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, a->workspace_bytes);
     if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(DTATTN_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
@@ -268,7 +335,8 @@ extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     p.kv[0] = reinterpret_cast<char*>(a->k_cache), p.kv[1] = reinterpret_cast<char*>(a->v_cache);
     p.scale[0] = a->k_scale, p.scale[1] = a->v_scale;
     p.w = a->weights, p.lengths = a->lengths, p.kept = a->kept;
-    p.order = reinterpret_cast<uint32_t*>(a->workspace);
+    p.plan = reinterpret_cast<int2*>(a->workspace);
+    p.order = reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(a->workspace) + space.plan);
     p.kv_b[0] = a->k_stride[0], p.kv_h[0] = a->k_stride[1], p.kv_s[0] = a->k_stride[2];
     p.kv_b[1] = a->v_stride[0], p.kv_h[1] = a->v_stride[1], p.kv_s[1] = a->v_stride[2];
     p.s_b[0] = a->k_scale_stride[0], p.s_h[0] = a->k_scale_stride[1];
@@ -282,12 +350,20 @@ extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     p.blocks_max = (int32_t)((a->S_max + a->block - 1) / a->block);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const unsigned heads = (unsigned)(a->B * a->Hkv);
-    hipLaunchKernelGGL(kv_evict_select_kernel, dim3(heads), dim3(kSelect), 0, stream, p);
+    if (p.blocks_max <= 4 * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<4>, dim3(heads), dim3(kSelect), 0, stream, p);
+    else if (p.blocks_max <= kHeldRows * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<kHeldRows>, dim3(heads), dim3(kSelect), 0, stream, p);
+    else hipLaunchKernelGGL(kv_evict_select_kernel<0>, dim3(heads), dim3(kSelect), 0, stream, p);
     int st = check_launch("kv_evict_select_kernel");
     if (st != DTATTN_OK) return st;
-    hipLaunchKernelGGL(kv_evict_move_kernel, dim3(heads, 3), dim3(1024), 0, stream, p);
-    st = check_launch("kv_evict_move_kernel");
-    if (st != DTATTN_OK) return st;
-    hipLaunchKernelGGL(kv_evict_lengths_kernel, dim3((unsigned)((a->B + 255) / 256)), dim3(256), 0, stream, p);
-    return check_launch("kv_evict_lengths_kernel");
+    // a row's chunks are shared until there is a workgroup for every CU, or one per chunk
+    const int cus = stream_cus(stream);
+    p.width = p.chunks;
+    while (p.width > 1 && 2 * (int64_t)heads * ((p.chunks + p.width - 1) / p.width) < cus) p.width = (p.width + 1) / 2;
+    p.width = std::min(p.width, 1024);
+    p.groups = (p.chunks + p.width - 1) / p.width;
+    const int64_t lots = (2 * (int64_t)heads + 7) / 8;
+    const int64_t grid = std::max<int64_t>(lots * 8 * p.groups, heads);
+    if (grid > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
+    hipLaunchKernelGGL(kv_evict_move_kernel, dim3((unsigned)grid, 2), dim3(1024), 0, stream, p);
+    return check_launch("kv_evict_move_kernel");
 }

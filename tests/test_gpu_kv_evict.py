@@ -203,6 +203,14 @@ def test_evict_long():
     _evict(rng, 1, 1, 70016, 16, [70001], 4000 * 16, 160, 16, torch.float8_e4m3fn, 16)
 
 
+def test_evict_many_and_few_heads():
+    # 300 workgroups of whole rows, and two whose rows' chunks are shared out, one of them with an odd number of chunks
+    rng = np.random.default_rng(11)
+    _evict(rng, 25, 6, 96, 16, [96 - 3 * (i % 7) for i in range(25)], 40, 4, 1, torch.bfloat16)
+    _evict(rng, 1, 1, 3001, 40, [3001], 1500, 7, 1, torch.bfloat16)
+    _evict(rng, 1, 1, 9000, 128, [8999], 4096, 16, 16, torch.float32)
+
+
 def test_evict_layouts():
     rng = np.random.default_rng(9)
     _evict(rng, 2, 3, 200, 64, [200, 151], 64, 4, 1, torch.float16, layout=lambda x: x.transpose(1, 2).contiguous().transpose(1, 2))
