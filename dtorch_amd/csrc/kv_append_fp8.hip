@@ -6,10 +6,13 @@
 // depend on the scale, only the range below the block's maximum does, and that is 2^-9 at the least), and a block that
 // grows over several appends then re-encodes its older rows by an exact shift instead of rounding them again each time.
 //
-// HBM-bound: one wave per (sequence, kv head, K or V, touched block).  It holds the block's new rows in registers
-// (up to 16 chunks of 8 elements per lane: 64 tokens of 128 elements), so that they are read once; larger
-// blocks read them twice, the second time from L2.  Few items per sequence (a decode step) run as one workgroup per
+// HBM-bound: an item per (sequence, kv head, K or V, touched block), whose threads hold its new rows in four chunks of 8
+// elements each, so that they are read once: a wave for up to 16 rows of 128, a workgroup of 2 to 16 waves for more.  A
+// thread runs the code once, so short code matters: 16 chunks per lane, one wave to a block of 64, took 20 us where this takes
+// 12 (4 x 2000 tokens of 8 heads of 128, bf16).  Few items per sequence (a decode step) run as one workgroup per
 // sequence, which also advances the length; with more a second launch on the same stream does.
+#include <algorithm>
+
 #include "fp8_cache.hpp"
 
 namespace dtattn {
@@ -31,8 +34,7 @@ struct Append8Params {
 
 namespace {
 
-constexpr int kHeld = 16;     // chunks of 8 elements that a lane holds: 64 rows of 128
-constexpr int kHeldStep = 4;  // in the step kernel, whose items are up to 16 rows
+constexpr int kHeld = 4;  // chunks of 8 elements that a lane holds: a wave holds 16 rows of 128
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 
@@ -57,6 +59,49 @@ __device__ __forceinline__ u32x2 encode8(const float* x, float inv) {
     return u32x2{codes4(y), codes4(y + 4)};
 }
 
+// Largest magnitude as bits: those of elements without their sign, which order as the values do, infinities and NaN on top.
+// Two 16-bit elements go at a time.
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, const Chunk<T>& c) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(c.v) / sizeof(c.v[0])); ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) m = max(m, c.v[i][j] & 0x7fffffffu);
+            else m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, c.v[i][j] & 0x7fff7fffu)));
+        }
+    return m;
+}
+// The value of max_bits over a wave's lanes.
+template <typename T>
+__device__ __forceinline__ float wave_max_bits(uint32_t m) {
+    if constexpr (sizeof(T) == 2) m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, m);
+    else return Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)m));
+}
+
+// 8 values of 16 bits, all finite, over a power of two s that holds them: one conversion per pair, which divides and rounds
+// once (the same codes as encode8's, checked over every value of both types).
+template <typename T>
+__device__ __forceinline__ u32x2 encode8_pow2(const Chunk<T>& c, float s) {
+    typedef T pair __attribute__((ext_vector_type(2)));
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = c.v[0][i];
+        const pair x = __builtin_bit_cast(pair, w);
+        s16x2 r = {};
+        if constexpr (__is_same(T, f16_t)) r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, x, s, false);
+        else r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, x, s, false);
+        o[i] = __builtin_bit_cast(uint32_t, r);
+    }
+    return u32x2{pack_lo_hi(o[0], o[1], 0), pack_lo_hi(o[2], o[3], 0)};
+}
+
 // 4 codes times `f`, rounded to codes again.
 __device__ __forceinline__ uint32_t recode4(uint32_t w, float f) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
@@ -64,10 +109,10 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float f) {
     return codes4(y);
 }
 
-// One wave's item: block i of those that the new tokens of (b, h) touch, of K (kv = 0) or V.
-template <typename T, bool PAGED, int HELD>
+// An item: block i of those that the new tokens of (b, h) touch, of K (kv = 0) or V.  WAVES: one wave's, or a workgroup's.
+template <typename T, bool PAGED, bool WAVES>
 __device__ __forceinline__ void append8_item(const Append8Params& p, int64_t b, int h, int kv, int i, int length) {
-    const int lane = threadIdx.x & 63;
+    const int t = WAVES ? threadIdx.x & 63 : threadIdx.x, threads = WAVES ? 64 : blockDim.x;
     const int start = max(length, 0);
     if (start >= p.capacity) return;
     const int t0 = ((start >> p.block_shift) + i) << p.block_shift;
@@ -85,70 +130,87 @@ __device__ __forceinline__ void append8_item(const Append8Params& p, int64_t b, 
     char* dst = p.dst[kv] + slot * p.d_b[kv] + h * p.d_h[kv] + row0 * p.d_s[kv];  // the block's first row
     float* sp = p.scale[kv] + slot * p.s_b[kv] + h * p.s_h[kv] + (row0 >> p.block_shift);
     const char* src = p.src[kv] + b * p.n_b[kv] + h * p.n_h[kv] + (int64_t)(first - start) * p.n_s[kv];
-    const int total = (stop - first) * p.cpr;
     const float old = first > t0 ? *sp : 0.f;
-
-    Chunk<T> raw[HELD];
-    auto load = [&](int base) {
+    // a thread's chunks: number c of rows r, r + step, ...; the launch has no more than kHeld * step rows in a block
+    const int step = threads / p.cpr, r = t / p.cpr, c = t - r * p.cpr;
+    const int rows = r < step ? stop - first : 0;  // threads past the last whole row idle
+    Chunk<T> raw[kHeld];
 #pragma unroll
-        for (int k = 0; k < HELD; ++k) {
-            const int idx = min(base + 64 * k + lane, total - 1);
-            if (base + 64 * k < total)
-                raw[k] = load_chunk<T, false>(reinterpret_cast<const T*>(src + (idx / p.cpr) * p.n_s[kv]) + (idx % p.cpr) * 8);
+    for (int k = 0; k < kHeld; ++k) {
+        raw[k] = Chunk<T>{};
+        if (r + k * step < rows) raw[k] = load_chunk<T, false>(reinterpret_cast<const T*>(src + (r + k * step) * p.n_s[kv]) + c * 8);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) top = max_bits<T>(top, raw[k]);
+    __shared__ float red[2][16];
+    auto largest = [&](float m, int which) {
+        if constexpr (!WAVES) {
+            if ((t & 63) == 0) red[which][t >> 6] = m;
+            __syncthreads();
+            for (int w = 0; w < threads >> 6; ++w) {  // NaN bits count as the largest here
+                const float x = red[which][w];
+                m = x != x || x > m ? x : m;
+            }
         }
+        return m;
     };
-    float m = 0.f;
-    for (int base = 0; base < total; base += 64 * HELD) {
-        load(base);
+    float m = largest(wave_max_bits<T>(top), 0);
+    const bool clean = finite(m);
+    if (!clean) {  // of the others, then
+        m = 0.f;
 #pragma unroll
-        for (int k = 0; k < HELD; ++k) {
-            if (base + 64 * k >= total) break;
+        for (int k = 0; k < kHeld; ++k) {
             float x[8];
             unpack_chunk<T>(raw[k], x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) m = fmaxf(m, finite(x[e]) ? fabsf(x[e]) : 0.f);
         }
+        m = largest(wave_max(m), 1);
     }
-    m = wave_max(m);
     float s = scale_for(m);
     if (first > t0) {
         s = fmaxf(old, s);
         if (s != old) {  // the block's older rows at its new scale
             const float f = old / s;
-            const int cells = (first - t0) * p.cpr;
-            for (int idx = lane; idx < cells; idx += 64) {
-                u32x2* at = reinterpret_cast<u32x2*>(dst + (idx / p.cpr) * p.d_s[kv] + (idx % p.cpr) * 8);
+            for (int i = r; i < (r < step ? first - t0 : 0); i += step) {
+                u32x2* at = reinterpret_cast<u32x2*>(dst + i * p.d_s[kv] + c * 8);
                 const u32x2 w = *at;
                 *at = u32x2{recode4(w.x, f), recode4(w.y, f)};
             }
         }
     }
-    if (lane == 0) *sp = s;
+    if (t == 0) *sp = s;
     const float inv = 1.f / s;
-    const int64_t skip = (int64_t)(first - t0) * p.d_s[kv];
-    for (int base = 0; base < total; base += 64 * HELD) {
-        if (total > 64 * HELD) load(base);
+    char* to = dst + (first - t0) * p.d_s[kv] + c * 8;
+    auto put = [&](auto encode) {
 #pragma unroll
-        for (int k = 0; k < HELD; ++k) {
-            const int idx = base + 64 * k + lane;
-            if (base + 64 * k >= total) break;
-            float x[8];
-            unpack_chunk<T>(raw[k], x);
-            const u32x2 w = encode8(x, inv);
-            if (idx < total) *reinterpret_cast<u32x2*>(dst + skip + (idx / p.cpr) * p.d_s[kv] + (idx % p.cpr) * 8) = w;
+        for (int k = 0; k < kHeld; ++k)
+            if (r + k * step < rows) *reinterpret_cast<u32x2*>(to + (r + k * step) * p.d_s[kv]) = encode(raw[k]);
+    };
+    if constexpr (sizeof(T) == 2) {
+        // an older scale of the caller's own need not be a power of two
+        if (clean && (__builtin_bit_cast(uint32_t, s) & 0x7fffffu) == 0) {
+            put([&](const Chunk<T>& w) { return encode8_pow2<T>(w, s); });
+            return;
         }
     }
+    put([&](const Chunk<T>& w) {
+        float x[8];
+        unpack_chunk<T>(w, x);
+        return encode8(x, inv);
+    });
 }
 
 }  // namespace
 
-template <typename T, bool PAGED>
-__global__ void __launch_bounds__(256) kv_append_fp8_kernel(const Append8Params p) {
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+template <typename T, bool PAGED, bool WAVES>
+__global__ void __launch_bounds__(WAVES ? 256 : 1024) kv_append_fp8_kernel(const Append8Params p) {
+    const int64_t item = WAVES ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
     if (item >= p.items) return;
     const int64_t bh = item / (2 * p.nblk), b = bh / p.Hkv;
     const int r = (int)(item % (2 * p.nblk));
-    append8_item<T, PAGED, kHeld>(p, b, (int)(bh % p.Hkv), r & 1, r >> 1, p.lengths[b]);
+    append8_item<T, PAGED, WAVES>(p, b, (int)(bh % p.Hkv), r & 1, r >> 1, p.lengths[b]);
 }
 
 // One sequence per workgroup, and its length.
@@ -158,7 +220,7 @@ __global__ void __launch_bounds__(1024) kv_append_fp8_step_kernel(const Append8P
     const int length = p.lengths[b];
     const int per = 2 * p.nblk, items = p.Hkv * per;
     for (int it = threadIdx.x >> 6; it < items; it += blockDim.x >> 6)
-        append8_item<T, PAGED, kHeldStep>(p, b, it / per, (it % per) & 1, (it % per) >> 1, length);
+        append8_item<T, PAGED, true>(p, b, it / per, (it % per) & 1, (it % per) >> 1, length);
     __syncthreads();  // every thread has read the length
     if (threadIdx.x == 0) p.lengths[b] = (int)min((int64_t)max(length, 0) + p.n_new, (int64_t)p.capacity);
 }
@@ -171,15 +233,22 @@ __global__ void __launch_bounds__(256) kv_lengths_fp8_kernel(int32_t* lengths, i
 template <typename T, bool PAGED>
 static int launch_append8(const Append8Params& p, int64_t B, hipStream_t stream) {
     const int64_t per_seq = p.items / B;
-    if (p.n_new > 0 && per_seq <= 64 && p.n_new <= 64 * kHeldStep / 16 && B <= 0x7fffffff) {
+    // rows that a wave holds: 16 of 128
+    const int held = kHeld * (64 / p.cpr);
+    if (p.n_new > 0 && per_seq <= 64 && p.n_new <= held && B <= 0x7fffffff) {
         const unsigned waves = (unsigned)(per_seq < 16 ? per_seq : 16);
         hipLaunchKernelGGL((kv_append_fp8_step_kernel<T, PAGED>), dim3((unsigned)B), dim3(64 * waves), 0, stream, p);
         return check_launch("kv_append_fp8_step_kernel");
     }
-    const int64_t blocks = (p.items + 3) / 4;
-    if (blocks > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "kv_append_fp8: grid too large");
     if (p.n_new > 0) {
-        hipLaunchKernelGGL((kv_append_fp8_kernel<T, PAGED>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        // a wave for a block that it holds, or else as many as hold it; 256 rows of 128 are 16 waves' (kHeld * (threads / cpr) rows)
+        const int rows = std::min(1 << p.block_shift, p.n_new);
+        unsigned waves = 1;
+        while (kHeld * (64 * (int)waves / p.cpr) < rows) ++waves;
+        const int64_t blocks = waves == 1 ? (p.items + 3) / 4 : p.items;
+        if (blocks > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "kv_append_fp8: grid too large");
+        if (waves == 1) hipLaunchKernelGGL((kv_append_fp8_kernel<T, PAGED, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((kv_append_fp8_kernel<T, PAGED, false>), dim3((unsigned)blocks), dim3(64 * waves), 0, stream, p);
         const int st = check_launch("kv_append_fp8_kernel");
         if (st != DTATTN_OK) return st;
     }

@@ -46,7 +46,7 @@ def append_fp8(codes, scale, table, lengths, new, block):
                     s = block_scale(float(fin.max(initial=0.0)))
                     if t > t0:
                         old = float(scale[slot, h, r0 // block])
-                        s = max(s, old)
+                        s = s if np.isnan(old) else max(s, old)
                         if s != old:
                             was = codes[slot, h, r0:r0 + t - t0]
                             val = e4m3fn_decode(was)

@@ -45,13 +45,15 @@ def _pool(rng, slots, H, rows, D, block):
     return k, s
 
 
-def _append(rng, lengths, H, D, cap, block, page, n, dtype, spoil=None, table=None):
+def _append(rng, lengths, H, D, cap, block, page, n, dtype, spoil=None, table=None, scales=None):
     B = len(lengths)
     if page and table is None:
         table = rng.permutation(B * (cap // page) + 2)[:B * (cap // page)].reshape(B, -1).astype(np.int32)
     slots, rows = (B * (cap // page) + 2, page) if page else (B, cap)
     k, ks = _pool(rng, slots, H, rows, D, block)
     v, vs = _pool(rng, slots, H, rows, D, block)
+    if scales is not None:
+        ks[:], vs[:] = scales(ks), scales(vs)
     new = [torch.from_numpy(rng.standard_normal((B, n, H, D)).astype(np.float32) * np.exp2(rng.integers(-8, 9, (1, n, H, 1))).astype(np.float32)).to(dtype)
            for _ in range(2)]
     if spoil is not None:
@@ -68,7 +70,7 @@ def _append(rng, lengths, H, D, cap, block, page, n, dtype, spoil=None, table=No
         _F().kv_cache_append_fp8(dk, dv, dks, dvs, dl, kn, vn)
     torch.cuda.synchronize()
     assert _same_codes(_codes(dk), k) and _same_codes(_codes(dv), v)
-    assert np.array_equal(dks.cpu().numpy(), ks) and np.array_equal(dvs.cpu().numpy(), vs)
+    assert np.array_equal(dks.cpu().numpy(), ks, equal_nan=True) and np.array_equal(dvs.cpu().numpy(), vs, equal_nan=True)
     assert dl.tolist() == [min(max(x, 0) + n, cap) for x in lengths]
 
 
@@ -113,6 +115,20 @@ def test_append_extreme_values(dtype):
 
     for n in (1, 4, 20):
         _append(rng, [0, 3, 0, 16, 2], 2, 64, 64, 16, 0, n, dtype, spoil if n > 3 else None)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_append_behind_scales_of_any_value(dtype):
+    # scales of the caller's own: kept where they hold the new values (the product with their reciprocal, rounded once to fp32, is
+    # what is encoded), replaced where they do not; 0 and NaN count as none
+    def scales(s):
+        s = np.where(np.arange(s.size).reshape(s.shape) % 2, np.float32(4.0), s * np.float32(2.0 ** -12))
+        s[0, 0], s[1, 0] = 0.0, np.nan
+        return s
+
+    rng = np.random.default_rng(12)
+    for n in (1, 9):
+        _append(rng, [3, 17, 40, 63], 2, 64, 128, 16, 0, n, dtype, scales=scales)
 
 
 def test_append_token_by_token_is_append_at_once():
