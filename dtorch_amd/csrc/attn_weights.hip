@@ -38,45 +38,46 @@ struct WeightParams {
 
 namespace {
 
-constexpr int kTiles = 4;  // key tiles of 16 per wave
+constexpr int kFewColumns = 64;
 
-// How a wave holds one tile's 16 keys (A operand: lane & 15 is the key) and one set's 16 queries (B operand), and their product.
+// How a wave holds one tile's 16 keys (B operand: lane & 15 is the key) and one set's 16 queries (A operand), and their product: a
+// lane has queries 4 (lane / 16) .. + 3 of key lane & 15, so a sum over queries is three adds and two exchanges.
 // 16-bit and 8-bit keys: 16x16x32 MFMAs on 16-bit operands; codes are exact there, and fp32 queries over codes are
-// three bf16 parts.
+// three bf16 parts.  Keys are loaded as they are, from rows and chunks that exist (what stands for a head dim past the last
+// meets a zero of the query), so that nothing stands between their loads and the next ones.
 template <typename TQ, typename TK, int D>
 struct Operands {
     typedef typename std::conditional<std::is_same<TQ, f16_t>::value, f16_t, bf16_t>::type E;
     typedef typename Elem<E>::vec8 V8;
     static constexpr bool codes = sizeof(TK) == 1;
     static constexpr int parts = std::is_same<TQ, float>::value ? 3 : 1;
-    static constexpr int steps = D / 32;
-    struct Keys { V8 v[steps]; };
+    static constexpr int steps = D / 32, loads = codes ? D / 64 : D / 32;
+    struct Keys { u32x4 v[loads]; };
     struct Queries { V8 v[parts][steps]; };
     // first head dim of the 8 of step s: chunks of 16 bytes of keys
     static __device__ __forceinline__ int dim(int g4, int s) { return codes ? 64 * (s >> 1) + 16 * g4 + 8 * (s & 1) : 32 * s + 8 * g4; }
-    // row: the key's first element; past: the row lies past the last key
-    static __device__ __forceinline__ void keys(Keys& f, const TK* row, int g4, int d, bool past) {
+    static __device__ __forceinline__ void keys(Keys& f, const TK* row, int g4, int d) {
 #pragma unroll
-        for (int s = 0; s < steps; s += codes ? 2 : 1) {
-            const int x = dim(g4, s);
-            const u32x4 w = x < d && !past ? ld16_nt(row + x) : u32x4{0u, 0u, 0u, 0u};
-            if constexpr (codes) f.v[s] = codes_to_vec8<E>(w.x, w.y), f.v[s + 1] = codes_to_vec8<E>(w.z, w.w);
-            else f.v[s] = __builtin_bit_cast(V8, w);
+        for (int i = 0; i < loads; ++i) {
+            const int x = dim(g4, codes ? 2 * i : i);
+            f.v[i] = ld16_nt(row + (x < d ? x : 0));
         }
     }
-    static __device__ __forceinline__ void queries(Queries& f, const TQ* row, int g4, int d, bool past, uint32_t q_and, uint32_t q_xor) {
+    // none: a query of zeros
+    static __device__ __forceinline__ void queries(Queries& f, const TQ* row, int g4, int d, bool none, uint32_t q_and, uint32_t q_xor) {
+        Chunk<TQ> w[steps];
+#pragma unroll
+        for (int s = 0; s < steps; ++s) w[s] = load_chunk<TQ, false>(row + (dim(g4, s) < d ? dim(g4, s) : 0));
 #pragma unroll
         for (int s = 0; s < steps; ++s) {
-            const int x = dim(g4, s);
-            Chunk<TQ> w = {};
-            if (x < d && !past) w = load_chunk<TQ, false>(row + x);
 #pragma unroll
-            for (int i = 0; i < (int)(sizeof(w.v) / sizeof(w.v[0])); ++i) w.v[i] = x < d && !past ? q_bits(w.v[i], q_and, q_xor) : w.v[i];
+            for (int i = 0; i < (int)(sizeof(w[s].v) / sizeof(w[s].v[0])); ++i)
+                w[s].v[i] = dim(g4, s) < d && !none ? q_bits(w[s].v[i], q_and, q_xor) : u32x4{0u, 0u, 0u, 0u};
             if constexpr (parts == 1) {
-                f.v[0][s] = __builtin_bit_cast(V8, w.v[0]);
+                f.v[0][s] = __builtin_bit_cast(V8, w[s].v[0]);
             } else {
                 float y[8];
-                unpack_chunk<TQ>(w, y);
+                unpack_chunk<TQ>(w[s], y);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     bf16_t t[3];
@@ -90,9 +91,13 @@ struct Operands {
     static __device__ __forceinline__ f32x4 product(const Keys& k, const Queries& q) {
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < steps; ++s)
+        for (int s = 0; s < steps; ++s) {
+            V8 kf;
+            if constexpr (codes) kf = s & 1 ? codes_to_vec8<E>(k.v[s >> 1].z, k.v[s >> 1].w) : codes_to_vec8<E>(k.v[s >> 1].x, k.v[s >> 1].y);
+            else kf = __builtin_bit_cast(V8, k.v[s]);
 #pragma unroll
-            for (int i = 0; i < parts; ++i) a = mfma16(k.v[s], q.v[i][s], a);
+            for (int i = 0; i < parts; ++i) a = mfma16(q.v[i][s], kf, a);
+        }
         return a;
     }
 };
@@ -102,95 +107,122 @@ struct Operands<float, float, D> {
     static constexpr int steps = D / 16;
     struct Keys { f32x4 v[steps]; };
     struct Queries { f32x4 v[steps]; };
-    static __device__ __forceinline__ void keys(Keys& f, const float* row, int g4, int d, bool past) {
+    static __device__ __forceinline__ void keys(Keys& f, const float* row, int g4, int d) {
 #pragma unroll
-        for (int s = 0; s < steps; ++s) {
-            const int x = 16 * s + 4 * g4;
-            f.v[s] = x < d && !past ? __builtin_bit_cast(f32x4, ld16_nt(row + x)) : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int s = 0; s < steps; ++s) f.v[s] = __builtin_bit_cast(f32x4, ld16_nt(row + (16 * s + 4 * g4 < d ? 16 * s + 4 * g4 : 0)));
     }
-    static __device__ __forceinline__ void queries(Queries& f, const float* row, int g4, int d, bool past, uint32_t q_and, uint32_t q_xor) {
+    static __device__ __forceinline__ void queries(Queries& f, const float* row, int g4, int d, bool none, uint32_t q_and, uint32_t q_xor) {
+        u32x4 w[steps];
 #pragma unroll
-        for (int s = 0; s < steps; ++s) {
-            const int x = 16 * s + 4 * g4;
-            f.v[s] = x < d && !past ? __builtin_bit_cast(f32x4, q_bits(ld16(row + x), q_and, q_xor)) : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int s = 0; s < steps; ++s) w[s] = ld16(row + (16 * s + 4 * g4 < d ? 16 * s + 4 * g4 : 0));
+#pragma unroll
+        for (int s = 0; s < steps; ++s)
+            f.v[s] = 16 * s + 4 * g4 < d && !none ? __builtin_bit_cast(f32x4, q_bits(w[s], q_and, q_xor)) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
     static __device__ __forceinline__ f32x4 product(const Keys& k, const Queries& q) {
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < steps; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a = __builtin_amdgcn_mfma_f32_16x16x4f32(k.v[s][e], q.v[s][e], a, 0, 0, 0);
+            for (int e = 0; e < 4; ++e) a = __builtin_amdgcn_mfma_f32_16x16x4f32(q.v[s][e], k.v[s][e], a, 0, 0, 0);
         return a;
     }
 };
 
 }  // namespace
 
-// Grid: (64-key chunks / 4, kv heads, sequences); one chunk per wave.  Column c of a set is (query, head) number 16 * set + c,
-// query-major: query c / group, head c % group.
-template <typename TQ, typename TK, int D, bool CAUSAL>
+// Few queries (up to kFewColumns of a kv head).  Grid: (workgroups of a (sequence, kv head), kv heads, sequences); the waves of those
+// workgroups take the chunks of TILES tiles in turn, whatever the sequence's length.  Column c of a set is (query, head) number
+// 16 * set + c, query-major: query c / group, head c % group.  A wave loads the next chunk's keys and weights when it
+// has this one's scores.
+template <typename TQ, typename TK, int D, bool CAUSAL, int TILES>
 __global__ void __launch_bounds__(256) attn_weights_kernel(const WeightParams p) {
     typedef Operands<TQ, TK, D> Op;
+    constexpr int KEYS = 16 * TILES;
     const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
     const int64_t b = blockIdx.z;
     const int hk = blockIdx.y;
-    const int k0 = ((int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 16 * kTiles;
     const int n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
+    const int stride = (int)gridDim.x * 4 * KEYS;
+    int k0 = ((int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * KEYS;
     if (k0 >= n) return;
     const TK* kb = reinterpret_cast<const TK*>(p.k) + b * p.k_b + hk * p.k_h;
     const TQ* qb = reinterpret_cast<const TQ*>(p.q) + b * p.q_b + (int64_t)hk * p.group * p.q_h;
     const float* lb = p.lse + b * p.lse_b + (int64_t)hk * p.group * p.lse_h;
-    typename Op::Keys kf[kTiles];
-    float c[kTiles];
+    float* const w = p.w + b * p.w_b + hk * p.w_h;
+    const int N = p.L * p.group;
+    int last = N;  // the end of the columns that are not padding
+    if constexpr (CAUSAL)
+        if (p.lengths != nullptr) last = (int)min(max(n - p.q_offset, (int64_t)0), (int64_t)p.L) * p.group;
+    if (last == 0) return;
+    typename Op::Keys kf[TILES];
+    float c[TILES], was[TILES];
+    auto load = [&](int key) {
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-        const int key = k0 + 16 * t + col;
-        Op::keys(kf[t], kb + (int64_t)min(key, n - 1) * p.k_s, g4, p.d, key >= n);
-        c[t] = p.c;
-        if constexpr (sizeof(TK) == 1) c[t] *= p.ks[b * p.ks_b + hk * p.ks_h + (min(k0 + 16 * t, n - 1) >> p.block_shift)];
-    }
-    const int64_t N = (int64_t)p.L * p.group;
-    // the first column that sees the chunk's first key, and the end of those that are not padding
-    int64_t first = 0, last = N;
-    if constexpr (CAUSAL) {
-        first = max((int64_t)k0 - p.q_offset, (int64_t)0) * p.group;
-        if (p.lengths != nullptr) last = min(N, max(n - p.q_offset, (int64_t)0) * p.group);
-    }
-    float sum[kTiles][4] = {};
-    for (int64_t n0 = first; n0 < last; n0 += 16) {
-        const int64_t at = n0 + col;
-        const int64_t i = min(at, last - 1) / p.group;
-        const int h = (int)(min(at, last - 1) - i * p.group);
-        const float lse = lb[h * p.lse_h + i];
-        // columns past the end, and rows that see no key: a query of zeros at a weight of 0
-        const bool none = at >= last || lse == kNegInf;
-        typename Op::Queries qf;
-        Op::queries(qf, qb + h * p.q_h + i * p.q_s, g4, p.d, none, p.q_and, p.q_xor);
-        const float nl = none ? kNegInf : -lse * kLog2e;
-        const int64_t sees = i + p.q_offset;  // the last key of this column
+        for (int t = 0; t < TILES; ++t) Op::keys(kf[t], kb + (int64_t)min(key + 16 * t + col, n - 1) * p.k_s, g4, p.d);
+    };
+    auto load_weights = [&](int key) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            const f32x4 s = Op::product(kf[t], qf);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x = fast_exp2(__builtin_fmaf(s[e], c[t], nl));
-                if constexpr (CAUSAL) x = k0 + 16 * t + 4 * g4 + e <= sees ? x : 0.f;
-                sum[t][e] += x;
-            }
+        for (int t = 0; t < TILES; ++t) {
+            c[t] = p.c;
+            if constexpr (sizeof(TK) == 1) c[t] *= p.ks[b * p.ks_b + hk * p.ks_h + (min(key + 16 * t, n - 1) >> p.block_shift)];
+            was[t] = w[min(key + 16 * t + col, n - 1)];
         }
-    }
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-        float v = 0.f;
+    };
+    typename Op::Queries qf;
+    float nl[4];
+    int64_t sees[4];  // the last keys of this lane's four columns
+    auto column = [&](int n0) {
+        float lse[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float s = group_sum<16>(sum[t][e]);
-            v = col == e ? s : v;
+            const int at = min(n0 + 4 * g4 + e, last - 1);
+            const int i = at / p.group;
+            lse[e] = lb[(at - i * p.group) * p.lse_h + i];
+            sees[e] = i + p.q_offset;
         }
-        const int key = k0 + 16 * t + 4 * g4 + col;
-        if (col < 4 && key < n) p.w[b * p.w_b + hk * p.w_h + key] += v;
+        const int at = min(n0 + col, last - 1);
+        const int i = at / p.group, h = at - i * p.group;
+        // columns past the end, and rows that see no key: a query of zeros at a weight of 0
+        const bool none = n0 + col >= last || lb[h * p.lse_h + i] == kNegInf;
+        Op::queries(qf, qb + h * p.q_h + i * p.q_s, g4, p.d, none, p.q_and, p.q_xor);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nl[e] = n0 + 4 * g4 + e >= last || lse[e] == kNegInf ? kNegInf : -lse[e] * kLog2e;
+    };
+    load(k0);
+    load_weights(k0);
+    column(0);
+    for (;; k0 += stride) {
+        float sum[TILES] = {};
+        const bool more = k0 + stride < n;
+        float cc[TILES], ww[TILES];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) cc[t] = c[t], ww[t] = was[t];
+        for (int n0 = 0; n0 < last; n0 += 16) {
+            if (last > 16) column(n0);
+            f32x4 s[TILES];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) s[t] = Op::product(kf[t], qf);
+            if (n0 + 16 >= last && more) {
+                load(k0 + stride);
+                load_weights(k0 + stride);
+            }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = fast_exp2(__builtin_fmaf(s[t][e], cc[t], nl[e]));
+                    if constexpr (CAUSAL) x = k0 + 16 * t + col <= sees[e] ? x : 0.f;
+                    sum[t] += x;
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const float v = sum_across_groups<16>(sum[t]);
+            const int key = k0 + 16 * t + col;
+            if (g4 == 0 && key < n) w[key] = ww[t] + v;
+        }
+        if (!more) break;
     }
 }
 
@@ -464,8 +496,7 @@ PromptPlan prompt_plan(const dtattn_weights_args* a, int keys, int cus) {
     return r;
 }
 
-// One set of 16 columns is the token form's; it reads the keys once and is done.
-bool is_prompt(const dtattn_weights_args* a) { return a->L * (a->Hq / a->Hkv) > 64; }
+bool is_prompt(const dtattn_weights_args* a) { return a->L * (a->Hq / a->Hkv) > kFewColumns; }
 
 int prompt_keys(const dtattn_weights_args* a) { return a->k_dtype == DTATTN_FP32 ? PromptTypes<float, float>::keys : PromptTypes<bf16_t, bf16_t>::keys; }
 
@@ -487,13 +518,24 @@ static int launch_prompt(WeightParams p, bool causal, const PromptPlan& plan, hi
     return check_launch("attn_weights_sum_kernel");
 }
 
+// per_cu: workgroups wanted per CU.  One set of columns: chunks of 32 keys; more sets load the queries again for each chunk, and take
+// 64.  us at 32 keys and 6 workgroups / 64 and 4: 16 of 700 to 8191, 28 heads over 4 (codes) 13.9 / 16.1, 16x8191 bf16 32 over 8 55 / 56,
+// 8 of 4000 to 8191 fp32 58 / 74; 8 of 20000 to 32768, 64 heads over 1 (codes) 32 / 25.
+template <typename TQ, typename TK, int D, int TILES>
+static int launch_few(const WeightParams& p, bool causal, int per_cu, hipStream_t stream) {
+    const int64_t slices = (int64_t)p.B * p.Hkv, most = (p.S + 64 * TILES - 1) / (64 * TILES);
+    const int64_t wanted = std::max<int64_t>(1, (int64_t)per_cu * std::max(stream_cus(stream), 1) / slices);
+    const dim3 grid((unsigned)std::min(most, wanted), (unsigned)p.Hkv, (unsigned)p.B);
+    if (causal) hipLaunchKernelGGL((attn_weights_kernel<TQ, TK, D, true, TILES>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attn_weights_kernel<TQ, TK, D, false, TILES>), grid, dim3(256), 0, stream, p);
+    return check_launch("attn_weights_kernel");
+}
+
 template <typename TQ, typename TK, int D>
 static int launch_weights(const WeightParams& p, bool causal, const PromptPlan* plan, hipStream_t stream) {
     if (plan != nullptr) return launch_prompt<TQ, TK, D>(p, causal, *plan, stream);
-    const dim3 grid((unsigned)((p.S + 64 * kTiles - 1) / (64 * kTiles)), (unsigned)p.Hkv, (unsigned)p.B);
-    if (causal) hipLaunchKernelGGL((attn_weights_kernel<TQ, TK, D, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((attn_weights_kernel<TQ, TK, D, false>), grid, dim3(256), 0, stream, p);
-    return check_launch("attn_weights_kernel");
+    if (p.L * p.group <= 16) return launch_few<TQ, TK, D, 2>(p, causal, 6, stream);
+    return launch_few<TQ, TK, D, 4>(p, causal, 4, stream);
 }
 
 template <typename TQ, typename TK>
