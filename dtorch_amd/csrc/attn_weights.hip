@@ -4,10 +4,12 @@
 // No counterpart in the reference, which keeps no KV cache (python/dtorch/test/modules/llama.py:126-156); the weights are
 // what dtattn_kv_evict chooses by.
 //
-// One query per sequence (decode) is bound by HBM: the keys are read once.  A prompt is bound by its products and
-// exponentials.  Both keep a wave's keys in registers as MFMA operands (64 keys: four tiles of 16) and pass the queries
-// by in sets of 16 (query, head) columns, so that the sum over queries stays in registers too and no two waves add
-// to one weight: the result does not depend on timing.
+// One query per sequence (decode) is bound by HBM: the keys are read once.  A prompt is bound by VALU issue: an exponential, an
+// fma and an add per (query, key) pair beside its MFMAs (16 MFMAs, 512 cycles, against 32 exponentials and 64 others, about
+// 512).  Both keep a wave's keys in registers as MFMA operands and pass the queries by, so that the sum over queries stays in
+// registers too and no two waves add to one weight: the result does not depend on timing.  Measured: 16 sequences of 700 to
+// 8191, 28 heads over 4 of 128, codes, one query 14 us; 4x2048 causal bf16, 32 heads over 8 of 128, 110-114 us, not causal
+// 158-168 us (850 TFLOP/s), at 4096 queries 1000 TFLOP/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -29,10 +31,11 @@ struct WeightParams {
     int64_t ks_b, ks_h, lse_b, lse_h;
     int64_t q_offset;
     int32_t B, Hkv, group, L, S, d, block_shift;
-    float c;  // scale * log2(e)
-    uint32_t q_and, q_xor;
-    float* part;               // prompts whose columns several workgroups share: [parts, B * Hkv, S]
-    int32_t parts, part_tiles; // and the column tiles of each
+    float c;  // scale * log2(e), of either sign
+    // prompts: columns go by in tiles of `rows` queries by `width` heads, the group's or a set of 32 of them
+    int32_t width, rows;
+    float* part;                // prompts whose columns several workgroups share: [parts, B * Hkv, S]
+    int32_t parts, row_parts, part_tiles;  // parts: head sets by row_parts parts of so many column tiles
     int32_t key_blocks;
 };
 
@@ -64,7 +67,7 @@ struct Operands {
         }
     }
     // none: a query of zeros
-    static __device__ __forceinline__ void queries(Queries& f, const TQ* row, int g4, int d, bool none, uint32_t q_and, uint32_t q_xor) {
+    static __device__ __forceinline__ void queries(Queries& f, const TQ* row, int g4, int d, bool none) {
         Chunk<TQ> w[steps];
 #pragma unroll
         for (int s = 0; s < steps; ++s) w[s] = load_chunk<TQ, false>(row + (dim(g4, s) < d ? dim(g4, s) : 0));
@@ -72,7 +75,7 @@ struct Operands {
         for (int s = 0; s < steps; ++s) {
 #pragma unroll
             for (int i = 0; i < (int)(sizeof(w[s].v) / sizeof(w[s].v[0])); ++i)
-                w[s].v[i] = dim(g4, s) < d && !none ? q_bits(w[s].v[i], q_and, q_xor) : u32x4{0u, 0u, 0u, 0u};
+                w[s].v[i] = dim(g4, s) < d && !none ? w[s].v[i] : u32x4{0u, 0u, 0u, 0u};
             if constexpr (parts == 1) {
                 f.v[0][s] = __builtin_bit_cast(V8, w[s].v[0]);
             } else {
@@ -111,13 +114,13 @@ struct Operands<float, float, D> {
 #pragma unroll
         for (int s = 0; s < steps; ++s) f.v[s] = __builtin_bit_cast(f32x4, ld16_nt(row + (16 * s + 4 * g4 < d ? 16 * s + 4 * g4 : 0)));
     }
-    static __device__ __forceinline__ void queries(Queries& f, const float* row, int g4, int d, bool none, uint32_t q_and, uint32_t q_xor) {
+    static __device__ __forceinline__ void queries(Queries& f, const float* row, int g4, int d, bool none) {
         u32x4 w[steps];
 #pragma unroll
         for (int s = 0; s < steps; ++s) w[s] = ld16(row + (16 * s + 4 * g4 < d ? 16 * s + 4 * g4 : 0));
 #pragma unroll
         for (int s = 0; s < steps; ++s)
-            f.v[s] = 16 * s + 4 * g4 < d && !none ? __builtin_bit_cast(f32x4, q_bits(w[s], q_and, q_xor)) : f32x4{0.f, 0.f, 0.f, 0.f};
+            f.v[s] = 16 * s + 4 * g4 < d && !none ? __builtin_bit_cast(f32x4, w[s]) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
     static __device__ __forceinline__ f32x4 product(const Keys& k, const Queries& q) {
         f32x4 a = {0.f, 0.f, 0.f, 0.f};
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(const WeightParams p)
         const int i = at / p.group, h = at - i * p.group;
         // columns past the end, and rows that see no key: a query of zeros at a weight of 0
         const bool none = n0 + col >= last || lb[h * p.lse_h + i] == kNegInf;
-        Op::queries(qf, qb + h * p.q_h + i * p.q_s, g4, p.d, none, p.q_and, p.q_xor);
+        Op::queries(qf, qb + h * p.q_h + i * p.q_s, g4, p.d, none);
 #pragma unroll
         for (int e = 0; e < 4; ++e) nl[e] = n0 + 4 * g4 + e >= last || lse[e] == kNegInf ? kNegInf : -lse[e] * kLog2e;
     };
@@ -244,6 +247,32 @@ struct PromptTypes {
     static constexpr int keys = 4 * 32 * tiles;        // per workgroup
 };
 
+// The queries that see a key block from kwg on: [first, last).
+template <bool CAUSAL>
+__device__ __forceinline__ void prompt_queries(const WeightParams& p, int kwg, int n, int& first, int& last) {
+    first = 0, last = p.L;
+    if constexpr (CAUSAL) {
+        first = (int)min(max((int64_t)kwg - p.q_offset, (int64_t)0), (int64_t)p.L);
+        if (p.lengths != nullptr) last = (int)min(max(n - p.q_offset, (int64_t)0), (int64_t)p.L);
+    }
+}
+
+// Parts that the tiles of queries [first, last) are cut in: equal ones of part_tiles or fewer.
+__device__ __forceinline__ int prompt_parts(const WeightParams& p, int first, int last) {
+    const int tiles = first < last ? (last + p.rows - 1) / p.rows - first / p.rows : 0;
+    return (tiles + p.part_tiles - 1) / p.part_tiles;
+}
+// The tiles [t0, t1) of one of them, if there is such a part.
+__device__ __forceinline__ bool prompt_part(const WeightParams& p, int first, int last, int part, int& t0, int& t1) {
+    const int parts = prompt_parts(p, first, last);
+    if (part >= parts) return false;
+    const int from = first / p.rows, tiles = (last + p.rows - 1) / p.rows - from;
+    const int each = tiles / parts, more = tiles - each * parts;
+    t0 = from + part * each + min(part, more);
+    t1 = t0 + each + (part < more ? 1 : 0);
+    return true;
+}
+
 // Elements x .. x + 7 of a row of d (a multiple of 16 bytes), zeros past its end.
 template <typename T>
 __device__ __forceinline__ Chunk<T> load8(const T* row, int x, int d) {
@@ -271,68 +300,120 @@ __device__ __forceinline__ void to_parts(const Chunk<T>& w, V8* out) {
     }
 }
 
-// (query, head) of a column, columns query-major, stepping by kCols.
-struct Column {
-    int64_t i;
-    int h;
-    __device__ __forceinline__ Column(int64_t n, int group) : i(n / group), h((int)(n - n / group * group)) {}
-    __device__ __forceinline__ void step(int di, int dh, int group) {
-        i += di;
-        h += dh;
-        if (h >= group) h -= group, ++i;
-    }
-};
-
 }  // namespace
 
 // A workgroup of four waves holds 256 keys (128 in fp32) as operands and passes column tiles by, which its threads stage
 // through LDS one tile ahead.  A column is a lane, so its lse is one register and the sums over columns are one
 // add per score; lanes meet once, at the end.  Per wave and tile of 16-bit operands 16 MFMAs against 32 exponentials and 64 other
-// VALU instructions.
+// VALU instructions: the exponentials of one 32-key tile go under the MFMAs of the next (the last one's under the next column
+// tile's), tiles on the causal border apart.
 template <typename TQ, typename TK, int D, bool CAUSAL>
 __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const WeightParams p) {
     typedef PromptTypes<TQ, TK> Types;
     typedef typename Types::E E;
     typedef typename Types::V8 V8;
     constexpr int QP = Types::qparts, KP = Types::kparts, KT = Types::tiles, KS = D / 16, DC = D / 8;
-    constexpr int PER = kCols * DC / 256;  // chunks of 8 elements that a thread stages
+    constexpr int PER = kCols * DC / 256, ROWS = 256 / DC;  // chunks of 8 elements that a thread stages, ROWS rows apart
     __shared__ __attribute__((aligned(16))) V8 stage[2][QP][kCols * DC];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
-    // workgroup -> (key block, part of the columns, slice); slices go round the XCDs, whose L2 then holds their queries
+    // workgroup -> (part of the columns, key block, slice): slices go round the XCDs, and the key blocks that a part's queries meet
+    // run side by side, so an L2 loads those queries once
     const int slices = p.B * p.Hkv;
     const int slice = blockIdx.x % slices;
     const int rest = blockIdx.x / slices;
-    const int part = rest % p.parts, kblock = rest / p.parts;
+    const int kblock = rest % p.key_blocks, part = rest / p.key_blocks;  // part: head set * row parts + row part
     const int64_t b = slice / p.Hkv;
     const int hk = slice % p.Hkv;
     const int n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
     const int kwg = kblock * Types::keys;
     if (kwg >= n) return;
-    const int64_t N = (int64_t)p.L * p.group;
-    int64_t first = 0, last = N;  // the block's columns
-    if constexpr (CAUSAL) {
-        first = min(max((int64_t)kwg - p.q_offset, (int64_t)0) * p.group, N);
-        if (p.lengths != nullptr) last = min(N, max(n - p.q_offset, (int64_t)0) * p.group);
-    }
-    const int64_t t0 = max(first / kCols, (int64_t)part * p.part_tiles);
-    const int64_t t1 = min((last + kCols - 1) / kCols, (int64_t)(part + 1) * p.part_tiles);
-    if (t0 >= t1) return;  // the sum knows
+    const int set = part / p.row_parts, row_part = part - set * p.row_parts;
+    int first, last;
+    prompt_queries<CAUSAL>(p, kwg, n, first, last);
+    int t0, t1;
+    if (!prompt_part(p, first, last, row_part, t0, t1)) return;  // the sum knows
     const int k0 = kwg + __builtin_amdgcn_readfirstlane(tid >> 6) * 32 * KT;
+
+    // What a thread stages of a tile: chunk x0 of columns r0, r0 + ROWS, ..., query-major (query column / width, head column % width).
+    // Chunk x of column r lies at x ^ swz(r): 16 columns read one chunk each without a conflict.  Columns that are none (heads past
+    // the group's, and where the width does not divide 32) and chunks past the head dim are zeros from the start.
+    auto swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+    const int r0 = tid / DC, x0 = tid % DC, heads = p.group - set * kCols;
+    for (int i = tid; i < 2 * QP * kCols * DC; i += 256) (&stage[0][0][0])[i] = V8{};
+    int srow[PER];
+    const TQ* src[PER];
+    const float* lse_src;
+    const int crow = col / p.width < p.rows && col % p.width < heads ? col / p.width : -1;  // this lane's column (-1: none)
+    {
+        const TQ* qb = reinterpret_cast<const TQ*>(p.q) + b * p.q_b + ((int64_t)hk * p.group + set * kCols) * p.q_h + (int64_t)t0 * p.rows * p.q_s;
+        const float* lb = p.lse + b * p.lse_b + ((int64_t)hk * p.group + set * kCols) * p.lse_h + (int64_t)t0 * p.rows;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int r = r0 + k * ROWS, head = r % p.width;
+            srow[k] = r / p.width;
+            if (8 * x0 >= p.d || srow[k] >= p.rows || head >= heads) srow[k] = -1;  // nothing to stage
+            src[k] = qb + (srow[k] >= 0 ? srow[k] * p.q_s + head * p.q_h + 8 * x0 : 0);
+        }
+        lse_src = lb + (crow >= 0 ? (int64_t)(col % p.width) * p.lse_h + crow : 0);
+    }
+    const int64_t step = p.rows * p.q_s;
+    const int tail = last % p.rows != 0 ? last / p.rows : 1 << 30;  // the tile with queries past the last
+    Chunk<TQ> raw[PER];
+    float lse;
+    auto load = [&](int t) {  // (what is loaded is not looked at here: that would wait for it)
+        const int rows = t == tail ? last % p.rows : p.rows;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const TQ* at = src[k];
+            if (t == tail && srow[k] >= rows) at -= srow[k] * p.q_s;  // a query that is there
+            raw[k] = load8(at, 0, p.d - 8 * x0 > 0 ? p.d - 8 * x0 : p.d);
+            src[k] += step;
+        }
+        const float* at = lse_src;
+        if (t == tail && crow >= rows) at -= crow;
+        lse = *at;
+        lse_src += p.rows;
+    };
+    V8* const put_at = &stage[0][0][r0 * DC + (x0 ^ swz(r0))];
+    constexpr int BUF = QP * kCols * DC;
+    auto put = [&](int buf, int t) {
+        // a row that sees no key (an lse of -inf) may hold anything: it counts as zeros at a weight of 0, and so do queries past the last
+        const bool blank = __ballot(lse == kNegInf) != 0;
+        if (blank || t == tail) {
+            if (t == tail && crow >= last % p.rows) lse = kNegInf;
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (__shfl(lse, r0 + k * ROWS, 64) == kNegInf) raw[k] = Chunk<TQ>{};
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            V8 o[QP];
+            to_parts<TQ, V8, QP>(raw[k], o);
+            // rows ROWS apart have one swz where ROWS is a multiple of its period
+            const int r = r0 + k * ROWS;
+            V8* const at = ROWS % 16 == 0 ? put_at + k * ROWS * DC : &stage[0][0][r * DC + (x0 ^ swz(r))];
+            if (srow[k] >= 0) {
+#pragma unroll
+                for (int i = 0; i < QP; ++i) at[buf * BUF + i * kCols * DC] = o[i];
+            }
+        }
+    };
+    load(t0);
 
     const TK* kb = reinterpret_cast<const TK*>(p.k) + b * p.k_b + hk * p.k_h;
     V8 kf[KT][KP][KS];
     float c[KT][2];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-        const TK* row = kb + (int64_t)min(k0 + 32 * t + col, n - 1) * p.k_s;
+        const TK* krow = kb + (int64_t)min(k0 + 32 * t + col, n - 1) * p.k_s;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int x = 16 * s + 8 * half;
             if constexpr (sizeof(TK) == 1) {
-                const u32x2 w = x < p.d ? *reinterpret_cast<const u32x2*>(row + x) : u32x2{0u, 0u};
+                const u32x2 w = x < p.d ? *reinterpret_cast<const u32x2*>(krow + x) : u32x2{0u, 0u};
                 kf[t][0][s] = codes_to_vec8<E>(w.x, w.y);
             } else {
-                const Chunk<TK> w = load8(row, x, p.d);
+                const Chunk<TK> w = load8(krow, x, p.d);
                 V8 o[KP];
                 to_parts<TK, V8, KP>(w, o);
 #pragma unroll
@@ -346,86 +427,106 @@ __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const Weigh
         }
     }
 
-    const TQ* qb = reinterpret_cast<const TQ*>(p.q) + b * p.q_b + (int64_t)hk * p.group * p.q_h;
-    const float* lb = p.lse + b * p.lse_b + (int64_t)hk * p.group * p.lse_h;
-    const int di = kCols / p.group, dh = kCols % p.group;
-    // chunk x of row r of a tile lies at x ^ swz(r): 16 rows read one chunk each without a conflict
-    auto swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
-    Column own(t0 * kCols + col, p.group);  // this lane's column
-    int64_t left = last - t0 * kCols;       // columns from the tile on
-    const int r0 = tid / DC, x0 = tid % DC;  // rows r0 + k * 256 / DC of a tile
-    Column src0(t0 * kCols + r0, p.group), src1(t0 * kCols + r0 + 256 / DC, p.group);
-    Chunk<TQ> raw[PER];
-    float lse;
-    auto load = [&]() {  // the tile that src0, src1 and own stand at, and on to the next
-        int64_t at[2] = {src0.i * p.q_s + src0.h * p.q_h, src1.i * p.q_s + src1.h * p.q_h};
+    const V8* get_at[KS];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const bool ok = r0 + k * (256 / DC) < left;
-            raw[k] = load8(qb + (ok ? at[k] : 0), 8 * x0, ok ? p.d : 0);
-        }
-        lse = col < left ? lb[own.h * p.lse_h + own.i] : kNegInf;
-        left -= kCols;
-        src0.step(di, dh, p.group);
-        src1.step(di, dh, p.group);
-    };
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int r = r0 + k * (256 / DC);
-            Chunk<TQ> w = raw[k];
-#pragma unroll
-            for (int i = 0; i < (int)(sizeof(w.v) / sizeof(w.v[0])); ++i) w.v[i] = q_bits(w.v[i], p.q_and, p.q_xor);
-            V8 o[QP];
-            to_parts<TQ, V8, QP>(w, o);
-#pragma unroll
-            for (int i = 0; i < QP; ++i) stage[buf][i][r * DC + (x0 ^ swz(r))] = o[i];
-        }
-    };
-
+    for (int x = 0; x < KS; ++x) get_at[x] = &stage[0][0][col * DC + ((2 * x) ^ (half ^ swz(col)))];
+    // every thread is past the zeros of the stage before the first tile is put there
+    lds_barrier();
     float sum[KT][16] = {};
-    load();
-    for (int64_t t = t0; t < t1; ++t) {
-        const int buf = (int)(t - t0) & 1;
-        put(buf);
-        const bool none = lse == kNegInf;
-        const float nl = -lse * kLog2e;
-        int lim = 32 * KT - 1;  // the last of the wave's keys that this column sees
-        if constexpr (CAUSAL) lim = (int)min(max(own.i + p.q_offset - k0, (int64_t)-1), (int64_t)(32 * KT - 1));
-        if (none) lim = -1;
-        own.step(di, dh, p.group);
-        if (t + 1 < t1) load();
+    float nl;
+    // Stages tile t and has the next one on its way.  Buffers alternate, and the barrier has every wave past its reads of the other
+    // one's last tile.
+    auto turn = [&](int buf, int t) {
+        put(buf, t);
+        nl = crow < 0 || lse == kNegInf ? kNegInf : -lse * kLog2e;
+        if (t + 1 < t1) load(t + 1);
         lds_barrier();
-        // buffers alternate, and this barrier has every wave past its reads of the other one's last tile
-        if (k0 < n && __ballot(lim >= 0) != 0) {
-            f32x16 s[KT] = {};
+    };
+    V8 qf[KS];  // held for the second key tile, but for the three parts of fp32
+    auto queries = [&](int buf) {
+        if constexpr (QP == 1) {
 #pragma unroll
-            for (int x = 0; x < KS; ++x) {
-                V8 qf[QP];
+            for (int x = 0; x < KS; ++x) qf[x] = get_at[x][buf * BUF];
+        }
+    };
+    auto product = [&](int buf, int kt) {
+        f32x16 s = {};
 #pragma unroll
-                for (int i = 0; i < QP; ++i) qf[i] = stage[buf][i][col * DC + ((2 * x + half) ^ swz(col))];
+        for (int x = 0; x < KS; ++x) {
+            V8 q[QP];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+            for (int j = 0; j < QP; ++j) q[j] = QP == 1 ? qf[x] : get_at[x][buf * BUF + j * kCols * DC];
 #pragma unroll
-                    for (int i = 0; i < KP; ++i)
+            for (int i = 0; i < KP; ++i)
 #pragma unroll
-                        for (int j = 0; j < QP && i + j < 3; ++j) s[kt] = Elem<E>::mfma32(kf[kt][i][x], qf[j], s[kt]);
-            }
-            if (__ballot(lim < 32 * KT - 1) == 0) {
+                for (int j = 0; j < QP && i + j < 3; ++j) s = Elem<E>::mfma32(kf[kt][i][x], q[j], s);
+        }
+        return s;
+    };
+    auto fold = [&](const f32x16& s, int kt, float at) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+        for (int i = 0; i < 16; ++i) sum[kt][i] += fast_exp2(__builtin_fmaf(s[i], c[kt][i >> 3], at));
+    };
+    int t = t0;
+    if constexpr (CAUSAL) {
+        // tiles whose first query does not see the wave's last key (an even number; a wave without keys runs through them all)
+        int64_t border = t1;
+        if (k0 < n) border = max(((int64_t)k0 + 32 * KT - 1 - p.q_offset + p.rows - 1) / p.rows, (int64_t)t0);
+        const int t_full = (int)min(border + ((border - t0) & 1), (int64_t)t1);
+        for (; t < t_full; ++t) {
+            const int buf = (t - t0) & 1;
+            turn(buf, t);
+            // the last of the wave's keys that this column sees
+            int lim = (int)min(max((int64_t)t * p.rows + p.q_offset - k0, (int64_t)-64), (int64_t)(32 * KT)) + max(crow, 0);
+            if (k0 >= n || __ballot(lim >= 0) == 0) continue;
+            lim -= 4 * half;
+            queries(buf);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[kt][i] += fast_exp2(__builtin_fmaf(s[kt][i], c[kt][i >> 3], nl));
-            } else {
+            for (int kt = 0; kt < KT; ++kt) {
+                const f32x16 s = product(buf, kt);
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float x = fast_exp2(__builtin_fmaf(s[kt][i], c[kt][i >> 3], nl));
-                        sum[kt][i] += 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3) <= lim ? x : 0.f;
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    const float x = fast_exp2(__builtin_fmaf(s[i], c[kt][i >> 3], nl));
+                    sum[kt][i] += 32 * kt + 8 * (i >> 2) + (i & 3) <= lim ? x : 0.f;
+                }
             }
         }
+    }
+    if (k0 < n) {
+        // scores that wait for their exponentials: the last key tile's of the column tile before
+        f32x16 wait = {};
+        float wait_nl = kNegInf;
+        auto full = [&](auto buffer) {
+            constexpr int buf = decltype(buffer)::value;
+            turn(buf, t++);
+            queries(buf);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const f32x16 s = product(buf, kt);
+                fold(wait, kt == 0 ? KT - 1 : kt - 1, kt == 0 ? wait_nl : nl);
+                wait = s;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {  // a step's MFMAs, and a KS-th of the VALU instructions and exponentials
+                    __builtin_amdgcn_sched_group_barrier(0x008, KP * QP == 9 ? 6 : QP, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 32 / KS, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x400, 16 / KS, 0);
+                }
+            }
+            wait_nl = nl;
+        };
+        while (t + 1 < t1) {
+            full(std::integral_constant<int, 0>());
+            // the sums stay under this tile's MFMAs: left alone they sink past the next barrier
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(sum[kt][i]));
+            full(std::integral_constant<int, 1>());
+        }
+        if (t < t1) full(std::integral_constant<int, 0>());
+        fold(wait, KT - 1, wait_nl);
+    } else {
+        for (; t < t1; ++t) turn((t - t0) & 1, t);
     }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -452,17 +553,13 @@ __global__ void __launch_bounds__(256) attn_weights_sum_kernel(const WeightParam
     const int hk = slice % p.Hkv;
     const int n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
     if (key >= n) return;
-    const int64_t N = (int64_t)p.L * p.group;
-    int64_t first = 0, last = N;
-    if constexpr (CAUSAL) {
-        first = min(max((int64_t)(key / keys * keys) - p.q_offset, (int64_t)0) * p.group, N);
-        if (p.lengths != nullptr) last = min(N, max(n - p.q_offset, (int64_t)0) * p.group);
-    }
-    const int64_t t0 = first / kCols, t1 = (last + kCols - 1) / kCols;
-    if (t0 >= t1) return;
-    const int x0 = (int)(t0 / p.part_tiles), x1 = (int)((t1 - 1) / p.part_tiles);
+    int first, last;
+    prompt_queries<CAUSAL>(p, key / keys * keys, n, first, last);
+    const int parts = prompt_parts(p, first, last);
+    if (parts == 0) return;
     float v = 0.f;
-    for (int x = x0; x <= x1; ++x) v += p.part[((int64_t)x * slices + slice) * p.S + key];
+    for (int set = 0; set < p.parts; set += p.row_parts)
+        for (int x = 0; x < parts; ++x) v += p.part[((int64_t)(set + x) * slices + slice) * p.S + key];
     p.w[b * p.w_b + hk * p.w_h + key] += v;
 }
 
@@ -470,28 +567,37 @@ namespace {
 
 // Parts that a prompt's columns are cut in, so that the workgroups (two fit a CU) go round a few times.
 struct PromptPlan {
-    int64_t key_blocks, parts, part_tiles;
+    int64_t key_blocks, parts, row_parts, part_tiles;
+    int32_t width, rows;
     size_t bytes;
 };
 
 PromptPlan prompt_plan(const dtattn_weights_args* a, int keys, int cus) {
     PromptPlan r;
     r.key_blocks = (a->S + keys - 1) / keys;
-    const int64_t group = a->Hq / a->Hkv, slices = a->B * a->Hkv;
-    const int64_t tiles = (a->L * group + kCols - 1) / kCols;
+    const int64_t group = a->Hq / a->Hkv, slices = a->B * a->Hkv, sets = (group + kCols - 1) / kCols;
+    // a tile is whole queries (of up to 32 heads each), so that a thread's part of it is the same in every tile
+    r.width = (int32_t)std::min<int64_t>(group, kCols);
+    r.rows = kCols / r.width;
+    const int64_t tiles = (a->L + r.rows - 1) / r.rows;
     double work = (double)r.key_blocks * (double)tiles;
-    if (a->causal != 0) {  // key block k sees the columns from key k * keys - q_offset on
+    if (a->causal != 0) {  // key block k sees the queries from key k * keys - q_offset on
         work = 0;
         const int64_t step = std::max<int64_t>(1, r.key_blocks / 256);  // sampled
         for (int64_t k = 0; k < r.key_blocks; k += step) {
             const int64_t from = std::min<int64_t>(std::max<int64_t>(k * keys - a->q_offset, 0), a->L);
-            work += (double)step * (double)((a->L - from) * group) / kCols;
+            work += (double)step * (double)(a->L - from) / r.rows;
         }
     }
-    work *= (double)slices;
-    r.part_tiles = std::max<int64_t>(8, (int64_t)(work / (2.0 * cus * 3)) + 1);
+    work *= (double)(slices * sets);
+    // two workgroups fit a CU.  us at 1 / 2 / 3 / 5 rounds of them (bf16 but for the last two): 4x2048 causal 32 heads over 8 127 /
+    // 114 / 114 / 121, not causal 163 / 168 / 171 / 172; 2x2000 causal 20 heads of 64 33 / 37 / 37 / 38; 1x4000 causal 28 over 4, fp16
+    // 133 / 122 / 129 / 147; 1x1500 causal 32 over 8, fp32 96 / 93 / 90 / 91.  Parts of less than 8 tiles cost more to start than
+    // they spread (1x777 causal 32 over 8 at 4 tiles 27, at 8 21).
+    r.part_tiles = std::max<int64_t>(8, (int64_t)(work / (2.0 * cus * 2)) + 1);
     r.part_tiles = std::min(r.part_tiles, tiles);
-    r.parts = (tiles + r.part_tiles - 1) / r.part_tiles;
+    r.row_parts = (tiles + r.part_tiles - 1) / r.part_tiles;
+    r.parts = r.row_parts * sets;
     r.bytes = r.parts > 1 ? (((size_t)r.parts * slices * a->S * sizeof(float) + 255) & ~(size_t)255) : 0;
     return r;
 }
@@ -506,6 +612,7 @@ template <typename TQ, typename TK, int D>
 static int launch_prompt(WeightParams p, bool causal, const PromptPlan& plan, hipStream_t stream) {
     const int64_t slices = (int64_t)p.B * p.Hkv;
     p.parts = (int32_t)plan.parts, p.part_tiles = (int32_t)plan.part_tiles, p.key_blocks = (int32_t)plan.key_blocks;
+    p.row_parts = (int32_t)plan.row_parts, p.width = plan.width, p.rows = plan.rows;
     const dim3 grid((unsigned)(slices * plan.parts * plan.key_blocks));
     if (causal) hipLaunchKernelGGL((attn_weights_prompt_kernel<TQ, TK, D, true>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((attn_weights_prompt_kernel<TQ, TK, D, false>), grid, dim3(256), 0, stream, p);
@@ -599,8 +706,8 @@ extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stre
     p.q_offset = a->q_offset;
     p.B = (int32_t)a->B, p.Hkv = (int32_t)a->Hkv, p.group = (int32_t)(a->Hq / a->Hkv);
     p.L = (int32_t)a->L, p.S = (int32_t)a->S, p.d = (int32_t)a->D;
-    p.c = sp.scale * kLog2e;
-    p.q_and = sp.q_and, p.q_xor = sp.q_xor;
+    // the sign of a scale and a scale of 0 as they are: no product is rounded by either
+    p.c = sp.q_and == 0u ? 0.f : (sp.q_xor != 0u ? -sp.scale : sp.scale) * kLog2e;
     const bool causal = a->causal != 0;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     PromptPlan prompt;
@@ -609,6 +716,7 @@ extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stre
         const int cus = stream_cus(stream);
         if (cus <= 0) return fail(DTATTN_ERR_DEVICE, "%s: cannot tell the stream's device", who);
         prompt = prompt_plan(a, prompt_keys(a), cus);
+        if (prompt.row_parts * prompt.part_tiles * prompt.rows > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many queries", who);
         if (prompt.key_blocks * prompt.parts * a->B * a->Hkv > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
         if (prompt.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < prompt.bytes))
             return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, prompt.bytes, a->workspace_bytes);
