@@ -43,11 +43,13 @@ namespace {
 
 constexpr int kFewColumns = 64;
 
+__device__ const uint32_t kZeros[4] = {0u, 0u, 0u, 0u};
+
 // How a wave holds one tile's 16 keys (B operand: lane & 15 is the key) and one set's 16 queries (A operand), and their product: a
 // lane has queries 4 (lane / 16) .. + 3 of key lane & 15, so a sum over queries is three adds and two exchanges.
 // 16-bit and 8-bit keys: 16x16x32 MFMAs on 16-bit operands; codes are exact there, and fp32 queries over codes are
-// three bf16 parts.  Keys are loaded as they are, from rows and chunks that exist (what stands for a head dim past the last
-// meets a zero of the query), so that nothing stands between their loads and the next ones.
+// three bf16 parts.  Keys are loaded as they are, from rows that exist (and from zeros for head dims past the last), so that
+// nothing stands between their loads and the next ones.
 template <typename TQ, typename TK, int D>
 struct Operands {
     typedef typename std::conditional<std::is_same<TQ, f16_t>::value, f16_t, bf16_t>::type E;
@@ -63,7 +65,7 @@ struct Operands {
 #pragma unroll
         for (int i = 0; i < loads; ++i) {
             const int x = dim(g4, codes ? 2 * i : i);
-            f.v[i] = ld16_nt(row + (x < d ? x : 0));
+            f.v[i] = ld16_nt(x < d ? row + x : reinterpret_cast<const TK*>(kZeros));
         }
     }
     // none: a query of zeros
@@ -112,7 +114,8 @@ struct Operands<float, float, D> {
     struct Queries { f32x4 v[steps]; };
     static __device__ __forceinline__ void keys(Keys& f, const float* row, int g4, int d) {
 #pragma unroll
-        for (int s = 0; s < steps; ++s) f.v[s] = __builtin_bit_cast(f32x4, ld16_nt(row + (16 * s + 4 * g4 < d ? 16 * s + 4 * g4 : 0)));
+        for (int s = 0; s < steps; ++s)
+            f.v[s] = __builtin_bit_cast(f32x4, ld16_nt(16 * s + 4 * g4 < d ? row + 16 * s + 4 * g4 : reinterpret_cast<const float*>(kZeros)));
     }
     static __device__ __forceinline__ void queries(Queries& f, const float* row, int g4, int d, bool none) {
         u32x4 w[steps];
@@ -186,8 +189,9 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(const WeightParams p)
         }
         const int at = min(n0 + col, last - 1);
         const int i = at / p.group, h = at - i * p.group;
-        // columns past the end, and rows that see no key: a query of zeros at a weight of 0
-        const bool none = n0 + col >= last || lb[h * p.lse_h + i] == kNegInf;
+        // rows that see no key may hold anything: a query of zeros.  Columns past the end are the last one again, so that an
+        // infinite key is no NaN where it is none there.  Both at a weight of 0.
+        const bool none = lb[h * p.lse_h + i] == kNegInf;
         Op::queries(qf, qb + h * p.q_h + i * p.q_s, g4, p.d, none);
 #pragma unroll
         for (int e = 0; e < 4; ++e) nl[e] = n0 + 4 * g4 + e >= last || lse[e] == kNegInf ? kNegInf : -lse[e] * kLog2e;
@@ -335,8 +339,9 @@ __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const Weigh
     const int k0 = kwg + __builtin_amdgcn_readfirstlane(tid >> 6) * 32 * KT;
 
     // What a thread stages of a tile: chunk x0 of columns r0, r0 + ROWS, ..., query-major (query column / width, head column % width).
-    // Chunk x of column r lies at x ^ swz(r): 16 columns read one chunk each without a conflict.  Columns that are none (heads past
-    // the group's, and where the width does not divide 32) and chunks past the head dim are zeros from the start.
+    // Chunk x of column r lies at x ^ swz(r): 16 columns read one chunk each without a conflict.  Chunks past the head dim are zeros
+    // from the start; columns that are none (heads past the group's, and where the width does not divide 32) are the tile's first
+    // one again, so that an infinite key is no NaN where it is none there.
     auto swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
     const int r0 = tid / DC, x0 = tid % DC, heads = p.group - set * kCols;
     for (int i = tid; i < 2 * QP * kCols * DC; i += 256) (&stage[0][0][0])[i] = V8{};
@@ -349,9 +354,10 @@ __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const Weigh
         const float* lb = p.lse + b * p.lse_b + ((int64_t)hk * p.group + set * kCols) * p.lse_h + (int64_t)t0 * p.rows;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            const int r = r0 + k * ROWS, head = r % p.width;
-            srow[k] = r / p.width;
-            if (8 * x0 >= p.d || srow[k] >= p.rows || head >= heads) srow[k] = -1;  // nothing to stage
+            const int r = r0 + k * ROWS;
+            const bool none = r / p.width >= p.rows || r % p.width >= heads;
+            const int head = none ? 0 : r % p.width;
+            srow[k] = 8 * x0 >= p.d ? -1 : none ? 0 : r / p.width;  // -1: nothing to stage
             src[k] = qb + (srow[k] >= 0 ? srow[k] * p.q_s + head * p.q_h + 8 * x0 : 0);
         }
         lse_src = lb + (crow >= 0 ? (int64_t)(col % p.width) * p.lse_h + crow : 0);
@@ -377,14 +383,13 @@ __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const Weigh
     V8* const put_at = &stage[0][0][r0 * DC + (x0 ^ swz(r0))];
     constexpr int BUF = QP * kCols * DC;
     auto put = [&](int buf, int t) {
-        // a row that sees no key (an lse of -inf) may hold anything: it counts as zeros at a weight of 0, and so do queries past the last
-        const bool blank = __ballot(lse == kNegInf) != 0;
-        if (blank || t == tail) {
-            if (t == tail && crow >= last % p.rows) lse = kNegInf;
+        // a row that sees no key (an lse of -inf) may hold anything: it counts as zeros, at a weight of 0
+        if (__ballot(lse == kNegInf) != 0) {
 #pragma unroll
             for (int k = 0; k < PER; ++k)
                 if (__shfl(lse, r0 + k * ROWS, 64) == kNegInf) raw[k] = Chunk<TQ>{};
         }
+        if (t == tail && crow >= last % p.rows) lse = kNegInf;  // past the last query
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             V8 o[QP];

@@ -637,6 +637,7 @@ extern "C" int dtattn_decode_fp8(const dtattn_decode_fp8_args* a, void* stream_)
     st = plan_scale(a->scale, a->D, a->dtype == DTATTN_FP32 ? kSign32 : kSign16, &sp);
     if (st != DTATTN_OK) return st;
     if (a->B == 0) return DTATTN_OK;
+    if (a->B * a->Hq > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
     if (a->q == nullptr || a->lengths == nullptr || a->o == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
     const int64_t esz = a->dtype == DTATTN_FP32 ? 4 : 2;
     for (int i = 0; i < 2; ++i)

@@ -263,7 +263,7 @@ using namespace dtattn;
 extern "C" int dtattn_kv_append_fp8(const dtattn_kv_append_fp8_args* a, void* stream_) {
     const char* who = "kv_append_fp8";
     if (a == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: args is NULL", who);
-    if (a->B < 0 || a->Hkv <= 0 || a->n_new < 0 || a->D <= 0 || a->Hkv > (1 << 20))
+    if (a->B < 0 || a->Hkv <= 0 || a->n_new < 0 || a->D <= 0 || a->Hkv > (1 << 20) || a->B > (1 << 24))
         return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
     Append8Params p = {};
     Fp8Cache c;
@@ -275,6 +275,8 @@ extern "C" int dtattn_kv_append_fp8(const dtattn_kv_append_fp8_args* a, void* st
     if (a->B == 0) return DTATTN_OK;
     if (a->lengths == nullptr || (a->n_new > 0 && (a->k_new == nullptr || a->v_new == nullptr)))
         return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    if (a->k_cache == a->v_cache || a->k_scale == a->v_scale)
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: keys and values are both written and cannot share memory", who);
     const int64_t esz = a->dtype == DTATTN_FP32 ? 4 : 2;
     for (int i = 0; i < 3; ++i)
         if ((a->k_new_stride[i] * esz) % 16 != 0 || (a->v_new_stride[i] * esz) % 16 != 0)
@@ -307,6 +309,7 @@ extern "C" int dtattn_kv_append_fp8(const dtattn_kv_append_fp8_args* a, void* st
     p.block_shift = c.block_shift;
     // the first new token may be the last row of its block
     p.nblk = a->n_new == 0 ? 0 : (int32_t)((a->block - 1 + a->n_new - 1) / a->block + 1);
+    if (a->B * a->Hkv > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
     p.items = a->B * a->Hkv * 2 * p.nblk;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const bool paged = a->block_table != nullptr;

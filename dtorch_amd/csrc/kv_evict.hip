@@ -302,7 +302,7 @@ extern "C" size_t dtattn_kv_evict_workspace_size(const dtattn_kv_evict_args* a) 
 extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     const char* who = "kv_evict";
     if (a == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: args is NULL", who);
-    if (a->B < 0 || a->Hkv <= 0 || a->S_max <= 0 || a->S_max > (1 << 29) || a->row_bytes <= 0)
+    if (a->B < 0 || a->Hkv <= 0 || a->B > 0x7fffffff || a->Hkv > 0x7fffffff || a->S_max <= 0 || a->S_max > (1 << 29) || a->row_bytes <= 0)
         return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
     if (a->block < 1 || a->block > 256 || (a->block & (a->block - 1)) != 0)
         return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: block %lld must be a power of two up to 256", who, (long long)a->block);
@@ -325,6 +325,8 @@ extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     if (a->B == 0) return DTATTN_OK;
     if (a->k_cache == nullptr || a->v_cache == nullptr || a->weights == nullptr || a->lengths == nullptr || a->kept == nullptr)
         return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    if (a->k_cache == a->v_cache || (scales && a->k_scale == a->v_scale))
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: keys and values are both moved in place and cannot share memory", who);
     if (a->B * a->Hkv > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
     const EvictSpace space = evict_workspace(a);
     const size_t need = space.plan + space.order;

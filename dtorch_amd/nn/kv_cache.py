@@ -11,6 +11,12 @@ attends with the split-KV decode kernels:
 
 Prompts in one prefill call share their length; per-sequence lengths then diverge only through the
 caller's own use of `lengths`.
+
+With ``dtype=torch.float8_e4m3fn`` a cache holds codes and a scale for each block of tokens and kv head
+(half the bytes of a 16-bit one): the prompt's own attention still runs on the tensors as they come, and
+decode reads the codes.  ``KVCache(track_weights=True)`` also sums the attention weight that each cached
+token has received, and ``evict(keep, recent)`` shrinks every sequence to the tokens that received the most
+(and the newest ones), so that a bounded cache serves an unbounded sequence.
 """
 from __future__ import annotations
 
@@ -22,13 +28,38 @@ import torch
 from . import functional as F
 
 
+_CODES = torch.float8_e4m3fn
+
+
+def _scales(cache: torch.Tensor, block: int):
+    """K and V scales of a cache of codes, one per block of tokens and kv head (None, None for other caches)."""
+    if cache.dtype != _CODES:
+        return None, None
+    if block not in (16, 32, 64, 128, 256) or cache.shape[2] % block:
+        raise ValueError(f"the tokens of a scale must be a power of two from 16 to 256 that divides a page; got {block}")
+    if cache.shape[3] % 16 or cache.shape[3] > 128:
+        raise ValueError(f"a cache of codes takes a head_dim that is a multiple of 16 up to 128; got {cache.shape[3]}")
+    scale = torch.ones(cache.shape[0], cache.shape[1], cache.shape[2] // block, device=cache.device)
+    return scale, torch.ones_like(scale)
+
+
 class KVCache:
-    """Padded cache [B, Hkv, max_len, D] plus device lengths [B] (int32)."""
+    """Padded cache [B, Hkv, max_len, D] plus device lengths [B] (int32).
+
+    dtype float8_e4m3fn: codes with fp32 scales [B, Hkv, max_len / block], max_len rounded up to whole blocks of
+    ``block`` tokens (a power of two from 16 to 256).  track_weights: fp32 ``weights`` [B, Hkv, max_len], for evict().
+    """
 
     def __init__(self, batch: int, kv_heads: int, max_len: int, head_dim: int, dtype=torch.bfloat16,
-                 device="cuda", scale: Optional[float] = None):
+                 device="cuda", scale: Optional[float] = None, block: int = 32, track_weights: bool = False):
+        self.block = max(block, 1) if dtype == _CODES else 1  # tokens that share a scale, and that evict() keeps or drops together
+        max_len = -(-max_len // self.block) * self.block
         self.k = torch.zeros(batch, kv_heads, max_len, head_dim, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
+        self.k_scale, self.v_scale = _scales(self.k, self.block)
+        if track_weights and (head_dim > 128 or head_dim * self.k.element_size() % 16):
+            raise ValueError(f"track_weights takes a head_dim up to 128 whose rows are multiples of 16 bytes; got {head_dim}")
+        self.weights = torch.zeros(batch, kv_heads, max_len, device=device) if track_weights else None
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.scale = scale
         self._host_len = np.zeros(batch, dtype=np.int64)  # mirrors `lengths` for capacity checks
@@ -48,14 +79,17 @@ class KVCache:
             self._host_stale = True
         if self._host_stale:
             return self.capacity
-        return max(int(self._host_len.max(initial=0)), 1)
+        return -(-max(int(self._host_len.max(initial=0)), 1) // self.block) * self.block
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
         """Append [B, Hkv, n, D] keys and values after each sequence's current length."""
         n = k_new.shape[2]
         if int(self._host_len.max(initial=0)) + n > self.capacity:
             raise ValueError(f"KV cache full: {int(self._host_len.max())} + {n} tokens > capacity {self.capacity}")
-        F.kv_cache_append(self.k, self.v, self.lengths, k_new, v_new)
+        if self.k_scale is not None:
+            F.kv_cache_append_fp8(self.k, self.v, self.k_scale, self.v_scale, self.lengths, k_new, v_new)
+        else:
+            F.kv_cache_append(self.k, self.v, self.lengths, k_new, v_new)
         self._host_len += n  # only once the append was accepted
 
     def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
@@ -63,15 +97,42 @@ class KVCache:
         causal alignment to hold), then the prompt's K/V into the cache."""
         if int(self._host_len.max(initial=0)) != 0:
             raise ValueError("prefill expects an empty cache; use decode() for later tokens")
-        out = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=self.scale, enable_gqa=True)
+        if self.weights is None:
+            out = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=self.scale, enable_gqa=True)
+            self.append(k, v)
+            return out
+        out, lse = F.scaled_dot_product_attention_with_lse(q, k, v, is_causal=True, scale=self.scale, enable_gqa=True)
         self.append(k, v)
+        F.attention_weight_accumulate(self.weights[:, :, :k.shape[2]], q, k, lse, is_causal=True, scale=self.scale)
         return out
 
     def decode(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> torch.Tensor:
         """One new token per sequence: append its K/V, then attend over everything cached."""
         self.append(k_new, v_new)
         n = self._span()
-        return F.decode_attention(q, self.k[:, :, :n], self.v[:, :, :n], self.lengths, scale=self.scale)[0]
+        k, v, ks = self.k[:, :, :n], self.v[:, :, :n], None
+        if self.k_scale is not None:
+            ks = self.k_scale[:, :, :n // self.block]
+            out, lse = F.decode_attention_fp8(q, k, v, ks, self.v_scale[:, :, :n // self.block], self.lengths, scale=self.scale)
+        else:
+            out, lse = F.decode_attention(q, k, v, self.lengths, scale=self.scale)
+        if self.weights is not None:
+            F.attention_weight_accumulate(self.weights[:, :, :n], q, k, lse, lengths=self.lengths, scale=self.scale, key_scale=ks)
+        return out
+
+    def evict(self, keep: int, recent: int) -> torch.Tensor:
+        """Shrink each sequence to ``keep`` tokens: its last ``recent`` and, kv head by kv head, those of the others
+        that received the most attention (F.kv_cache_evict; both are multiples of ``block``).  The order of the
+        tokens stays, and keys keep the positions they were rotated with.  Returns the kept block indices."""
+        if self.weights is None:
+            raise ValueError("evict needs a cache with track_weights=True")
+        kept = F.kv_cache_evict(self.k, self.v, self.lengths, self.weights, keep, recent, block=self.block,
+                                k_scale=self.k_scale, v_scale=self.v_scale)
+        if torch.cuda.is_current_stream_capturing():
+            self._host_stale = True
+        blocks = -(-self._host_len // self.block)  # as the kernel shortens them
+        self._host_len = np.where(blocks > keep // self.block, keep + self._host_len - blocks * self.block, self._host_len)
+        return kept
 
     def sync_lengths(self) -> np.ndarray:
         """Refresh the host copy of the lengths from the device (one synchronising copy).
@@ -80,10 +141,14 @@ class KVCache:
         advances only the device lengths.  Call this after replays and before eager use, so that the
         capacity check sees the true lengths.  The caller bounds the number of replays by
         capacity - current length: the append kernel drops tokens past the capacity (and the lengths
-        saturate there), so later replays would attend over a truncated cache.
+        saturate there), so later replays would attend over a truncated cache.  A caller that has shortened
+        `lengths` itself calls it as well; it then clears the weights of the tokens that are gone.
         """
         self._host_len = self.lengths.to("cpu", torch.int64).numpy().copy()
         self._host_stale = False
+        if self.weights is not None:
+            gone = torch.arange(self.capacity, device=self.weights.device) >= self.lengths[:, None]
+            self.weights.masked_fill_(gone[:, None], 0.0)
         return self._host_len.copy()
 
 
@@ -91,13 +156,15 @@ class PagedKVCache:
     """Paged cache: pools [num_pages, Hkv, page_size, D], a block table [B, max_pages] and lengths [B].
 
     Pages come from a host-side free list when a sequence's next tokens cross into a new page; the block
-    table rows that change are copied to the device before the append that writes them.
+    table rows that change are copied to the device before the append that writes them.  dtype float8_e4m3fn:
+    codes with fp32 scales [num_pages, Hkv, page_size / block], ``block`` tokens (at most a page) to a scale.
     """
 
     def __init__(self, batch: int, kv_heads: int, num_pages: int, page_size: int, max_pages: int, head_dim: int,
-                 dtype=torch.bfloat16, device="cuda", scale: Optional[float] = None):
+                 dtype=torch.bfloat16, device="cuda", scale: Optional[float] = None, block: int = 32):
         self.k = torch.zeros(num_pages, kv_heads, page_size, head_dim, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
+        self.k_scale, self.v_scale = _scales(self.k, min(block, page_size))
         self.page_size = page_size
         self.scale = scale
         self._free = list(range(num_pages - 1, -1, -1))
@@ -135,7 +202,10 @@ class PagedKVCache:
                 changed = True
         if changed:
             self.block_table.copy_(torch.from_numpy(self._table), non_blocking=False)
-        F.kv_cache_append_paged(self.k, self.v, self.block_table, self.lengths, k_new, v_new)
+        if self.k_scale is not None:
+            F.kv_cache_append_fp8_paged(self.k, self.v, self.k_scale, self.v_scale, self.block_table, self.lengths, k_new, v_new)
+        else:
+            F.kv_cache_append_paged(self.k, self.v, self.block_table, self.lengths, k_new, v_new)
         self._host_len += n  # only once the append was accepted
 
     def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
@@ -148,6 +218,9 @@ class PagedKVCache:
     def decode(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> torch.Tensor:
         self.append(k_new, v_new)
         n = self._span_pages()
+        if self.k_scale is not None:
+            return F.decode_attention_fp8_paged(q, self.k, self.v, self.k_scale, self.v_scale, self.block_table[:, :n],
+                                                self.lengths, scale=self.scale)[0]
         return F.decode_attention_paged(q, self.k, self.v, self.block_table[:, :n], self.lengths, scale=self.scale)[0]
 
     def sync_lengths(self) -> np.ndarray:

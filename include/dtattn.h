@@ -311,7 +311,8 @@ int dtattn_kv_append_paged(const dtattn_kv_append_paged_args* args, void* stream
  * of its scale and the needed one; when that is a new scale, its r older rows become
  * e4m3fn_rne(code * (old / new)), which is exact for the powers of two that this call writes, subnormal
  * codes apart.  New codes are e4m3fn_rne(x * (1 / scale)); NaN and infinities become NaN codes.  Rows past
- * the written ones are left as they were. */
+ * the written ones are left as they were.  A page that is written belongs to one sequence; keys and values lie
+ * apart (equal pointers are refused). */
 typedef struct {
     const void* k_new;     /* [B, Hkv, n_new, D], `dtype` (any strides that are multiples of 16 bytes, D stride 1) */
     const void* v_new;
@@ -382,7 +383,9 @@ int dtattn_decode_fp8(const dtattn_decode_fp8_args* args, void* stream);
  * where lse is what the attention over the same keys returned.  Key j is visible to query i iff
  * j < n = lengths[b] (S without lengths) and, when causal, j <= i + q_offset; with causal and lengths a query at
  * i + q_offset >= n is padding and adds nothing.  A row whose lse is -inf (it sees no key) adds nothing.
- * Sums are fp32 in an order that depends on the sizes alone.  Only weights[b, hk, j < n] are touched. */
+ * Sums are fp32, without atomics, in an order that depends on the sizes, the lengths and the device's CU count.  Only
+ * weights[b, hk, j < n] are touched.  Where an fp32 query or key is infinite its products with another's zero parts are NaN, and
+ * so may be a weight that is 0 in exact arithmetic; keys that a row does not see never count. */
 typedef struct {
     float* weights;          /* [B, Hkv, S], key stride 1 */
     const void* q;           /* [B, Hq, L, D] */
@@ -418,7 +421,8 @@ int dtattn_attention_weights(const dtattn_weights_args* args, void* stream);
  * 0, and lengths[b] becomes keep - block + the tokens of the last block.  Rows behind are left as they were.  A sequence
  * of no more than keep / block blocks is left alone.  kept[b, h, i] is the index of the i-th block that stayed, -1 past
  * them.  1 <= block <= recent <= keep, both multiples of block, block a power of two up to 256; with codes, block is a multiple of
- * scale_block.  K and V rows are `row_bytes` bytes, a multiple of 16, at strides that are multiples of 16 bytes. */
+ * scale_block.  K and V rows are `row_bytes` bytes, a multiple of 16, at strides that are multiples of 16 bytes; K and V
+ * lie apart (equal pointers are refused). */
 typedef struct {
     void* k_cache;           /* [B, Hkv, S_max, row] */
     void* v_cache;
