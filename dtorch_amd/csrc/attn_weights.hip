@@ -8,8 +8,8 @@
 // fma and an add per (query, key) pair beside its MFMAs (16 MFMAs, 512 cycles, against 32 exponentials and 64 others, about
 // 512).  Both keep a wave's keys in registers as MFMA operands and pass the queries by, so that the sum over queries stays in
 // registers too and no two waves add to one weight: the result does not depend on timing.  Measured: 16 sequences of 700 to
-// 8191, 28 heads over 4 of 128, codes, one query 14 us; 4x2048 causal bf16, 32 heads over 8 of 128, 110-114 us, not causal
-// 158-168 us (850 TFLOP/s), at 4096 queries 1000 TFLOP/s.
+// 8191, 28 heads over 4 of 128, codes, one query 14 us; 4x2048 causal bf16, 32 heads over 8 of 128, 98 us, not causal 138 us
+// (990 TFLOP/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -34,8 +34,8 @@ struct WeightParams {
     float c;  // scale * log2(e), of either sign
     // prompts: columns go by in tiles of `rows` queries by `width` heads, the group's or a set of 32 of them
     int32_t width, rows;
-    float* part;                // prompts whose columns several workgroups share: [parts, B * Hkv, S]
-    int32_t parts, row_parts, part_tiles;  // parts: head sets by row_parts parts of so many column tiles
+    float* part;  // records of blocks that several shares meet: [B * Hkv, sets, shares + key_blocks, keys of a block]
+    int32_t sets, shares;  // head sets; shares of a (sequence, kv head, head set) at most
     int32_t key_blocks;
 };
 
@@ -237,7 +237,9 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(const WeightParams p)
 
 namespace {
 
-constexpr int kCols = 32;  // columns of a tile: 32x32 products
+constexpr int kCols = 32;       // columns of a tile: 32x32 products
+constexpr int kShareTiles = 4;  // column tiles that a share has at least
+constexpr int kStartTiles = 4;  // column tiles whose time it takes to start a key block
 
 // 16-bit and 8-bit keys are one operand; fp32 ones are three bf16 parts (8 bits each, exact), of whose nine products with the
 // query's parts the six largest count: what is left out is below 2^-23 of |q| |k|, an fp32 sum's own rounding.
@@ -251,31 +253,58 @@ struct PromptTypes {
     static constexpr int keys = 4 * 32 * tiles;        // per workgroup
 };
 
-// The queries that see a key block from kwg on: [first, last).
+// The column tiles that the key blocks of a sequence meet, one block after another: block k meets those from first(k) to end.  Their
+// list is cut in equal shares, one per workgroup, so that all run for the same time however a causal mask cuts the blocks.
 template <bool CAUSAL>
-__device__ __forceinline__ void prompt_queries(const WeightParams& p, int kwg, int n, int& first, int& last) {
-    first = 0, last = p.L;
-    if constexpr (CAUSAL) {
-        first = (int)min(max((int64_t)kwg - p.q_offset, (int64_t)0), (int64_t)p.L);
-        if (p.lengths != nullptr) last = (int)min(max(n - p.q_offset, (int64_t)0), (int64_t)p.L);
+struct PromptTiles {
+    const WeightParams& p;
+    int keys, n, end, last;  // keys of a block and of the sequence; tiles, and queries that are not padding
+    __device__ __forceinline__ PromptTiles(const WeightParams& p_, int keys_, int64_t b) : p(p_), keys(keys_) {
+        n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
+        last = p.L;
+        if (CAUSAL && p.lengths != nullptr) last = (int)min(max(n - p.q_offset, (int64_t)0), (int64_t)p.L);
+        end = (last + p.rows - 1) / p.rows;
     }
+    __device__ __forceinline__ int first(int k) const {
+        if constexpr (!CAUSAL) return 0;
+        const int64_t query = (int64_t)k * keys - p.q_offset;
+        return query >= last ? end : (int)max(query, (int64_t)0) / p.rows;
+    }
+    __device__ __forceinline__ int count(int k) const { return (int64_t)k * keys < n ? end - first(k) : 0; }
+    // f(k0, c, pre) for 64 blocks at a time: lane's block k0 + lane meets c tiles, and those up to it pre
+    template <typename F>
+    __device__ __forceinline__ int scan(F f) const {
+        const int lane = threadIdx.x & 63;
+        int total = 0;
+        for (int k0 = 0; k0 < p.key_blocks; k0 += 64) {
+            const int c = k0 + lane < p.key_blocks ? count(k0 + lane) : 0;
+            const int pre = scan64(c) + total;
+            f(k0, c, pre);
+            total = __builtin_amdgcn_readlane(pre, 63);
+        }
+        return total;
+    }
+};
+
+// A share's record of a key block: the sum of the two numbers is another one for each of a list's records.
+__device__ __forceinline__ int64_t prompt_record(const WeightParams& p, int slice, int set, int share, int kblock) {
+    return ((int64_t)slice * p.sets + set) * (p.shares + p.key_blocks) + share + kblock;
 }
 
-// Parts that the tiles of queries [first, last) are cut in: equal ones of part_tiles or fewer.
-__device__ __forceinline__ int prompt_parts(const WeightParams& p, int first, int last) {
-    const int tiles = first < last ? (last + p.rows - 1) / p.rows - first / p.rows : 0;
-    return (tiles + p.part_tiles - 1) / p.part_tiles;
-}
-// The tiles [t0, t1) of one of them, if there is such a part.
-__device__ __forceinline__ bool prompt_part(const WeightParams& p, int first, int last, int part, int& t0, int& t1) {
-    const int parts = prompt_parts(p, first, last);
-    if (part >= parts) return false;
-    const int from = first / p.rows, tiles = (last + p.rows - 1) / p.rows - from;
-    const int each = tiles / parts, more = tiles - each * parts;
-    t0 = from + part * each + min(part, more);
-    t1 = t0 + each + (part < more ? 1 : 0);
-    return true;
-}
+// V tiles in up to `most` shares of V / n or one more, of kShareTiles at least.
+struct PromptShares {
+    int n, q, rem;
+    __device__ __forceinline__ PromptShares(int V, int most) {
+        n = min(most, max(1, V / kShareTiles));
+        q = V / n;
+        rem = V - q * n;
+    }
+    __device__ __forceinline__ int start(int r) const { return r * q + min(r, rem); }
+    __device__ __forceinline__ int of(int x) const {
+        const int big = rem * (q + 1);
+        return x < big ? x / (q + 1) : rem + (x - big) / q;
+    }
+};
 
 // Elements x .. x + 7 of a row of d (a multiple of 16 bytes), zeros past its end.
 template <typename T>
@@ -310,9 +339,11 @@ __device__ __forceinline__ void to_parts(const Chunk<T>& w, V8* out) {
 // through LDS one tile ahead.  A column is a lane, so its lse is one register and the sums over columns are one
 // add per score; lanes meet once, at the end.  Per wave and tile of 16-bit operands 16 MFMAs against 32 exponentials and 64 other
 // VALU instructions: the exponentials of one 32-key tile go under the MFMAs of the next (the last one's under the next column
-// tile's), tiles on the causal border apart.
+// tile's), tiles on the causal border apart.  Workgroups take equal shares of the tiles, from one key block into the next, and
+// as many as run at a time: parts of one block each, of even sizes, left places idle (4x2048 causal 32 heads over 8, bf16 108 us,
+// equal shares 98; 1x4000 causal 28 over 4, fp16 122, shares 100).
 template <typename TQ, typename TK, int D, bool CAUSAL>
-__global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const WeightParams p) {
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) attn_weights_prompt_kernel(const WeightParams p) {
     typedef PromptTypes<TQ, TK> Types;
     typedef typename Types::E E;
     typedef typename Types::V8 V8;
@@ -320,23 +351,34 @@ __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const Weigh
     constexpr int PER = kCols * DC / 256, ROWS = 256 / DC;  // chunks of 8 elements that a thread stages, ROWS rows apart
     __shared__ __attribute__((aligned(16))) V8 stage[2][QP][kCols * DC];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
-    // workgroup -> (part of the columns, key block, slice): slices go round the XCDs, and the key blocks that a part's queries meet
-    // run side by side, so an L2 loads those queries once
+    // workgroup -> (share, head set, slice): slices go round the XCDs, so an L2 loads a slice's queries and keys once
     const int slices = p.B * p.Hkv;
     const int slice = blockIdx.x % slices;
-    const int rest = blockIdx.x / slices;
-    const int kblock = rest % p.key_blocks, part = rest / p.key_blocks;  // part: head set * row parts + row part
+    const int set = blockIdx.x / slices % p.sets, share = blockIdx.x / slices / p.sets;
     const int64_t b = slice / p.Hkv;
     const int hk = slice % p.Hkv;
-    const int n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
-    const int kwg = kblock * Types::keys;
-    if (kwg >= n) return;
-    const int set = part / p.row_parts, row_part = part - set * p.row_parts;
-    int first, last;
-    prompt_queries<CAUSAL>(p, kwg, n, first, last);
-    int t0, t1;
-    if (!prompt_part(p, first, last, row_part, t0, t1)) return;  // the sum knows
-    const int k0 = kwg + __builtin_amdgcn_readfirstlane(tid >> 6) * 32 * KT;
+    const PromptTiles<CAUSAL> tiles(p, Types::keys, b);
+    const int n = tiles.n;
+    int c0 = 0, pre0 = 0;  // of the first 64 blocks
+    const int all = tiles.scan([&](int k0, int c, int pre) {
+        if (k0 == 0) c0 = c, pre0 = pre;
+    });
+    if (all == 0) return;
+    const PromptShares shares(all, p.shares);
+    if (share >= shares.n) return;
+    int todo = shares.start(share + 1) - shares.start(share);
+    int kblock = 0, t0 = shares.start(share);  // the first tile: so far counted in the list
+    auto find = [&](int k0, int c, int pre) {
+        const uint64_t hit = __ballot(pre > shares.start(share) && pre - c <= shares.start(share));
+        if (hit == 0) return;
+        const int l = __builtin_ctzll(hit);
+        kblock = k0 + l;
+        t0 -= __builtin_amdgcn_readlane(pre - c, l);
+    };
+    if (p.key_blocks <= 64) find(0, c0, pre0);
+    else tiles.scan(find);
+    t0 += tiles.first(kblock);
+    int t1 = min(t0 + todo, tiles.end);
 
     // What a thread stages of a tile: chunk x0 of columns r0, r0 + ROWS, ..., query-major (query column / width, head column % width).
     // Chunk x of column r lies at x ^ swz(r): 16 columns read one chunk each without a conflict.  Chunks past the head dim are zeros
@@ -363,11 +405,12 @@ __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const Weigh
         lse_src = lb + (crow >= 0 ? (int64_t)(col % p.width) * p.lse_h + crow : 0);
     }
     const int64_t step = p.rows * p.q_s;
-    const int tail = last % p.rows != 0 ? last / p.rows : 1 << 30;  // the tile with queries past the last
+    const int tail_rows = tiles.last % p.rows;
+    const int tail = tail_rows != 0 ? tiles.end - 1 : -1;  // the tile with queries past the last
     Chunk<TQ> raw[PER];
     float lse;
     auto load = [&](int t) {  // (what is loaded is not looked at here: that would wait for it)
-        const int rows = t == tail ? last % p.rows : p.rows;
+        const int rows = t == tail ? tail_rows : p.rows;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const TQ* at = src[k];
@@ -389,7 +432,7 @@ __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const Weigh
             for (int k = 0; k < PER; ++k)
                 if (__shfl(lse, r0 + k * ROWS, 64) == kNegInf) raw[k] = Chunk<TQ>{};
         }
-        if (t == tail && crow >= last % p.rows) lse = kNegInf;  // past the last query
+        if (t == tail && crow >= tail_rows) lse = kNegInf;  // past the last query
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             V8 o[QP];
@@ -405,174 +448,202 @@ __global__ void __launch_bounds__(256, 2) attn_weights_prompt_kernel(const Weigh
     };
     load(t0);
 
-    const TK* kb = reinterpret_cast<const TK*>(p.k) + b * p.k_b + hk * p.k_h;
-    V8 kf[KT][KP][KS];
-    float c[KT][2];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        const TK* krow = kb + (int64_t)min(k0 + 32 * t + col, n - 1) * p.k_s;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int x = 16 * s + 8 * half;
-            if constexpr (sizeof(TK) == 1) {
-                const u32x2 w = x < p.d ? *reinterpret_cast<const u32x2*>(krow + x) : u32x2{0u, 0u};
-                kf[t][0][s] = codes_to_vec8<E>(w.x, w.y);
-            } else {
-                const Chunk<TK> w = load8(krow, x, p.d);
-                V8 o[KP];
-                to_parts<TK, V8, KP>(w, o);
-#pragma unroll
-                for (int i = 0; i < KP; ++i) kf[t][i][s] = o[i];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            c[t][u] = p.c;
-            if constexpr (sizeof(TK) == 1) c[t][u] *= p.ks[b * p.ks_b + hk * p.ks_h + (min(k0 + 32 * t + 16 * u, n - 1) >> p.block_shift)];
-        }
-    }
-
     const V8* get_at[KS];
 #pragma unroll
     for (int x = 0; x < KS; ++x) get_at[x] = &stage[0][0][col * DC + ((2 * x) ^ (half ^ swz(col)))];
-    // every thread is past the zeros of the stage before the first tile is put there
-    lds_barrier();
-    float sum[KT][16] = {};
-    float nl;
-    // Stages tile t and has the next one on its way.  Buffers alternate, and the barrier has every wave past its reads of the other
-    // one's last tile.
-    auto turn = [&](int buf, int t) {
-        put(buf, t);
-        nl = crow < 0 || lse == kNegInf ? kNegInf : -lse * kLog2e;
-        if (t + 1 < t1) load(t + 1);
+    const TK* kb = reinterpret_cast<const TK*>(p.k) + b * p.k_b + hk * p.k_h;
+    int k0 = 0;
+    V8 kf[KT][KP][KS];
+    float c[KT][2];
+    auto load_keys = [&] {
+        k0 = kblock * Types::keys + __builtin_amdgcn_readfirstlane(tid >> 6) * 32 * KT;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            const TK* krow = kb + (int64_t)min(k0 + 32 * t + col, n - 1) * p.k_s;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int x = 16 * s + 8 * half;
+                if constexpr (sizeof(TK) == 1) {
+                    const u32x2 w = x < p.d ? *reinterpret_cast<const u32x2*>(krow + x) : u32x2{0u, 0u};
+                    kf[t][0][s] = codes_to_vec8<E>(w.x, w.y);
+                } else {
+                    const Chunk<TK> w = load8(krow, x, p.d);
+                    V8 o[KP];
+                    to_parts<TK, V8, KP>(w, o);
+#pragma unroll
+                    for (int i = 0; i < KP; ++i) kf[t][i][s] = o[i];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                c[t][u] = p.c;
+                if constexpr (sizeof(TK) == 1) c[t][u] *= p.ks[b * p.ks_b + hk * p.ks_h + (min(k0 + 32 * t + 16 * u, n - 1) >> p.block_shift)];
+            }
+        }
+    };
+    load_keys();
+
+    for (;;) {  // a key block, or what of its tiles is this share's
+        // every thread is past the zeros of the stage, and past the last block's tiles, before the first tile is put there
         lds_barrier();
-    };
-    V8 qf[KS];  // held for the second key tile, but for the three parts of fp32
-    auto queries = [&](int buf) {
-        if constexpr (QP == 1) {
-#pragma unroll
-            for (int x = 0; x < KS; ++x) qf[x] = get_at[x][buf * BUF];
-        }
-    };
-    auto product = [&](int buf, int kt) {
-        f32x16 s = {};
-#pragma unroll
-        for (int x = 0; x < KS; ++x) {
-            V8 q[QP];
-#pragma unroll
-            for (int j = 0; j < QP; ++j) q[j] = QP == 1 ? qf[x] : get_at[x][buf * BUF + j * kCols * DC];
-#pragma unroll
-            for (int i = 0; i < KP; ++i)
-#pragma unroll
-                for (int j = 0; j < QP && i + j < 3; ++j) s = Elem<E>::mfma32(kf[kt][i][x], q[j], s);
-        }
-        return s;
-    };
-    auto fold = [&](const f32x16& s, int kt, float at) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum[kt][i] += fast_exp2(__builtin_fmaf(s[i], c[kt][i >> 3], at));
-    };
-    int t = t0;
-    if constexpr (CAUSAL) {
-        // tiles whose first query does not see the wave's last key (an even number; a wave without keys runs through them all)
-        int64_t border = t1;
-        if (k0 < n) border = max(((int64_t)k0 + 32 * KT - 1 - p.q_offset + p.rows - 1) / p.rows, (int64_t)t0);
-        const int t_full = (int)min(border + ((border - t0) & 1), (int64_t)t1);
-        for (; t < t_full; ++t) {
-            const int buf = (t - t0) & 1;
-            turn(buf, t);
-            // the last of the wave's keys that this column sees
-            int lim = (int)min(max((int64_t)t * p.rows + p.q_offset - k0, (int64_t)-64), (int64_t)(32 * KT)) + max(crow, 0);
-            if (k0 >= n || __ballot(lim >= 0) == 0) continue;
-            lim -= 4 * half;
-            queries(buf);
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const f32x16 s = product(buf, kt);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float x = fast_exp2(__builtin_fmaf(s[i], c[kt][i >> 3], nl));
-                    sum[kt][i] += 32 * kt + 8 * (i >> 2) + (i & 3) <= lim ? x : 0.f;
-                }
-            }
-        }
-    }
-    if (k0 < n) {
-        // scores that wait for their exponentials: the last key tile's of the column tile before
-        f32x16 wait = {};
-        float wait_nl = kNegInf;
-        auto full = [&](auto buffer) {
-            constexpr int buf = decltype(buffer)::value;
-            turn(buf, t++);
-            queries(buf);
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const f32x16 s = product(buf, kt);
-                fold(wait, kt == 0 ? KT - 1 : kt - 1, kt == 0 ? wait_nl : nl);
-                wait = s;
-#pragma unroll
-                for (int i = 0; i < KS; ++i) {  // a step's MFMAs, and a KS-th of the VALU instructions and exponentials
-                    __builtin_amdgcn_sched_group_barrier(0x008, KP * QP == 9 ? 6 : QP, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x002, 32 / KS, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x400, 16 / KS, 0);
-                }
-            }
-            wait_nl = nl;
+        float sum[KT][16] = {};
+        float nl;
+        // Stages tile t and has the next one on its way.  Buffers alternate, and the barrier has every wave past its reads of the other
+        // one's last tile.
+        auto turn = [&](int buf, int t) {
+            put(buf, t);
+            nl = crow < 0 || lse == kNegInf ? kNegInf : -lse * kLog2e;
+            if (t + 1 < t1) load(t + 1);
+            lds_barrier();
         };
-        while (t + 1 < t1) {
-            full(std::integral_constant<int, 0>());
-            // the sums stay under this tile's MFMAs: left alone they sink past the next barrier
+        V8 qf[KS];  // held for the second key tile, but for the three parts of fp32
+        auto queries = [&](int buf) {
+            if constexpr (QP == 1) {
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+                for (int x = 0; x < KS; ++x) qf[x] = get_at[x][buf * BUF];
+            }
+        };
+        auto product = [&](int buf, int kt) {
+            f32x16 s = {};
 #pragma unroll
-                for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(sum[kt][i]));
-            full(std::integral_constant<int, 1>());
+            for (int x = 0; x < KS; ++x) {
+                V8 q[QP];
+#pragma unroll
+                for (int j = 0; j < QP; ++j) q[j] = QP == 1 ? qf[x] : get_at[x][buf * BUF + j * kCols * DC];
+#pragma unroll
+                for (int i = 0; i < KP; ++i)
+#pragma unroll
+                    for (int j = 0; j < QP && i + j < 3; ++j) s = Elem<E>::mfma32(kf[kt][i][x], q[j], s);
+            }
+            return s;
+        };
+        auto fold = [&](const f32x16& s, int kt, float at) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[kt][i] += fast_exp2(__builtin_fmaf(s[i], c[kt][i >> 3], at));
+        };
+        int t = t0;
+        if constexpr (CAUSAL) {
+            // tiles whose first query does not see the wave's last key (an even number; a wave without keys runs through them all)
+            int64_t border = t1;
+            if (k0 < n) border = max(((int64_t)k0 + 32 * KT - 1 - p.q_offset + p.rows - 1) / p.rows, (int64_t)t0);
+            const int t_full = (int)min(border + ((border - t0) & 1), (int64_t)t1);
+            for (; t < t_full; ++t) {
+                const int buf = (t - t0) & 1;
+                turn(buf, t);
+                // the last of the wave's keys that this column sees
+                int lim = (int)min(max((int64_t)t * p.rows + p.q_offset - k0, (int64_t)-64), (int64_t)(32 * KT)) + max(crow, 0);
+                if (k0 >= n || __ballot(lim >= 0) == 0) continue;
+                lim -= 4 * half;
+                queries(buf);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const f32x16 s = product(buf, kt);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = fast_exp2(__builtin_fmaf(s[i], c[kt][i >> 3], nl));
+                        sum[kt][i] += 32 * kt + 8 * (i >> 2) + (i & 3) <= lim ? x : 0.f;
+                    }
+                }
+            }
         }
-        if (t < t1) full(std::integral_constant<int, 0>());
-        fold(wait, KT - 1, wait_nl);
-    } else {
-        for (; t < t1; ++t) turn((t - t0) & 1, t);
-    }
+        if (k0 < n) {
+            // scores that wait for their exponentials: the last key tile's of the column tile before
+            f32x16 wait = {};
+            float wait_nl = kNegInf;
+            auto full = [&](auto buffer) {
+                constexpr int buf = decltype(buffer)::value;
+                turn(buf, t++);
+                queries(buf);
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-        float v = 0.f;
+                for (int kt = 0; kt < KT; ++kt) {
+                    const f32x16 s = product(buf, kt);
+                    fold(wait, kt == 0 ? KT - 1 : kt - 1, kt == 0 ? wait_nl : nl);
+                    wait = s;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float s = group_sum<32>(sum[kt][i]);
-            v = col == i ? s : v;
+                    for (int i = 0; i < KS; ++i) {  // a step's MFMAs, and a KS-th of the VALU instructions and exponentials
+                        __builtin_amdgcn_sched_group_barrier(0x008, KP * QP == 9 ? 6 : QP, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 32 / KS, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x400, 16 / KS, 0);
+                    }
+                }
+                wait_nl = nl;
+            };
+            while (t + 1 < t1) {
+                full(std::integral_constant<int, 0>());
+                // the sums stay under this tile's MFMAs: left alone they sink past the next barrier
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(sum[kt][i]));
+                full(std::integral_constant<int, 1>());
+            }
+            if (t < t1) full(std::integral_constant<int, 0>());
+            fold(wait, KT - 1, wait_nl);
+        } else {
+            for (; t < t1; ++t) turn((t - t0) & 1, t);
         }
-        const int key = k0 + 32 * kt + 8 * (col >> 2) + 4 * half + (col & 3);
-        if (col < 16 && key < n) {
-            if (p.parts == 1) p.w[b * p.w_b + hk * p.w_h + key] += v;
-            else p.part[((int64_t)part * slices + slice) * p.S + key] = v;
+        // the next block's first loads go out before this one's sums meet (its keys' in one part: three would not fit the registers)
+        const int done = kblock, done_k0 = k0;
+        const bool whole = p.sets == 1 && t1 - t0 == tiles.count(kblock);
+        todo -= t1 - t0;
+        if (todo > 0) {
+            t0 = tiles.first(++kblock);
+            // the loads are past t1
+#pragma unroll
+            for (int k = 0; k < PER; ++k) src[k] += (t0 - t1) * step;
+            lse_src += (int64_t)(t0 - t1) * p.rows;
+            t1 = min(t0 + todo, tiles.end);
+            load(t0);
+            if constexpr (QP * KP == 1) load_keys();
         }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            float v = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float s = group_sum<32>(sum[kt][i]);
+                v = col == i ? s : v;
+            }
+            const int at = done_k0 + 32 * kt + 8 * (col >> 2) + 4 * half + (col & 3);
+            if (col < 16 && at < n) {
+                // a block whose tiles are all here is done
+                if (whole) p.w[b * p.w_b + hk * p.w_h + at] += v;
+                else p.part[prompt_record(p, slice, set, share, done) * Types::keys + at - done * Types::keys] = v;
+            }
+        }
+        if (todo == 0) break;
+        if constexpr (QP * KP != 1) load_keys();
     }
 }
 
-// Adds the parts of a key in their order: those whose workgroup had columns.
-template <bool CAUSAL>
-__global__ void __launch_bounds__(256) attn_weights_sum_kernel(const WeightParams p, int keys) {
-    const int key = blockIdx.x * 256 + threadIdx.x;
-    const int slices = p.B * p.Hkv, slice = blockIdx.y;
+// Adds a key block's records in the order of their shares.
+template <bool CAUSAL, int KEYS>
+__global__ void __launch_bounds__(KEYS) attn_weights_sum_kernel(const WeightParams p) {
+    const int slice = blockIdx.y, kblock = blockIdx.x, key = kblock * KEYS + threadIdx.x;
     const int64_t b = slice / p.Hkv;
     const int hk = slice % p.Hkv;
-    const int n = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.S) : p.S;
-    if (key >= n) return;
-    int first, last;
-    prompt_queries<CAUSAL>(p, key / keys * keys, n, first, last);
-    const int parts = prompt_parts(p, first, last);
-    if (parts == 0) return;
+    const PromptTiles<CAUSAL> tiles(p, KEYS, b);
+    int from = 0, to = 0;  // the block's tiles in the list
+    const int all = tiles.scan([&](int k0, int c, int pre) {
+        if (kblock - k0 < 0 || kblock - k0 >= 64) return;
+        to = __builtin_amdgcn_readlane(pre, kblock - k0);
+        from = to - __builtin_amdgcn_readlane(c, kblock - k0);
+    });
+    if (from == to || key >= tiles.n) return;
+    const PromptShares shares(all, p.shares);
+    const int first = shares.of(from), last = shares.of(to - 1);
+    if (p.sets == 1 && first == last) return;  // done already
     float v = 0.f;
-    for (int set = 0; set < p.parts; set += p.row_parts)
-        for (int x = 0; x < parts; ++x) v += p.part[((int64_t)(set + x) * slices + slice) * p.S + key];
+    for (int set = 0; set < p.sets; ++set)
+        for (int share = first; share <= last; ++share) v += p.part[prompt_record(p, slice, set, share, kblock) * KEYS + threadIdx.x];
     p.w[b * p.w_b + hk * p.w_h + key] += v;
 }
 
 namespace {
 
-// Parts that a prompt's columns are cut in, so that the workgroups (two fit a CU) go round a few times.
+// Shares that the tiles of a (sequence, kv head, head set) are cut in.
 struct PromptPlan {
-    int64_t key_blocks, parts, row_parts, part_tiles;
+    int64_t key_blocks, sets, shares, tiles;
     int32_t width, rows;
     size_t bytes;
 };
@@ -580,12 +651,13 @@ struct PromptPlan {
 PromptPlan prompt_plan(const dtattn_weights_args* a, int keys, int cus) {
     PromptPlan r;
     r.key_blocks = (a->S + keys - 1) / keys;
-    const int64_t group = a->Hq / a->Hkv, slices = a->B * a->Hkv, sets = (group + kCols - 1) / kCols;
+    const int64_t group = a->Hq / a->Hkv, slices = a->B * a->Hkv;
+    r.sets = (group + kCols - 1) / kCols;
     // a tile is whole queries (of up to 32 heads each), so that a thread's part of it is the same in every tile
     r.width = (int32_t)std::min<int64_t>(group, kCols);
     r.rows = kCols / r.width;
-    const int64_t tiles = (a->L + r.rows - 1) / r.rows;
-    double work = (double)r.key_blocks * (double)tiles;
+    r.tiles = (a->L + r.rows - 1) / r.rows;
+    double work = (double)r.key_blocks * (double)r.tiles;
     if (a->causal != 0) {  // key block k sees the queries from key k * keys - q_offset on
         work = 0;
         const int64_t step = std::max<int64_t>(1, r.key_blocks / 256);  // sampled
@@ -594,16 +666,20 @@ PromptPlan prompt_plan(const dtattn_weights_args* a, int keys, int cus) {
             work += (double)step * (double)(a->L - from) / r.rows;
         }
     }
-    work *= (double)(slices * sets);
-    // two workgroups fit a CU.  us at 1 / 2 / 3 / 5 rounds of them (bf16 but for the last two): 4x2048 causal 32 heads over 8 127 /
-    // 114 / 114 / 121, not causal 163 / 168 / 171 / 172; 2x2000 causal 20 heads of 64 33 / 37 / 37 / 38; 1x4000 causal 28 over 4, fp16
-    // 133 / 122 / 129 / 147; 1x1500 causal 32 over 8, fp32 96 / 93 / 90 / 91.  Parts of less than 8 tiles cost more to start than
-    // they spread (1x777 causal 32 over 8 at 4 tiles 27, at 8 21).
-    r.part_tiles = std::max<int64_t>(8, (int64_t)(work / (2.0 * cus * 2)) + 1);
-    r.part_tiles = std::min(r.part_tiles, tiles);
-    r.row_parts = (tiles + r.part_tiles - 1) / r.part_tiles;
-    r.parts = r.row_parts * sets;
-    r.bytes = r.parts > 1 ? (((size_t)r.parts * slices * a->S * sizeof(float) + 255) & ~(size_t)255) : 0;
+    // Two workgroups fit a CU, three at head dims up to 64: the shares that fill so many places, one turn or more of them, for the
+    // turns that take the least time (a share starts a key block, or goes on with it, at the price of kStartTiles tiles).  us at 0.8 / 0.9 /
+    // 1 / 1.2 / 2 workgroups per place: 4x2048 causal 32 heads over 8, bf16 132 / 112 / 98 / 119 / 104, not causal 170 / 156 / 138 / 173 /
+    // 140; 1x4000 causal 28 over 4, fp16 112 / 102 / 100 / 118 / 103; 1x1500 causal 32 over 8, fp32 76 / 75 / 72 / 91 / 80; 2x2000 causal 20
+    // of 64 at 0.5 / 0.67 / 1 / 1.1 / 1.3: 45 / 36 / 32 / 37 / 39.  2x777 causal 12 of 64, fp32, shares of 2 / 4 / 8 tiles at least: 22 / 21 / 26.
+    const int64_t items = slices * r.sets, slots = (a->D <= 64 ? 3 : 2) * (int64_t)cus, least = (items + slots - 1) / slots;
+    const int64_t most = std::max<int64_t>(1, (int64_t)(work / kShareTiles));
+    double best = 0;
+    for (int64_t turns = least; turns < least + 3; ++turns) {
+        const int64_t shares = std::min(most, std::max<int64_t>(1, turns * slots / items));
+        const double us = (double)((items * shares + slots - 1) / slots) * (work / shares + kStartTiles * (1. + (double)r.key_blocks / shares));
+        if (turns == least || us < best) best = us, r.shares = shares;
+    }
+    r.bytes = r.shares * r.sets > 1 ? (((size_t)items * (r.shares + r.key_blocks) * keys * sizeof(float) + 255) & ~(size_t)255) : 0;
     return r;
 }
 
@@ -616,17 +692,17 @@ int prompt_keys(const dtattn_weights_args* a) { return a->k_dtype == DTATTN_FP32
 template <typename TQ, typename TK, int D>
 static int launch_prompt(WeightParams p, bool causal, const PromptPlan& plan, hipStream_t stream) {
     const int64_t slices = (int64_t)p.B * p.Hkv;
-    p.parts = (int32_t)plan.parts, p.part_tiles = (int32_t)plan.part_tiles, p.key_blocks = (int32_t)plan.key_blocks;
-    p.row_parts = (int32_t)plan.row_parts, p.width = plan.width, p.rows = plan.rows;
-    const dim3 grid((unsigned)(slices * plan.parts * plan.key_blocks));
+    p.shares = (int32_t)plan.shares, p.sets = (int32_t)plan.sets, p.key_blocks = (int32_t)plan.key_blocks;
+    p.width = plan.width, p.rows = plan.rows;
+    const dim3 grid((unsigned)(slices * plan.sets * plan.shares));
     if (causal) hipLaunchKernelGGL((attn_weights_prompt_kernel<TQ, TK, D, true>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((attn_weights_prompt_kernel<TQ, TK, D, false>), grid, dim3(256), 0, stream, p);
     const int st = check_launch("attn_weights_prompt_kernel");
-    if (st != DTATTN_OK || plan.parts == 1) return st;
-    const dim3 sums((unsigned)((p.S + 255) / 256), (unsigned)slices);
-    const int keys = PromptTypes<TQ, TK>::keys;
-    if (causal) hipLaunchKernelGGL(attn_weights_sum_kernel<true>, sums, dim3(256), 0, stream, p, keys);
-    else hipLaunchKernelGGL(attn_weights_sum_kernel<false>, sums, dim3(256), 0, stream, p, keys);
+    if (st != DTATTN_OK || plan.bytes == 0) return st;
+    constexpr int KEYS = PromptTypes<TQ, TK>::keys;
+    const dim3 sums((unsigned)plan.key_blocks, (unsigned)slices);
+    if (causal) hipLaunchKernelGGL((attn_weights_sum_kernel<true, KEYS>), sums, dim3(KEYS), 0, stream, p);
+    else hipLaunchKernelGGL((attn_weights_sum_kernel<false, KEYS>), sums, dim3(KEYS), 0, stream, p);
     return check_launch("attn_weights_sum_kernel");
 }
 
@@ -721,8 +797,8 @@ extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stre
         const int cus = stream_cus(stream);
         if (cus <= 0) return fail(DTATTN_ERR_DEVICE, "%s: cannot tell the stream's device", who);
         prompt = prompt_plan(a, prompt_keys(a), cus);
-        if (prompt.row_parts * prompt.part_tiles * prompt.rows > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many queries", who);
-        if (prompt.key_blocks * prompt.parts * a->B * a->Hkv > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
+        if (prompt.key_blocks * prompt.tiles > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many queries and keys", who);
+        if (a->B * a->Hkv * prompt.sets * prompt.shares > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
         if (prompt.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < prompt.bytes))
             return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, prompt.bytes, a->workspace_bytes);
         if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(DTATTN_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);

@@ -68,20 +68,6 @@ constexpr int kShareLeast = kWaves8;
 __device__ __forceinline__ int tokens8(const Decode8Params& p, int64_t b) { return min(max(p.lengths[b], 0), p.capacity); }
 __device__ __forceinline__ int units8(const Decode8Params& p, int64_t b) { return (tokens8(p, b) + kUnit8 - 1) / kUnit8; }
 
-// Inclusive prefix sum over the wave's lanes, by DPP: within rows of 16, then the last lanes of rows to those behind.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int scan64(int v) {
-    v = dpp_add<0x111, 0xf>(v);  // row_shr:1
-    v = dpp_add<0x112, 0xf>(v);
-    v = dpp_add<0x114, 0xf>(v);
-    v = dpp_add<0x118, 0xf>(v);
-    v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-    return dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-}
-
 // V units in `n` shares of V / n or one more (all the longer ones first); the host keeps V below 2^31.
 struct Shares8 {
     int n, q, rem;

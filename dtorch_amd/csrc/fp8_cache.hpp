@@ -63,6 +63,20 @@ __device__ __forceinline__ typename Elem<T>::vec8 codes_to_vec8(uint32_t lo, uin
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// Inclusive prefix sum over the wave's lanes, by DPP: within rows of 16, then the last lanes of rows to those behind.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int scan64(int v) {
+    v = dpp_add<0x111, 0xf>(v);  // row_shr:1
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    return dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+}
+
 // The three bf16 parts of an fp32 value: 24 bits of mantissa as 8 + 8 + 8, by truncation, so that their sum is the value (parts
 // below the smallest bf16 normal apart).  A value that is not finite is its first part.
 __device__ __forceinline__ void split3(float x, bf16_t out[3]) {

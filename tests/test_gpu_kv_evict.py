@@ -101,6 +101,15 @@ def test_prompt(dtype, L, S, Hq, Hkv, D, causal, q_offset, lengths):
     _check_weights(rng, 3, Hq, Hkv, L, S, D, dtype, lengths=lengths, causal=causal, q_offset=q_offset)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("L,S,Hq,Hkv,D,causal,q_offset,lengths", [
+    (70, 20000, 2, 1, 64, True, 19930, [20000, 17000, 300]), (66, 9000, 2, 2, 64, False, 0, None), (65, 9000, 1, 1, 128, True, 8000, [9000, 8030, 0]),
+    (30, 2900, 40, 1, 64, True, 2870, [2900, 2875, 100]), (1000, 1500, 2, 2, 16, True, 250, None)])
+def test_prompt_over_many_keys(dtype, L, S, Hq, Hkv, D, causal, q_offset, lengths):
+    """Shares of several key blocks, blocks of several shares, and more blocks than lanes."""
+    _check_weights(np.random.default_rng(S), 3, Hq, Hkv, L, S, D, dtype, lengths=lengths, causal=causal, q_offset=q_offset)
+
+
 def test_prompt_over_codes():
     rng = np.random.default_rng(2)
     for dtype in (torch.bfloat16, torch.float32):
