@@ -12,7 +12,7 @@
 #include <algorithm>
 
 #include "decode_params.hpp"
-#include "dtattn_common.hpp"
+#include "fp8_cache.hpp"
 
 namespace dtattn {
 
@@ -43,17 +43,12 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive prefix sum over the workgroup (kSelect threads), and the total.
+// Exclusive prefix sum over the workgroup (kSelect threads), and the total.  `lds` is not in use before the call or, until every
+// thread is past a barrier, after it.
 __device__ __forceinline__ int scan_all(int v, int* lds, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int s = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(s, d, 64);
-        if (lane >= d) s += o;
-    }
-    __syncthreads();
-    if (lane == 63) lds[wave] = s;
+    const int wave = threadIdx.x >> 6;
+    const int s = scan64(v);
+    if ((threadIdx.x & 63) == 63) lds[wave] = s;
     __syncthreads();
     int before = 0;
     total = 0;
@@ -76,13 +71,13 @@ __device__ __forceinline__ int tokens_of(const EvictParams& p, int64_t b) { retu
 
 }  // namespace
 
-// The candidates' weights: PER per thread in registers (candidate tid + kSelect * k), or PER = 0 in memory.
+// The candidates' weights: PER per thread in registers (candidate PER * tid + k), or PER = 0 in memory.
 template <int PER>
 __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictParams p) {
     constexpr int BINS = 2048;
-    __shared__ int hist[BINS];
-    __shared__ int waves[kSelect / 64];
-    __shared__ int found[2];
+    __shared__ int hist[3][BINS];  // one a round: nothing is cleared between them
+    __shared__ int waves[4][kSelect / 64];
+    __shared__ int found[3][2];
     const int tid = threadIdx.x;
     const int64_t bh = blockIdx.x, b = bh / p.Hkv;
     const int h = (int)(bh % p.Hkv);
@@ -103,77 +98,81 @@ __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictPar
         if (p.block_shift == 0) return ordered(w[i]);
         double s = 0.;
         const float* x = w + ((int64_t)i << p.block_shift);
+#pragma unroll 16
         for (int j = 0; j < (1 << p.block_shift); ++j) s += (double)x[j];
         return ordered((float)s);
     };
     uint32_t mine[PER > 0 ? PER : 1];
     if constexpr (PER > 0) {
 #pragma unroll
-        for (int k = 0; k < PER; ++k) mine[k] = tid + k * kSelect < cand ? weight(tid + k * kSelect) : 0u;
+        for (int k = 0; k < PER; ++k) mine[k] = PER * tid + k < cand ? weight(PER * tid + k) : 0u;
     } else {
         for (int i = tid; i < cand; i += kSelect) order[i] = weight(i);
-        __syncthreads();
     }
-    // f(candidate, its weight) for this thread's candidates
-    auto each = [&](auto f) {
-        if constexpr (PER > 0) {
-#pragma unroll
-            for (int k = 0; k < PER; ++k)
-                if (tid + k * kSelect < cand) f(tid + k * kSelect, mine[k]);
-        } else {
-            for (int i = tid; i < cand; i += kSelect) f(i, order[i]);
-        }
-    };
+    for (int i = tid; i < 3 * BINS; i += kSelect) (&hist[0][0])[i] = 0;
+    __syncthreads();
     // The need-th largest, some bits a round: `prefix` holds the bits found so far, and `need` how many stay of those that share them
     uint32_t prefix = 0, mask = 0;
     if (need > 0) {
+#pragma unroll
         for (int round = 0; round < 3; ++round) {
             const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bins = round < 2 ? 2048 : 1024;
-            for (int i = tid; i < BINS; i += kSelect) hist[i] = 0;
-            __syncthreads();
-            each([&](int, uint32_t u) {
-                if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & (bins - 1)], 1);
-            });
-            __syncthreads();
-            // two bins a thread, from the largest down
-            const int hi = hist[BINS - 1 - 2 * tid], lo = hist[BINS - 2 - 2 * tid];
-            int total;
-            const int before = scan_all(hi + lo, waves, total);
-            if (before < need && before + hi + lo >= need) {
-                const bool upper = before + hi >= need;
-                found[0] = BINS - 1 - 2 * tid - (upper ? 0 : 1);
-                found[1] = need - before - (upper ? 0 : hi);
+            auto count = [&](uint32_t u) {
+                if ((u & mask) == prefix) atomicAdd(&hist[round][(u >> shift) & (bins - 1)], 1);
+            };
+            if constexpr (PER > 0) {
+#pragma unroll
+                for (int k = 0; k < PER; ++k)
+                    if (PER * tid + k < cand) count(mine[k]);
+            } else {
+                for (int i = tid; i < cand; i += kSelect) count(order[i]);
             }
             __syncthreads();
-            prefix |= (uint32_t)found[0] << shift;
-            mask |= (uint32_t)(bins - 1) << shift;
-            need = found[1];
+            // two bins a thread, from the largest down
+            const int hi = hist[round][BINS - 1 - 2 * tid], lo = hist[round][BINS - 2 - 2 * tid];
+            int total;
+            const int before = scan_all(hi + lo, waves[round], total);
+            if (before < need && before + hi + lo >= need) {
+                const bool upper = before + hi >= need;
+                found[round][0] = BINS - 1 - 2 * tid - (upper ? 0 : 1);
+                found[round][1] = need - before - (upper ? 0 : hi);
+            }
             __syncthreads();
+            prefix |= (uint32_t)found[round][0] << shift;
+            mask |= (uint32_t)(bins - 1) << shift;
+            need = found[round][1];
         }
     } else {
         prefix = 0xffffffffu;  // above every weight
     }
-    // those above stay, and the first `need` of those at it: one row of kSelect candidates after another
-    int out = 0, seen = 0;  // kept, and met at the prefix, in the rows before
-    const int rows = (cand + kSelect - 1) / kSelect;
-    auto row = [&](int k, uint32_t u) {
-        const int i = tid + k * kSelect;
-        const bool above = i < cand && u > prefix, at = i < cand && u == prefix;
-        int total;
-        const int before = scan_all(((int)above << 16) + (int)at, waves, total);
-        const int at_before = seen + (before & 0xffff);
-        // of those before me in this row: all above, and those at it that stay
-        const int stay_at = min(max(need - seen, 0), before & 0xffff);
-        if (above || (at && at_before < need)) kept[out + (before >> 16) + stay_at] = i;
-        out += (total >> 16) + min(max(need - seen, 0), total & 0xffff);
-        seen += total & 0xffff;
-    };
+    // those above stay, and the first `need` of those at it
     if constexpr (PER > 0) {
+        int counts = 0;  // above << 16, and at it: up to 16384 of both
 #pragma unroll
         for (int k = 0; k < PER; ++k)
-            if (k < rows) row(k, mine[k]);
+            if (PER * tid + k < cand) counts += mine[k] > prefix ? 1 << 16 : mine[k] == prefix ? 1 : 0;
+        int total;
+        const int before = scan_all(counts, waves[3], total);
+        int above = before >> 16, at = before & 0xffff;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (PER * tid + k < cand) {
+                const bool over = mine[k] > prefix, same = mine[k] == prefix;
+                if (over || (same && at < need)) kept[above + min(at, need)] = PER * tid + k;
+                above += over, at += same;
+            }
     } else {
-        for (int k = 0; k < rows; ++k) row(k, tid + k * kSelect < cand ? order[tid + k * kSelect] : 0u);
+        int above = 0, at = 0;  // of the candidates before: one row of kSelect after another
+        for (int i0 = 0; i0 < cand; i0 += kSelect) {
+            const uint32_t u = i0 + tid < cand ? order[i0 + tid] : 0u;
+            const bool over = i0 + tid < cand && u > prefix, same = i0 + tid < cand && u == prefix;
+            int total;
+            const int before = scan_all(((int)over << 16) + (int)same, waves[3], total);
+            const int mine_at = at + (before & 0xffff);
+            if (over || (same && mine_at < need)) kept[above + (before >> 16) + min(mine_at, need)] = i0 + tid;
+            above += total >> 16, at += total & 0xffff;
+            __syncthreads();
+        }
     }
     for (int i = tid; i < p.recent; i += kSelect) kept[p.keep - p.recent + i] = cand + i;
 }
@@ -352,7 +351,9 @@ extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     p.blocks_max = (int32_t)((a->S_max + a->block - 1) / a->block);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const unsigned heads = (unsigned)(a->B * a->Hkv);
-    if (p.blocks_max <= 4 * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<4>, dim3(heads), dim3(kSelect), 0, stream, p);
+    // (8192 tokens in blocks of 32, 16 of 8 heads: four candidates a thread 16.8 us, one 5.8)
+    if (p.blocks_max <= kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<1>, dim3(heads), dim3(kSelect), 0, stream, p);
+    else if (p.blocks_max <= 4 * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<4>, dim3(heads), dim3(kSelect), 0, stream, p);
     else if (p.blocks_max <= kHeldRows * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<kHeldRows>, dim3(heads), dim3(kSelect), 0, stream, p);
     else hipLaunchKernelGGL(kv_evict_select_kernel<0>, dim3(heads), dim3(kSelect), 0, stream, p);
     int st = check_launch("kv_evict_select_kernel");
