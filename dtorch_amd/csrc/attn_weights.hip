@@ -8,7 +8,7 @@
 // fma and an add per (query, key) pair beside its MFMAs (16 MFMAs, 512 cycles, against 32 exponentials and 64 others, about
 // 512).  Both keep a wave's keys in registers as MFMA operands and pass the queries by, so that the sum over queries stays in
 // registers too and no two waves add to one weight: the result does not depend on timing.  Measured: 16 sequences of 700 to
-// 8191, 28 heads over 4 of 128, codes, one query 14 us; 4x2048 causal bf16, 32 heads over 8 of 128, 98 us, not causal 138 us
+// 8191, 28 heads over 4 of 128, codes, one query 13 us (a decode step has just read these keys: loads that bypass the caches take 14); 4x2048 causal bf16, 32 heads over 8 of 128, 98 us, not causal 138 us
 // (990 TFLOP/s).
 #include <algorithm>
 #include <type_traits>
@@ -65,7 +65,7 @@ struct Operands {
 #pragma unroll
         for (int i = 0; i < loads; ++i) {
             const int x = dim(g4, codes ? 2 * i : i);
-            f.v[i] = ld16_nt(x < d ? row + x : reinterpret_cast<const TK*>(kZeros));
+            f.v[i] = ld16(x < d ? row + x : reinterpret_cast<const TK*>(kZeros));
         }
     }
     // none: a query of zeros
@@ -115,7 +115,7 @@ struct Operands<float, float, D> {
     static __device__ __forceinline__ void keys(Keys& f, const float* row, int g4, int d) {
 #pragma unroll
         for (int s = 0; s < steps; ++s)
-            f.v[s] = __builtin_bit_cast(f32x4, ld16_nt(16 * s + 4 * g4 < d ? row + 16 * s + 4 * g4 : reinterpret_cast<const float*>(kZeros)));
+            f.v[s] = __builtin_bit_cast(f32x4, ld16(16 * s + 4 * g4 < d ? row + 16 * s + 4 * g4 : reinterpret_cast<const float*>(kZeros)));
     }
     static __device__ __forceinline__ void queries(Queries& f, const float* row, int g4, int d, bool none) {
         u32x4 w[steps];
@@ -707,7 +707,7 @@ static int launch_prompt(WeightParams p, bool causal, const PromptPlan& plan, hi
 }
 
 // per_cu: workgroups wanted per CU.  One set of columns: chunks of 32 keys; more sets load the queries again for each chunk, and take
-// 64.  us at 32 keys and 6 workgroups / 64 and 4: 16 of 700 to 8191, 28 heads over 4 (codes) 13.9 / 16.1, 16x8191 bf16 32 over 8 55 / 56,
+// 64.  us (of loads that bypass the caches) at 32 keys and 6 workgroups / 64 and 4: 16 of 700 to 8191, 28 heads over 4 (codes) 13.9 / 16.1, 16x8191 bf16 32 over 8 55 / 56,
 // 8 of 4000 to 8191 fp32 58 / 74; 8 of 20000 to 32768, 64 heads over 1 (codes) 32 / 25.
 template <typename TQ, typename TK, int D, int TILES>
 static int launch_few(const WeightParams& p, bool causal, int per_cu, hipStream_t stream) {
