@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) attn_weights_prompt_kern
 // Adds a key block's records in the order of their shares.
 template <bool CAUSAL, int KEYS>
 __global__ void __launch_bounds__(KEYS) attn_weights_sum_kernel(const WeightParams p) {
-    const int slice = blockIdx.y, kblock = blockIdx.x, key = kblock * KEYS + threadIdx.x;
+    const int slices = p.B * p.Hkv, slice = blockIdx.x % slices, kblock = blockIdx.x / slices, key = kblock * KEYS + threadIdx.x;
     const int64_t b = slice / p.Hkv;
     const int hk = slice % p.Hkv;
     const PromptTiles<CAUSAL> tiles(p, KEYS, b);
@@ -700,7 +700,7 @@ static int launch_prompt(WeightParams p, bool causal, const PromptPlan& plan, hi
     const int st = check_launch("attn_weights_prompt_kernel");
     if (st != DTATTN_OK || plan.bytes == 0) return st;
     constexpr int KEYS = PromptTypes<TQ, TK>::keys;
-    const dim3 sums((unsigned)plan.key_blocks, (unsigned)slices);
+    const dim3 sums((unsigned)(plan.key_blocks * slices));
     if (causal) hipLaunchKernelGGL((attn_weights_sum_kernel<true, KEYS>), sums, dim3(KEYS), 0, stream, p);
     else hipLaunchKernelGGL((attn_weights_sum_kernel<false, KEYS>), sums, dim3(KEYS), 0, stream, p);
     return check_launch("attn_weights_sum_kernel");
@@ -755,7 +755,7 @@ extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stre
     const int64_t qe = a->q_dtype == DTATTN_FP32 ? 4 : 2, ke = codes ? 1 : qe;
     if (a->D > 128 || (a->D * ke) % 16 != 0)
         return fail(DTATTN_ERR_UNSUPPORTED, "%s: head dim %lld not supported (rows of a multiple of 16 bytes, up to 128)", who, (long long)a->D);
-    if (a->S > (1 << 29) || a->L > (1 << 29) || a->B > 65535 || a->Hkv > 65535 || a->B * a->Hkv > 65535)
+    if (a->S > (1 << 29) || a->L > (1 << 29) || a->B > 65535 || a->Hkv > 65535 || a->B * a->Hkv > 0x7fffffff)
         return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
     const int64_t most = (int64_t)1 << 40;
     if (a->q_offset > most || a->q_offset < -most) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: q_offset out of range", who);
@@ -798,7 +798,7 @@ extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stre
         if (cus <= 0) return fail(DTATTN_ERR_DEVICE, "%s: cannot tell the stream's device", who);
         prompt = prompt_plan(a, prompt_keys(a), cus);
         if (prompt.key_blocks * prompt.tiles > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many queries and keys", who);
-        if (a->B * a->Hkv * prompt.sets * prompt.shares > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
+        if (a->B * a->Hkv * prompt.sets * prompt.shares > 0x7fffffff || a->B * a->Hkv * prompt.key_blocks > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
         if (prompt.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < prompt.bytes))
             return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, prompt.bytes, a->workspace_bytes);
         if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(DTATTN_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);

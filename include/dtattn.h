@@ -299,7 +299,8 @@ int dtattn_kv_append_paged(const dtattn_kv_append_paged_args* args, void* stream
  * k_scale[b, h, i]; S_max is a multiple of `block`.  In a paged cache a page holds page_size / block whole
  * blocks and the scale of the block that row r of a page lies in is k_scale[page, h, r / block].  Scales
  * have a stride of 1 between the blocks of a head.  Head dims D: multiples of 16 up to 128; code strides
- * are multiples of 16 bytes, a row stride is at least D, and code pointers are 16-byte aligned.
+ * are multiples of 16 bytes, a row stride is at least D, and code pointers are 16-byte aligned.  Lengths and
+ * block tables do not change while a call that reads them runs.
  */
 
 /* Quantised append: the new tokens' keys and values as codes into the cache.

@@ -489,3 +489,20 @@ def test_empty_shapes(dtype):
     w = torch.ones(2, 2, 64, device="cuda")
     F.attention_weight_accumulate(w, z(2, 4, 0, 64), z(2, 2, 64, 64), z(2, 4, 0, dtype=torch.float32))
     assert (w == 1).all()
+
+
+def test_weights_of_more_slices_than_a_grid_axis():
+    """65920 (sequence, kv head) pairs of 33 heads each: one query, and two as a prompt of two head sets whose sums meet."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    B, Hkv, group, S, D = 1030, 64, 33, 16, 8
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()
+    k = r(B, Hkv, S, D)
+    for L in (1, 2):
+        q = r(B, Hkv * group, L, D)
+        s = (q.float().view(B, Hkv, group * L, D) @ k.float().transpose(2, 3).contiguous()) * D ** -0.5
+        lse = torch.logsumexp(s, -1).view(B, Hkv * group, L)
+        w = torch.zeros(B, Hkv, S, device="cuda")
+        _F().attention_weight_accumulate(w, q, k, lse)
+        want = torch.softmax(s.double(), -1).sum(2)
+        # scores and lse below 32 in fp32 on both sides, and sums of 66 terms
+        assert ((w.double() - want).abs() <= want * (2 * (2 * D + 8) * 32 + 8 * 32 + 2 * 66 + 32) * E).all()
