@@ -8,8 +8,8 @@
 // fma and an add per (query, key) pair beside its MFMAs (16 MFMAs, 512 cycles, against 32 exponentials and 64 others, about
 // 512).  Both keep a wave's keys in registers as MFMA operands and pass the queries by, so that the sum over queries stays in
 // registers too and no two waves add to one weight: the result does not depend on timing.  Measured: 16 sequences of 700 to
-// 8191, 28 heads over 4 of 128, codes, one query 13 us (a decode step has just read these keys: loads that bypass the caches take 14); 4x2048 causal bf16, 32 heads over 8 of 128, 98 us, not causal 138 us
-// (990 TFLOP/s).
+// 8191, 28 heads over 4 of 128, codes, one query 11.6 us (through the caches, which a decode step has just filled; loads that
+// bypass them take 13.4); 4x2048 causal bf16, 32 heads over 8 of 128, 98 us, not causal 138 us (990 TFLOP/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -667,10 +667,11 @@ PromptPlan prompt_plan(const dtattn_weights_args* a, int keys, int cus) {
         }
     }
     // Two workgroups fit a CU, three at head dims up to 64: the shares that fill so many places, one turn or more of them, for the
-    // turns that take the least time (a share starts a key block, or goes on with it, at the price of kStartTiles tiles).  us at 0.8 / 0.9 /
-    // 1 / 1.2 / 2 workgroups per place: 4x2048 causal 32 heads over 8, bf16 132 / 112 / 98 / 119 / 104, not causal 170 / 156 / 138 / 173 /
-    // 140; 1x4000 causal 28 over 4, fp16 112 / 102 / 100 / 118 / 103; 1x1500 causal 32 over 8, fp32 76 / 75 / 72 / 91 / 80; 2x2000 causal 20
-    // of 64 at 0.5 / 0.67 / 1 / 1.1 / 1.3: 45 / 36 / 32 / 37 / 39.  2x777 causal 12 of 64, fp32, shares of 2 / 4 / 8 tiles at least: 22 / 21 / 26.
+    // turns that take the least time (a share starts a key block, or goes on with it, at the price of kStartTiles tiles).  us
+    // at 0.8 / 0.9 / 1 / 1.2 / 2 workgroups per place: 4x2048 causal 32 heads over 8, bf16 132 / 112 / 98 / 119 / 104, not causal
+    // 170 / 156 / 138 / 173 / 140; 1x4000 causal 28 over 4, fp16 112 / 102 / 100 / 118 / 103; 1x1500 causal 32 over 8, fp32
+    // 76 / 75 / 72 / 91 / 80; 2x2000 causal 20 of 64 at 0.5 / 0.67 / 1 / 1.1 / 1.3: 45 / 36 / 32 / 37 / 39.  2x777 causal 12 of 64,
+    // fp32, shares of 2 / 4 / 8 tiles at least: 22 / 21 / 26.
     const int64_t items = slices * r.sets, slots = (a->D <= 64 ? 3 : 2) * (int64_t)cus, least = (items + slots - 1) / slots;
     const int64_t most = std::max<int64_t>(1, (int64_t)(work / kShareTiles));
     double best = 0;

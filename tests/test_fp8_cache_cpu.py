@@ -2,6 +2,7 @@
 parameters keep through serialisation.  Every pointer here is made up: a call that is not refused is an empty one."""
 import ctypes
 import pickle
+import struct
 
 import numpy as np
 import pytest
@@ -181,6 +182,20 @@ def test_params_round_trip():
     p = pickle.loads(pickle.dumps(host.KvCacheEvictParam(1 << 33, 64, 16)))
     assert (p.keep, p.recent, p.block) == (1 << 33, 64, 16)
     assert host.SdpaDecodeFp8Op(0.5).param.scale == 0.5 and host.SdpaDecodeFp8Op().param.scale is None
+
+
+def test_param_bytes():
+    """The fields in their order: little-endian scalars, a presence byte before the optional scale."""
+    host = _lib.load()
+    cases = [(host.KvCacheAppendFp8Param(), b""), (host.KvCacheAppendFp8PagedParam(), b""),
+             (host.SdpaDecodeFp8Param(0.5), struct.pack("<Bd", 1, 0.5)), (host.SdpaDecodeFp8PagedParam(None), struct.pack("<B", 0)),
+             (host.AttentionWeightsParam(0.25, True, -3), struct.pack("<BdBq", 1, 0.25, 1, -3)),
+             (host.KvCacheEvictParam(64, 16, 8), struct.pack("<qqq", 64, 16, 8))]
+    for p, want in cases:
+        assert p.to_bytes() == want, type(p)
+        assert type(p).from_bytes(want).to_bytes() == want and type(pickle.loads(pickle.dumps(p))) is type(p)
+        with pytest.raises(ValueError, match="trailing"):
+            type(p).from_bytes(want + b"x")
 
 
 def test_host_operators_need_the_device():
