@@ -213,7 +213,7 @@ def _tolerances(c, o, a, mag, ln):
     u = U[dtype]
     to = a * (rel + (u if terms == 1 else 0))[..., None] + np.abs(o) * u + np.finfo(np.float32).tiny
     if dtype == torch.float16:
-        to = to + 2.0 ** -25 + (n * 2.0 ** -40)[..., None] * np.nanmax(np.abs(orc.values(c["v"], c["vs"])))
+        to = to + 2.0 ** -25 + (n * 2.0 ** -40)[..., None] * np.nanmax(np.abs(orc.values(c["v"], c["vs"])), initial=0)
     return to, ds + (n + 64) * E + 8 * E * np.abs(np.where(np.isfinite(ln), ln, 0))
 
 
