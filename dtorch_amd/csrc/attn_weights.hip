@@ -238,8 +238,11 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(const WeightParams p)
 namespace {
 
 constexpr int kCols = 32;       // columns of a tile: 32x32 products
-constexpr int kShareTiles = 4;  // column tiles that a share has at least
-constexpr int kStartTiles = 4;  // column tiles whose time it takes to start a key block
+// Column tiles whose time it takes to start a key block, and places that a share has at least.  us at 0 and 4 / 4 and 4 / 4 and 8 /
+// 6 and 6 (causal): 4x2048 32 heads over 8, bf16 103 / 100 / 104 / 101; 1x1500 the same, fp32 71 / 67 / 67 / 69; 2x777 12 of 64, fp32
+// 21 / 20 / 22 / 20; 1x777 32 over 8, bf16 22 / 20 / 20 / 21; 1x1200 8 heads, fp32 31 / 26 / 28 / 30; not causal 4x2048 141 / 144 / 145 / 146.
+constexpr int kStartTiles = 4;
+constexpr int kShareTiles = 4;
 
 // 16-bit and 8-bit keys are one operand; fp32 ones are three bf16 parts (8 bits each, exact), of whose nine products with the
 // query's parts the six largest count: what is left out is below 2^-23 of |q| |k|, an fp32 sum's own rounding.
@@ -254,7 +257,8 @@ struct PromptTypes {
 };
 
 // The column tiles that the key blocks of a sequence meet, one block after another: block k meets those from first(k) to end.  Their
-// list is cut in equal shares, one per workgroup, so that all run for the same time however a causal mask cuts the blocks.
+// list, with kStartTiles places before each block's tiles for the time that the block's start takes, is cut in equal shares, one
+// per workgroup, so that all run for the same time however a causal mask cuts the blocks.
 template <bool CAUSAL>
 struct PromptTiles {
     const WeightParams& p;
@@ -271,13 +275,14 @@ struct PromptTiles {
         return query >= last ? end : (int)max(query, (int64_t)0) / p.rows;
     }
     __device__ __forceinline__ int count(int k) const { return (int64_t)k * keys < n ? end - first(k) : 0; }
-    // f(k0, c, pre) for 64 blocks at a time: lane's block k0 + lane meets c tiles, and those up to it pre
+    // f(k0, c, pre) for 64 blocks at a time: lane's block k0 + lane has c places in the list, and those up to it pre
     template <typename F>
     __device__ __forceinline__ int scan(F f) const {
         const int lane = threadIdx.x & 63;
         int total = 0;
         for (int k0 = 0; k0 < p.key_blocks; k0 += 64) {
-            const int c = k0 + lane < p.key_blocks ? count(k0 + lane) : 0;
+            int c = k0 + lane < p.key_blocks ? count(k0 + lane) : 0;
+            if (c > 0) c += kStartTiles;
             const int pre = scan64(c) + total;
             f(k0, c, pre);
             total = __builtin_amdgcn_readlane(pre, 63);
@@ -291,7 +296,7 @@ __device__ __forceinline__ int64_t prompt_record(const WeightParams& p, int slic
     return ((int64_t)slice * p.sets + set) * (p.shares + p.key_blocks) + share + kblock;
 }
 
-// V tiles in up to `most` shares of V / n or one more, of kShareTiles at least.
+// V places in up to `most` shares of V / n or one more, of kShareTiles at least.
 struct PromptShares {
     int n, q, rem;
     __device__ __forceinline__ PromptShares(int V, int most) {
@@ -366,19 +371,21 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) attn_weights_prompt_kern
     if (all == 0) return;
     const PromptShares shares(all, p.shares);
     if (share >= shares.n) return;
-    int todo = shares.start(share + 1) - shares.start(share);
-    int kblock = 0, t0 = shares.start(share);  // the first tile: so far counted in the list
-    auto find = [&](int k0, int c, int pre) {
-        const uint64_t hit = __ballot(pre > shares.start(share) && pre - c <= shares.start(share));
+    const int begin = shares.start(share);
+    // the block there, its tiles before the share, and the share's places from the block's first place on
+    int kblock = 0, skip = 0, ahead = shares.start(share + 1);
+    auto look = [&](int k0, int c, int pre) {
+        const uint64_t hit = __ballot(pre > begin && pre - c <= begin);
         if (hit == 0) return;
-        const int l = __builtin_ctzll(hit);
+        const int l = __builtin_ctzll(hit), place = __builtin_amdgcn_readlane(pre - c, l);
         kblock = k0 + l;
-        t0 -= __builtin_amdgcn_readlane(pre - c, l);
+        skip = max(begin - place - kStartTiles, 0);
+        ahead -= place;
     };
-    if (p.key_blocks <= 64) find(0, c0, pre0);
-    else tiles.scan(find);
-    t0 += tiles.first(kblock);
-    int t1 = min(t0 + todo, tiles.end);
+    if (p.key_blocks <= 64) look(0, c0, pre0);
+    else tiles.scan(look);
+    int t0 = tiles.first(kblock) + skip, t1 = min(tiles.first(kblock) + ahead - kStartTiles, tiles.end);
+    if (t0 >= t1) return;  // the share ends before the block's first tile
 
     // What a thread stages of a tile: chunk x0 of columns r0, r0 + ROWS, ..., query-major (query column / width, head column % width).
     // Chunk x of column r lies at x ^ swz(r): 16 columns read one chunk each without a conflict.  Chunks past the head dim are zeros
@@ -585,14 +592,14 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) attn_weights_prompt_kern
         // the next block's first loads go out before this one's sums meet (its keys' in one part: three would not fit the registers)
         const int done = kblock, done_k0 = k0;
         const bool whole = p.sets == 1 && t1 - t0 == tiles.count(kblock);
-        todo -= t1 - t0;
-        if (todo > 0) {
+        ahead -= kStartTiles + tiles.count(kblock);
+        if (ahead > kStartTiles) {
             t0 = tiles.first(++kblock);
             // the loads are past t1
 #pragma unroll
             for (int k = 0; k < PER; ++k) src[k] += (t0 - t1) * step;
             lse_src += (int64_t)(t0 - t1) * p.rows;
-            t1 = min(t0 + todo, tiles.end);
+            t1 = min(t0 + ahead - kStartTiles, tiles.end);
             load(t0);
             if constexpr (QP * KP == 1) load_keys();
         }
@@ -611,7 +618,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) attn_weights_prompt_kern
                 else p.part[prompt_record(p, slice, set, share, done) * Types::keys + at - done * Types::keys] = v;
             }
         }
-        if (todo == 0) break;
+        if (done == kblock) break;
         if constexpr (QP * KP != 1) load_keys();
     }
 }
@@ -632,10 +639,16 @@ __global__ void __launch_bounds__(KEYS) attn_weights_sum_kernel(const WeightPara
     if (from == to || key >= tiles.n) return;
     const PromptShares shares(all, p.shares);
     const int first = shares.of(from), last = shares.of(to - 1);
-    if (p.sets == 1 && first == last) return;  // done already
+    // a share with tiles of the block has a record of it, but for one that has them all, which is done already
+    const int count = to - from - kStartTiles;
+    auto tile = [&](int x) { return min(max(x - from - kStartTiles, 0), count); };
     float v = 0.f;
-    for (int set = 0; set < p.sets; ++set)
-        for (int share = first; share <= last; ++share) v += p.part[prompt_record(p, slice, set, share, kblock) * KEYS + threadIdx.x];
+    for (int share = first; share <= last; ++share) {
+        const int a = tile(shares.start(share)), b = tile(shares.start(share + 1));
+        if (p.sets == 1 && a == 0 && b == count) return;
+        if (a < b)
+            for (int set = 0; set < p.sets; ++set) v += p.part[prompt_record(p, slice, set, share, kblock) * KEYS + threadIdx.x];
+    }
     p.w[b * p.w_b + hk * p.w_h + key] += v;
 }
 
@@ -666,18 +679,18 @@ PromptPlan prompt_plan(const dtattn_weights_args* a, int keys, int cus) {
             work += (double)step * (double)(a->L - from) / r.rows;
         }
     }
+    work += (double)r.key_blocks * kStartTiles;
     // Two workgroups fit a CU, three at head dims up to 64: the shares that fill so many places, one turn or more of them, for the
-    // turns that take the least time (a share starts a key block, or goes on with it, at the price of kStartTiles tiles).  us
-    // at 0.8 / 0.9 / 1 / 1.2 / 2 workgroups per place: 4x2048 causal 32 heads over 8, bf16 132 / 112 / 98 / 119 / 104, not causal
+    // turns that take the least time (with the price of a start for every share).  us, without places for starts, at
+    // 0.8 / 0.9 / 1 / 1.2 / 2 workgroups per place: 4x2048 causal 32 heads over 8, bf16 132 / 112 / 98 / 119 / 104, not causal
     // 170 / 156 / 138 / 173 / 140; 1x4000 causal 28 over 4, fp16 112 / 102 / 100 / 118 / 103; 1x1500 causal 32 over 8, fp32
-    // 76 / 75 / 72 / 91 / 80; 2x2000 causal 20 of 64 at 0.5 / 0.67 / 1 / 1.1 / 1.3: 45 / 36 / 32 / 37 / 39.  2x777 causal 12 of 64,
-    // fp32, shares of 2 / 4 / 8 tiles at least: 22 / 21 / 26.
+    // 76 / 75 / 72 / 91 / 80; 2x2000 causal 20 of 64 at 0.5 / 0.67 / 1 / 1.1 / 1.3: 45 / 36 / 32 / 37 / 39.
     const int64_t items = slices * r.sets, slots = (a->D <= 64 ? 3 : 2) * (int64_t)cus, least = (items + slots - 1) / slots;
     const int64_t most = std::max<int64_t>(1, (int64_t)(work / kShareTiles));
     double best = 0;
     for (int64_t turns = least; turns < least + 3; ++turns) {
         const int64_t shares = std::min(most, std::max<int64_t>(1, turns * slots / items));
-        const double us = (double)((items * shares + slots - 1) / slots) * (work / shares + kStartTiles * (1. + (double)r.key_blocks / shares));
+        const double us = (double)((items * shares + slots - 1) / slots) * (work / shares + kStartTiles);
         if (turns == least || us < best) best = us, r.shares = shares;
     }
     r.bytes = r.shares * r.sets > 1 ? (((size_t)items * (r.shares + r.key_blocks) * keys * sizeof(float) + 255) & ~(size_t)255) : 0;
@@ -798,7 +811,7 @@ extern "C" int dtattn_attention_weights(const dtattn_weights_args* a, void* stre
         const int cus = stream_cus(stream);
         if (cus <= 0) return fail(DTATTN_ERR_DEVICE, "%s: cannot tell the stream's device", who);
         prompt = prompt_plan(a, prompt_keys(a), cus);
-        if (prompt.key_blocks * prompt.tiles > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many queries and keys", who);
+        if (prompt.key_blocks * (prompt.tiles + kStartTiles) > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many queries and keys", who);
         if (a->B * a->Hkv * prompt.sets * prompt.shares > 0x7fffffff || a->B * a->Hkv * prompt.key_blocks > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
         if (prompt.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < prompt.bytes))
             return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, prompt.bytes, a->workspace_bytes);
