@@ -233,9 +233,10 @@ __global__ void __launch_bounds__(256) kv_lengths_fp8_kernel(int32_t* lengths, i
 template <typename T, bool PAGED>
 static int launch_append8(const Append8Params& p, int64_t B, hipStream_t stream) {
     const int64_t per_seq = p.items / B;
-    // rows that a wave holds: 16 of 128
+    // One launch for few items of few rows (a wave holds 16 rows of 128): us with 16 / 32 / 64 / 128 items a sequence against two
+    // launches 6.0 and 8.8 / 7.8 and 9.1 / 11.5 and 9.0 / 19.3 and 9.5 (1 token, 64 to 16 sequences of 8 to 64 heads).
     const int held = kHeld * (64 / p.cpr);
-    if (p.n_new > 0 && per_seq <= 64 && p.n_new <= held && B <= 0x7fffffff) {
+    if (p.n_new > 0 && per_seq <= 32 && p.n_new <= held && B <= 0x7fffffff) {
         const unsigned waves = (unsigned)(per_seq < 16 ? per_seq : 16);
         hipLaunchKernelGGL((kv_append_fp8_step_kernel<T, PAGED>), dim3((unsigned)B), dim3(64 * waves), 0, stream, p);
         return check_launch("kv_append_fp8_step_kernel");

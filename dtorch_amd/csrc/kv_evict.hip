@@ -4,7 +4,7 @@
 //
 // kv_evict_select_kernel: one workgroup per (sequence, kv head) finds the weight of the last block that stays by a radix
 // select over the blocks' weights (as unsigned numbers in their order; 11, 11 and 10 bits a round), takes of the blocks at that
-// weight the first ones, and writes the list of blocks that stay, in order.  Up to 16384 candidates are held in registers.
+// weight the first ones, and writes the list of blocks that stay, in order.  Up to 4096 candidates are held in registers.
 // kv_evict_move_kernel: moves rows to the front in place.  Row i of the result comes from a row at or past i, so a tile
 // of rows may be written as soon as the tile itself has been read: what a write covers belongs to rows already read.  A workgroup
 // has the next tile's loads in flight while it writes one, and that tile's list entries before them.  Few heads share a row's chunks
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictPar
     }
     // those above stay, and the first `need` of those at it
     if constexpr (PER > 0) {
-        int counts = 0;  // above << 16, and at it: up to 16384 of both
+        int counts = 0;  // above << 16, and at it: up to 4096 of both
 #pragma unroll
         for (int k = 0; k < PER; ++k)
             if (PER * tid + k < cand) counts += mine[k] > prefix ? 1 << 16 : mine[k] == prefix ? 1 : 0;
@@ -277,7 +277,7 @@ struct EvictSpace {
     size_t plan, order;  // bytes
 };
 
-constexpr int kHeldRows = 16;  // candidates a thread holds
+constexpr int kHeldRows = 4;  // candidates a thread holds
 
 static EvictSpace evict_workspace(const dtattn_kv_evict_args* a) {
     const int64_t blocks = (a->S_max + a->block - 1) / a->block;
@@ -351,17 +351,20 @@ extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     p.blocks_max = (int32_t)((a->S_max + a->block - 1) / a->block);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const unsigned heads = (unsigned)(a->B * a->Hkv);
-    // (8192 tokens in blocks of 32, 16 of 8 heads: four candidates a thread 16.8 us, one 5.8)
+    // Candidates in registers, as few a thread as hold them, or in memory.  us of the launch, 64 heads of 4096 tokens: four a thread
+    // 7.2, in memory 10.8; 128 of 256 blocks of 32: one 5.8, four 16.8, in memory 6.8; the whole call, 8 heads of 16384:
+    // sixteen 24.4, in memory 21.6.
     if (p.blocks_max <= kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<1>, dim3(heads), dim3(kSelect), 0, stream, p);
-    else if (p.blocks_max <= 4 * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<4>, dim3(heads), dim3(kSelect), 0, stream, p);
     else if (p.blocks_max <= kHeldRows * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<kHeldRows>, dim3(heads), dim3(kSelect), 0, stream, p);
     else hipLaunchKernelGGL(kv_evict_select_kernel<0>, dim3(heads), dim3(kSelect), 0, stream, p);
     int st = check_launch("kv_evict_select_kernel");
     if (st != DTATTN_OK) return st;
-    // a row's chunks are shared until there is a workgroup for every CU, or one per chunk
-    const int cus = stream_cus(stream);
+    // A row's chunks are shared until three CUs in four have a workgroup, or each chunk has one.  us at a workgroup for no CU / half
+    // of them / three in four / all / all twice, heads of 128 bf16, 8192 -> 4096 tokens: 1 sequence of 8 heads 45 / 29 / 33 / 33 / 34,
+    // 3 61 / 44 / 44 / 49 / 62, 6 68 / 52 / 52 / 69 / 80, 8 72 / 72 / 64 / 63 / 81, 12 81 / 81 / 81 / 83 / 109.
+    const int wanted = std::max(stream_cus(stream) * 3 / 4, 1);
     p.width = p.chunks;
-    while (p.width > 1 && 2 * (int64_t)heads * ((p.chunks + p.width - 1) / p.width) < cus) p.width = (p.width + 1) / 2;
+    while (p.width > 1 && 2 * (int64_t)heads * ((p.chunks + p.width - 1) / p.width) < wanted) p.width = (p.width + 1) / 2;
     p.width = std::min(p.width, 1024);
     p.groups = (p.chunks + p.width - 1) / p.width;
     const int64_t lots = (2 * (int64_t)heads + 7) / 8;
