@@ -640,16 +640,14 @@ __global__ void __launch_bounds__(KEYS) attn_weights_sum_kernel(const WeightPara
     });
     if (from == to || key >= tiles.n) return;
     const PromptShares shares(all, p.shares);
-    const int first = shares.of(from), last = shares.of(to - 1);
-    // a share with tiles of the block has a record of it, but for one that has them all, which is done already
-    const int count = to - from - kStartTiles;
-    auto tile = [&](int x) { return min(max(x - from - kStartTiles, 0), count); };
+    // the shares with tiles of the block; one that has them all is done already
+    const int first = shares.of(from + kStartTiles), last = shares.of(to - 1);
+    if (p.sets == 1 && first == last) return;
     float v = 0.f;
-    for (int share = first; share <= last; ++share) {
-        const int a = tile(shares.start(share)), b = tile(shares.start(share + 1));
-        if (p.sets == 1 && a == 0 && b == count) return;
-        if (a < b)
-            for (int set = 0; set < p.sets; ++set) v += p.part[prompt_record(p, slice, set, share, kblock) * KEYS + threadIdx.x];
+    for (int set = 0; set < p.sets; ++set) {
+        const float* record = p.part + prompt_record(p, slice, set, first, kblock) * KEYS + threadIdx.x;
+#pragma unroll 8
+        for (int share = first; share <= last; ++share, record += KEYS) v += *record;
     }
     p.w[b * p.w_b + hk * p.w_h + key] += v;
 }
