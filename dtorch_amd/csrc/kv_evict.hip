@@ -4,7 +4,7 @@
 //
 // kv_evict_select_kernel: one workgroup per (sequence, kv head) finds the weight of the last block that stays by a radix
 // select over the blocks' weights (as unsigned numbers in their order; 11, 11 and 10 bits a round), takes of the blocks at that
-// weight the first ones, and writes the list of blocks that stay, in order.  Up to 4096 candidates are held in registers.
+// weight the first ones, and writes the list of blocks that stay, in order.  Up to 16384 candidates are held in registers.
 // kv_evict_move_kernel: moves rows to the front in place.  Row i of the result comes from a row at or past i, so a tile
 // of rows may be written as soon as the tile itself has been read: what a write covers belongs to rows already read.  A workgroup
 // has the next tile's loads in flight while it writes one, and that tile's list entries before them.  Few heads share a row's chunks
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictPar
     }
     // those above stay, and the first `need` of those at it
     if constexpr (PER > 0) {
-        int counts = 0;  // above << 16, and at it: up to 4096 of both
+        int counts = 0;  // above << 16, and at it: up to 16384 of both
 #pragma unroll
         for (int k = 0; k < PER; ++k)
             if (PER * tid + k < cand) counts += mine[k] > prefix ? 1 << 16 : mine[k] == prefix ? 1 : 0;
@@ -277,7 +277,7 @@ struct EvictSpace {
     size_t plan, order;  // bytes
 };
 
-constexpr int kHeldRows = 4;  // candidates a thread holds
+constexpr int kHeldRows = 16;  // candidates a thread holds
 
 static EvictSpace evict_workspace(const dtattn_kv_evict_args* a) {
     const int64_t blocks = (a->S_max + a->block - 1) / a->block;
@@ -351,10 +351,11 @@ extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     p.blocks_max = (int32_t)((a->S_max + a->block - 1) / a->block);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     const unsigned heads = (unsigned)(a->B * a->Hkv);
-    // Candidates in registers, as few a thread as hold them, or in memory.  us of the launch, 64 heads of 4096 tokens: four a thread
-    // 7.2, in memory 10.8; 128 of 256 blocks of 32: one 5.8, four 16.8, in memory 6.8; the whole call, 8 heads of 16384:
-    // sixteen 24.4, in memory 21.6.
+    // Candidates in registers, as few a thread as hold them, or in memory.  us of the launch: 64 heads of 4096 tokens, four a thread
+    // 7.3, sixteen 11.6, in memory 10.8; 16 of 10319, sixteen 13.5, in memory 21.1; 8 of 16384 17.7, 28.2; 128 of 256 blocks of 32,
+    // one 5.8, four 16.8, in memory 6.8.
     if (p.blocks_max <= kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<1>, dim3(heads), dim3(kSelect), 0, stream, p);
+    else if (p.blocks_max <= 4 * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<4>, dim3(heads), dim3(kSelect), 0, stream, p);
     else if (p.blocks_max <= kHeldRows * kSelect) hipLaunchKernelGGL(kv_evict_select_kernel<kHeldRows>, dim3(heads), dim3(kSelect), 0, stream, p);
     else hipLaunchKernelGGL(kv_evict_select_kernel<0>, dim3(heads), dim3(kSelect), 0, stream, p);
     int st = check_launch("kv_evict_select_kernel");

@@ -212,6 +212,13 @@ def test_evict_long():
     _evict(rng, 1, 1, 70016, 16, [70001], 4000 * 16, 160, 16, torch.float8_e4m3fn, 16)
 
 
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 4096, 4097, 9001, 16384, 16385])
+def test_evict_candidates_around_what_a_thread_holds(n):
+    rng = np.random.default_rng(n)
+    w = np.round(np.exp(rng.standard_normal((1, 2, n)) * 2)).astype(np.float32)  # many ties
+    _evict(rng, 1, 2, n, 16, [n], n // 2 + 3, 5, 1, torch.bfloat16, weights=w)
+
+
 def test_evict_many_and_few_heads():
     # 300 workgroups of whole rows, and two whose rows' chunks are shared out, one of them with an odd number of chunks
     rng = np.random.default_rng(11)
