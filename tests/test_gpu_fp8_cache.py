@@ -305,6 +305,18 @@ def test_decode_layouts():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("page", [16, 64])
+def test_decode_of_shared_and_of_bad_pages(page):
+    """A prefix that two sequences share, a page twice in one sequence, and page ids outside the pool, which count as its ends."""
+    rng = np.random.default_rng(page)
+    c = _decode_case(rng, [300, 290, 256, 200], 8, 2, 128, 16, page, torch.bfloat16, 320, junk=False)
+    t = c["table"]
+    t[1, :2] = t[0, :2]
+    t[2, 3] = t[2, 0]
+    t[3, 0], t[3, 1] = -5, 1 << 30
+    _check(c, *_run_decode(c))
+
+
 def test_decode_of_a_longer_cache_view():
     # the same tokens in a larger cache: other shares, the same values within their rounding; and a view of its first blocks
     rng = np.random.default_rng(16)
