@@ -9,11 +9,13 @@
 // order of the head dims inside a product is free, so long as the query's is the same), and for the values 8 (D = 128)
 // or 4 bytes of each of 8 tokens, whose bytes pair up by token with one v_perm for four of them.  Codes become
 // 16-bit floats exactly (e4m3 has 4 significant bits); scales are applied to scores, and to P through its exponent, in
-// fp32, so any positive scale does.  Per 32 tokens: 80 conversions and permutes, 16 MFMAs and about 150 other
-// instructions for 8 KB.
+// fp32, so any positive scale does.
 //
 // fp32 queries: q and P are each the sum of three bf16 numbers (8 mantissa bits apiece, exact), and codes are exact in
-// bf16, so three MFMAs give the fp32 product.
+// bf16, so three MFMAs give the fp32 product.  16-bit queries: P is two numbers of their type, which leaves 2^-16 (bf16) or 2^-22
+// (fp16) of it, far below the one rounding of the output; P rounded to 16 bits would add half a step of the type.  The second
+// part costs 1 to 3% (64 sequences of 512 to 8192 in pages 104 us against 103, 16 of 20000 to 32768 141 against 137, one of 4000
+// 12.0 against 11.9).
 //
 // All (kv head, sequence, 32-token unit) triples are laid end to end by a prefix sum of the lengths and cut in equal
 // shares, one per workgroup, whose four waves take its units in turn and meet in LDS where a sequence ends.  What a share cuts (its
@@ -83,26 +85,27 @@ struct Shares8 {
     }
 };
 
-// Operand types by query type: bf16 products for bf16 and (in three parts) fp32 queries, fp16 ones for fp16.
+// Operand types by query type: bf16 products for bf16 and fp32 queries, fp16 ones for fp16; parts of a query and of P.
 template <typename T>
 struct Q8 {
     typedef T E;
-    static constexpr int parts = 1;
+    static constexpr int parts = 1, pparts = 2;
 };
 template <>
 struct Q8<float> {
     typedef bf16_t E;
-    static constexpr int parts = 3;
+    static constexpr int parts = 3, pparts = 3;
 };
 
-// x[0..7] as `parts` operands whose sum they are.
+// x[0..7] as the two or three operands whose sum they are.
 template <typename T>
 __device__ __forceinline__ void operands(const float* x, typename Elem<typename Q8<T>::E>::vec8* out) {
     typedef typename Q8<T>::E E;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        if constexpr (Q8<T>::parts == 1) {
+        if constexpr (Q8<T>::pparts == 2) {
             out[0][e] = Elem<E>::from_f32(x[e]);
+            out[1][e] = Elem<E>::from_f32(x[e] - Elem<E>::to_f32(out[0][e]));
         } else {
             bf16_t t[3];
             split3(x[e], t);
@@ -140,7 +143,7 @@ __global__ void __launch_bounds__(64 * kWaves8, kSharesPerCu) decode_fp8_kernel(
     typedef typename Q8<T>::E E;
     typedef typename Elem<E>::vec8 V8;
     constexpr int NT = kTiles8;
-    constexpr int NP = Q8<T>::parts, DH = D / 64, DPL = D / 16;  // DPL: V bytes (dims) per lane and token
+    constexpr int NP = Q8<T>::parts, PP = Q8<T>::pparts, DH = D / 64, DPL = D / 16;  // DPL: V bytes (dims) per lane and token
     constexpr int NR = PAGES == 2 ? NT : 1;                      // buffer resources of a unit
     constexpr int RP = D + 4;  // floats per row of red_o: rows 16 bytes apart in the banks
     __shared__ __attribute__((aligned(16))) float red_o[kWaves8][16][RP];
@@ -370,9 +373,9 @@ __global__ void __launch_bounds__(64 * kWaves8, kSharesPerCu) decode_fp8_kernel(
         if (more) load_scales(nx);
         // The row sum is on the running max of the scores.  P is on a base of its own, E, where the exponents of a tile's
         // scores and of its V scale add up, so the product of P and codes needs no scaling.  E is the unit's own largest
-        // value, so that the largest P is a power of two and rounds exactly, but at most 2^24 below the running one, which
+        // value, so that the largest P is a power of two, but at most 2^24 below the running one, which
         // keeps alpha and the accumulators finite.  That power is 1, and in fp16 2^15: its subnormals then begin 2^-29
-        // below the largest P and not 2^-14, and a small P next to it keeps its precision.
+        // below the largest P and not 2^-14, and a small P and its second part keep their precision.
         float Mn = ML, e0 = kNegInf;
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt) {
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(64 * kWaves8, kSharesPerCu) decode_fp8_kernel(
         const float alpha = fast_exp2(eb - base);
         eb = en;
         float us = 0.f;
-        V8 pk[NT / 2][NP];
+        V8 pk[NT / 2][PP];
 #pragma unroll
         for (int tp = 0; tp < NT / 2; ++tp) {
             float pf[8];
@@ -412,9 +415,9 @@ __global__ void __launch_bounds__(64 * kWaves8, kSharesPerCu) decode_fp8_kernel(
                 V8 vf[4];
                 transpose4x8<E>(vr[tp][h], vf);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int i = 0; i < PP; ++i)
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) acc[4 * h + j] = mfma16(vf[j], pk[tp][i], acc[4 * h + j]);
+                    for (int j = 0; j < 4; ++j) acc[4 * h + j] = mfma16(vf[j], pk[tp][i], acc[4 * h + j]);
             }
         if (more) load_v(nx);
       }

@@ -339,11 +339,11 @@ typedef struct {
 
 int dtattn_kv_append_fp8(const dtattn_kv_append_fp8_args* args, void* stream);
 
-/* Single-token attention over such a cache: dtattn_decode_splitkv's arithmetic with K = code * k_scale and
+/* Single-token attention over such a cache: dtattn_decode_splitkv's formula with K = code * k_scale and
  * V = code * v_scale, any positive finite scales.  Scores, softmax statistics and accumulators are fp32; codes enter the products
- * exactly.  With 16-bit queries P is rounded to their type for the second product, as in the 16-bit decode; with FP32
- * queries both products carry fp32 operands (three bf16 parts of each).  Rows at or past lengths[b] are never read; page ids are
- * clamped into the pool. */
+ * exactly.  With 16-bit queries P enters the second product as two numbers of their type (its rounding and the remainder's), which
+ * leaves 2^-16 (BF16) or 2^-22 (FP16) of it; with FP32 queries both products carry fp32 operands (three bf16 parts of each).  O is
+ * rounded once.  Rows at or past lengths[b] are never read; page ids are clamped into the pool. */
 typedef struct {
     const void* q;           /* [B, Hq, 1, D], 16-byte aligned, strides multiples of 16 bytes */
     const void* k_cache;     /* codes, as above */
