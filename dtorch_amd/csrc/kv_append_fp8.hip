@@ -38,9 +38,9 @@ constexpr int kHeld = 4;  // chunks of 8 elements that a lane holds: a wave hold
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 
-// The smallest power of two s >= 2^-126 with m <= 448 s; 1 for m = 0.  m = f 2^e with 1 <= f < 2: 448 = 1.75 * 2^8.
+// The smallest power of two s >= 2^-126 with m <= 448 s.  m = f 2^e with 1 <= f < 2: 448 = 1.75 * 2^8.  For m = 0 that is 2^-126, which
+// no other value's scale is below: tokens without a finite value other than 0 leave the scale to those before and behind them.
 __device__ __forceinline__ float scale_for(float m) {
-    if (m == 0.f) return 1.f;
     const uint32_t bits = __builtin_bit_cast(uint32_t, m);
     const int k = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);  // biased by 127
     return __builtin_bit_cast(float, (uint32_t)max(k, 1) << 23);

@@ -163,8 +163,9 @@ def kv_cache_append_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: t
     k_cache / v_cache float8_e4m3fn [B, Hkv, S_max, D]; k_scale / v_scale fp32 [B, Hkv, S_max / block] (the block,
     a power of two from 16 to 256, follows from the shapes); k_new / v_new bf16, fp16 or fp32 [B, Hkv, n_new, D].
     A value is code * scale.  A block's scale is the smallest power of two that holds its largest value within
-    +-448; a block that outgrows its scale re-encodes its older tokens (exact, subnormal codes apart).  NaN and
-    infinite inputs become NaN codes and leave the scale to the others.
+    +-448 (and at least 2^-126, which is that of a block of zeros); a block that outgrows its scale re-encodes its older
+    tokens (exact, subnormal codes apart).  NaN and infinite inputs become NaN codes; they and zeros leave the scale to
+    the others, whichever come first.
     """
     _h.KvCacheAppendFp8Op().compute([k_cache, v_cache, k_scale, v_scale, lengths, k_new, v_new])
 

@@ -11,7 +11,7 @@ from .sdpa import e4m3fn_decode, e4m3fn_encode
 
 
 def block_scale(amax: float) -> float:
-    """The smallest power of two s >= 2^-126 with amax <= 448 s; 1 for amax = 0."""
+    """The smallest power of two s >= 2^-126 with amax <= 448 s, for a block that has an amax (1 for amax = 0)."""
     if amax == 0:
         return 1.0
     k = -126
@@ -43,7 +43,8 @@ def append_fp8(codes, scale, table, lengths, new, block):
                 for h in range(heads):
                     x = new[b, h, t - start:stop - start]
                     fin = np.abs(x[np.isfinite(x)])
-                    s = block_scale(float(fin.max(initial=0.0)))
+                    amax = float(fin.max(initial=0.0))
+                    s = block_scale(amax) if amax > 0 else 2.0 ** -126  # no value to hold: no scale is too small
                     if t > t0:
                         old = float(scale[slot, h, r0 // block])
                         s = s if np.isnan(old) else max(s, old)
