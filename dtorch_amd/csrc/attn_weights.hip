@@ -247,7 +247,8 @@ constexpr int kStartTiles = 4;
 constexpr int kShareTiles = 4;
 
 // 16-bit and 8-bit keys are one operand; fp32 ones are three bf16 parts (8 bits each, exact), of whose nine products with the
-// query's parts the six largest count: what is left out is below 2^-23 of |q| |k|, an fp32 sum's own rounding.
+// query's parts the six largest count.  The second part is at most 2^-8 of a value and the third 2^-16, of either sign, so what is left
+// out is at most 2^-23 of |q| |k|, what one fp32 addition rounds by (parts cut off instead of rounded: 2^-21, always of one sign).
 template <typename TQ, typename TK>
 struct PromptTypes {
     typedef typename std::conditional<std::is_same<TQ, f16_t>::value, f16_t, bf16_t>::type E;

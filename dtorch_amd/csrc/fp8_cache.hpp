@@ -77,17 +77,18 @@ __device__ __forceinline__ int scan64(int v) {
     return dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
 
-// The three bf16 parts of an fp32 value: 24 bits of mantissa as 8 + 8 + 8, by truncation, so that their sum is the value (parts
-// below the smallest bf16 normal apart).  A value that is not finite is its first part.
+// The three bf16 parts of an fp32 value, each the rest rounded to nearest: 24 bits of mantissa as 8 + 8 + 8, so that their sum is the
+// value (parts below the smallest bf16 normal apart), with the second at most 2^-8 and the third 2^-16 of it.  A value that is
+// not finite is its first part; of one that would round to infinity that is cut off instead.
 __device__ __forceinline__ void split3(float x, bf16_t out[3]) {
-    float r = x;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        const bool finite = fabsf(r) < __builtin_inff();
-        const float t = finite ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, r) & 0xffff0000u) : r;
-        out[i] = static_cast<bf16_t>(t);
-        r = finite ? r - t : 0.f;
-    }
+    const float mag = fabsf(x);
+    const bool finite = mag < __builtin_inff();
+    const bool cut = finite && mag > 0x1.fep127f;
+    out[0] = static_cast<bf16_t>(cut ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u) : x);
+    float r = finite ? x - static_cast<float>(out[0]) : 0.f;
+    out[1] = static_cast<bf16_t>(r);
+    r -= static_cast<float>(out[1]);
+    out[2] = static_cast<bf16_t>(r);
 }
 
 }  // namespace dtattn
