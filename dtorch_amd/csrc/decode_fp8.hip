@@ -115,6 +115,12 @@ __device__ __forceinline__ void operands(const float* x, typename Elem<typename 
     }
 }
 
+// log2 of any float >= 0: the instruction takes a subnormal for 0.
+__device__ __forceinline__ float log2_any(float x) {
+    const bool small = __builtin_bit_cast(uint32_t, x) < 0x00800000u;
+    return __log2f(small ? x * 0x1p24f : x) - (small ? 24.f : 0.f);
+}
+
 // Largest and sum over the four lane groups that hold a column.
 __device__ __forceinline__ float colmax(float x) { return max_across_groups<16>(x); }
 __device__ __forceinline__ float colsum(float x) { return sum_across_groups<16>(x); }
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(64 * kWaves8, kSharesPerCu) decode_fp8_kernel(
                 for (int i = 0; i < NP; ++i) a = mfma16(kf, qf[i][k], a);
             }
             sc[tt] = a * (p.c * ks[tt]);
-            lv[tt] = __log2f(vs[tt]);
+            lv[tt] = log2_any(vs[tt]);
         }
         if (more) load_k(nx);  // the keys are used up
         if (left < kUnit8) {
@@ -452,9 +458,10 @@ __global__ void __launch_bounds__(64 * kWaves8, kSharesPerCu) decode_fp8_kernel(
         const float lse = __builtin_fmaf(M, kLn2, __log2f(lt) * kLn2);
         const bool whole = cur.tok == 0 && u + m <= n && m * kUnit8 >= cur.L;
         // every score -inf: a record of O = 0 at the LSE of -inf, which drops it in the merge; the output itself is 0 / 0
-        const float f = lt == 0.f && !whole ? 0.f : fast_exp2(X - M) / lt;
+        // (2^(X - M), which the smallest scales of V take below what the instruction gives, is the product of two powers)
+        const float f = lt == 0.f && !whole ? 0.f : fast_exp2(fmaxf(X - M, -100.f)) / lt, small = fast_exp2(fminf(X - M + 100.f, 0.f));
 #pragma unroll
-        for (int j = 0; j < DPL; ++j) o[j] *= f;
+        for (int j = 0; j < DPL; ++j) o[j] = o[j] * f * small;
         if (whole) {
             T* op = reinterpret_cast<T*>(p.o) + b * p.o_b + hq * p.o_h + dim;
             if (dim < p.d) {

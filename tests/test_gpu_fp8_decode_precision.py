@@ -56,3 +56,30 @@ def test_same_call_same_bits(dtype):
     for _ in range(5):
         again = _run_decode(c)
         assert torch.equal(first[0].view(torch.uint8), again[0].view(torch.uint8)) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("exponents", [(-126,), (-128,), (-130, -127), (-149,), (-140, -100), (118, 119)])
+@pytest.mark.parametrize("lengths,Hq,Hkv,page", [([100, 17, 1], 8, 2, 0), ([3000], 4, 4, 16)])
+def test_value_scales_at_the_ends_of_the_range(dtype, exponents, lengths, Hq, Hkv, page):
+    """Any positive finite scale: subnormal ones and the largest, in one share and in records that merge.
+
+    Outputs near the smallest normal: half a step of the type's subnormals more, 2^-134 in bf16 and 2^-150 in fp32, and one of fp32
+    for each product that brings the accumulators there (three) and each record that is added (a share has 128 tokens at least)."""
+    rng = np.random.default_rng(23 + len(lengths))
+    D, cap = 64, -(-max(lengths) // 16) * 16
+    c = _decode_case(rng, lengths, Hq, Hkv, D, 16, page, dtype, cap, scales=lambda r, s: np.exp2(r.choice(exponents, s).astype(np.float64)).astype(np.float32), junk=False)
+    for name in "kv":  # every finite code, up to 448
+        bits = rng.integers(0, 256, c[name].shape).astype(np.uint8)
+        c[name] = np.where((bits & 0x7F) == 0x7F, np.uint8(0x18), bits)
+    c["ks"][:] = 2.0 ** -8
+    if max(exponents) > 0:  # outputs within the range
+        c["v"] = np.where((c["v"] & 0x78) > 0x50, (c["v"] & 0x87) | 0x50, c["v"]).astype(np.uint8)
+    o, _ = _run_decode(c)
+    want, _, a, mag = orc.decode_fp8(c["q"].double().numpy()[:, :, 0], c["k"], c["v"], c["ks"], c["vs"], c["lengths"], c["table"])
+    n = np.maximum(np.asarray(lengths, dtype=np.float64), 1)[:, None]
+    u, parts = (U[dtype], 2) if dtype == torch.bfloat16 else (0.0, 3)
+    tol = a * (2 * (parts * D + 8) * E * mag + (3 * n + 64) * E + u * u)[..., None]
+    tol = tol * (1 + u) + np.abs(want) * max(u, E) + (2.0 ** -134 if dtype == torch.bfloat16 else 2.0 ** -150) + ((4 + n / 128) * 2.0 ** -150)[..., None]
+    off = np.abs(o.double().cpu().numpy()[:, :, 0] - want)
+    assert np.all(off <= tol), float((off / tol).max())
