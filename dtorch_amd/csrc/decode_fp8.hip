@@ -14,8 +14,8 @@
 // fp32 queries: q and P are each the sum of three bf16 numbers (8 mantissa bits apiece, exact), and codes are exact in
 // bf16, so three MFMAs give the fp32 product.  16-bit queries: P is two numbers of their type, which leaves 2^-16 (bf16) or 2^-22
 // (fp16) of it, far below the one rounding of the output; P rounded to 16 bits would add half a step of the type.  The second
-// part costs 1 to 3% (64 sequences of 512 to 8192 in pages 104 us against 103, 16 of 20000 to 32768 141 against 137, one of 4000
-// 12.0 against 11.9).
+// part costs 1% (us without it and with: 64 sequences of 512 to 8192 in pages 103.0 and 103.4, 16 of 20000 to 32768 136.2 and 137.8,
+// one of 4000 12.0 and 12.2).
 //
 // All (kv head, sequence, 32-token unit) triples are laid end to end by a prefix sum of the lengths and cut in equal
 // shares, one per workgroup, whose four waves take its units in turn and meet in LDS where a sequence ends.  What a share cuts (its

@@ -42,7 +42,7 @@ static int fp8_cache_checks(const Args* a, bool paged, const char* who, Fp8Cache
     for (int i = 0; i < 3; ++i)
         if (a->k_stride[i] % 16 != 0 || a->v_stride[i] % 16 != 0)
             return fail(DTATTN_ERR_UNSUPPORTED, "%s: cache strides must be multiples of 16 bytes", who);
-    // up to 64 rows are addressed with 32-bit offsets below 2^30, and what must not be read with offsets from 3 * 2^30 on
+    // the 32 rows of a decode unit are addressed with 32-bit offsets below 2^30, and what must not be read with offsets from 3 * 2^30 on
     if (a->k_stride[2] < a->D || a->v_stride[2] < a->D || a->k_stride[2] > (1 << 24) || a->v_stride[2] > (1 << 24))
         return fail(DTATTN_ERR_UNSUPPORTED, "%s: the row stride of a cache must be from D to 2^24 bytes", who);
     return DTATTN_OK;

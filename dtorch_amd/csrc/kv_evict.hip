@@ -360,9 +360,10 @@ extern "C" int dtattn_kv_evict(const dtattn_kv_evict_args* a, void* stream_) {
     else hipLaunchKernelGGL(kv_evict_select_kernel<0>, dim3(heads), dim3(kSelect), 0, stream, p);
     int st = check_launch("kv_evict_select_kernel");
     if (st != DTATTN_OK) return st;
-    // A row's chunks are shared until three CUs in four have a workgroup, or each chunk has one.  us at a workgroup for no CU / half
-    // of them / three in four / all / all twice, heads of 128 bf16, 8192 -> 4096 tokens: 1 sequence of 8 heads 45 / 29 / 33 / 33 / 34,
-    // 3 61 / 44 / 44 / 49 / 62, 6 68 / 52 / 52 / 69 / 80, 8 72 / 72 / 64 / 63 / 81, 12 81 / 81 / 81 / 83 / 109.
+    // A row's chunks are halved among workgroups until three CUs in four have one, or each chunk has one.  us where that bound is no CU /
+    // half of them / three in four / all / all twice, heads of 128 bf16, 8192 -> 4096 tokens: 1 sequence of 8 heads 45 / 29 / 33 / 33 / 34,
+    // 3 61 / 44 / 44 / 49 / 62, 6 68 / 52 / 52 / 69 / 80, 8 72 / 72 / 64 / 63 / 81, 12 81 / 81 / 81 / 83 / 109.  Workgroups double, so one
+    // sequence goes from 128 of them, which half of the CUs would take, to 256 of single chunks: 33 us, and not the 29 of two.
     const int wanted = std::max(stream_cus(stream) * 3 / 4, 1);
     p.width = p.chunks;
     while (p.width > 1 && 2 * (int64_t)heads * ((p.chunks + p.width - 1) / p.width) < wanted) p.width = (p.width + 1) / 2;

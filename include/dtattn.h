@@ -385,8 +385,9 @@ int dtattn_decode_fp8(const dtattn_decode_fp8_args* args, void* stream);
  * j < n = lengths[b] (S without lengths) and, when causal, j <= i + q_offset; with causal and lengths a query at
  * i + q_offset >= n is padding and adds nothing.  A row whose lse is -inf (it sees no key) adds nothing.
  * Sums are fp32, without atomics, in an order that depends on the sizes, the lengths and the device's CU count.  Only
- * weights[b, hk, j < n] are touched.  Where an fp32 query or key is infinite its products with another's zero parts are NaN, and
- * so may be a weight that is 0 in exact arithmetic; keys that a row does not see never count.
+ * weights[b, hk, j < n] are touched.  An infinite value's product with a zero is NaN, and so may be a weight that is 0 in exact
+ * arithmetic: an fp32 query or key that is infinite meets the zero parts of another, and an infinite key the zeros that stand for a
+ * row whose lse is -inf.  Keys that a row does not see never count.
  * D up to 128, rows of a multiple of 16 bytes; B and Hkv up to 65535. */
 typedef struct {
     float* weights;          /* [B, Hkv, S], key stride 1 */
