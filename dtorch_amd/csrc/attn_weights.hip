@@ -7,10 +7,11 @@
 // One query per sequence (decode) is bound by HBM: the keys are read once.  A prompt is bound by the matrix cores and VALU issue
 // together: an exponential, an fma and an add per (query, key) pair beside its MFMAs.  Counters at 4x2048 causal bf16, 32 heads over
 // 8 of 128, per wave and column tile: 16 MFMAs, 512 cycles, and 32 exponentials (two issue slots each) and 112 other VALU
-// instructions on average, 773 cycles with the MFMAs' issue; the two waves of a SIMD take 1294 cycles each.  Both forms keep a wave's keys in registers as MFMA operands and pass the queries by, so that the sum over queries stays in
-// registers too and no two waves add to one weight: the result does not depend on timing.  Measured: 16 sequences of 700 to
-// 8191, 28 heads over 4 of 128, codes, one query 11.6 us (through the caches, which a decode step has just filled; loads that
-// bypass them take 13.4); 4x2048 causal bf16, 32 heads over 8 of 128, 98 us, not causal 138 us (990 TFLOP/s).
+// instructions on average, 773 cycles with the MFMAs' issue; the two waves of a SIMD take 1294 cycles each.  Both forms
+// keep a wave's keys in registers as MFMA operands and pass the queries by, so that the sum over queries stays in registers too and
+// no two waves add to one weight: the result does not depend on timing.  Measured: 16 sequences of 700 to 8191, 28 heads over 4 of
+// 128, codes, one query 11.6 us (through the caches, which a decode step has just filled; loads that bypass them take 13.4); 4x2048
+// causal bf16, 32 heads over 8 of 128, 96 us, not causal 138 us (990 TFLOP/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -347,8 +348,8 @@ __device__ __forceinline__ void to_parts(const Chunk<T>& w, V8* out) {
 // A workgroup of four waves holds 256 keys (128 in fp32) as operands and passes column tiles by, which its threads stage
 // through LDS one tile ahead.  A column is a lane, so its lse is one register and the sums over columns are one
 // add per score; lanes meet once, at the end.  Per wave and tile of 16-bit operands 16 MFMAs against 32 exponentials and 68 to 83 other
-// VALU instructions (145 on the causal border): the exponentials of one 32-key tile go under the MFMAs of the next (the last one's under the next column
-// tile's), tiles on the causal border apart.  Workgroups take equal shares of the tiles, from one key block into the next, and
+// VALU instructions (145 on the causal border): the exponentials of one 32-key tile go under the MFMAs of the next (the last one's
+// under the next column tile's), tiles on the causal border apart.  Workgroups take equal shares of the tiles, from one key block into the next, and
 // as many as run at a time: parts of one block each, of even sizes, left places idle (4x2048 causal 32 heads over 8, bf16 108 us,
 // equal shares 98; 1x4000 causal 28 over 4, fp16 122, shares 100).
 template <typename TQ, typename TK, int D, bool CAUSAL>

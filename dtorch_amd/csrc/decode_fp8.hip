@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(64 * kWaves8, kSharesPerCu) decode_fp8_kernel(
     typedef typename Elem<E>::vec8 V8;
     constexpr int NT = kTiles8;
     constexpr int NP = Q8<T>::parts, PP = Q8<T>::pparts, DH = D / 64, DPL = D / 16;  // DPL: V bytes (dims) per lane and token
-    constexpr int NR = PAGES == 2 ? NT : 1;                      // buffer resources of a unit
+    constexpr int NR = PAGES == 2 ? NT : 1;  // buffer resources of a unit
     constexpr int RP = D + 4;  // floats per row of red_o: rows 16 bytes apart in the banks
     __shared__ __attribute__((aligned(16))) float red_o[kWaves8][16][RP];
     __shared__ float red_m[kWaves8][16], red_l[kWaves8][16], red_e[kWaves8][16];

@@ -308,9 +308,9 @@ int dtattn_kv_append_paged(const dtattn_kv_append_paged_args* args, void* stream
  * Positions, capacity, unassigned pages and the lengths' advance are those of dtattn_kv_append[_paged].
  * With amax the largest |x| over the finite new values of a block (of K or of V), the block needs the scale
  * 2^k, the smallest power of two with amax <= 448 * 2^k and k >= -126 (so 2^-126 when amax is 0: such tokens
- * leave the scale to the others).  A block whose first row is among the new tokens takes that scale.  A block that already holds tokens keeps the larger
- * of its scale and the needed one; when that is a new scale, its r older rows become
- * e4m3fn_rne(code * (old / new)), which is exact for the powers of two that this call writes, subnormal
+ * leave the scale to the others).  A block whose first row is among the new tokens takes that scale.  A block
+ * that already holds tokens keeps the larger of its scale and the needed one; when that is a new scale, its r
+ * older rows become e4m3fn_rne(code * (old / new)), which is exact for the powers of two that this call writes, subnormal
  * codes apart.  New codes are e4m3fn_rne(x * (1 / scale)); NaN and infinities become NaN codes.  Rows past
  * the written ones are left as they were.  A page that is written belongs to one sequence; keys and values lie
  * apart (equal pointers are refused). */
