@@ -1,0 +1,193 @@
+// Single-token decode of sequences that share a prefix (semantics: dtattn.h, "attention over a shared prefix"): the arithmetic of
+// SdpaOp::Compute (dtorch/core/operators/standard/scaled_dot_product_attention_op.cc:107-109) at Lq = 1.  The reference has no KV cache.
+//
+// The prefix's keys meet the query heads of all sequences of a group as one matrix product of 16, 32 or 64 columns a wave, so they are
+// read once per so many query rows instead of once per sequence; a long prefix of many sequences is bound by the matrix cores, the
+// sequences' own tokens by HBM.  Both write records, which one more launch merges by LSE.
+#include <algorithm>
+
+#include "decode_parts.hpp"
+
+namespace dtattn {
+
+namespace {
+
+// Waves per SIMD that a part's registers leave room for.
+template <typename T>
+constexpr int part_waves(int nc) { return nc == 1 || (nc == 2 && sizeof(T) == 2) ? 2 : 1; }
+
+}  // namespace
+
+template <typename T, int D, int NC, int KIND, bool TWO>
+__global__ void __launch_bounds__(64 * kPartWaves, part_waves<T>(NC)) decode_shared_kernel(const PartsParams p) {
+    __shared__ __attribute__((aligned(16))) float red_o[kPartWaves][16][D + 4];
+    __shared__ float red_m[kPartWaves][16], red_l[kPartWaves][16];
+    __shared__ int eff[kPartGroups], lead[kPartGroups];
+    decode_part<T, D, NC, KIND, TWO>(p, blockIdx.x, red_o, red_m, red_l, eff, lead);
+}
+
+namespace {
+
+struct SharedPlan {
+    int32_t kernel_d, nc, nsub[2], shares[2], columns[2];
+    size_t meta[2], rec_o[2], rec_lse[2], whole_o, whole_lse, bytes;
+};
+
+int64_t units_in(int64_t tokens) { return (tokens + kPartUnit - 1) / kPartUnit; }
+
+SharedPlan plan_shared(const dtattn_decode_shared_args* a, int cus) {
+    SharedPlan r = {};
+    const bool paged = a->block_table != nullptr;
+    const int64_t capacity = std::max<int64_t>(paged ? a->max_pages * a->page_size : a->S_max, 1);
+    const int64_t prefix = std::max<int64_t>(paged ? capacity : a->S_prefix, 1);
+    const int64_t group = a->Hq / a->Hkv, rows = a->B / a->groups * group;
+    r.kernel_d = a->D <= 64 ? 64 : 128;
+    r.nc = rows <= 16 ? 1 : rows <= 32 || a->dtype == DTATTN_FP32 ? 2 : 4;
+    r.columns[0] = 16 * r.nc, r.columns[1] = 16;
+    const int waves = r.nc == 1 || (r.nc == 2 && a->dtype != DTATTN_FP32) ? 2 : 1;
+    const int64_t cols[2] = {rows, group}, sets[2] = {a->groups, a->B}, tokens[2] = {prefix, capacity};
+    for (int s = 0; s < 2; ++s) {
+        r.nsub[s] = (int32_t)((cols[s] + r.columns[s] - 1) / r.columns[s]);
+        const int64_t units = a->Hkv * r.nsub[s] * sets[s] * units_in(tokens[s]);
+        r.shares[s] = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)(s == 0 ? waves : 2) * cus, units / kPartLeast));
+        const size_t records = (size_t)2 * r.shares[s] * r.columns[s];
+        r.meta[s] = part_up((1 + 2 * (size_t)sets[s]) * sizeof(int32_t));
+        r.rec_o[s] = part_up(records * r.kernel_d * sizeof(float));
+        r.rec_lse[s] = part_up(records * sizeof(float));
+    }
+    r.whole_o = part_up((size_t)a->B * a->Hq * r.kernel_d * sizeof(float));
+    r.whole_lse = part_up((size_t)a->B * a->Hq * sizeof(float));
+    r.bytes = 2 * (r.whole_o + r.whole_lse);
+    for (int s = 0; s < 2; ++s) r.bytes += r.meta[s] + r.rec_o[s] + r.rec_lse[s];
+    return r;
+}
+
+template <typename T, int D, int NC>
+void launch_prefix(const PartsParams& p, bool two, hipStream_t stream) {
+    const dim3 grid((unsigned)p.shares[0]), block(64 * kPartWaves);
+    if (two) hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, kPrefixPart, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, kPrefixPart, false>), grid, block, 0, stream, p);
+}
+
+template <typename T, int D>
+int launch_shared(const PartsParams& p, int nc, hipStream_t stream) {
+    const bool two = p.table != nullptr && p.page_shift < 5;
+    if (nc == 1) launch_prefix<T, D, 1>(p, two, stream);
+    else if (nc == 2) launch_prefix<T, D, 2>(p, two, stream);
+    else if constexpr (sizeof(T) == 2) launch_prefix<T, D, 4>(p, two, stream);
+    int st = check_launch("decode_shared_kernel");
+    if (st != DTATTN_OK) return st;
+    const dim3 grid((unsigned)p.shares[1]), block(64 * kPartWaves);
+    if (two) hipLaunchKernelGGL((decode_shared_kernel<T, D, 1, kOwnPart, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((decode_shared_kernel<T, D, 1, kOwnPart, false>), grid, block, 0, stream, p);
+    st = check_launch("decode_shared_kernel");
+    if (st != DTATTN_OK) return st;
+    const int64_t pairs = (int64_t)p.B * p.Hq;
+    // Few pairs are cut into many records each: four waves to a pair
+    if (pairs <= 256) hipLaunchKernelGGL((decode_parts_merge_kernel<T, D, 4, true>), dim3((unsigned)pairs), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((decode_parts_merge_kernel<T, D, 1, true>), dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, stream, p);
+    return check_launch("decode_parts_merge_kernel");
+}
+
+}  // namespace
+
+}  // namespace dtattn
+
+using namespace dtattn;
+
+extern "C" size_t dtattn_decode_shared_workspace_size(const dtattn_decode_shared_args* a, void* stream) {
+    if (a == nullptr || a->B <= 0 || a->groups <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->D <= 0 || a->Hq < a->Hkv || a->B < a->groups) return 0;
+    const int cus = stream_cus(reinterpret_cast<hipStream_t>(stream));
+    return plan_shared(a, cus > 0 ? cus : 256).bytes;
+}
+
+extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* stream_) {
+    const char* who = "decode_shared";
+    if (a == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: args is NULL", who);
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    if (a->B < 0 || a->groups <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->D <= 0 || a->B > (1 << 24) || a->Hq > (1 << 20))
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
+    if (a->Hq % a->Hkv != 0) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: Hq is not a multiple of Hkv", who);
+    if (a->B % a->groups != 0) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: %lld sequences are not %lld equal groups", who, (long long)a->B, (long long)a->groups);
+    if (a->groups > kPartGroups) return fail(DTATTN_ERR_UNSUPPORTED, "%s: %lld groups (up to %d)", who, (long long)a->groups, kPartGroups);
+    const bool paged = a->block_table != nullptr;
+    if (paged) {
+        if (a->page_size < 16 || (a->page_size & (a->page_size - 1)) != 0 || a->page_size > (1 << 20))
+            return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: page_size %lld must be a power of two >= 16", who, (long long)a->page_size);
+        if (a->num_pages <= 0 || a->max_pages <= 0 || a->num_pages > 0x7fffffff || a->max_pages > (1 << 29) / a->page_size)
+            return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad page counts", who);
+    } else if (a->S_prefix <= 0 || a->S_max <= 0 || a->S_prefix > (1 << 29) || a->S_max > (1 << 29)) {
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad capacities", who);
+    }
+    const int64_t strides[16] = {a->q_stride[0], a->q_stride[1], a->o_stride[0], a->o_stride[1], a->k_stride[0], a->k_stride[1], a->k_stride[2],
+                                 a->v_stride[0], a->v_stride[1], a->v_stride[2], a->k_prefix_stride[0], a->k_prefix_stride[1], a->k_prefix_stride[2],
+                                 a->v_prefix_stride[0], a->v_prefix_stride[1], a->v_prefix_stride[2]};
+    const int64_t rows[4] = {a->k_stride[2], a->v_stride[2], a->k_prefix_stride[2], a->v_prefix_stride[2]};
+    uintptr_t bits = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->o) | reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache);
+    if (!paged) bits |= reinterpret_cast<uintptr_t>(a->k_prefix) | reinterpret_cast<uintptr_t>(a->v_prefix);
+    int st = part_tensor_checks(a->D, a->dtype, strides, paged ? 10 : 16, rows, paged ? 2 : 4, bits, who);
+    if (st != DTATTN_OK) return st;
+    ScalePlan sp;
+    st = plan_scale(a->scale, a->D, a->dtype == DTATTN_FP32 ? kSign32 : kSign16, &sp);
+    if (st != DTATTN_OK || a->B == 0) return st;
+    if (a->q == nullptr || a->o == nullptr || a->k_cache == nullptr || a->v_cache == nullptr || a->lengths == nullptr || a->prefix_lengths == nullptr ||
+        (!paged && (a->k_prefix == nullptr || a->v_prefix == nullptr)))
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    const int cus = stream_cus(stream);
+    if (cus <= 0) return fail(DTATTN_ERR_DEVICE, "%s: cannot tell the stream's device", who);
+    const SharedPlan plan = plan_shared(a, cus);
+    const int64_t capacity = paged ? a->max_pages * a->page_size : a->S_max, most_prefix = paged ? capacity : a->S_prefix;
+    if (a->groups * a->Hkv * plan.nsub[0] * units_in(most_prefix) >= ((int64_t)1 << 31) ||
+        a->B * a->Hkv * plan.nsub[1] * units_in(capacity) >= ((int64_t)1 << 31) || a->B * a->Hq > 0x7fffffff)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: cache too large", who);
+    if (a->workspace == nullptr || a->workspace_bytes < plan.bytes)
+        return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, plan.bytes, a->workspace_bytes);
+    if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0)
+        return fail(DTATTN_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+
+    PartsParams p = {};
+    const int64_t esz = a->dtype == DTATTN_FP32 ? 4 : 2;
+    p.q = reinterpret_cast<const char*>(a->q), p.o = reinterpret_cast<char*>(a->o), p.lse = a->lse;
+    p.k[1] = reinterpret_cast<const char*>(a->k_cache), p.v[1] = reinterpret_cast<const char*>(a->v_cache);
+    p.k_b[1] = a->k_stride[0] * esz, p.k_h[1] = a->k_stride[1] * esz, p.k_s[1] = a->k_stride[2] * esz;
+    p.v_b[1] = a->v_stride[0] * esz, p.v_h[1] = a->v_stride[1] * esz, p.v_s[1] = a->v_stride[2] * esz;
+    if (paged) {
+        p.k[0] = p.k[1], p.k_b[0] = p.k_b[1], p.k_h[0] = p.k_h[1], p.k_s[0] = p.k_s[1];
+        p.v[0] = p.v[1], p.v_b[0] = p.v_b[1], p.v_h[0] = p.v_h[1], p.v_s[0] = p.v_s[1];
+        p.table = a->block_table, p.bt_s = a->block_table_stride;
+        p.page_shift = __builtin_ctzll((unsigned long long)a->page_size), p.num_pages = (int32_t)a->num_pages;
+    } else {
+        p.k[0] = reinterpret_cast<const char*>(a->k_prefix), p.v[0] = reinterpret_cast<const char*>(a->v_prefix);
+        p.k_b[0] = a->k_prefix_stride[0] * esz, p.k_h[0] = a->k_prefix_stride[1] * esz, p.k_s[0] = a->k_prefix_stride[2] * esz;
+        p.v_b[0] = a->v_prefix_stride[0] * esz, p.v_h[0] = a->v_prefix_stride[1] * esz, p.v_s[0] = a->v_prefix_stride[2] * esz;
+    }
+    p.capacity[0] = (int32_t)most_prefix, p.capacity[1] = (int32_t)capacity;
+    p.lengths = a->lengths, p.prefix = a->prefix_lengths;
+    char* ws = reinterpret_cast<char*>(a->workspace);
+    auto take = [&](size_t bytes) {
+        char* at = ws;
+        ws += bytes;
+        return at;
+    };
+    for (int s = 0; s < 2; ++s) {
+        p.nsub[s] = plan.nsub[s], p.shares[s] = plan.shares[s], p.columns[s] = plan.columns[s];
+        p.meta[s] = reinterpret_cast<int32_t*>(take(plan.meta[s]));
+        p.rec_o[s] = reinterpret_cast<float*>(take(plan.rec_o[s]));
+        p.rec_lse[s] = reinterpret_cast<float*>(take(plan.rec_lse[s]));
+        p.whole_o[s] = reinterpret_cast<float*>(take(plan.whole_o));
+        p.whole_lse[s] = reinterpret_cast<float*>(take(plan.whole_lse));
+    }
+    p.q_b = a->q_stride[0], p.q_h = a->q_stride[1], p.o_b = a->o_stride[0], p.o_h = a->o_stride[1];
+    p.lse_b = a->lse != nullptr ? a->lse_stride[0] : 0;
+    p.B = (int32_t)a->B, p.Hq = (int32_t)a->Hq, p.Hkv = (int32_t)a->Hkv, p.group = (int32_t)(a->Hq / a->Hkv);
+    p.groups = (int32_t)a->groups, p.per = (int32_t)(a->B / a->groups);
+    p.d = (int32_t)a->D;
+    p.c = sp.scale * kLog2e;
+    p.q_and = sp.q_and, p.q_xor = sp.q_xor;
+    const bool wide = plan.kernel_d == 128;
+    switch (a->dtype) {
+        case DTATTN_BF16: return wide ? launch_shared<bf16_t, 128>(p, plan.nc, stream) : launch_shared<bf16_t, 64>(p, plan.nc, stream);
+        case DTATTN_FP16: return wide ? launch_shared<f16_t, 128>(p, plan.nc, stream) : launch_shared<f16_t, 64>(p, plan.nc, stream);
+        default: return wide ? launch_shared<float, 128>(p, plan.nc, stream) : launch_shared<float, 64>(p, plan.nc, stream);
+    }
+}

@@ -7,6 +7,7 @@
 #include "cache_ops.h"
 #include "dtattn.h"
 #include "sdpa_op.h"
+#include "shared_ops.h"
 
 namespace py = pybind11;
 using namespace dtorch_amd::core;
@@ -34,6 +35,17 @@ void BindSerialisation(C& cls) {
         .def_static("from_bytes", [](const py::bytes& b) { return FromBytes<P>(std::string(b)); })
         .def(py::pickle([](const P& p) { return py::make_tuple(py::bytes(ToBytes(p))); },
                         [](py::tuple t) { return FromBytes<P>(t[0].cast<std::string>()); }));
+}
+
+// An operator with its param.
+template <typename Op, typename P>
+void BindOp(py::module_& m, const char* name) {
+    py::class_<Op>(m, name)
+        .def(py::init<P>(), py::arg("param"))
+        .def_property_readonly("param", &Op::Param)
+        .def("compute", [](const Op& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
 }
 
 }  // namespace
@@ -242,6 +254,54 @@ PYBIND11_MODULE(_dtattn_host, m) {
         .def("compute", [](const KvCacheEvictOp& op, const std::vector<std::optional<at::Tensor>>& in) {
             return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
         });
+
+    // Shared pages, a shared prefix and selected key blocks.
+    auto fork = py::class_<KvPagesForkParam>(m, "KvPagesForkParam").def(py::init<>());
+    BindSerialisation<KvPagesForkParam>(fork);
+    auto compact = py::class_<KvPagesCompactParam>(m, "KvPagesCompactParam").def(py::init<>());
+    BindSerialisation<KvPagesCompactParam>(compact);
+    auto count = py::class_<TokenCountParam>(m, "TokenCountParam")
+                     .def(py::init<>())
+                     .def(py::init<int64_t>(), py::arg("tokens"))
+                     .def_readwrite("tokens", &TokenCountParam::tokens);
+    BindSerialisation<TokenCountParam>(count);
+    auto shp = py::class_<SdpaDecodeSharedParam>(m, "SdpaDecodeSharedParam")
+                   .def(py::init<>())
+                   .def(py::init<std::optional<double>>(), py::arg("scale"))
+                   .def_readwrite("scale", &SdpaDecodeSharedParam::scale);
+    BindSerialisation<SdpaDecodeSharedParam>(shp);
+    auto selp = py::class_<SelectKeyBlocksParam>(m, "SelectKeyBlocksParam")
+                    .def(py::init<>())
+                    .def(py::init<int64_t, int64_t, int64_t, std::optional<double>>(), py::arg("keep"), py::arg("recent"), py::arg("block"),
+                         py::arg("scale") = std::nullopt)
+                    .def_readwrite("keep", &SelectKeyBlocksParam::keep)
+                    .def_readwrite("recent", &SelectKeyBlocksParam::recent)
+                    .def_readwrite("block", &SelectKeyBlocksParam::block)
+                    .def_readwrite("scale", &SelectKeyBlocksParam::scale);
+    BindSerialisation<SelectKeyBlocksParam>(selp);
+    auto blp = py::class_<SdpaDecodeBlocksParam>(m, "SdpaDecodeBlocksParam")
+                   .def(py::init<>())
+                   .def(py::init<int64_t, std::optional<double>>(), py::arg("block"), py::arg("scale") = std::nullopt)
+                   .def_readwrite("block", &SdpaDecodeBlocksParam::block)
+                   .def_readwrite("scale", &SdpaDecodeBlocksParam::scale);
+    BindSerialisation<SdpaDecodeBlocksParam>(blp);
+
+    py::class_<KvPagesForkOp>(m, "KvPagesForkOp")
+        .def(py::init<>())
+        .def("compute", [](const KvPagesForkOp& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
+    py::class_<KvPagesCompactOp>(m, "KvPagesCompactOp")
+        .def(py::init<>())
+        .def("compute", [](const KvPagesCompactOp& op, const std::vector<std::optional<at::Tensor>>& in) {
+            return RunCompute([&](const TorchTensorOptArray& i, TorchTensorArray& o) { op.Compute(i, o); }, in);
+        });
+    BindOp<KvPagesReserveOp, TokenCountParam>(m, "KvPagesReserveOp");
+    BindOp<SdpaDecodeSharedOp, SdpaDecodeSharedParam>(m, "SdpaDecodeSharedOp");
+    BindOp<SdpaDecodeSharedPagedOp, SdpaDecodeSharedParam>(m, "SdpaDecodeSharedPagedOp");
+    BindOp<KeyBoundsOp, TokenCountParam>(m, "KeyBoundsOp");
+    BindOp<SelectKeyBlocksOp, SelectKeyBlocksParam>(m, "SelectKeyBlocksOp");
+    BindOp<SdpaDecodeBlocksOp, SdpaDecodeBlocksParam>(m, "SdpaDecodeBlocksOp");
 
     py::class_<DevicePeaks>(m, "DevicePeaks")
         .def_readonly("cu_count", &DevicePeaks::cuCount)

@@ -1,0 +1,395 @@
+// Key bounds of a cache's blocks, and the selection of blocks by them (formulas: dtattn.h, "attention over selected key blocks").
+//
+// No counterpart in the reference, which keeps no KV cache (python/dtorch/test/modules/llama.py:126-156).
+//
+// The bound: a token's key lies between k_min and k_max in every dimension, so q . k <= sum_d q_d x_d with x_d = k_max_d where
+// q_d > 0 and k_min_d elsewhere.  Reading 2 D values per block instead of D per token, it says which blocks can hold large scores.
+//
+// key_bounds_kernel: a workgroup per (block, sequence and kv head); every 16-byte chunk of a row belongs to one column of threads,
+// which meet by lane exchanges and then in LDS.  Bound by HBM: the rows are read once.
+// select_blocks_kernel: one workgroup per (sequence, kv head) scores its blocks, four lanes to a block, with the query's heads in LDS as
+// 64-bit numbers, and takes the largest scores by a radix select.  Sums in 64 bits are exact for 16-bit types (products have at
+// most 22 bits), so scores next to one another are told apart alike in any order of summation, and the vector units' 64-bit rate
+// is that of 32 bits.
+#include <algorithm>
+
+#include "decode_params.hpp"
+#include "radix_select.hpp"
+
+namespace dtattn {
+
+struct BlockCache {  // where blocks lie
+    const int32_t* table;  // NULL: padded
+    const int32_t* lengths;
+    int64_t bt_s;
+    int32_t capacity, page_shift, num_pages, block_shift;
+};
+
+struct BoundsParams {
+    BlockCache c;
+    const char* k;
+    char* lo;
+    char* hi;
+    int64_t k_b, k_h, k_s, lo_b, lo_h, lo_s, hi_b, hi_h, hi_s;  // bytes
+    int32_t Hkv, n_new, chunks;
+};
+
+struct SelectParams {
+    BlockCache c;
+    const char* q;
+    const char* lo;
+    const char* hi;
+    uint32_t* order;  // [B, Hkv, blocks_max], where LDS does not hold the scores
+    int32_t* kept;
+    int64_t q_b, q_h;  // elements
+    int64_t lo_b, lo_h, lo_s, hi_b, hi_h, hi_s;  // bytes
+    int32_t Hkv, group, d, keep, recent, blocks_max;
+    uint32_t q_and, q_xor;
+};
+
+namespace {
+
+__device__ __forceinline__ int tokens_in(const BlockCache& c, int64_t b) { return min(max(c.lengths[b], 0), c.capacity); }
+
+}  // namespace
+
+// W: chunks of a row's columns of threads, a power of two.
+template <typename T, int W>
+__global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
+    constexpr int E = 16 / (int)sizeof(T), ROWS = 256 / W;
+    __shared__ float red[4][2][W * E];
+    const int tid = threadIdx.x, col = tid % W, row = tid / W;
+    const int64_t bh = blockIdx.x, b = bh / p.Hkv;
+    const int h = (int)(bh % p.Hkv);
+    const int n = tokens_in(p.c, b);
+    const int block = 1 << p.c.block_shift;
+    const int64_t j = (max(n - p.n_new, 0) >> p.c.block_shift) + (int64_t)blockIdx.y;  // this workgroup's block
+    const int64_t t0 = j << p.c.block_shift;
+    if (t0 >= n) return;
+    const int rows = (int)min((int64_t)block, n - t0);
+    int64_t slot = b, r0 = t0;
+    if (p.c.table != nullptr) {
+        slot = p.c.table[b * p.c.bt_s + (t0 >> p.c.page_shift)];
+        r0 = t0 & ((1 << p.c.page_shift) - 1);
+        if (slot < 0 || slot >= p.c.num_pages) return;
+    }
+    const char* k = p.k + slot * p.k_b + h * p.k_h + r0 * p.k_s + col * 16;
+    float lo[E], hi[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) lo[e] = __builtin_inff(), hi[e] = kNegInf;
+    if (col < p.chunks) {
+        constexpr int PER = 4;  // rows in flight
+        for (int r = row; r < rows; r += ROWS * PER) {
+            u32x4 w[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) w[i] = ld16(k + min(r + ROWS * i, rows - 1) * p.k_s);  // a row twice changes nothing
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                float x[E];
+                if constexpr (sizeof(T) == 4) {
+                    const f32x4 f = __builtin_bit_cast(f32x4, w[i]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = f[e];
+                } else {
+                    unpack8<T>(w[i], x);
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) lo[e] = fminf(lo[e], x[e]), hi[e] = fmaxf(hi[e], x[e]);  // NaN is passed over
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (W == 8) lo[e] = fminf(lo[e], dpp_f<0x128>(lo[e])), hi[e] = fmaxf(hi[e], dpp_f<0x128>(hi[e]));  // lane ^ 8
+        if (W <= 16) lo[e] = -max_xor16(-lo[e]), hi[e] = max_xor16(hi[e]);
+        lo[e] = -max_xor32(-lo[e]), hi[e] = max_xor32(hi[e]);
+    }
+    if ((tid & 63) < W) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) red[tid >> 6][0][col * E + e] = lo[e], red[tid >> 6][1][col * E + e] = hi[e];
+    }
+    __syncthreads();
+    const int64_t jb = r0 >> p.c.block_shift;
+    T* out_lo = reinterpret_cast<T*>(p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s);
+    T* out_hi = reinterpret_cast<T*>(p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s);
+    for (int i = tid; i < p.chunks * E; i += 256) {
+        out_lo[i] = Elem<T>::from_f32(fminf(fminf(red[0][0][i], red[1][0][i]), fminf(red[2][0][i], red[3][0][i])));
+        out_hi[i] = Elem<T>::from_f32(fmaxf(fmaxf(red[0][1][i], red[1][1][i]), fmaxf(red[2][1][i], red[3][1][i])));
+    }
+}
+
+// HB: query heads at a time; IN_LDS: the scores are held in LDS (up to kSelectLds blocks).
+constexpr int kSelectLds = 4096;
+
+template <typename T, int D, int HB, bool IN_LDS>
+__global__ void __launch_bounds__(kSelect) select_blocks_kernel(const SelectParams p) {
+    constexpr int E = 16 / (int)sizeof(T), NI = D / E / 4;  // chunks of a row per lane
+    __shared__ __attribute__((aligned(16))) double qd[HB][D];
+    __shared__ uint32_t held[IN_LDS ? kSelectLds : 1];
+    const int tid = threadIdx.x;
+    const int64_t bh = blockIdx.x, b = bh / p.Hkv;
+    const int h = (int)(bh % p.Hkv);
+    const int n = tokens_in(p.c, b);
+    const int blocks = (n + (1 << p.c.block_shift) - 1) >> p.c.block_shift;
+    int32_t* kept = p.kept + bh * p.keep;
+    if (blocks <= p.keep) {
+        for (int i = tid; i < p.keep; i += kSelect) kept[i] = i < blocks ? i : -1;
+        return;
+    }
+    const int cand = blocks - p.recent;
+    uint32_t* order = IN_LDS ? held : p.order + bh * p.blocks_max;
+    const int quad = tid >> 2, l = tid & 3;
+    const int in_page = p.c.page_shift - p.c.block_shift;  // log2 of a page's blocks
+    for (int g0 = 0; g0 < p.group; g0 += HB) {
+        if (g0 > 0) __syncthreads();  // the last heads have been used
+        for (int i = tid; i < HB * D; i += kSelect) {
+            const int g = min(g0 + i / D, p.group - 1), dim = i % D;  // a head twice changes nothing
+            double x = 0.;
+            if (dim < p.d) {
+                const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_b + (h * p.group + g) * p.q_h + dim;
+                if constexpr (sizeof(T) == 4) x = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, *q) & p.q_and) ^ p.q_xor);
+                else x = Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)((__builtin_bit_cast(uint16_t, *q) & p.q_and) ^ p.q_xor)));
+            }
+            qd[i / D][dim] = x;
+        }
+        __syncthreads();
+        for (int j = quad; j < cand; j += kSelect / 4) {
+            int64_t slot = b, jb = j;
+            if (p.c.table != nullptr) {
+                slot = min(max(p.c.table[b * p.c.bt_s + (j >> in_page)], 0), p.c.num_pages - 1);
+                jb = j & ((1 << in_page) - 1);
+            }
+            const char* lo = p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s;
+            const char* hi = p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s;
+            u32x4 wl[NI], wh[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int c = min(l + 4 * i, p.d / E - 1);  // past the head dim: a valid chunk, which meets zeros
+                wl[i] = ld16_nt(lo + 16 * c);
+                wh[i] = ld16_nt(hi + 16 * c);
+            }
+            asm volatile("" ::: "memory");  // the query's numbers stay in LDS: held over the loop, they would be spilled
+            double s[HB];
+#pragma unroll
+            for (int g = 0; g < HB; ++g) s[g] = 0.;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                float fl[E], fh[E];
+                if constexpr (sizeof(T) == 4) {
+                    const f32x4 a = __builtin_bit_cast(f32x4, wl[i]), c = __builtin_bit_cast(f32x4, wh[i]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) fl[e] = a[e], fh[e] = c[e];
+                } else {
+                    unpack8<T>(wl[i], fl);
+                    unpack8<T>(wh[i], fh);
+                }
+                const int dim = (l + 4 * i) * E;
+                const bool there = dim < p.d;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+#pragma unroll
+                    for (int g = 0; g < HB; ++g) {
+                        const double q = qd[g][dim + e];
+                        const double x = (double)(there ? (q > 0. ? fh[e] : fl[e]) : 0.f);
+                        s[g] = __builtin_fma(q, x, s[g]);
+                    }
+                }
+            }
+            float best = kNegInf;
+#pragma unroll
+            for (int g = 0; g < HB; ++g) {
+                s[g] += __shfl_xor(s[g], 1, 64);
+                s[g] += __shfl_xor(s[g], 2, 64);
+                best = fmaxf(best, (float)s[g]);  // NaN is passed over
+            }
+            if (l == 0) {
+                const uint32_t u = ordered(best);
+                order[j] = g0 == 0 ? u : max(order[j], u);
+            }
+        }
+    }
+    __syncthreads();
+    select_largest<0>(cand, p.keep - p.recent, p.recent, order, kept, [&](int i) { return order[i]; });
+}
+
+namespace {
+
+struct BlockSizes {
+    int64_t S_max, num_pages, page_size, max_pages, block_table_stride;
+    const int32_t* table;
+    const int32_t* lengths;
+    int32_t block;
+};
+
+int block_checks(const BlockSizes& a, const char* who, BlockCache* out) {
+    if (a.block < 16 || a.block > 256 || (a.block & (a.block - 1)) != 0)
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: block %d must be a power of two from 16 to 256", who, a.block);
+    out->table = a.table;
+    out->lengths = a.lengths;
+    out->bt_s = a.block_table_stride;
+    out->block_shift = __builtin_ctz((unsigned)a.block);
+    out->page_shift = 0, out->num_pages = 0;
+    if (a.table != nullptr) {
+        if (a.page_size < 16 || (a.page_size & (a.page_size - 1)) != 0 || a.page_size > (1 << 20))
+            return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: page_size %lld must be a power of two >= 16", who, (long long)a.page_size);
+        if (a.page_size < a.block)
+            return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: a page of %lld tokens does not hold a block of %d", who, (long long)a.page_size, a.block);
+        if (a.num_pages <= 0 || a.max_pages <= 0 || a.num_pages > 0x7fffffff || a.max_pages > (1 << 29) / a.page_size)
+            return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad page counts", who);
+        out->capacity = (int32_t)(a.max_pages * a.page_size);
+        out->page_shift = __builtin_ctzll((unsigned long long)a.page_size);
+        out->num_pages = (int32_t)a.num_pages;
+    } else {
+        if (a.S_max <= 0 || a.S_max > (1 << 29) || a.S_max % a.block != 0)
+            return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: S_max=%lld must be a positive multiple of the block of %d tokens", who, (long long)a.S_max, a.block);
+        out->capacity = (int32_t)a.S_max;
+    }
+    return DTATTN_OK;
+}
+
+// Rows of 16-byte chunks at 16-byte strides, D up to 128.
+int row_checks(int64_t D, int32_t dtype, const int64_t* strides, int n, uintptr_t bits, const char* who) {
+    if (dtype != DTATTN_BF16 && dtype != DTATTN_FP16 && dtype != DTATTN_FP32)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: dtype %d not supported (bf16, fp16, fp32)", who, dtype);
+    const int64_t esz = dtype == DTATTN_FP32 ? 4 : 2;
+    if (D <= 0 || D > 128 || (D * esz) % 16 != 0)
+        return fail(DTATTN_ERR_UNSUPPORTED, "%s: head dim %lld not supported (up to 128, a multiple of 16 bytes)", who, (long long)D);
+    for (int i = 0; i < n; ++i)
+        if (strides[i] < 0 || (strides[i] * esz) % 16 != 0)
+            return fail(DTATTN_ERR_UNSUPPORTED, "%s: strides must be multiples of 16 bytes", who);
+    if (bits & 15) return fail(DTATTN_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned", who);
+    return DTATTN_OK;
+}
+
+template <typename T>
+void launch_bounds_of(const BoundsParams& p, dim3 grid, hipStream_t stream) {
+    if (p.chunks <= 8) hipLaunchKernelGGL((key_bounds_kernel<T, 8>), grid, dim3(256), 0, stream, p);
+    else if (p.chunks <= 16) hipLaunchKernelGGL((key_bounds_kernel<T, 16>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((key_bounds_kernel<T, 32>), grid, dim3(256), 0, stream, p);
+}
+
+template <typename T, int D, int HB>
+void launch_select(const SelectParams& p, dim3 grid, hipStream_t stream) {
+    if (p.blocks_max <= kSelectLds) hipLaunchKernelGGL((select_blocks_kernel<T, D, HB, true>), grid, dim3(kSelect), 0, stream, p);
+    else hipLaunchKernelGGL((select_blocks_kernel<T, D, HB, false>), grid, dim3(kSelect), 0, stream, p);
+}
+template <typename T, int D>
+void select_heads(const SelectParams& p, dim3 grid, hipStream_t stream) {
+    if (p.group == 1) launch_select<T, D, 1>(p, grid, stream);
+    else if (p.group <= 4) launch_select<T, D, 4>(p, grid, stream);
+    else launch_select<T, D, 8>(p, grid, stream);
+}
+template <typename T>
+void select_dims(const SelectParams& p, dim3 grid, hipStream_t stream) {
+    if (p.d <= 64) select_heads<T, 64>(p, grid, stream);
+    else select_heads<T, 128>(p, grid, stream);
+}
+
+template <typename Args>
+BlockSizes sizes_of(const Args* a) {
+    return {a->S_max, a->num_pages, a->page_size, a->max_pages, a->block_table_stride, a->block_table, a->lengths, a->block};
+}
+
+int64_t blocks_max_of(const dtattn_select_blocks_args* a) {
+    const int64_t capacity = a->block_table != nullptr ? a->max_pages * a->page_size : a->S_max;
+    return (capacity + a->block - 1) / a->block;
+}
+
+}  // namespace
+
+}  // namespace dtattn
+
+using namespace dtattn;
+
+extern "C" int dtattn_key_bounds(const dtattn_key_bounds_args* a, void* stream_) {
+    const char* who = "key_bounds";
+    if (a == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: args is NULL", who);
+    if (a->B < 0 || a->Hkv <= 0 || a->B > (1 << 24) || a->Hkv > (1 << 20) || a->n_new < 0) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
+    BoundsParams p = {};
+    int st = block_checks(sizes_of(a), who, &p.c);
+    if (st != DTATTN_OK) return st;
+    const int64_t strides[9] = {a->k_stride[0], a->k_stride[1], a->k_stride[2], a->min_stride[0], a->min_stride[1], a->min_stride[2],
+                                a->max_stride[0], a->max_stride[1], a->max_stride[2]};
+    st = row_checks(a->D, a->dtype, strides, 9,
+                    reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->k_min) | reinterpret_cast<uintptr_t>(a->k_max), who);
+    if (st != DTATTN_OK || a->B == 0 || a->n_new == 0) return st;
+    if (a->k_cache == nullptr || a->k_min == nullptr || a->k_max == nullptr || a->lengths == nullptr)
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    if (a->k_min == a->k_max || a->k_min == a->k_cache || a->k_max == a->k_cache)
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: keys and bounds cannot share memory", who);
+    const int64_t esz = a->dtype == DTATTN_FP32 ? 4 : 2;
+    p.k = reinterpret_cast<const char*>(a->k_cache);
+    p.lo = reinterpret_cast<char*>(a->k_min), p.hi = reinterpret_cast<char*>(a->k_max);
+    p.k_b = a->k_stride[0] * esz, p.k_h = a->k_stride[1] * esz, p.k_s = a->k_stride[2] * esz;
+    p.lo_b = a->min_stride[0] * esz, p.lo_h = a->min_stride[1] * esz, p.lo_s = a->min_stride[2] * esz;
+    p.hi_b = a->max_stride[0] * esz, p.hi_h = a->max_stride[1] * esz, p.hi_s = a->max_stride[2] * esz;
+    p.Hkv = (int32_t)a->Hkv, p.chunks = (int32_t)(a->D * esz / 16);
+    const int64_t n = std::min<int64_t>(a->n_new, p.c.capacity);
+    p.n_new = (int32_t)n;
+    const int64_t blocks = (n + a->block - 2) / a->block + 1, heads = a->B * a->Hkv;  // that n tokens touch, at most
+    if (heads > 0x7fffffff || blocks > 65535) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
+    const dim3 grid((unsigned)heads, (unsigned)blocks);
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    switch (a->dtype) {
+        case DTATTN_BF16: launch_bounds_of<bf16_t>(p, grid, stream); break;
+        case DTATTN_FP16: launch_bounds_of<f16_t>(p, grid, stream); break;
+        default: launch_bounds_of<float>(p, grid, stream);
+    }
+    return check_launch("key_bounds_kernel");
+}
+
+extern "C" size_t dtattn_select_key_blocks_workspace_size(const dtattn_select_blocks_args* a) {
+    if (a == nullptr || a->B <= 0 || a->Hkv <= 0 || a->block <= 0) return 0;
+    const int64_t blocks = blocks_max_of(a);
+    return blocks <= kSelectLds ? 0 : ((size_t)a->B * a->Hkv * blocks * sizeof(uint32_t) + 255) & ~(size_t)255;
+}
+
+extern "C" int dtattn_select_key_blocks(const dtattn_select_blocks_args* a, void* stream_) {
+    const char* who = "select_key_blocks";
+    if (a == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: args is NULL", who);
+    if (a->B < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->B > (1 << 24) || a->Hq > (1 << 20)) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
+    if (a->Hq % a->Hkv != 0) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: Hq is not a multiple of Hkv", who);
+    SelectParams p = {};
+    int st = block_checks(sizes_of(a), who, &p.c);
+    if (st != DTATTN_OK) return st;
+    if (a->recent < a->block || a->keep < a->recent || a->keep % a->block != 0 || a->recent % a->block != 0 || a->keep > (1 << 29))
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: keep %lld and recent %lld must be multiples of the block of %d tokens with block <= recent <= keep",
+                    who, (long long)a->keep, (long long)a->recent, a->block);
+    const int64_t strides[8] = {a->q_stride[0], a->q_stride[1], a->min_stride[0], a->min_stride[1], a->min_stride[2],
+                                a->max_stride[0], a->max_stride[1], a->max_stride[2]};
+    st = row_checks(a->D, a->dtype, strides, 8,
+                    reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_min) | reinterpret_cast<uintptr_t>(a->k_max), who);
+    if (st != DTATTN_OK) return st;
+    ScalePlan sp;
+    st = plan_scale(a->scale, a->D, a->dtype == DTATTN_FP32 ? kSign32 : kSign16, &sp);
+    if (st != DTATTN_OK || a->B == 0) return st;
+    if (a->q == nullptr || a->k_min == nullptr || a->k_max == nullptr || a->lengths == nullptr || a->blocks == nullptr)
+        return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    if (a->B * a->Hkv > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
+    const size_t need = dtattn_select_key_blocks_workspace_size(a);
+    if (need > 0) {
+        if (a->workspace == nullptr || a->workspace_bytes < need)
+            return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, a->workspace_bytes);
+        if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(DTATTN_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+    }
+    const int64_t esz = a->dtype == DTATTN_FP32 ? 4 : 2;
+    p.q = reinterpret_cast<const char*>(a->q);
+    p.lo = reinterpret_cast<const char*>(a->k_min), p.hi = reinterpret_cast<const char*>(a->k_max);
+    p.order = reinterpret_cast<uint32_t*>(a->workspace);
+    p.kept = a->blocks;
+    p.q_b = a->q_stride[0], p.q_h = a->q_stride[1];
+    p.lo_b = a->min_stride[0] * esz, p.lo_h = a->min_stride[1] * esz, p.lo_s = a->min_stride[2] * esz;
+    p.hi_b = a->max_stride[0] * esz, p.hi_h = a->max_stride[1] * esz, p.hi_s = a->max_stride[2] * esz;
+    p.Hkv = (int32_t)a->Hkv, p.group = (int32_t)(a->Hq / a->Hkv), p.d = (int32_t)a->D;
+    p.keep = (int32_t)(a->keep / a->block), p.recent = (int32_t)(a->recent / a->block);
+    p.blocks_max = (int32_t)blocks_max_of(a);
+    p.q_and = sp.q_and, p.q_xor = sp.q_xor;
+    const dim3 grid((unsigned)(a->B * a->Hkv));
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    switch (a->dtype) {
+        case DTATTN_BF16: select_dims<bf16_t>(p, grid, stream); break;
+        case DTATTN_FP16: select_dims<f16_t>(p, grid, stream); break;
+        default: select_dims<float>(p, grid, stream);
+    }
+    return check_launch("select_blocks_kernel");
+}

@@ -12,7 +12,7 @@
 #include <algorithm>
 
 #include "decode_params.hpp"
-#include "fp8_cache.hpp"
+#include "radix_select.hpp"
 
 namespace dtattn {
 
@@ -34,33 +34,6 @@ struct EvictParams {
 
 namespace {
 
-constexpr int kSelect = 1024;
-
-// Floats as unsigned numbers of the same order; NaN as -inf, -0 as 0.
-__device__ __forceinline__ uint32_t ordered(float x) {
-    if (x != x) x = kNegInf;
-    const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-// Exclusive prefix sum over the workgroup (kSelect threads), and the total.  `lds` is not in use before the call or, until every
-// thread is past a barrier, after it.
-__device__ __forceinline__ int scan_all(int v, int* lds, int& total) {
-    const int wave = threadIdx.x >> 6;
-    const int s = scan64(v);
-    if ((threadIdx.x & 63) == 63) lds[wave] = s;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < kSelect / 64; ++i) {
-        const int t = lds[i];
-        before += i < wave ? t : 0;
-        total += t;
-    }
-    return before + s - v;
-}
-
 // Every wave's loads have returned (a barrier alone orders what they see, not when they are done).
 __device__ __forceinline__ void read_all() {
     wait_vmem();
@@ -74,10 +47,6 @@ __device__ __forceinline__ int tokens_of(const EvictParams& p, int64_t b) { retu
 // The candidates' weights: PER per thread in registers (candidate PER * tid + k), or PER = 0 in memory.
 template <int PER>
 __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictParams p) {
-    constexpr int BINS = 2048;
-    __shared__ int hist[3][BINS];  // one a round: nothing is cleared between them
-    __shared__ int waves[4][kSelect / 64];
-    __shared__ int found[3][2];
     const int tid = threadIdx.x;
     const int64_t bh = blockIdx.x, b = bh / p.Hkv;
     const int h = (int)(bh % p.Hkv);
@@ -91,8 +60,6 @@ __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictPar
         return;
     }
     const int cand = blocks - p.recent;  // candidates: 0 .. cand - 1, all of them whole blocks
-    int need = p.keep - p.recent;        // of which so many stay; fewer than cand
-    uint32_t* order = p.order + bh * p.blocks_max;
     const float* w = p.w + b * p.w_b + h * p.w_h;
     auto weight = [&](int i) {
         if (p.block_shift == 0) return ordered(w[i]);
@@ -102,79 +69,7 @@ __global__ void __launch_bounds__(kSelect) kv_evict_select_kernel(const EvictPar
         for (int j = 0; j < (1 << p.block_shift); ++j) s += (double)x[j];
         return ordered((float)s);
     };
-    uint32_t mine[PER > 0 ? PER : 1];
-    if constexpr (PER > 0) {
-#pragma unroll
-        for (int k = 0; k < PER; ++k) mine[k] = PER * tid + k < cand ? weight(PER * tid + k) : 0u;
-    } else {
-        for (int i = tid; i < cand; i += kSelect) order[i] = weight(i);
-    }
-    for (int i = tid; i < 3 * BINS; i += kSelect) (&hist[0][0])[i] = 0;
-    __syncthreads();
-    // The need-th largest, some bits a round: `prefix` holds the bits found so far, and `need` how many stay of those that share them
-    uint32_t prefix = 0, mask = 0;
-    if (need > 0) {
-#pragma unroll
-        for (int round = 0; round < 3; ++round) {
-            const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bins = round < 2 ? 2048 : 1024;
-            auto count = [&](uint32_t u) {
-                if ((u & mask) == prefix) atomicAdd(&hist[round][(u >> shift) & (bins - 1)], 1);
-            };
-            if constexpr (PER > 0) {
-#pragma unroll
-                for (int k = 0; k < PER; ++k)
-                    if (PER * tid + k < cand) count(mine[k]);
-            } else {
-                for (int i = tid; i < cand; i += kSelect) count(order[i]);
-            }
-            __syncthreads();
-            // two bins a thread, from the largest down
-            const int hi = hist[round][BINS - 1 - 2 * tid], lo = hist[round][BINS - 2 - 2 * tid];
-            int total;
-            const int before = scan_all(hi + lo, waves[round], total);
-            if (before < need && before + hi + lo >= need) {
-                const bool upper = before + hi >= need;
-                found[round][0] = BINS - 1 - 2 * tid - (upper ? 0 : 1);
-                found[round][1] = need - before - (upper ? 0 : hi);
-            }
-            __syncthreads();
-            prefix |= (uint32_t)found[round][0] << shift;
-            mask |= (uint32_t)(bins - 1) << shift;
-            need = found[round][1];
-        }
-    } else {
-        prefix = 0xffffffffu;  // above every weight
-    }
-    // those above stay, and the first `need` of those at it
-    if constexpr (PER > 0) {
-        int counts = 0;  // above << 16, and at it: up to 16384 of both
-#pragma unroll
-        for (int k = 0; k < PER; ++k)
-            if (PER * tid + k < cand) counts += mine[k] > prefix ? 1 << 16 : mine[k] == prefix ? 1 : 0;
-        int total;
-        const int before = scan_all(counts, waves[3], total);
-        int above = before >> 16, at = before & 0xffff;
-#pragma unroll
-        for (int k = 0; k < PER; ++k)
-            if (PER * tid + k < cand) {
-                const bool over = mine[k] > prefix, same = mine[k] == prefix;
-                if (over || (same && at < need)) kept[above + min(at, need)] = PER * tid + k;
-                above += over, at += same;
-            }
-    } else {
-        int above = 0, at = 0;  // of the candidates before: one row of kSelect after another
-        for (int i0 = 0; i0 < cand; i0 += kSelect) {
-            const uint32_t u = i0 + tid < cand ? order[i0 + tid] : 0u;
-            const bool over = i0 + tid < cand && u > prefix, same = i0 + tid < cand && u == prefix;
-            int total;
-            const int before = scan_all(((int)over << 16) + (int)same, waves[3], total);
-            const int mine_at = at + (before & 0xffff);
-            if (over || (same && mine_at < need)) kept[above + (before >> 16) + min(mine_at, need)] = i0 + tid;
-            above += total >> 16, at += total & 0xffff;
-            __syncthreads();
-        }
-    }
-    for (int i = tid; i < p.recent; i += kSelect) kept[p.keep - p.recent + i] = cand + i;
+    select_largest<PER>(cand, p.keep - p.recent, p.recent, p.order + bh * p.blocks_max, kept, weight);
 }
 
 // A workgroup per (sequence, kv head, K or V, group of chunks), eight of them in a row on different XCDs; blockIdx.y = 1: the

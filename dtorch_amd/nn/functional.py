@@ -9,7 +9,9 @@ New entry points (no reference counterpart, see the host operators):
 ``scaled_dot_product_attention_with_lse``, ``decode_attention``, ``lse_merge``,
 ``ring_attention_step`` and ``quantize_fp8_per_head``; over an 8-bit KV cache ``kv_cache_append_fp8`` and
 ``decode_attention_fp8`` (and their paged forms); to bound a cache ``attention_weight_accumulate`` and
-``kv_cache_evict``.
+``kv_cache_evict``; over pages that sequences share ``kv_pages_fork``, ``kv_pages_reserve`` and ``kv_pages_compact``;
+over a prefix that sequences share ``decode_attention_shared`` (and ``_paged``); to read a long cache in part
+``kv_key_bounds``, ``select_key_blocks`` and ``decode_attention_blocks`` (and their paged forms).
 """
 from __future__ import annotations
 
@@ -232,6 +234,121 @@ def kv_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.
     """
     param = _h.KvCacheEvictParam(int(keep), int(recent), 0 if block is None else int(block))
     return _h.KvCacheEvictOp(param).compute([k_cache, v_cache, lengths, weights, k_scale, v_scale])[0]
+
+
+def kv_pages_fork(block_table: torch.Tensor, lengths: torch.Tensor, page_refs: torch.Tensor, parents: torch.Tensor) -> None:
+    """Sequences of a paged cache continue their parents, in place and without copying a page.
+
+    block_table int32 [B, max_pages] (slots outside the pool, such as -1, are empty), lengths int32 [B], page_refs int32
+    [num_pages] (how many slots name each page), parents int32 [B], all on the device.  Row b and lengths[b] become what row
+    parents[b] and its length were; a parent outside [0, B) frees the sequence.  B up to 8192.
+    """
+    _h.KvPagesForkOp().compute([block_table, lengths, page_refs, parents])
+
+
+def kv_pages_reserve(pools: Sequence[torch.Tensor], block_table: torch.Tensor, lengths: torch.Tensor, page_refs: torch.Tensor,
+                     n_new: int) -> torch.Tensor:
+    """Pages of their own for the next ``n_new`` tokens of every sequence (copy on write), in place.
+
+    pools: keys [num_pages, Hkv, page_size, D] first, then values, scales [num_pages, Hkv, page_size / block] or key bounds
+    [num_pages, Hkv, page_size / block, D]; up to 8.  Empty slots take free pages (page_refs 0), the lowest first, sequence by
+    sequence; a sequence whose next token falls into a page that others share takes a copy of its rows (of sequences that
+    all write a page the last one keeps it).  Returns int32 [1] on the device: the pages that were lacking (0: none); slots
+    that got none hold -1, and what was cached in them is lost to the sequence.  lengths stay as they are.
+    """
+    return _h.KvPagesReserveOp(_h.TokenCountParam(int(n_new))).compute([block_table, lengths, page_refs, *pools])[0]
+
+
+def kv_pages_compact(pools: Sequence[torch.Tensor], block_table: torch.Tensor, page_refs: torch.Tensor) -> torch.Tensor:
+    """Move the pages in use to the front of the pool, in place.
+
+    With U pages in use (page_refs > 0), those at or above index U move to the free ones below it, lowest to lowest, in
+    every pool, with their counts; the table follows.  pools as for kv_pages_reserve.  Returns U, int32 [1] on the device.
+    """
+    return _h.KvPagesCompactOp().compute([block_table, page_refs, *pools])[0]
+
+
+def decode_attention_shared(query: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, prefix_lengths: torch.Tensor,
+                            k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                            scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """decode_attention of sequences behind a prefix that they share, which is read once for all of them.
+
+    query [B, Hq, 1, D]; k_prefix / v_prefix [G, Hkv, S, D] with int32 prefix_lengths [G]: prefix g belongs to the B / G
+    sequences from g * B / G on; k_cache / v_cache [B, Hkv, S_max, D] with int32 lengths [B]: each sequence's tokens behind it.
+    bf16, fp16 or fp32, D up to 128.  Returns (O [B, Hq, 1, D], LSE [B, Hq] fp32).
+    """
+    op = _h.SdpaDecodeSharedOp(_h.SdpaDecodeSharedParam(None if scale is None else float(scale)))
+    return tuple(op.compute([query, k_prefix, v_prefix, prefix_lengths, k_cache, v_cache, lengths]))
+
+
+def decode_attention_shared_paged(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                                  lengths: torch.Tensor, prefix_lengths: torch.Tensor,
+                                  scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """decode_attention_paged of sequences whose first pages are the same, which are read once for all of them.
+
+    Arguments as for decode_attention_paged, and int32 prefix_lengths [G]: the first prefix_lengths[g] tokens (rounded down to whole
+    pages) of the B / G sequences from g * B / G on lie in the same pages.  lengths count all tokens; sequences of length 0
+    take no part.  Where a sequence is shorter than its group's prefix, the group shares no more than that sequence's whole pages.
+    """
+    op = _h.SdpaDecodeSharedPagedOp(_h.SdpaDecodeSharedParam(None if scale is None else float(scale)))
+    return tuple(op.compute([query, k_pages, v_pages, block_table, lengths, prefix_lengths]))
+
+
+def kv_key_bounds(k_cache: torch.Tensor, k_min: torch.Tensor, k_max: torch.Tensor, lengths: torch.Tensor, n_new: int) -> None:
+    """Refresh the key bounds of the blocks that hold the last ``n_new`` tokens of each sequence, in place.
+
+    k_cache [B, Hkv, S_max, D]; k_min / k_max [B, Hkv, S_max / block, D] of its dtype (the block, a power of two from 16 to 256,
+    follows from the shapes): the smallest and the largest value of each dimension over a block's tokens, NaN passed over.
+    Call it after the append of n_new tokens.
+    """
+    _h.KeyBoundsOp(_h.TokenCountParam(int(n_new))).compute([k_cache, k_min, k_max, lengths, None])
+
+
+def kv_key_bounds_paged(k_pages: torch.Tensor, k_min: torch.Tensor, k_max: torch.Tensor, block_table: torch.Tensor,
+                        lengths: torch.Tensor, n_new: int) -> None:
+    """kv_key_bounds of a paged cache: bounds [num_pages, Hkv, page_size / block, D]."""
+    _h.KeyBoundsOp(_h.TokenCountParam(int(n_new))).compute([k_pages, k_min, k_max, lengths, block_table])
+
+
+def select_key_blocks(query: torch.Tensor, k_min: torch.Tensor, k_max: torch.Tensor, lengths: torch.Tensor, keep: int, recent: int,
+                      block: int, scale: Optional[float] = None) -> torch.Tensor:
+    """The blocks of a cache whose keys can score highest for a single-token query, by their key bounds (kv_key_bounds).
+
+    For every kv head the last ``recent`` tokens' blocks and the best of the others, ``keep`` tokens in all (both multiples
+    of ``block``): int32 [B, Hkv, keep / block], ascending, -1 behind the blocks of a shorter sequence.  A block's score is the
+    largest over the kv head's query heads of the bound sum_d max(q_d k_min_d, q_d k_max_d), of equal ones the first
+    counts.  Only the sign of ``scale`` matters.
+    """
+    param = _h.SelectKeyBlocksParam(int(keep), int(recent), int(block), None if scale is None else float(scale))
+    return _h.SelectKeyBlocksOp(param).compute([query, k_min, k_max, lengths, None])[0]
+
+
+def select_key_blocks_paged(query: torch.Tensor, k_min: torch.Tensor, k_max: torch.Tensor, block_table: torch.Tensor,
+                            lengths: torch.Tensor, keep: int, recent: int, block: int,
+                            scale: Optional[float] = None) -> torch.Tensor:
+    """select_key_blocks of a paged cache (kv_key_bounds_paged)."""
+    param = _h.SelectKeyBlocksParam(int(keep), int(recent), int(block), None if scale is None else float(scale))
+    return _h.SelectKeyBlocksOp(param).compute([query, k_min, k_max, lengths, block_table])[0]
+
+
+def decode_attention_blocks(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                            blocks: torch.Tensor, block: int, scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """decode_attention over listed blocks of tokens only.
+
+    blocks int32 [B, Hkv, n]: kv head hk of sequence b attends to tokens blocks[b, hk, i] * block + (0 .. block - 1) before
+    lengths[b]; an index outside the sequence's blocks (-1) stands for none.  ``block`` is a power of two from 16 to 256.
+    bf16, fp16 or fp32, D up to 128.  Returns (O [B, Hq, 1, D], LSE [B, Hq] fp32) over those tokens.
+    """
+    op = _h.SdpaDecodeBlocksOp(_h.SdpaDecodeBlocksParam(int(block), None if scale is None else float(scale)))
+    return tuple(op.compute([query, k_cache, v_cache, lengths, blocks, None]))
+
+
+def decode_attention_blocks_paged(query: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                                  lengths: torch.Tensor, blocks: torch.Tensor, block: int,
+                                  scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """decode_attention_blocks over a paged cache whose pages hold whole blocks."""
+    op = _h.SdpaDecodeBlocksOp(_h.SdpaDecodeBlocksParam(int(block), None if scale is None else float(scale)))
+    return tuple(op.compute([query, k_pages, v_pages, lengths, blocks, block_table]))
 
 
 def lse_merge(outs: Sequence[torch.Tensor], lses: Sequence[torch.Tensor],

@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define DTATTN_ABI_VERSION 12
+#define DTATTN_ABI_VERSION 13
 
 /* Softmax scale fields (ABI version 8): NaN selects 1/sqrt(D) (computed in double and rounded once to
  * float, as libtorch computes its default, from ABI version 10); any finite value is used as given,
@@ -447,6 +447,204 @@ typedef struct {
 
 size_t dtattn_kv_evict_workspace_size(const dtattn_kv_evict_args* args);
 int dtattn_kv_evict(const dtattn_kv_evict_args* args, void* stream);
+
+/* ---- pages that sequences share (ABI version 13) ------------------------------------------------------
+ *
+ * Block tables, lengths and reference counts on the device: page_refs[p] is the number of table slots that name page p, 0 for a
+ * free page.  A slot outside [0, num_pages) is empty.  The calls below keep the counts in step with the table, change nothing
+ * else, and can be captured.
+ *
+ * Fork: row b of the table and lengths[b] become what row parents[b] and lengths[parents[b]] were; a parent outside [0, B) frees the
+ * sequence (every slot -1, length 0).  No page is copied: a page that several sequences are about to write is dtattn_kv_pages_reserve's
+ * matter.  B up to 8192. */
+typedef struct {
+    int32_t* block_table;    /* [B, max_pages], slot stride 1 */
+    int32_t* lengths;        /* [B] */
+    int32_t* page_refs;      /* [num_pages] */
+    const int32_t* parents;  /* [B] */
+    int64_t B, max_pages, num_pages;
+    int64_t block_table_stride;
+} dtattn_kv_fork_args;
+
+int dtattn_kv_pages_fork(const dtattn_kv_fork_args* args, void* stream);
+
+/* One array of pages: [num_pages, heads, page_size / row_tokens] rows of row_bytes bytes.  Keys and values have a row per token
+ * (row_tokens 1); scales and key bounds one per block of row_tokens tokens.  Addresses, strides and row_bytes are multiples of 4. */
+typedef struct {
+    void* data;
+    int64_t heads, row_bytes, row_tokens;
+    int64_t page_stride, head_stride, row_stride; /* bytes */
+} dtattn_page_pool;
+
+#define DTATTN_MAX_PAGE_POOLS 8
+
+/* Reserve: pages of their own for the next n_new tokens of every sequence.  The slots of positions lengths[b] to
+ * lengths[b] + n_new - 1 (those inside the table; lengths clamped to [0, max_pages * page_size]) are taken in the order of b and then
+ * of the slot.  An empty one takes a free page.  One whose page is shared takes a free page as well, so long as others still name
+ * the page: of sequences that all write a page, the last one keeps it.  The rows of the tokens that the sequence has in such a page
+ * are copied, in every pool.  Free pages are taken from the lowest index up; once they run out, slots that need one become -1 (tokens
+ * written through them are dropped, those they held are lost to the sequence), and *short_by says how many (0 otherwise).
+ * A copied row's other bytes, and rows behind a sequence's tokens, are left as they were. */
+typedef struct {
+    dtattn_page_pool pools[DTATTN_MAX_PAGE_POOLS];
+    int32_t n_pools;
+    int32_t* block_table;    /* [B, max_pages], slot stride 1 */
+    const int32_t* lengths;  /* [B] */
+    int32_t* page_refs;      /* [num_pages] */
+    int32_t* short_by;       /* [1] */
+    int64_t B, max_pages, num_pages, page_size, n_new;
+    int64_t block_table_stride;
+    void* workspace;         /* >= dtattn_kv_pages_reserve_workspace_size(args) bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} dtattn_kv_reserve_args;
+
+size_t dtattn_kv_pages_reserve_workspace_size(const dtattn_kv_reserve_args* args);
+int dtattn_kv_pages_reserve(const dtattn_kv_reserve_args* args, void* stream);
+
+/* Compact: with U pages in use, those at or above index U move to the free ones below it, the lowest to the lowest, with their
+ * reference counts, and the table follows.  *used becomes U.  What the pages left behind hold stays. */
+typedef struct {
+    dtattn_page_pool pools[DTATTN_MAX_PAGE_POOLS];
+    int32_t n_pools;
+    int32_t* block_table;    /* [B, max_pages], slot stride 1 */
+    int32_t* page_refs;      /* [num_pages] */
+    int32_t* used;           /* [1] */
+    int64_t B, max_pages, num_pages, page_size;
+    int64_t block_table_stride;
+    void* workspace;         /* >= dtattn_kv_pages_compact_workspace_size(args) bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} dtattn_kv_compact_args;
+
+size_t dtattn_kv_pages_compact_workspace_size(const dtattn_kv_compact_args* args);
+int dtattn_kv_pages_compact(const dtattn_kv_compact_args* args, void* stream);
+
+/* ---- attention over a shared prefix (ABI version 13) --------------------------------------------------
+ *
+ * Single-token attention (dtattn_decode_splitkv's formula) of B sequences in `groups` equal groups of consecutive ones, whose
+ * sequences share their first tokens.  Those are read once for the group's query heads together, and each sequence's own tokens
+ * behind them as by the decode; both parts meet by their LSE in fp32, and O is rounded once.
+ *
+ * Padded (block_table NULL): sequence b attends to the first prefix_lengths[g] rows of k_prefix[g], v_prefix[g] and to the first
+ * lengths[b] rows of k_cache[b], v_cache[b], g = b / (B / groups).
+ * Paged: lengths[b] counts all of a sequence's tokens, and the first prefix_lengths[g] of them, rounded down to whole pages, lie in
+ * the same pages for every sequence of the group with any tokens (the slots of its first such sequence are read).  Where a sequence with
+ * tokens is shorter than that, the whole group shares as many whole pages as that sequence fills, no more.
+ * Lengths are clamped to their capacity, page ids into the pool.  No rows: O = 0, LSE = -inf.
+ * D up to 128, a multiple of 16 bytes; up to 2048 groups.  16-bit types: scores, softmax statistics and accumulators are fp32, and P
+ * enters the second product as two numbers of its type (its rounding and the remainder's).  FP32: fp32 matrix instructions. */
+typedef struct {
+    const void* q;           /* [B, Hq, 1, D], 16-byte aligned, strides multiples of 16 bytes */
+    const void* k_prefix;    /* padded: [groups, Hkv, S_prefix, D] */
+    const void* v_prefix;
+    const void* k_cache;     /* padded: [B, Hkv, S_max, D]; paged: [num_pages, Hkv, page_size, D] */
+    const void* v_cache;
+    const int32_t* block_table;    /* [B, max_pages], slot stride 1; NULL: padded */
+    const int32_t* prefix_lengths; /* [groups] */
+    const int32_t* lengths;  /* [B] */
+    void* o;                 /* [B, Hq, 1, D] */
+    float* lse;              /* [B, Hq] fp32, head stride 1; may be NULL */
+    int64_t B, groups, Hq, Hkv, D;
+    int64_t S_prefix, S_max;
+    int64_t num_pages, page_size, max_pages;
+    int64_t q_stride[2];     /* B, H (elements) */
+    int64_t k_prefix_stride[3], v_prefix_stride[3]; /* group, H, row (elements) */
+    int64_t k_stride[3], v_stride[3]; /* (B | page), H, row (elements) */
+    int64_t o_stride[2];     /* B, H */
+    int64_t lse_stride[1];   /* B */
+    int64_t block_table_stride;
+    int32_t dtype;           /* BF16, FP16 or FP32 */
+    float scale;             /* NaN means 1/sqrt(D) */
+    void* workspace;         /* >= dtattn_decode_shared_workspace_size(args, stream) bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} dtattn_decode_shared_args;
+
+/* Workspace of a call on `stream`'s device; reads the sizes and `block_table` (whether it is NULL) of `args` only. */
+size_t dtattn_decode_shared_workspace_size(const dtattn_decode_shared_args* args, void* stream);
+int dtattn_decode_shared(const dtattn_decode_shared_args* args, void* stream);
+
+/* ---- attention over selected key blocks (ABI version 13) ----------------------------------------------
+ *
+ * Bounds: for every block of `block` tokens (a power of two from 16 to 256) that holds one of the last n_new of lengths[b] tokens, k_min
+ * and k_max become the smallest and the largest value of each dimension over the block's tokens (rows at or past lengths[b] are not
+ * read; NaN is passed over, and a dimension of nothing else gets +inf and -inf).  Other blocks are left alone.  A block table's
+ * slots outside the pool are passed over. */
+typedef struct {
+    const void* k_cache;     /* [B, Hkv, S_max, D]; paged: [num_pages, Hkv, page_size, D] */
+    void* k_min;             /* [B, Hkv, S_max / block, D]; paged: [num_pages, Hkv, page_size / block, D]; dtype of the keys */
+    void* k_max;
+    const int32_t* block_table; /* NULL: padded */
+    const int32_t* lengths;
+    int64_t B, Hkv, D, n_new;
+    int64_t S_max;
+    int64_t num_pages, page_size, max_pages;
+    int64_t k_stride[3];     /* (B | page), H, row (elements) */
+    int64_t min_stride[3], max_stride[3]; /* (B | page), H, block (elements) */
+    int64_t block_table_stride;
+    int32_t block;
+    int32_t dtype;           /* BF16, FP16 or FP32 */
+} dtattn_key_bounds_args;
+
+int dtattn_key_bounds(const dtattn_key_bounds_args* args, void* stream);
+
+/* Selection: for each kv head of a sequence of ceil(lengths[b] / block) blocks, the indices of keep / block blocks in ascending
+ * order: the last recent / block ones, and of the others those with the largest score, of equal ones the lowest index.  With no more
+ * blocks than that all of them, and -1 behind.  A block's score is the largest over the kv head's query heads of
+ *   sum_d s q_d x_d,   x_d = k_max_d where s q_d > 0 and k_min_d elsewhere,   s = the sign of `scale` (0: every score is 0)
+ * which no score q . k of its tokens exceeds (times |scale|); sums are taken in 64 bits and rounded once to fp32, and a head whose
+ * sum is NaN is passed over (-inf where all are).  `keep` and `recent` are multiples of block, block <= recent <= keep. */
+typedef struct {
+    const void* q;           /* [B, Hq, 1, D], 16-byte aligned, strides multiples of 16 bytes */
+    const void* k_min;       /* as above */
+    const void* k_max;
+    const int32_t* block_table; /* NULL: padded */
+    const int32_t* lengths;
+    int32_t* blocks;         /* [B, Hkv, keep / block] contiguous */
+    int64_t B, Hq, Hkv, D, keep, recent;
+    int64_t S_max;
+    int64_t num_pages, page_size, max_pages;
+    int64_t q_stride[2];     /* B, H (elements) */
+    int64_t min_stride[3], max_stride[3];
+    int64_t block_table_stride;
+    int32_t block;
+    int32_t dtype;
+    float scale;             /* only its sign counts; NaN means 1/sqrt(D) */
+    void* workspace;         /* >= dtattn_select_key_blocks_workspace_size(args) bytes (it may be 0), 256-byte aligned */
+    size_t workspace_bytes;
+} dtattn_select_blocks_args;
+
+size_t dtattn_select_key_blocks_workspace_size(const dtattn_select_blocks_args* args);
+int dtattn_select_key_blocks(const dtattn_select_blocks_args* args, void* stream);
+
+/* Single-token attention over the listed blocks of each kv head: dtattn_decode_splitkv's formula over the tokens
+ * blocks[b, hk, i] * block + (0 .. block - 1) that lie before lengths[b].  An index that is negative or past the sequence's blocks
+ * stands for no token; a block listed twice counts twice.  No token: O = 0, LSE = -inf.  Types as for dtattn_decode_shared. */
+typedef struct {
+    const void* q;
+    const void* k_cache;     /* [B, Hkv, S_max, D]; paged: [num_pages, Hkv, page_size, D] */
+    const void* v_cache;
+    const int32_t* block_table; /* NULL: padded */
+    const int32_t* lengths;
+    const int32_t* blocks;   /* [B, Hkv, n_blocks], index stride 1 */
+    void* o;
+    float* lse;              /* may be NULL */
+    int64_t B, Hq, Hkv, D, n_blocks;
+    int64_t S_max;
+    int64_t num_pages, page_size, max_pages;
+    int64_t q_stride[2];
+    int64_t k_stride[3], v_stride[3];
+    int64_t blocks_stride[2]; /* B, H */
+    int64_t o_stride[2];
+    int64_t lse_stride[1];
+    int64_t block_table_stride;
+    int32_t block;
+    int32_t dtype;
+    float scale;
+    void* workspace;         /* >= dtattn_decode_blocks_workspace_size(args, stream) bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} dtattn_decode_blocks_args;
+
+size_t dtattn_decode_blocks_workspace_size(const dtattn_decode_blocks_args* args, void* stream);
+int dtattn_decode_blocks(const dtattn_decode_blocks_args* args, void* stream);
 
 /* LSE merge of n partial attention blocks over the same queries.
  *
