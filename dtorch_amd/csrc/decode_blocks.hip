@@ -14,7 +14,9 @@ template <typename T, int D, bool TWO>
 __global__ void __launch_bounds__(64 * kPartWaves, 2) decode_blocks_kernel(const PartsParams p) {
     __shared__ __attribute__((aligned(16))) float red_o[kPartWaves][16][D + 4];
     __shared__ float red_m[kPartWaves][16], red_l[kPartWaves][16];
-    decode_part<T, D, 1, kListPart, TWO>(p, blockIdx.x, red_o, red_m, red_l, nullptr, nullptr);
+    const int U = p.B * part_places(p.list_units);
+    const PartShares sh(U * p.Hkv * p.nsub[1], p.shares);
+    if ((int)blockIdx.x < sh.n) decode_part<T, D, 1, kListPart, TWO>(p, PartLengths{nullptr, nullptr}, U, sh, blockIdx.x, red_o, red_m, red_l);
 }
 
 namespace {
@@ -29,8 +31,8 @@ BlocksPlan plan_blocks(const dtattn_decode_blocks_args* a, int cus) {
     r.kernel_d = a->D <= 64 ? 64 : 128;
     r.nsub = (int32_t)((a->Hq / a->Hkv + 15) / 16);
     r.units = (int32_t)((a->n_blocks * a->block + kPartUnit - 1) / kPartUnit);
-    const int64_t units = a->B * a->Hkv * r.nsub * r.units;
-    r.shares = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)2 * cus, units / kPartLeast));
+    const int64_t places = a->B * a->Hkv * r.nsub * (int64_t)(r.units + kPartExtra);
+    r.shares = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)2 * cus, places / kPartLeast));
     const size_t records = (size_t)2 * r.shares * 16;
     r.rec_o = part_up(records * r.kernel_d * sizeof(float));
     r.rec_lse = part_up(records * sizeof(float));
@@ -39,7 +41,7 @@ BlocksPlan plan_blocks(const dtattn_decode_blocks_args* a, int cus) {
 
 template <typename T, int D>
 int launch_blocks(const PartsParams& p, hipStream_t stream) {
-    const dim3 grid((unsigned)p.shares[1]), block(64 * kPartWaves);
+    const dim3 grid((unsigned)p.shares), block(64 * kPartWaves);
     if (p.block_shift < 5) hipLaunchKernelGGL((decode_blocks_kernel<T, D, true>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((decode_blocks_kernel<T, D, false>), grid, block, 0, stream, p);
     const int st = check_launch("decode_blocks_kernel");
@@ -98,7 +100,7 @@ extern "C" int dtattn_decode_blocks(const dtattn_decode_blocks_args* a, void* st
     const int cus = stream_cus(stream);
     if (cus <= 0) return fail(DTATTN_ERR_DEVICE, "%s: cannot tell the stream's device", who);
     const BlocksPlan plan = plan_blocks(a, cus);
-    if (a->B * a->Hkv * plan.nsub * (int64_t)plan.units >= ((int64_t)1 << 31) || a->B * a->Hq > 0x7fffffff)
+    if (a->B * a->Hkv * plan.nsub * (int64_t)(plan.units + kPartExtra) >= ((int64_t)1 << 31) || a->B * a->Hq > 0x7fffffff)
         return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many blocks", who);
     const size_t need = plan.rec_o + plan.rec_lse;
     if (a->workspace == nullptr || a->workspace_bytes < need)
@@ -120,7 +122,7 @@ extern "C" int dtattn_decode_blocks(const dtattn_decode_blocks_args* a, void* st
     p.lengths = a->lengths, p.list = a->blocks;
     p.list_b = a->blocks_stride[0], p.list_h = a->blocks_stride[1];
     p.n_list = (int32_t)a->n_blocks, p.list_units = plan.units, p.block_shift = __builtin_ctz((unsigned)a->block);
-    p.nsub[1] = plan.nsub, p.shares[1] = plan.shares, p.columns[1] = 16;
+    p.nsub[1] = plan.nsub, p.shares = plan.shares, p.columns[1] = 16;
     p.rec_o[1] = reinterpret_cast<float*>(a->workspace);
     p.rec_lse[1] = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + plan.rec_o);
     p.q_b = a->q_stride[0], p.q_h = a->q_stride[1], p.o_b = a->o_stride[0], p.o_h = a->o_stride[1];

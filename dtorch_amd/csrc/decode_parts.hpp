@@ -2,7 +2,8 @@
 // their own tokens behind it, and for listed blocks of tokens; and the kernel that merges what its shares leave.
 //
 // A part is a set of segments, (column set, sequence or group) pairs with a number of 32-token units each.  All units are laid end to
-// end and cut in equal shares, one per workgroup, whose four waves take its units in turn and meet in LDS where a segment ends.
+// end, each segment's behind places that stand for its own cost, and cut in equal shares, one per workgroup, whose four waves take its
+// units in turn and meet in LDS where a segment ends.
 // A segment's columns are query rows that read the same keys: the query heads of a kv head (a sequence's own tokens and listed blocks), or
 // those of all sequences of a group (the prefix), 16 NC of them.
 //
@@ -39,8 +40,10 @@ struct PartsParams {
     float* rec_lse[2];
     float* whole_o[2];  // [B, Hq, kernel D]: segments inside one share
     float* whole_lse[2];
-    int32_t* meta[2];   // units of all; then of each group or sequence: units before it, and its own
-    int32_t nsub[2], shares[2], columns[2];  // column sets of a kv head; shares at most; columns of a set
+    int32_t* meta[2];   // places of all, and shares at most; then of each group or sequence: places before it, and its units
+    int32_t nsub[2], columns[2];  // column sets of a kv head; columns of a set
+    int32_t shares;     // of both parts, or of the listed blocks, at most
+    int32_t weight[2];  // what a unit of each part costs
     int32_t capacity[2];
     int64_t q_b, q_h, o_b, o_h, lse_b, bt_s, list_b, list_h;  // elements
     int32_t B, Hq, Hkv, group, groups, per;  // per: sequences of a group
@@ -55,10 +58,12 @@ namespace {
 
 constexpr int kPartUnit = 32;  // tokens
 constexpr int kPartWaves = 4;
-constexpr int kPartLeast = kPartWaves;  // units of a share, at least
+constexpr int kPartLeast = kPartWaves + 1;  // places of a share, at least
 constexpr int kPartGroups = 2048;
+// What a segment costs besides its units, in units: its waves meet, and the last of them take turns that others have no unit for.
+constexpr int kPartExtra = 4;
 
-// V units in `n` shares of V / n or one more (all the longer ones first); the host keeps V below 2^31.
+// V places in `n` shares of V / n or one more (all the longer ones first); the host keeps V below 2^31.
 struct PartShares {
     int n, q, rem;
     __device__ __forceinline__ PartShares(int V, int most) {
@@ -67,7 +72,7 @@ struct PartShares {
         rem = V - q * n;
     }
     __device__ __forceinline__ int start(int r) const { return r * q + min(r, rem); }
-    __device__ __forceinline__ int of(int x) const {  // the share of unit x
+    __device__ __forceinline__ int of(int x) const {  // the share of place x
         const int big = rem * (q + 1);
         return x < big ? x / (q + 1) : rem + (x - big) / q;
     }
@@ -90,9 +95,256 @@ __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __
 
 }  // namespace
 
+// What both parts of a shared call need to know of the lengths.
+struct PartLengths {
+    int* eff;   // LDS, paged: tokens that a group shares: whole pages that each of its sequences with tokens has
+    int* lead;  // LDS, paged: the first of those sequences
+};
+
+__device__ __forceinline__ int part_clamp(int n, int most) { return min(max(n, 0), most); }
+
+__device__ __forceinline__ void part_lengths(const PartsParams& p, const PartLengths& at) {
+    if (p.table == nullptr) return;
+    const int tid = threadIdx.x;
+    for (int g = tid; g < p.groups; g += 256) at.eff[g] = at.lead[g] = 0x7fffffff;
+    __syncthreads();
+    for (int b = tid; b < p.B; b += 256) {
+        const int n = part_clamp(p.lengths[b], p.capacity[1]);
+        if (n > 0) {
+            atomicMin(&at.eff[b / p.per], n);
+            atomicMin(&at.lead[b / p.per], b);
+        }
+    }
+    __syncthreads();
+    for (int g = tid; g < p.groups; g += 256) {
+        const int n = at.eff[g] == 0x7fffffff ? 0 : min(at.eff[g], max(p.prefix[g], 0));
+        at.eff[g] = n >> p.page_shift << p.page_shift;
+    }
+    __syncthreads();
+}
+
+// Units of group or sequence z, per lane.
+template <int KIND>
+__device__ __forceinline__ int part_units(const PartsParams& p, const PartLengths& at, int z) {
+    const bool paged = p.table != nullptr;
+    int n;
+    if constexpr (KIND == kPrefixPart) n = paged ? at.eff[z] : part_clamp(p.prefix[z], p.capacity[0]);
+    else n = part_clamp(p.lengths[z], p.capacity[1]) - (paged ? at.eff[z / p.per] : 0);
+    return (max(n, 0) + kPartUnit - 1) / kPartUnit;
+}
+
+// Places of units and of what segments cost besides.
+__device__ __forceinline__ int part_places(int units) { return units > 0 ? units + kPartExtra : 0; }
+
+// Places of all groups or sequences; the wave that `tells` leaves them for the merge.
+template <int KIND>
+__device__ __forceinline__ int part_total(const PartsParams& p, const PartLengths& at, bool tells) {
+    const int Z = KIND == kPrefixPart ? p.groups : p.B, lane = threadIdx.x & 63;
+    int32_t* meta = p.meta[KIND == kPrefixPart ? 0 : 1];
+    int U = 0;
+    for (int j0 = 0; j0 < Z; j0 += 64) {
+        const int units = j0 + lane < Z ? part_units<KIND>(p, at, j0 + lane) : 0, own = part_places(units);
+        const int s = scan64(own);
+        if (tells && j0 + lane < Z) {
+            meta[2 + 2 * (j0 + lane)] = U + s - own;
+            meta[3 + 2 * (j0 + lane)] = units;
+        }
+        U += __builtin_amdgcn_readlane(s, 63);
+    }
+    return U;
+}
+
+// Walks the units of one part.  Lengths, page ids and lists are scalar loads, which leave the vector loads in flight alone.
+// NR: tiles of a unit that are found apart.
+template <int KIND, int NR>
+struct PartWalk {
+    static constexpr int S = KIND == kPrefixPart ? 0 : 1;
+    typedef const __attribute__((address_space(4))) int32_t cint32;
+    struct At {              // a unit
+        int slot, hk, z;     // slot: kv head * nsub + column set
+        int u, units;        // of the segment
+        int start, end, row; // the segment's tokens; its row of the table
+        int t[NR], rows[NR], page[NR];
+    };
+    const PartsParams& p;
+    const PartLengths& lens;
+    const int U, Z;
+    const bool paged;
+
+    __device__ __forceinline__ PartWalk(const PartsParams& p_, const PartLengths& lens_, int U_)
+        : p(p_), lens(lens_), U(U_), Z(KIND == kPrefixPart ? p_.groups : p_.B), paged(p_.table != nullptr) {}
+
+    // a segment's tokens: from `start` to before `end`
+    __device__ __forceinline__ int start_of(int z) const {
+        return KIND == kOwnPart && paged ? __builtin_amdgcn_readfirstlane(lens.eff[z / p.per]) : 0;
+    }
+    __device__ __forceinline__ int end_of(int z) const {
+        if constexpr (KIND == kPrefixPart) return paged ? __builtin_amdgcn_readfirstlane(lens.eff[z]) : part_clamp(((cint32*)p.prefix)[z], p.capacity[0]);
+        else return part_clamp(((cint32*)p.lengths)[z], p.capacity[1]);
+    }
+    __device__ __forceinline__ void enter(At& a) const {
+        a.hk = p.nsub[S] == 1 ? a.slot : a.slot / p.nsub[S];
+        a.start = start_of(a.z);
+        a.end = end_of(a.z);
+        a.units = KIND == kListPart ? p.list_units : (max(a.end - a.start, 0) + kPartUnit - 1) / kPartUnit;
+        a.row = KIND == kPrefixPart && paged && a.units > 0 ? __builtin_amdgcn_readfirstlane(lens.lead[a.z]) : a.z;
+    }
+    __device__ __forceinline__ void next(At& a) const {  // the next segment with units; there is one
+        do {
+            if (++a.z == Z) a.z = 0, ++a.slot;
+            enter(a);
+        } while (a.units == 0);
+    }
+    __device__ __forceinline__ void advance(At& a, int k) const {
+        a.u += k;
+        while (a.u >= a.units) {
+            a.u -= a.units;
+            next(a);
+        }
+    }
+    // The tokens of a unit's tile i, from `skip` on, of up to `most`; and the page that holds them.
+    __device__ __forceinline__ void find_tile(At& a, int i, int skip, int most) const {
+        cint32* const list = (cint32*)p.list;
+        const int x = a.u * kPartUnit + skip;
+        if constexpr (KIND == kListPart) {
+            const int e = x >> p.block_shift;
+            const int j = e < p.n_list ? list[a.z * p.list_b + a.hk * p.list_h + e] : -1;
+            const bool there = (uint32_t)j < (uint32_t)((a.end + (1 << p.block_shift) - 1) >> p.block_shift);
+            a.t[i] = there ? (j << p.block_shift) + (x & ((1 << p.block_shift) - 1)) : 0;
+            a.rows[i] = there ? part_clamp(a.end - a.t[i], most) : 0;
+        } else {
+            a.t[i] = a.start + x;
+            a.rows[i] = part_clamp(a.end - a.t[i], most);
+            if (a.rows[i] == 0) a.t[i] = 0;
+        }
+        a.page[i] = paged ? ((cint32*)p.table)[a.row * p.bt_s + (a.t[i] >> p.page_shift)] : a.z;
+    }
+    __device__ __forceinline__ void find(At& a) const {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) find_tile(a, i, 16 * i, kPartUnit / NR);
+    }
+    // The first row of a tile.
+    __device__ __forceinline__ const char* base(const At& a, int i, const char* x, int64_t sb, int64_t s_h, int64_t ss) const {
+        const int64_t where = paged ? part_clamp(a.page[i], p.num_pages - 1) : a.page[i];
+        const int row = paged ? a.t[i] & ((1 << p.page_shift) - 1) : a.t[i];
+        return x + where * sb + a.hk * s_h + row * ss;
+    }
+    // The first unit at or behind a place, and its index among all.
+    __device__ __forceinline__ int locate(int place, At& a) const {
+        const int lane = threadIdx.x & 63;
+        a.slot = place / U;
+        int x = place - a.slot * U, before;
+        if constexpr (KIND == kListPart) {
+            const int each = part_places(p.list_units);
+            a.z = x / each;
+            x -= a.z * each;
+            before = (a.slot * p.B + a.z) * p.list_units;
+        } else {
+            int total = 0, left = 0;  // units of all groups or sequences, and of those before z
+            bool found = false;
+            for (int j0 = 0; j0 < Z; j0 += 64) {
+                const int units = j0 + lane < Z ? part_units<KIND>(p, lens, j0 + lane) : 0, own = part_places(units);
+                const int s = scan64(own), su = scan64(units);
+                const uint64_t hit = __ballot(s > x);  // segments ending past x
+                if (!found && hit != 0) {
+                    const int l = __builtin_ctzll(hit);
+                    found = true;
+                    a.z = j0 + l;
+                    left = total + __builtin_amdgcn_readlane(su - units, l);
+                    x -= __builtin_amdgcn_readlane(s - own, l);
+                } else if (!found) {
+                    x -= __builtin_amdgcn_readlane(s, 63);
+                }
+                total += __builtin_amdgcn_readlane(su, 63);
+            }
+            before = a.slot * total + left;
+        }
+        a.u = max(x - kPartExtra, 0);
+        return before + a.u;
+    }
+    // A share's first unit, and how many it has.
+    __device__ __forceinline__ int units(const PartShares& sh, int r, At& a) const {
+        const int all = U * p.Hkv * p.nsub[S], end = sh.start(r + 1);
+        At behind;
+        const int u0 = locate(sh.start(r), a);
+        const int n = (end < all ? locate(end, behind) : locate(all - 1, behind) + 1) - u0;
+        // said to be the same in every lane, so that what follows from them stays in scalar registers
+        a.slot = __builtin_amdgcn_readfirstlane(a.slot), a.z = __builtin_amdgcn_readfirstlane(a.z), a.u = __builtin_amdgcn_readfirstlane(a.u);
+        return __builtin_amdgcn_readfirstlane(n);
+    }
+    __device__ __forceinline__ int rows_of_head() const { return KIND == kPrefixPart ? p.per * p.group : p.group; }
+    // The sequence and head of a segment's row.
+    __device__ __forceinline__ void where(int z, int hk, int row, int& b, int& hq) const {
+        const int i = KIND == kPrefixPart ? row / p.group : 0;
+        b = KIND == kPrefixPart ? z * p.per + i : z;
+        hq = hk * p.group + row - i * p.group;
+    }
+};
+
+// A row of the query, in pieces of 16 bytes whose order the keys share: piece 4 k + lane / 16 in w[k].
+template <typename T, int NK>
+__device__ __forceinline__ void part_query(const PartsParams& p, int b, int hq, u32x4 (&w)[NK]) {
+    const int g4 = (threadIdx.x & 63) >> 4, row_bytes = p.d * (int)sizeof(T);
+    const char* qp = p.q + (b * p.q_b + hq * p.q_h) * (int64_t)sizeof(T);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        const int at16 = 16 * (4 * k + g4);
+        w[k] = ld16(qp + (at16 < row_bytes ? at16 : 0));
+    }
+}
+// The same once it has arrived: signed, and zeros past the head dim.
+template <typename T, int NK>
+__device__ __forceinline__ void part_query_bits(const PartsParams& p, u32x4 (&w)[NK]) {
+    const int g4 = (threadIdx.x & 63) >> 4, row_bytes = p.d * (int)sizeof(T);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) w[k] = 16 * (4 * k + g4) < row_bytes ? q_bits(w[k], p.q_and, p.q_xor) : u32x4{0u, 0u, 0u, 0u};
+}
+
+// The running maxima of NC sets of columns rise to those of a unit's scores; what was summed on the old base is scaled to the new one.
+template <int NC, int DPL>
+__device__ __forceinline__ void part_rise(const f32x4 (&sc)[NC][2], float scale, float (&M)[NC], float (&l)[NC], f32x4 (&acc)[NC][DPL]) {
+    float Mn[NC];
+    bool grows = false;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        float mx = kNegInf;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) mx = fmaxf(mx, fmaxf(fmaxf(sc[c][tt][0], sc[c][tt][1]), fmaxf(sc[c][tt][2], sc[c][tt][3])));
+        Mn[c] = fmaxf(M[c], max_across_groups<16>(mx) * scale);
+        grows |= Mn[c] > M[c];
+    }
+    if (__ballot(grows) == 0) return;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const float alpha = fast_exp2(M[c] - (Mn[c] == kNegInf ? 0.f : Mn[c]));
+        M[c] = Mn[c];
+        l[c] *= alpha;
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) acc[c][j] *= alpha;
+    }
+}
+
+// P of a unit's scores in one set of columns, as numbers and (16 bits) as two matrix operands, and its part of the row sum.
+template <typename T>
+__device__ __forceinline__ void part_weights(const f32x4 (&sc)[2], float scale, float M, float& l, float (&pf)[8],
+                                             typename PartType<T>::vec8 (&pk)[PartType<T>::parts]) {
+    const float base = (M == kNegInf ? 0.f : M) - PartType<T>::offset;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        pf[i] = fast_exp2(__builtin_fmaf(sc[i >> 2][i & 3], scale, -base));
+        l += pf[i];
+        if constexpr (sizeof(T) == 2) {
+            pk[0][i] = Elem<T>::from_f32(pf[i]);
+            pk[1][i] = Elem<T>::from_f32(pf[i] - Elem<T>::to_f32(pk[0][i]));
+        }
+    }
+}
+
+// Share r of the segments of one part, U places in each of Hkv * nsub column sets.
 // NC: sets of 16 columns.  TWO: a unit's two tiles of 16 tokens may lie apart (pages or blocks of 16 tokens).
 template <typename T, int D, int NC, int KIND, bool TWO>
-__device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][D + 4], float (*red_m)[16], float (*red_l)[16], int* eff, int* lead) {
+__device__ void decode_part(const PartsParams& p, const PartLengths& lens, int U, const PartShares& sh, int r, float (*red_o)[16][D + 4],
+                            float (*red_m)[16], float (*red_l)[16]) {
     typedef typename PartType<T>::vec8 V8;
     constexpr bool kF32 = sizeof(T) == 4;
     constexpr int S = KIND == kPrefixPart ? 0 : 1;
@@ -102,138 +354,15 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
     constexpr int NR = TWO ? 2 : 1;              // buffer resources of a unit
     constexpr int PP = PartType<T>::parts;
     constexpr float kOff = PartType<T>::offset;
+    typedef PartWalk<KIND, NR> Walk;
+    typedef typename Walk::At At;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g4 = lane >> 4;
-    typedef const __attribute__((address_space(4))) int32_t cint32;
-    cint32* const lengths = (cint32*)p.lengths;
-    cint32* const prefix = (cint32*)p.prefix;
-    cint32* const table = (cint32*)p.table;
-    cint32* const list = (cint32*)p.list;
-    const bool paged = p.table != nullptr;
-    const int Z = KIND == kPrefixPart ? p.groups : p.B;
-    auto clamped = [](int n, int most) { return min(max(n, 0), most); };
-
-    // Tokens that a group shares: whole pages that each of its sequences with tokens has, and the first of those sequences
-    if constexpr (KIND != kListPart) {
-        if (paged) {
-            for (int g = tid; g < p.groups; g += 256) eff[g] = lead[g] = 0x7fffffff;
-            __syncthreads();
-            for (int b = tid; b < p.B; b += 256) {
-                const int n = clamped(p.lengths[b], p.capacity[1]);
-                if (n > 0) {
-                    atomicMin(&eff[b / p.per], n);
-                    atomicMin(&lead[b / p.per], b);
-                }
-            }
-            __syncthreads();
-            for (int g = tid; g < p.groups; g += 256) {
-                const int n = eff[g] == 0x7fffffff ? 0 : min(eff[g], max(p.prefix[g], 0));
-                eff[g] = n >> p.page_shift << p.page_shift;
-            }
-            __syncthreads();
-        }
-    }
-    // a segment's tokens: from `start` to before `end`
-    auto start_of = [&](int z) { return KIND == kOwnPart && paged ? __builtin_amdgcn_readfirstlane(eff[z / p.per]) : 0; };
-    auto end_of = [&](int z) {
-        if constexpr (KIND == kPrefixPart) return paged ? __builtin_amdgcn_readfirstlane(eff[z]) : clamped(prefix[z], p.capacity[0]);
-        else return clamped(lengths[z], p.capacity[1]);
-    };
-    auto units_of = [&](int z) {  // per lane
-        int n;
-        if constexpr (KIND == kPrefixPart) n = paged ? eff[z] : clamped(p.prefix[z], p.capacity[0]);
-        else n = clamped(p.lengths[z], p.capacity[1]) - (paged ? eff[z / p.per] : 0);
-        return (max(n, 0) + kPartUnit - 1) / kPartUnit;
-    };
-    int U = 0, own0 = 0, pre0 = 0;
-    if constexpr (KIND == kListPart) {
-        U = p.B * p.list_units;
-    } else {
-        const bool tells = share == 0 && wave == 0;
-        for (int j0 = 0; j0 < Z; j0 += 64) {
-            const int own = j0 + lane < Z ? units_of(j0 + lane) : 0;
-            const int s = scan64(own);
-            if (j0 == 0) own0 = own, pre0 = s;
-            if (tells && j0 + lane < Z) {
-                p.meta[S][1 + 2 * (j0 + lane)] = U + s - own;
-                p.meta[S][2 + 2 * (j0 + lane)] = own;
-            }
-            U += __builtin_amdgcn_readlane(s, 63);
-        }
-        if (tells && lane == 0) p.meta[S][0] = U;
-    }
-    if (U == 0) return;
-    const PartShares sh(U * p.Hkv * p.nsub[S], p.shares[S]);
-    const int r = share;
-    if (r >= sh.n) return;
-    const int u0 = sh.start(r), n = sh.start(r + 1) - u0;  // first unit and units of this workgroup
-
-    struct At {  // a unit
-        int slot, hk, z;     // slot: kv head * nsub + column set
-        int u, units;        // of the segment
-        int start, end, row; // row: of the table
-        int t[NR], rows[NR], page[NR];
-    };
-    auto enter = [&](At& a) {
-        a.hk = p.nsub[S] == 1 ? a.slot : a.slot / p.nsub[S];
-        a.start = start_of(a.z);
-        a.end = end_of(a.z);
-        a.units = KIND == kListPart ? p.list_units : (max(a.end - a.start, 0) + kPartUnit - 1) / kPartUnit;
-        a.row = KIND == kPrefixPart && paged && a.units > 0 ? __builtin_amdgcn_readfirstlane(lead[a.z]) : a.z;
-    };
-    auto next = [&](At& a) {  // the next segment with units; there is one
-        do {
-            if (++a.z == Z) a.z = 0, ++a.slot;
-            enter(a);
-        } while (a.units == 0);
-    };
-    auto advance = [&](At& a, int k) {
-        a.u += k;
-        while (a.u >= a.units) {
-            a.u -= a.units;
-            next(a);
-        }
-    };
-    auto find = [&](At& a) {  // the tokens of a unit, and the pages that hold them
-#pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const int x = a.u * kPartUnit + 16 * i;
-            if constexpr (KIND == kListPart) {
-                const int e = x >> p.block_shift;
-                const int j = e < p.n_list ? list[a.z * p.list_b + a.hk * p.list_h + e] : -1;
-                const bool there = (uint32_t)j < (uint32_t)((a.end + (1 << p.block_shift) - 1) >> p.block_shift);
-                a.t[i] = there ? (j << p.block_shift) + (x & ((1 << p.block_shift) - 1)) : 0;
-                a.rows[i] = there ? clamped(a.end - a.t[i], kPartUnit / NR) : 0;
-            } else {
-                a.t[i] = a.start + x;
-                a.rows[i] = clamped(a.end - a.t[i], kPartUnit / NR);
-                if (a.rows[i] == 0) a.t[i] = 0;
-            }
-            a.page[i] = paged ? table[a.row * p.bt_s + (a.t[i] >> p.page_shift)] : a.z;
-        }
-    };
+    const Walk walk(p, lens, U);
     At at;
-    at.slot = u0 / U;
-    int x = u0 - at.slot * U;
-    if constexpr (KIND == kListPart) {
-        at.z = x / p.list_units;
-        x -= at.z * p.list_units;
-    } else {
-        for (int j0 = 0;; j0 += 64) {
-            const int own = j0 == 0 ? own0 : j0 + lane < Z ? units_of(j0 + lane) : 0;
-            const int s = j0 == 0 ? pre0 : scan64(own);
-            const uint64_t hit = __ballot(s > x);  // segments ending past x
-            if (hit != 0) {
-                const int l = __builtin_ctzll(hit);
-                at.z = j0 + l;
-                x -= __builtin_amdgcn_readlane(s - own, l);
-                break;
-            }
-            x -= __builtin_amdgcn_readlane(s, 63);
-        }
-    }
-    at.u = x;
-    enter(at);
+    const int n = walk.units(sh, r, at);  // units of this workgroup
+    if (n == 0) return;
+    walk.enter(at);
 
     // byte offsets of this lane's loads from a tile's first row; pieces past the real head dim lie past any resource
     const int row_bytes = p.d * (int)sizeof(T);
@@ -247,16 +376,11 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
 
     u32x4 kr[2][NK];
     uint32_t vr[8][VW];
-    auto base_of = [&](const At& a, int i, const char* x, int64_t sb, int64_t s_h, int64_t ss) {
-        const int64_t where = paged ? clamped(a.page[i], p.num_pages - 1) : a.page[i];
-        const int row = paged ? a.t[i] & ((1 << p.page_shift) - 1) : a.t[i];
-        return x + where * sb + a.hk * s_h + row * ss;
-    };
     auto ld16b = [&](__amdgpu_buffer_rsrc_t rs, uint32_t off) { return KIND == kPrefixPart ? buf_ld16(rs, off) : buf_ld16_nt(rs, off); };
     auto load_k = [&](const At& a) {
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            const auto rs = make_rsrc(base_of(a, i, p.k[S], p.k_b[S], p.k_h[S], p.k_s[S]), a.rows[i] > 0 ? (uint32_t)(a.rows[i] - 1) * kp + (uint32_t)row_bytes : 0u);
+            const auto rs = make_rsrc(walk.base(a, i, p.k[S], p.k_b[S], p.k_h[S], p.k_s[S]), a.rows[i] > 0 ? (uint32_t)(a.rows[i] - 1) * kp + (uint32_t)row_bytes : 0u);
 #pragma unroll
             for (int tt = TWO ? i : 0; tt < (TWO ? i + 1 : 2); ++tt)
 #pragma unroll
@@ -266,7 +390,7 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
     auto load_v = [&](const At& a) {
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            const auto rs = make_rsrc(base_of(a, i, p.v[S], p.v_b[S], p.v_h[S], p.v_s[S]), a.rows[i] > 0 ? (uint32_t)(a.rows[i] - 1) * vp + (uint32_t)row_bytes : 0u);
+            const auto rs = make_rsrc(walk.base(a, i, p.v[S], p.v_b[S], p.v_h[S], p.v_s[S]), a.rows[i] > 0 ? (uint32_t)(a.rows[i] - 1) * vp + (uint32_t)row_bytes : 0u);
 #pragma unroll
             for (int tt = TWO ? i : 0; tt < (TWO ? i + 1 : 2); ++tt)
 #pragma unroll
@@ -292,42 +416,33 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
     u32x4 qf[NC][NK];
     At cur = at, nx = at;
     if (wave < n) {
-        if (wave > 0) advance(nx, wave);
-        find(nx);
+        if (wave > 0) walk.advance(nx, wave);
+        walk.find(nx);
         load_k(nx);
         load_v(nx);
     }
+    const int R = walk.rows_of_head();
+    auto load_q = [&](const At& a) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            int b, hq;
+            walk.where(a.z, a.hk, min(16 * NC * (a.slot - a.hk * p.nsub[S]) + 16 * c + col, R - 1), b, hq);
+            part_query<T, NK>(p, b, hq, qf[c]);
+        }
+    };
+    load_q(cur);
     int s = wave;  // this wave's next unit of the share
     for (int u = 0; u < n;) {
         const int m = min(cur.units - cur.u, n - u);  // units of the segment
-        const int hk = cur.hk, z = cur.z, sub = cur.slot - hk * p.nsub[S];
-        const int R = KIND == kPrefixPart ? p.per * p.group : p.group;
-        const int R0 = 16 * NC * sub;
+        const int hk = cur.hk, z = cur.z, R0 = 16 * NC * (cur.slot - hk * p.nsub[S]);
+        const bool whole = cur.u == 0 && m == cur.units;
         bool seen = false;
-        auto where = [&](int row, int& b, int& hq) {  // the sequence and head of a row
-            const int i = KIND == kPrefixPart ? row / p.group : 0;
-            b = KIND == kPrefixPart ? z * p.per + i : z;
-            hq = hk * p.group + row - i * p.group;
-        };
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             M[c] = kNegInf, l[c] = 0.f;
 #pragma unroll
             for (int j = 0; j < DPL; ++j) acc[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        if (s < u + m) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                int b, hq;
-                where(min(R0 + 16 * c + col, R - 1), b, hq);
-                const char* qp = p.q + (b * p.q_b + hq * p.q_h) * (int64_t)sizeof(T);
-#pragma unroll
-                for (int k = 0; k < NK; ++k) {
-                    const int at16 = 16 * (4 * k + g4);
-                    const u32x4 w = ld16(qp + (at16 < row_bytes ? at16 : 0));
-                    qf[c][k] = at16 < row_bytes ? q_bits(w, p.q_and, p.q_xor) : u32x4{0u, 0u, 0u, 0u};
-                }
-            }
+            part_query_bits<T, NK>(p, qf[c]);
         }
         for (; s < u + m; s += kPartWaves) {
             int rows[NR];
@@ -335,8 +450,8 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
             for (int i = 0; i < NR; ++i) rows[i] = nx.rows[i], seen |= rows[i] > 0;
             const bool more = s + kPartWaves < n;
             if (more) {
-                advance(nx, kPartWaves);
-                find(nx);
+                walk.advance(nx, kPartWaves);
+                walk.find(nx);
             }
             f32x4 sc[NC][2];
 #pragma unroll
@@ -369,73 +484,60 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
                             for (int c = 0; c < NC; ++c) sc[c][tt][i] = kNegInf;
                         }
             }
-            float Mn[NC];
-            bool grows = false;
+            part_rise<NC, DPL>(sc, p.c, M, l, acc);
+            // two tokens' values of one dim side by side
+            auto pair_up = [&](int w, V8* out) {
+                uint32_t a[4], b[4];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float mx = kNegInf;
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt) mx = fmaxf(mx, fmaxf(fmaxf(sc[c][tt][0], sc[c][tt][1]), fmaxf(sc[c][tt][2], sc[c][tt][3])));
-                Mn[c] = fmaxf(M[c], max_across_groups<16>(mx) * p.c);
-                grows |= Mn[c] > M[c];
-            }
-            if (__ballot(grows) != 0) {
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const float alpha = fast_exp2(M[c] - (Mn[c] == kNegInf ? 0.f : Mn[c]));
-                    M[c] = Mn[c];
-                    l[c] *= alpha;
-#pragma unroll
-                    for (int j = 0; j < DPL; ++j) acc[c][j] *= alpha;
+                for (int t = 0; t < 4; ++t) {
+                    a[t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x05040100u);
+                    b[t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x07060302u);
                 }
-            }
-            V8 vf[kF32 ? 1 : DPL];
-            if constexpr (!kF32) {
-                // two tokens' values of one dim side by side
+                out[0] = __builtin_bit_cast(V8, u32x4{a[0], a[1], a[2], a[3]});
+                out[1] = __builtin_bit_cast(V8, u32x4{b[0], b[1], b[2], b[3]});
+            };
+            // one set of columns leaves room for all operands, so that the values' registers take the next unit's at once
+            constexpr bool kAhead = !kF32 && NC == 1;
+            V8 vf[kAhead ? DPL : 2];
+            if constexpr (kAhead) {
 #pragma unroll
-                for (int w = 0; w < VW; ++w) {
-                    uint32_t a[4], b[4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        a[t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x05040100u);
-                        b[t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x07060302u);
-                    }
-                    vf[2 * w] = __builtin_bit_cast(V8, u32x4{a[0], a[1], a[2], a[3]});
-                    vf[2 * w + 1] = __builtin_bit_cast(V8, u32x4{b[0], b[1], b[2], b[3]});
-                }
+                for (int w = 0; w < VW; ++w) pair_up(w, &vf[2 * w]);
                 if (more) load_v(nx);
             }
+            V8 pk[NC][PP];
+            float pf[NC][8];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const float base = (M[c] == kNegInf ? 0.f : M[c]) - kOff;
-                float pf[8];
+            for (int c = 0; c < NC; ++c) part_weights<T>(sc[c], p.c, M[c], l[c], pf[c], pk[c]);
+            if constexpr (kF32) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    pf[i] = fast_exp2(__builtin_fmaf(sc[c][i >> 2][i & 3], p.c, -base));
-                    l[c] += pf[i];
-                }
-                if constexpr (kF32) {
+                for (int i = 0; i < 8; ++i)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
+                    for (int j = 0; j < DPL; ++j)
 #pragma unroll
-                        for (int j = 0; j < DPL; ++j) acc[c][j] = mfma_f32(__builtin_bit_cast(float, vr[i][j]), pf[i], acc[c][j]);
-                } else {
-                    V8 pk[PP];
+                        for (int c = 0; c < NC; ++c) acc[c][j] = mfma_f32(__builtin_bit_cast(float, vr[i][j]), pf[c][i], acc[c][j]);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        pk[0][i] = Elem<T>::from_f32(pf[i]);
-                        pk[PP - 1][i] = Elem<T>::from_f32(pf[i] - Elem<T>::to_f32(pk[0][i]));
-                    }
+                for (int w = 0; w < VW; ++w) {
+                    if constexpr (!kAhead) pair_up(w, vf);
 #pragma unroll
                     for (int h = 0; h < PP; ++h)
 #pragma unroll
-                        for (int j = 0; j < DPL; ++j) acc[c][j] = mfma16(vf[j], pk[h], acc[c][j]);
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int c = 0; c < NC; ++c) acc[c][2 * w + j] = mfma16(vf[kAhead ? 2 * w + j : j], pk[c][h], acc[c][2 * w + j]);
                 }
             }
-            if (kF32 && more) load_v(nx);
+            if (!kAhead && more) load_v(nx);
+        }
+        // the next segment's query is on its way while this one's waves meet
+        const bool cut_first = u == 0;
+        u += m;
+        if (u < n) {
+            cur.u = 0;
+            walk.next(cur);
+            load_q(cur);
         }
         // the waves meet, 16 columns at a time
-        const bool whole = cur.u == 0 && m == cur.units;
         const bool any = KIND != kListPart || __syncthreads_or(seen);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -469,7 +571,7 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
                     }
                 }
                 int b, hq;
-                where(R0 + 16 * c + g, b, hq);
+                walk.where(z, hk, R0 + 16 * c + g, b, hq);
                 const int dim = DPL * (tid & 15);
                 const bool direct = KIND == kListPart && whole;
                 const float lse = __builtin_fmaf(X - kOff, kLn2, __log2f(lt) * kLn2);
@@ -487,7 +589,7 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
                         }
                     if (p.lse != nullptr && (tid & 15) == 0) p.lse[b * p.lse_b + hq] = lse;
                 } else {
-                    const int64_t rec = whole ? (int64_t)b * p.Hq + hq : (int64_t)(2 * r + (u == 0 ? 0 : 1)) * (16 * NC) + 16 * c + g;
+                    const int64_t rec = whole ? (int64_t)b * p.Hq + hq : (int64_t)(2 * r + (cut_first ? 0 : 1)) * (16 * NC) + 16 * c + g;
                     float* op = (whole ? p.whole_o[S] : p.rec_o[S]) + rec * D + dim;
 #pragma unroll
                     for (int j = 0; j < DPL; j += 4) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
@@ -495,11 +597,168 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
                 }
             }
         }
-        u += m;
+        if (u < n) lds_barrier();  // every wave has read the others' before they write again
+    }
+}
+
+// 16-byte chunk c of row r of a tile in LDS lies at c ^ part_swizzle(r): without bank conflicts for the 16-byte reads of keys (16 rows, one
+// chunk) and the 8-byte transposed ones of values (rows 16 apart alike).
+template <int D>
+__device__ __forceinline__ int part_swizzle(int r) { return D == 128 ? 2 * (r & 7) + ((r >> 3) & 1) : (r >> 1) & 7; }
+
+// Share r of the prefix for many rows (16-bit types): the four waves hold 16 NC rows each, and a unit's keys and values go through LDS once
+// for all of them, by direct loads into a ring of three stages.  A unit then costs a wave half the instructions of the form above
+// (no addresses of its own, no pairing of values, which a transposed read replaces).
+template <typename T, int D, int NC>
+__device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, int U, const PartShares& sh, int r, T (*kv)[2][kPartUnit * D]) {
+    typedef typename Elem<T>::vec8 V8;
+    typedef typename Elem<T>::vec4 V4;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    typedef PartWalk<kPrefixPart, 1> Walk;
+    typedef typename Walk::At At;
+    constexpr int NK = D / 32, NV = D / 16, CH = D / 8, RPL = 64 / CH, NL = 8 / RPL;  // CH: chunks of a row; a wave's loads of 8 rows: NL of RPL
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g4 = lane >> 4;
+    const Walk walk(p, lens, U);
+    At cur;
+    const int n = walk.units(sh, r, cur);
+    if (n == 0) return;
+    walk.enter(cur);
+
+    // rows 8 wave .. 8 wave + 7 of a unit, which lie in its tile wave / 2
+    const uint32_t kp = (uint32_t)p.k_s[0], vp = (uint32_t)p.v_s[0];
+    uint32_t koff[NL], voff[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        const int row = 8 * wave + RPL * i + lane / CH, c = (lane % CH) ^ part_swizzle<D>(row);
+        const bool there = 8 * c < p.d;  // chunks past the real head dim come as zeros
+        koff[i] = there ? (uint32_t)(row & 15) * kp + (uint32_t)(16 * c) : 0xc0000000u;
+        voff[i] = there ? (uint32_t)(row & 15) * vp + (uint32_t)(16 * c) : 0xc0000000u;
+    }
+    auto issue = [&](int buf, At& a) {
+        walk.find_tile(a, 0, 16 * (wave >> 1), 16);
+        const uint32_t row_bytes = (uint32_t)(p.d * (int)sizeof(T));
+        const auto krs = make_rsrc(walk.base(a, 0, p.k[0], p.k_b[0], p.k_h[0], p.k_s[0]), a.rows[0] > 0 ? (uint32_t)(a.rows[0] - 1) * kp + row_bytes : 0u);
+        const auto vrs = make_rsrc(walk.base(a, 0, p.v[0], p.v_b[0], p.v_h[0], p.v_s[0]), a.rows[0] > 0 ? (uint32_t)(a.rows[0] - 1) * vp + row_bytes : 0u);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            buf_ld16_lds_async(krs, &kv[buf][0][(8 * wave + RPL * i) * D], koff[i]);
+            buf_ld16_lds_async(vrs, &kv[buf][1][(8 * wave + RPL * i) * D], voff[i]);
+        }
+    };
+    const int R = walk.rows_of_head();
+    u32x4 qf[NC][NK];
+    auto row_of = [&](const At& a, int c) { return 16 * NC * (kPartWaves * (a.slot - a.hk * p.nsub[0]) + wave) + 16 * c + col; };
+    auto load_q = [&](const At& a) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            int b, hq;
+            walk.where(a.z, a.hk, min(row_of(a, c), R - 1), b, hq);
+            part_query<T, NK>(p, b, hq, qf[c]);
+        }
+    };
+    load_q(cur);
+    At nx = cur;
+    issue(0, nx);
+    if (n > 1) {
+        walk.advance(nx, 1);
+        issue(1, nx);
+    }
+    f32x4 acc[NC][NV];
+    float M[NC], l[NC];
+    int buf = 0;
+    for (int u = 0; u < n;) {
+        const int m = min(cur.units - cur.u, n - u);
+        const bool whole = cur.u == 0 && m == cur.units, cut_first = u == 0;
+        const At seg = cur;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            M[c] = kNegInf, l[c] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) acc[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            part_query_bits<T, NK>(p, qf[c]);
+        }
+        for (int i = 0; i < m; ++i, ++u) {
+            // this wave's loads of stage u have landed when no more are left than those of stage u + 1; then everybody's
+            if (u + 1 < n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            lds_barrier();
+            if (u + 2 < n) {  // every wave is done with stage u - 1
+                walk.advance(nx, 1);
+                issue(buf == 0 ? 2 : buf - 1, nx);
+            }
+            const T* K = kv[buf][0];
+            const T* V = kv[buf][1];
+            f32x4 sc[NC][2];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                V8 kf[NK];
+#pragma unroll
+                for (int k = 0; k < NK; ++k) {
+                    const int row = 16 * tt + col;
+                    kf[k] = __builtin_bit_cast(V8, ld16(K + row * D + 8 * ((4 * k + g4) ^ part_swizzle<D>(row))));
+                }
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    sc[c][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < NK; ++k) sc[c][tt] = mfma16(kf[k], __builtin_bit_cast(V8, qf[c][k]), sc[c][tt]);
+                }
+            }
+            const int left = seg.end - seg.start - (seg.u + i) * kPartUnit;
+            if (left < kPartUnit) {
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (16 * tt + 4 * g4 + e >= left) {
+#pragma unroll
+                            for (int c = 0; c < NC; ++c) sc[c][tt][e] = kNegInf;
+                        }
+            }
+            part_rise<NC, NV>(sc, p.c, M, l, acc);
+            V8 pk[NC][2];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float pf[8];
+                part_weights<T>(sc[c], p.c, M[c], l[c], pf, pk[c]);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int row = 4 * g4 + (col >> 2), ch = (2 * j + ((col & 3) >> 1)) ^ part_swizzle<D>(row);
+                const int off = row * D + 8 * ch + 4 * (col & 1);
+                const V4 lo = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + off)));
+                const V4 hi = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + off + 16 * D)));
+                const V8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) acc[c][j] = mfma16(vf, pk[c][h], acc[c][j]);
+            }
+            buf = buf == 2 ? 0 : buf + 1;
+        }
         if (u < n) {
-            lds_barrier();  // every wave has read the others' before they write again
             cur.u = 0;
-            next(cur);
+            walk.next(cur);
+            load_q(cur);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const float lt = sum_across_groups<16>(l[c]);
+            const int row = row_of(seg, c);
+            if (row < R) {
+                int b, hq;
+                walk.where(seg.z, seg.hk, row, b, hq);
+                const float lse = __builtin_fmaf(M[c] - PartType<T>::offset, kLn2, __log2f(lt) * kLn2);
+                const float inv = lt == 0.f ? 0.f : 1.f / lt;  // every score -inf: a record of O = 0 that its LSE drops
+                const int in_set = 16 * NC * wave + 16 * c + col;
+                const int64_t rec = whole ? (int64_t)b * p.Hq + hq : (int64_t)(2 * r + (cut_first ? 0 : 1)) * (16 * NC * kPartWaves) + in_set;
+                float* op = (whole ? p.whole_o[0] : p.rec_o[0]) + rec * D + 4 * g4;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4*>(op + 16 * j) = acc[c][j] * inv;
+                if (g4 == 0) (whole ? p.whole_lse[0] : p.rec_lse[0])[rec] = lse;
+            }
         }
     }
 }
@@ -509,79 +768,73 @@ __device__ void decode_part(const PartsParams& p, int share, float (*red_o)[16][
 template <typename T, int D, int W, bool SHARED>
 __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsParams p) {
     constexpr int DL = D / 64;  // dims per lane
-    __shared__ float red[W > 1 ? W : 1][D];
+    __shared__ float red[W > 1 ? W : 1][D + 2];
     const int lane = threadIdx.x & 63, wave = W > 1 ? threadIdx.x >> 6 : 0;
     const int64_t pair = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (pair >= (int64_t)p.B * p.Hq) return;
     const int b = (int)(pair / p.Hq), hq = (int)(pair % p.Hq), hk = hq / p.group, g = hq - hk * p.group;
-    int64_t first[2] = {0, 0}, later[2] = {0, 0};  // the record of a part's first share, and of the one behind it
-    int ns[2] = {0, 0};
-    bool whole[2] = {false, false};
-#pragma unroll
-    for (int S = SHARED ? 0 : 1; S < 2; ++S) {
-        const int z = S == 0 ? b / p.per : b;
-        const int row = S == 0 ? (b - z * p.per) * p.group + g : g;
-        const int U = SHARED ? p.meta[S][0] : p.B * p.list_units;
-        const int before = SHARED ? p.meta[S][1 + 2 * z] : b * p.list_units, own = SHARED ? p.meta[S][2 + 2 * z] : p.list_units;
-        if (own == 0) continue;
-        const int cols = p.columns[S], sub = row / cols;
-        const PartShares sh(U * p.Hkv * p.nsub[S], p.shares[S]);
-        const int x0 = (hk * p.nsub[S] + sub) * U + before, r0 = sh.of(x0), r1 = sh.of(x0 + own - 1);
-        ns[S] = r1 - r0 + 1;
-        whole[S] = r0 == r1;
-        // share r0 holds the segment first only if it begins with it
-        first[S] = whole[S] ? pair : (int64_t)(2 * r0 + (sh.start(r0) < x0 ? 1 : 0)) * cols + row - sub * cols;
-        later[S] = (int64_t)2 * (r0 + 1) * cols + row - sub * cols;
-    }
-    if (!SHARED && ns[1] == 1) return;  // written directly
-    // a padded prefix is read for every sequence; a paged one holds the first of a sequence's tokens, if it has any
-    if (SHARED && p.table != nullptr && p.lengths[b] <= 0) ns[0] = ns[1] = 0;
-    const int n = ns[0] + ns[1];
-    T* op = reinterpret_cast<T*>(p.o) + b * p.o_b + hq * p.o_h;
-    auto nothing = [&]() {  // no token: O = 0, LSE = -inf
-        if (wave > 0) return;
-#pragma unroll
-        for (int e = 0; e < DL; ++e)
-            if (DL * lane + e < p.d) op[DL * lane + e] = Elem<T>::from_f32(0.f);
-        if (p.lse != nullptr && lane == 0) p.lse[b * p.lse_b + hq] = kNegInf;
-    };
-    if (n == 0) return nothing();
-    struct Rec {
+    struct Part {
+        int n;                // records
+        int64_t first, later; // that of the part's first share, and of the one behind it
         const float* o;
         const float* lse;
     };
-    auto rec = [&](int j) {
-        const int S = SHARED && j < ns[0] ? 0 : 1, i = S == 1 ? j - ns[0] : j;
-        const int64_t q = i == 0 ? first[S] : later[S] + (int64_t)(i - 1) * 2 * p.columns[S];
-        return Rec{(whole[S] ? p.whole_o[S] : p.rec_o[S]) + q * D, (whole[S] ? p.whole_lse[S] : p.rec_lse[S]) + q};
+    auto part = [&](int S, int z, int row) {
+        Part r = {0, 0, 0, nullptr, nullptr};
+        const int U = SHARED ? p.meta[S][0] : p.B * part_places(p.list_units), most = SHARED ? p.meta[S][1] : p.shares;
+        const int before = SHARED ? p.meta[S][2 + 2 * z] : b * part_places(p.list_units), own = SHARED ? p.meta[S][3 + 2 * z] : p.list_units;
+        if (own == 0) return r;
+        const int cols = p.columns[S], sub = row / cols;
+        const PartShares sh(U * p.Hkv * p.nsub[S], most);
+        const int x0 = (hk * p.nsub[S] + sub) * U + before + kPartExtra, r0 = sh.of(x0), r1 = sh.of(x0 + own - 1);
+        const bool whole = r0 == r1;
+        r.n = r1 - r0 + 1;
+        // the segment is share r0's first, unless units of another lie before it there
+        r.first = whole ? pair : (int64_t)(2 * r0 + (sh.start(r0) < x0 - kPartExtra ? 1 : 0)) * cols + row - sub * cols;
+        r.later = (int64_t)2 * (r0 + 1) * cols + row - sub * cols;
+        r.o = whole ? p.whole_o[S] : p.rec_o[S];
+        r.lse = whole ? p.whole_lse[S] : p.rec_lse[S];
+        return r;
     };
-    float mx = kNegInf;
-    for (int j = lane; j < n; j += 64) mx = fmaxf(mx, *rec(j).lse);
-    mx = wave_max(mx);
-    if (!SHARED && mx == kNegInf) {  // no listed block with a token, or scores of -inf
-        const int tokens = min(max(p.lengths[b], 0), p.capacity[1]), blocks = (tokens + (1 << p.block_shift) - 1) >> p.block_shift;
-        bool there = false;
-        for (int j = lane; j < p.n_list; j += 64) there |= (uint32_t)p.list[b * p.list_b + hk * p.list_h + j] < (uint32_t)blocks;
-        if (__ballot(there) == 0) return nothing();
+    Part pre = {0, 0, 0, nullptr, nullptr}, own = part(1, b, g);
+    if (!SHARED && own.n == 1) return;  // written directly
+    if constexpr (SHARED) {
+        const int z = b / p.per;
+        pre = part(0, z, (b - z * p.per) * p.group + g);
+        // a padded prefix is read for every sequence; a paged one holds the first of a sequence's tokens, if it has any
+        if (p.table != nullptr && p.lengths[b] <= 0) pre.n = own.n = 0;
     }
-    float sum = 0.f;
-    for (int j = lane; j < n; j += 64) sum += __expf(*rec(j).lse - mx);
-    sum = wave_sum(sum);
-    const float inv = 1.f / sum;
-    float acc[DL] = {};
+    const int n = pre.n + own.n;
+    T* op = reinterpret_cast<T*>(p.o) + b * p.o_b + hq * p.o_h;
+    float M = kNegInf, sum = 0.f, acc[DL] = {};
     constexpr int MB = 8;  // records in flight
     for (int j0 = wave; j0 < n; j0 += W * MB) {
-        float lw[MB], v[MB][DL];
+        float lw[MB], v[MB][DL], top = M;
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
-            const Rec q = rec(min(j0 + W * j, n - 1));
-            lw[j] = *q.lse;
+            const int i = min(j0 + W * j, n - 1);
+            const bool is_own = !SHARED || i >= pre.n;
+            const int k = i - (SHARED && is_own ? pre.n : 0);
+            const int64_t q = k == 0 ? (is_own ? own.first : pre.first) : (is_own ? own.later : pre.later) + (int64_t)(k - 1) * 2 * p.columns[is_own ? 1 : 0];
+            lw[j] = (is_own ? own.lse : pre.lse)[q];
+            const float* o = (is_own ? own.o : pre.o) + q * D + DL * lane;
 #pragma unroll
-            for (int e = 0; e < DL; ++e) v[j][e] = q.o[DL * lane + e];
+            for (int e = 0; e < DL; ++e) v[j][e] = o[e];
         }
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
-            const float w = j0 + W * j < n ? __expf(lw[j] - mx) * inv : 0.f;
+            if (j0 + W * j >= n) lw[j] = kNegInf;
+            top = fmaxf(top, lw[j]);
+        }
+        const float base = top == kNegInf ? 0.f : top, alpha = __expf(M - base);
+        M = top;
+        sum *= alpha;
+#pragma unroll
+        for (int e = 0; e < DL; ++e) acc[e] *= alpha;
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+            const float w = __expf(lw[j] - base);
+            sum += w;
 #pragma unroll
             for (int e = 0; e < DL; ++e) acc[e] = __builtin_fmaf(w, v[j][e], acc[e]);
         }
@@ -589,17 +842,37 @@ __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsPara
     if constexpr (W > 1) {
 #pragma unroll
         for (int e = 0; e < DL; ++e) red[wave][DL * lane + e] = acc[e];
+        if (lane == 0) red[wave][D] = M, red[wave][D + 1] = sum;
         __syncthreads();
         if (wave > 0) return;
+        float top = kNegInf;
 #pragma unroll
-        for (int w = 1; w < W; ++w)
+        for (int w = 0; w < W; ++w) top = fmaxf(top, red[w][D]);
+        const float base = top == kNegInf ? 0.f : top;
+        sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < DL; ++e) acc[e] += red[w][DL * lane + e];
+        for (int e = 0; e < DL; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = __expf(red[w][D] - base);
+            sum = __builtin_fmaf(red[w][D + 1], f, sum);
+#pragma unroll
+            for (int e = 0; e < DL; ++e) acc[e] = __builtin_fmaf(red[w][DL * lane + e], f, acc[e]);
+        }
+        M = top;
     }
+    bool nothing = n == 0;  // no token: O = 0, LSE = -inf
+    if (!SHARED && M == kNegInf) {  // no listed block with a token, or scores of -inf
+        const int tokens = part_clamp(p.lengths[b], p.capacity[1]), blocks = (tokens + (1 << p.block_shift) - 1) >> p.block_shift;
+        bool there = false;
+        for (int j = lane; j < p.n_list; j += 64) there |= (uint32_t)p.list[b * p.list_b + hk * p.list_h + j] < (uint32_t)blocks;
+        nothing = __ballot(there) == 0;
+    }
+    const float inv = nothing ? 0.f : 1.f / sum;
 #pragma unroll
     for (int e = 0; e < DL; ++e)
-        if (DL * lane + e < p.d) op[DL * lane + e] = Elem<T>::from_f32(acc[e]);
-    if (p.lse != nullptr && lane == 0) p.lse[b * p.lse_b + hq] = mx + __logf(sum);
+        if (DL * lane + e < p.d) op[DL * lane + e] = Elem<T>::from_f32(nothing ? 0.f : acc[e] * inv);
+    if (p.lse != nullptr && lane == 0) p.lse[b * p.lse_b + hq] = M + __logf(sum);
 }
 
 namespace {

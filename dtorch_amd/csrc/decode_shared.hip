@@ -12,46 +12,79 @@ namespace dtattn {
 
 namespace {
 
-// Waves per SIMD that a part's registers leave room for.
-template <typename T>
-constexpr int part_waves(int nc) { return nc == 1 || (nc == 2 && sizeof(T) == 2) ? 2 : 1; }
+// Sets of 16 columns of a wave that two waves per SIMD have registers for.
+constexpr int part_columns(bool f32, int kernel_d) { return f32 && kernel_d == 128 ? 1 : 2; }
+
+// Workgroups of the prefix, in eighths of all: as its units' cost is to that of all, with one of either kind at least where there is
+// any work for it.
+__device__ __forceinline__ int prefix_shares(int64_t cost0, int64_t cost1, int most) {
+    const int eighth = most / 8;
+    if (cost0 == 0) return 0;
+    if (cost1 == 0) return most;
+    return 8 * (int)min(max((cost0 * eighth + (cost0 + cost1) / 2) / (cost0 + cost1), (int64_t)1), (int64_t)(eighth - 1));
+}
 
 }  // namespace
 
-template <typename T, int D, int NC, int KIND, bool TWO>
-__global__ void __launch_bounds__(64 * kPartWaves, part_waves<T>(NC)) decode_shared_kernel(const PartsParams p) {
-    __shared__ __attribute__((aligned(16))) float red_o[kPartWaves][16][D + 4];
+// One launch for both parts.  Workgroups go to the XCDs in turn; of those on an XCD the first ones take the prefix, so that a CU has some
+// of both, and consecutive shares, whose column sets read the same keys, lie on one XCD and its L2.
+// ROWS: the prefix by rows (16-bit types).
+template <typename T, int D, int NC, bool TWO, bool ROWS>
+__global__ void __launch_bounds__(64 * kPartWaves, 2) decode_shared_kernel(const PartsParams p) {
+    constexpr size_t kMeet = sizeof(float) * kPartWaves * 16 * (D + 4), kRing = ROWS ? sizeof(T) * 3 * 2 * kPartUnit * D : 0;
+    __shared__ __attribute__((aligned(1024))) char lds[kMeet > kRing ? kMeet : kRing];
+    float (*const red_o)[16][D + 4] = reinterpret_cast<float (*)[16][D + 4]>(lds);
     __shared__ float red_m[kPartWaves][16], red_l[kPartWaves][16];
     __shared__ int eff[kPartGroups], lead[kPartGroups];
-    decode_part<T, D, NC, KIND, TWO>(p, blockIdx.x, red_o, red_m, red_l, eff, lead);
+    const PartLengths lens = {eff, lead};
+    part_lengths(p, lens);
+    const bool tells = blockIdx.x == 0 && threadIdx.x < 64;
+    const int U0 = part_total<kPrefixPart>(p, lens, tells), U1 = part_total<kOwnPart>(p, lens, tells);
+    const int V0 = U0 * p.Hkv * p.nsub[0], V1 = U1 * p.Hkv * p.nsub[1];
+    const int most0 = prefix_shares((int64_t)V0 * p.weight[0], (int64_t)V1 * p.weight[1], p.shares), most1 = p.shares - most0;
+    if (tells && threadIdx.x == 0) {
+        p.meta[0][0] = U0, p.meta[0][1] = most0;
+        p.meta[1][0] = U1, p.meta[1][1] = most1;
+    }
+    const int x = blockIdx.x & 7, y = blockIdx.x >> 3;
+    const bool first = y < most0 / 8;
+    const PartShares sh(first ? V0 : V1, first ? most0 : most1);
+    const int per = (sh.n + 7) / 8, at = first ? y : y - most0 / 8;  // shares of an XCD
+    const int r = first && p.nsub[0] > 1 ? x * per + at : at * 8 + x;
+    if ((first ? V0 : V1) == 0 || at >= per || r >= sh.n) return;
+    if (first) {
+        if constexpr (ROWS) decode_part_rows<T, D, NC>(p, lens, U0, sh, r, reinterpret_cast<T (*)[2][kPartUnit * D]>(lds));
+        else decode_part<T, D, NC, kPrefixPart, TWO>(p, lens, U0, sh, r, red_o, red_m, red_l);
+        return;
+    }
+    decode_part<T, D, 1, kOwnPart, TWO>(p, lens, U1, sh, r, red_o, red_m, red_l);
 }
 
 namespace {
 
 struct SharedPlan {
-    int32_t kernel_d, nc, nsub[2], shares[2], columns[2];
+    int32_t kernel_d, nc, nsub[2], shares, columns[2];
+    bool rows;
     size_t meta[2], rec_o[2], rec_lse[2], whole_o, whole_lse, bytes;
 };
 
-int64_t units_in(int64_t tokens) { return (tokens + kPartUnit - 1) / kPartUnit; }
+// Places of a segment of so many tokens.
+int64_t places_in(int64_t tokens) { return (tokens + kPartUnit - 1) / kPartUnit + kPartExtra; }
 
 SharedPlan plan_shared(const dtattn_decode_shared_args* a, int cus) {
     SharedPlan r = {};
-    const bool paged = a->block_table != nullptr;
-    const int64_t capacity = std::max<int64_t>(paged ? a->max_pages * a->page_size : a->S_max, 1);
-    const int64_t prefix = std::max<int64_t>(paged ? capacity : a->S_prefix, 1);
     const int64_t group = a->Hq / a->Hkv, rows = a->B / a->groups * group;
     r.kernel_d = a->D <= 64 ? 64 : 128;
-    r.nc = rows <= 16 ? 1 : rows <= 32 || a->dtype == DTATTN_FP32 ? 2 : 4;
-    r.columns[0] = 16 * r.nc, r.columns[1] = 16;
-    const int waves = r.nc == 1 || (r.nc == 2 && a->dtype != DTATTN_FP32) ? 2 : 1;
-    const int64_t cols[2] = {rows, group}, sets[2] = {a->groups, a->B}, tokens[2] = {prefix, capacity};
+    const bool f32 = a->dtype == DTATTN_FP32;
+    r.rows = !f32 && rows > 32;
+    r.nc = r.rows ? (rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : part_columns(f32, r.kernel_d);
+    r.columns[0] = 16 * r.nc * (r.rows ? kPartWaves : 1), r.columns[1] = 16;
+    r.shares = std::max(2 * cus / 8 * 8, 16);
+    const int64_t cols[2] = {rows, group}, sets[2] = {a->groups, a->B};
     for (int s = 0; s < 2; ++s) {
         r.nsub[s] = (int32_t)((cols[s] + r.columns[s] - 1) / r.columns[s]);
-        const int64_t units = a->Hkv * r.nsub[s] * sets[s] * units_in(tokens[s]);
-        r.shares[s] = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)(s == 0 ? waves : 2) * cus, units / kPartLeast));
-        const size_t records = (size_t)2 * r.shares[s] * r.columns[s];
-        r.meta[s] = part_up((1 + 2 * (size_t)sets[s]) * sizeof(int32_t));
+        const size_t records = (size_t)2 * r.shares * r.columns[s];
+        r.meta[s] = part_up((2 + 2 * (size_t)sets[s]) * sizeof(int32_t));
         r.rec_o[s] = part_up(records * r.kernel_d * sizeof(float));
         r.rec_lse[s] = part_up(records * sizeof(float));
     }
@@ -62,29 +95,29 @@ SharedPlan plan_shared(const dtattn_decode_shared_args* a, int cus) {
     return r;
 }
 
-template <typename T, int D, int NC>
-void launch_prefix(const PartsParams& p, bool two, hipStream_t stream) {
-    const dim3 grid((unsigned)p.shares[0]), block(64 * kPartWaves);
-    if (two) hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, kPrefixPart, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, kPrefixPart, false>), grid, block, 0, stream, p);
+template <typename T, int D, int NC, bool ROWS>
+void launch_parts(const PartsParams& p, hipStream_t stream) {
+    const dim3 grid((unsigned)p.shares), block(64 * kPartWaves);
+    if (p.table != nullptr && p.page_shift < 5) hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, true, ROWS>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, false, ROWS>), grid, block, 0, stream, p);
 }
 
 template <typename T, int D>
-int launch_shared(const PartsParams& p, int nc, hipStream_t stream) {
-    const bool two = p.table != nullptr && p.page_shift < 5;
-    if (nc == 1) launch_prefix<T, D, 1>(p, two, stream);
-    else if (nc == 2) launch_prefix<T, D, 2>(p, two, stream);
-    else if constexpr (sizeof(T) == 2) launch_prefix<T, D, 4>(p, two, stream);
-    int st = check_launch("decode_shared_kernel");
-    if (st != DTATTN_OK) return st;
-    const dim3 grid((unsigned)p.shares[1]), block(64 * kPartWaves);
-    if (two) hipLaunchKernelGGL((decode_shared_kernel<T, D, 1, kOwnPart, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((decode_shared_kernel<T, D, 1, kOwnPart, false>), grid, block, 0, stream, p);
-    st = check_launch("decode_shared_kernel");
+int launch_shared(const PartsParams& p, int nc, bool rows, hipStream_t stream) {
+    if (!rows) {
+        if (nc == 1) launch_parts<T, D, 1, false>(p, stream);
+        else launch_parts<T, D, part_columns(sizeof(T) == 4, D), false>(p, stream);
+    } else if constexpr (sizeof(T) == 2) {
+        if (nc == 1) launch_parts<T, D, 1, true>(p, stream);
+        else launch_parts<T, D, 2, true>(p, stream);
+    }
+    const int st = check_launch("decode_shared_kernel");
     if (st != DTATTN_OK) return st;
     const int64_t pairs = (int64_t)p.B * p.Hq;
-    // Few pairs are cut into many records each: four waves to a pair
-    if (pairs <= 256) hipLaunchKernelGGL((decode_parts_merge_kernel<T, D, 4, true>), dim3((unsigned)pairs), dim3(256), 0, stream, p);
+    // Few pairs are cut into many records each: four waves to a pair.  Up to `most` records of the prefix; us of a call with four waves and
+    // with one: 384 pairs of 10 records 32.6 and 35.8, 2048 of 9 71.9 and 70.0.
+    const int64_t most = p.shares / ((int64_t)p.Hkv * p.nsub[0] * p.groups);
+    if (pairs <= 256 || (pairs <= 1024 && most > 8)) hipLaunchKernelGGL((decode_parts_merge_kernel<T, D, 4, true>), dim3((unsigned)pairs), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((decode_parts_merge_kernel<T, D, 1, true>), dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, stream, p);
     return check_launch("decode_parts_merge_kernel");
 }
@@ -137,8 +170,8 @@ extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* st
     if (cus <= 0) return fail(DTATTN_ERR_DEVICE, "%s: cannot tell the stream's device", who);
     const SharedPlan plan = plan_shared(a, cus);
     const int64_t capacity = paged ? a->max_pages * a->page_size : a->S_max, most_prefix = paged ? capacity : a->S_prefix;
-    if (a->groups * a->Hkv * plan.nsub[0] * units_in(most_prefix) >= ((int64_t)1 << 31) ||
-        a->B * a->Hkv * plan.nsub[1] * units_in(capacity) >= ((int64_t)1 << 31) || a->B * a->Hq > 0x7fffffff)
+    if (a->groups * a->Hkv * plan.nsub[0] * places_in(most_prefix) >= ((int64_t)1 << 31) ||
+        a->B * a->Hkv * plan.nsub[1] * places_in(capacity) >= ((int64_t)1 << 31) || a->B * a->Hq > 0x7fffffff)
         return fail(DTATTN_ERR_UNSUPPORTED, "%s: cache too large", who);
     if (a->workspace == nullptr || a->workspace_bytes < plan.bytes)
         return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, plan.bytes, a->workspace_bytes);
@@ -170,13 +203,15 @@ extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* st
         return at;
     };
     for (int s = 0; s < 2; ++s) {
-        p.nsub[s] = plan.nsub[s], p.shares[s] = plan.shares[s], p.columns[s] = plan.columns[s];
+        p.nsub[s] = plan.nsub[s], p.columns[s] = plan.columns[s];
         p.meta[s] = reinterpret_cast<int32_t*>(take(plan.meta[s]));
         p.rec_o[s] = reinterpret_cast<float*>(take(plan.rec_o[s]));
         p.rec_lse[s] = reinterpret_cast<float*>(take(plan.rec_lse[s]));
         p.whole_o[s] = reinterpret_cast<float*>(take(plan.whole_o));
         p.whole_lse[s] = reinterpret_cast<float*>(take(plan.whole_lse));
     }
+    p.shares = plan.shares;
+    p.weight[0] = plan.rows ? 3 : 2, p.weight[1] = plan.rows ? 2 : 3;
     p.q_b = a->q_stride[0], p.q_h = a->q_stride[1], p.o_b = a->o_stride[0], p.o_h = a->o_stride[1];
     p.lse_b = a->lse != nullptr ? a->lse_stride[0] : 0;
     p.B = (int32_t)a->B, p.Hq = (int32_t)a->Hq, p.Hkv = (int32_t)a->Hkv, p.group = (int32_t)(a->Hq / a->Hkv);
@@ -186,8 +221,8 @@ extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* st
     p.q_and = sp.q_and, p.q_xor = sp.q_xor;
     const bool wide = plan.kernel_d == 128;
     switch (a->dtype) {
-        case DTATTN_BF16: return wide ? launch_shared<bf16_t, 128>(p, plan.nc, stream) : launch_shared<bf16_t, 64>(p, plan.nc, stream);
-        case DTATTN_FP16: return wide ? launch_shared<f16_t, 128>(p, plan.nc, stream) : launch_shared<f16_t, 64>(p, plan.nc, stream);
-        default: return wide ? launch_shared<float, 128>(p, plan.nc, stream) : launch_shared<float, 64>(p, plan.nc, stream);
+        case DTATTN_BF16: return wide ? launch_shared<bf16_t, 128>(p, plan.nc, plan.rows, stream) : launch_shared<bf16_t, 64>(p, plan.nc, plan.rows, stream);
+        case DTATTN_FP16: return wide ? launch_shared<f16_t, 128>(p, plan.nc, plan.rows, stream) : launch_shared<f16_t, 64>(p, plan.nc, plan.rows, stream);
+        default: return wide ? launch_shared<float, 128>(p, plan.nc, plan.rows, stream) : launch_shared<float, 64>(p, plan.nc, plan.rows, stream);
     }
 }

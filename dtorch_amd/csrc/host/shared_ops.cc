@@ -358,12 +358,9 @@ void SelectKeyBlocksOp::Compute(const TorchTensorOptArray& in, TorchTensorArray&
         a.dtype = DtypeCode(q.scalar_type());
         a.scale = s;
         const size_t ws = dtattn_select_key_blocks_workspace_size(&a);
-        at::Tensor wst;
-        if (ws > 0) {
-            wst = Bytes(ws, q);
-            a.workspace = wst.data_ptr();
-            a.workspace_bytes = ws;
-        }
+        at::Tensor wst = Bytes(ws, q);
+        a.workspace = wst.data_ptr();
+        a.workspace_bytes = ws;
         Check(dtattn_select_key_blocks(&a, CurrentStream(q)), "dtattn_select_key_blocks");
     }
     outputs.push_back(blocks);

@@ -7,10 +7,10 @@
 //
 // key_bounds_kernel: a workgroup per (block, sequence and kv head); every 16-byte chunk of a row belongs to one column of threads,
 // which meet by lane exchanges and then in LDS.  Bound by HBM: the rows are read once.
-// select_blocks_kernel: one workgroup per (sequence, kv head) scores its blocks, four lanes to a block, with the query's heads in LDS as
-// 64-bit numbers, and takes the largest scores by a radix select.  Sums in 64 bits are exact for 16-bit types (products have at
+// score_blocks_kernel: four lanes to a block, with the query's heads in LDS as 64-bit numbers.  Sums in 64 bits are exact for 16-bit types (products have at
 // most 22 bits), so scores next to one another are told apart alike in any order of summation, and the vector units' 64-bit rate
 // is that of 32 bits.
+// select_blocks_kernel: one workgroup per (sequence, kv head) takes the largest scores by a radix select.
 #include <algorithm>
 
 #include "decode_params.hpp"
@@ -39,7 +39,7 @@ struct SelectParams {
     const char* q;
     const char* lo;
     const char* hi;
-    uint32_t* order;  // [B, Hkv, blocks_max], where LDS does not hold the scores
+    uint32_t* order;  // [B, Hkv, blocks_max]: scores in unsigned order
     int32_t* kept;
     int64_t q_b, q_h;  // elements
     int64_t lo_b, lo_h, lo_s, hi_b, hi_h, hi_s;  // bytes
@@ -118,98 +118,139 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
     }
 }
 
-// HB: query heads at a time; IN_LDS: the scores are held in LDS (up to kSelectLds blocks).
-constexpr int kSelectLds = 4096;
+// A workgroup scores blocks 64 W blockIdx.y, ... of one (sequence, kv head), four lanes to W blocks; HB: heads at a time.
+// What costs is the vector units: a value's choice by a mask (for 16-bit types two values at once), its conversion and the product, for
+// every head, and the reads of the query from LDS, which two blocks of a quad share.  The 64-bit matrix cores, at the vector units' rate
+// with 16 columns for a group's 4 heads, take 29 us where this takes 18 (32 sequences of 3000 to 32000 tokens in blocks of 64).
+constexpr int kScoreHeads = 16;
 
-template <typename T, int D, int HB, bool IN_LDS>
-__global__ void __launch_bounds__(kSelect) select_blocks_kernel(const SelectParams p) {
+template <typename T, int D, int HB, int W>
+__global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p) {
     constexpr int E = 16 / (int)sizeof(T), NI = D / E / 4;  // chunks of a row per lane
-    __shared__ __attribute__((aligned(16))) double qd[HB][D];
-    __shared__ uint32_t held[IN_LDS ? kSelectLds : 1];
+    __shared__ __attribute__((aligned(16))) double qd[kScoreHeads][D];
+    __shared__ __attribute__((aligned(16))) uint32_t qm[kScoreHeads][D * sizeof(T) / 4];  // all ones where q > 0
     const int tid = threadIdx.x;
     const int64_t bh = blockIdx.x, b = bh / p.Hkv;
     const int h = (int)(bh % p.Hkv);
     const int n = tokens_in(p.c, b);
     const int blocks = (n + (1 << p.c.block_shift) - 1) >> p.c.block_shift;
-    int32_t* kept = p.kept + bh * p.keep;
-    if (blocks <= p.keep) {
-        for (int i = tid; i < p.keep; i += kSelect) kept[i] = i < blocks ? i : -1;
-        return;
-    }
     const int cand = blocks - p.recent;
-    uint32_t* order = IN_LDS ? held : p.order + bh * p.blocks_max;
+    if (blocks <= p.keep || (int)blockIdx.y * 64 * W >= cand) return;
+    uint32_t* order = p.order + bh * p.blocks_max;
     const int quad = tid >> 2, l = tid & 3;
     const int in_page = p.c.page_shift - p.c.block_shift;  // log2 of a page's blocks
-    for (int g0 = 0; g0 < p.group; g0 += HB) {
+    for (int g0 = 0; g0 < p.group; g0 += kScoreHeads) {
+        const int heads = min(p.group - g0, kScoreHeads);
         if (g0 > 0) __syncthreads();  // the last heads have been used
-        for (int i = tid; i < HB * D; i += kSelect) {
-            const int g = min(g0 + i / D, p.group - 1), dim = i % D;  // a head twice changes nothing
-            double x = 0.;
-            if (dim < p.d) {
-                const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_b + (h * p.group + g) * p.q_h + dim;
-                if constexpr (sizeof(T) == 4) x = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, *q) & p.q_and) ^ p.q_xor);
-                else x = Elem<T>::to_f32(__builtin_bit_cast(T, (uint16_t)((__builtin_bit_cast(uint16_t, *q) & p.q_and) ^ p.q_xor)));
+        for (int i = tid; i < (heads + HB - 1) / HB * HB * D / E; i += 256) {
+            const int g = i / (D / E), dim = i % (D / E) * E;
+            u32x4 w = {0u, 0u, 0u, 0u}, mask;
+            if (g < heads && dim < p.d)
+                w = q_bits(ld16(reinterpret_cast<const T*>(p.q) + b * p.q_b + (h * p.group + g0 + g) * p.q_h + dim), p.q_and, p.q_xor);
+            if constexpr (sizeof(T) == 4) {
+                const f32x4 x = __builtin_bit_cast(f32x4, w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) qd[g][dim + e] = x[e], mask[e] = x[e] > 0.f ? 0xffffffffu : 0u;
+            } else {
+                float x[E];
+                unpack8<T>(w, x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) qd[g][dim + e] = x[e];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mask[e] = (x[2 * e] > 0.f ? 0xffffu : 0u) | (x[2 * e + 1] > 0.f ? 0xffff0000u : 0u);
             }
-            qd[i / D][dim] = x;
+            *reinterpret_cast<u32x4*>(&qm[g][dim * (int)sizeof(T) / 4]) = mask;
         }
         __syncthreads();
-        for (int j = quad; j < cand; j += kSelect / 4) {
-            int64_t slot = b, jb = j;
-            if (p.c.table != nullptr) {
-                slot = min(max(p.c.table[b * p.c.bt_s + (j >> in_page)], 0), p.c.num_pages - 1);
-                jb = j & ((1 << in_page) - 1);
-            }
-            const char* lo = p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s;
-            const char* hi = p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s;
-            u32x4 wl[NI], wh[NI];
+        for (int j0 = blockIdx.y * 64 * W; j0 < cand; j0 += gridDim.y * 64 * W) {
+            u32x4 wl[W][NI], wh[W][NI];
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int c = min(l + 4 * i, p.d / E - 1);  // past the head dim: a valid chunk, which meets zeros
-                wl[i] = ld16_nt(lo + 16 * c);
-                wh[i] = ld16_nt(hi + 16 * c);
-            }
-            asm volatile("" ::: "memory");  // the query's numbers stay in LDS: held over the loop, they would be spilled
-            double s[HB];
-#pragma unroll
-            for (int g = 0; g < HB; ++g) s[g] = 0.;
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                float fl[E], fh[E];
-                if constexpr (sizeof(T) == 4) {
-                    const f32x4 a = __builtin_bit_cast(f32x4, wl[i]), c = __builtin_bit_cast(f32x4, wh[i]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) fl[e] = a[e], fh[e] = c[e];
-                } else {
-                    unpack8<T>(wl[i], fl);
-                    unpack8<T>(wh[i], fh);
+            for (int w = 0; w < W; ++w) {
+                const int j = min(j0 + quad + 64 * w, cand - 1);
+                int64_t slot = b, jb = j;
+                if (p.c.table != nullptr) {
+                    slot = min(max(p.c.table[b * p.c.bt_s + (j >> in_page)], 0), p.c.num_pages - 1);
+                    jb = j & ((1 << in_page) - 1);
                 }
-                const int dim = (l + 4 * i) * E;
-                const bool there = dim < p.d;
+                const char* lo = p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s;
+                const char* hi = p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
+                for (int i = 0; i < NI; ++i) {
+                    const int c = l + 4 * i;
+                    const bool there = E * c < p.d;
+                    wl[w][i] = ld16_nt(lo + (there ? 16 * c : 0));
+                    wh[w][i] = ld16_nt(hi + (there ? 16 * c : 0));
+                    if (!there) wl[w][i] = wh[w][i] = u32x4{0u, 0u, 0u, 0u};
+                }
+            }
+            float best[W];
+#pragma unroll
+            for (int w = 0; w < W; ++w) best[w] = kNegInf;
+            for (int hb = 0; hb < heads; hb += HB) {
+                double s[W][HB];
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int g = 0; g < HB; ++g) s[w][g] = 0.;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const int dim = (l + 4 * i) * E;
 #pragma unroll
                     for (int g = 0; g < HB; ++g) {
-                        const double q = qd[g][dim + e];
-                        const double x = (double)(there ? (q > 0. ? fh[e] : fl[e]) : 0.f);
-                        s[g] = __builtin_fma(q, x, s[g]);
+                        const u32x4 mask = *reinterpret_cast<const u32x4*>(&qm[hb + g][dim * (int)sizeof(T) / 4]);
+                        double q[E];
+#pragma unroll
+                        for (int e = 0; e < E; ++e) q[e] = qd[hb + g][dim + e];
+#pragma unroll
+                        for (int w = 0; w < W; ++w) {
+                            const u32x4 x = (wh[w][i] & mask) | (wl[w][i] & ~mask);
+                            float f[E];
+                            if constexpr (sizeof(T) == 4) {
+                                const f32x4 v = __builtin_bit_cast(f32x4, x);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) f[e] = v[e];
+                            } else {
+                                unpack8<T>(x, f);
+                            }
+#pragma unroll
+                            for (int e = 0; e < E; ++e) s[w][g] = __builtin_fma(q[e], (double)f[e], s[w][g]);
+                        }
                     }
                 }
-            }
-            float best = kNegInf;
 #pragma unroll
-            for (int g = 0; g < HB; ++g) {
-                s[g] += __shfl_xor(s[g], 1, 64);
-                s[g] += __shfl_xor(s[g], 2, 64);
-                best = fmaxf(best, (float)s[g]);  // NaN is passed over
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int g = 0; g < HB; ++g) {
+                        s[w][g] += __shfl_xor(s[w][g], 1, 64);
+                        s[w][g] += __shfl_xor(s[w][g], 2, 64);
+                        if (hb + g < heads) best[w] = fmaxf(best[w], (float)s[w][g]);  // NaN is passed over
+                    }
             }
-            if (l == 0) {
-                const uint32_t u = ordered(best);
-                order[j] = g0 == 0 ? u : max(order[j], u);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const int j = j0 + quad + 64 * w;
+                if (l == 0 && j < cand) {
+                    const uint32_t u = ordered(best[w]);
+                    order[j] = g0 == 0 ? u : max(order[j], u);
+                }
             }
         }
     }
-    __syncthreads();
-    select_largest<0>(cand, p.keep - p.recent, p.recent, order, kept, [&](int i) { return order[i]; });
+}
+
+// The scores: PER per thread in registers, or PER = 0 in memory.
+template <int PER>
+__global__ void __launch_bounds__(kSelect) select_blocks_kernel(const SelectParams p) {
+    const int64_t bh = blockIdx.x, b = bh / p.Hkv;
+    const int n = tokens_in(p.c, b);
+    const int blocks = (n + (1 << p.c.block_shift) - 1) >> p.c.block_shift;
+    int32_t* kept = p.kept + bh * p.keep;
+    if (blocks <= p.keep) {
+        for (int i = threadIdx.x; i < p.keep; i += kSelect) kept[i] = i < blocks ? i : -1;
+        return;
+    }
+    uint32_t* order = p.order + bh * p.blocks_max;
+    select_largest<PER>(blocks - p.recent, p.keep - p.recent, p.recent, order, kept, [&](int i) { return order[i]; });
 }
 
 namespace {
@@ -269,20 +310,21 @@ void launch_bounds_of(const BoundsParams& p, dim3 grid, hipStream_t stream) {
 }
 
 template <typename T, int D, int HB>
-void launch_select(const SelectParams& p, dim3 grid, hipStream_t stream) {
-    if (p.blocks_max <= kSelectLds) hipLaunchKernelGGL((select_blocks_kernel<T, D, HB, true>), grid, dim3(kSelect), 0, stream, p);
-    else hipLaunchKernelGGL((select_blocks_kernel<T, D, HB, false>), grid, dim3(kSelect), 0, stream, p);
-}
-template <typename T, int D>
-void select_heads(const SelectParams& p, dim3 grid, hipStream_t stream) {
-    if (p.group == 1) launch_select<T, D, 1>(p, grid, stream);
-    else if (p.group <= 4) launch_select<T, D, 4>(p, grid, stream);
-    else launch_select<T, D, 8>(p, grid, stream);
+void launch_score(const SelectParams& p, unsigned heads, int64_t cus, hipStream_t stream) {
+    // A workgroup for every 64 blocks; where that is more than two to a CU, for every 128 (the query is then read from LDS half as
+    // often), until each CU has four.  us: 8 heads of 465 blocks 6.2 with 64 and 8.6 with 128, 256 of up to 492 19.1 and 18.0.
+    const int64_t chunks = (p.blocks_max + 63) / 64;
+    if (heads * chunks <= 2 * cus) {
+        hipLaunchKernelGGL((score_blocks_kernel<T, D, HB, 1>), dim3(heads, (unsigned)chunks), dim3(256), 0, stream, p);
+    } else {
+        const int64_t most = std::max<int64_t>((4 * cus + heads - 1) / heads, 1);
+        hipLaunchKernelGGL((score_blocks_kernel<T, D, HB, 2>), dim3(heads, (unsigned)std::min<int64_t>((chunks + 1) / 2, most)), dim3(256), 0, stream, p);
+    }
 }
 template <typename T>
-void select_dims(const SelectParams& p, dim3 grid, hipStream_t stream) {
-    if (p.d <= 64) select_heads<T, 64>(p, grid, stream);
-    else select_heads<T, 128>(p, grid, stream);
+void score(const SelectParams& p, unsigned heads, int64_t cus, hipStream_t stream) {
+    if (p.d <= 64) p.group == 1 ? launch_score<T, 64, 1>(p, heads, cus, stream) : launch_score<T, 64, 4>(p, heads, cus, stream);
+    else p.group == 1 ? launch_score<T, 128, 1>(p, heads, cus, stream) : launch_score<T, 128, 4>(p, heads, cus, stream);
 }
 
 template <typename Args>
@@ -340,8 +382,7 @@ extern "C" int dtattn_key_bounds(const dtattn_key_bounds_args* a, void* stream_)
 
 extern "C" size_t dtattn_select_key_blocks_workspace_size(const dtattn_select_blocks_args* a) {
     if (a == nullptr || a->B <= 0 || a->Hkv <= 0 || a->block <= 0) return 0;
-    const int64_t blocks = blocks_max_of(a);
-    return blocks <= kSelectLds ? 0 : ((size_t)a->B * a->Hkv * blocks * sizeof(uint32_t) + 255) & ~(size_t)255;
+    return ((size_t)a->B * a->Hkv * blocks_max_of(a) * sizeof(uint32_t) + 255) & ~(size_t)255;
 }
 
 extern "C" int dtattn_select_key_blocks(const dtattn_select_blocks_args* a, void* stream_) {
@@ -367,11 +408,9 @@ extern "C" int dtattn_select_key_blocks(const dtattn_select_blocks_args* a, void
         return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
     if (a->B * a->Hkv > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
     const size_t need = dtattn_select_key_blocks_workspace_size(a);
-    if (need > 0) {
-        if (a->workspace == nullptr || a->workspace_bytes < need)
-            return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, a->workspace_bytes);
-        if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(DTATTN_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
-    }
+    if (a->workspace == nullptr || a->workspace_bytes < need)
+        return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, a->workspace_bytes);
+    if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(DTATTN_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
     const int64_t esz = a->dtype == DTATTN_FP32 ? 4 : 2;
     p.q = reinterpret_cast<const char*>(a->q);
     p.lo = reinterpret_cast<const char*>(a->k_min), p.hi = reinterpret_cast<const char*>(a->k_max);
@@ -384,12 +423,20 @@ extern "C" int dtattn_select_key_blocks(const dtattn_select_blocks_args* a, void
     p.keep = (int32_t)(a->keep / a->block), p.recent = (int32_t)(a->recent / a->block);
     p.blocks_max = (int32_t)blocks_max_of(a);
     p.q_and = sp.q_and, p.q_xor = sp.q_xor;
-    const dim3 grid((unsigned)(a->B * a->Hkv));
+    const unsigned heads = (unsigned)(a->B * a->Hkv);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    const int64_t cus = std::max(stream_cus(stream), 1);
     switch (a->dtype) {
-        case DTATTN_BF16: select_dims<bf16_t>(p, grid, stream); break;
-        case DTATTN_FP16: select_dims<f16_t>(p, grid, stream); break;
-        default: select_dims<float>(p, grid, stream);
+        case DTATTN_BF16: score<bf16_t>(p, heads, cus, stream); break;
+        case DTATTN_FP16: score<f16_t>(p, heads, cus, stream); break;
+        default: score<float>(p, heads, cus, stream);
     }
+    st = check_launch("score_blocks_kernel");
+    if (st != DTATTN_OK) return st;
+    // as few a thread as hold them
+    if (p.blocks_max <= kSelect) hipLaunchKernelGGL(select_blocks_kernel<1>, dim3(heads), dim3(kSelect), 0, stream, p);
+    else if (p.blocks_max <= 4 * kSelect) hipLaunchKernelGGL(select_blocks_kernel<4>, dim3(heads), dim3(kSelect), 0, stream, p);
+    else if (p.blocks_max <= 16 * kSelect) hipLaunchKernelGGL(select_blocks_kernel<16>, dim3(heads), dim3(kSelect), 0, stream, p);
+    else hipLaunchKernelGGL(select_blocks_kernel<0>, dim3(heads), dim3(kSelect), 0, stream, p);
     return check_launch("select_blocks_kernel");
 }

@@ -9,8 +9,8 @@
 // kv_reserve_plan_kernel: one workgroup. The (sequence, slot) pairs that are about to be written are its items, in order; an item's
 // place among those that need a page is a prefix sum, and its place among the writers of a shared page a count of equal
 // entries before it, which makes the outcome independent of any order of execution.
-// kv_compact_plan_kernel: one workgroup. Two passes over the counts: how many pages are used, then the k-th hole and the k-th page
-// to move.
+// kv_compact_plan_kernel: one workgroup. How many pages are used, then the k-th hole and the k-th page to move, by prefix sums over the
+// counts.
 #include <algorithm>
 
 #include "decode_params.hpp"
@@ -46,7 +46,7 @@ struct PagesParams {
     int32_t* items;  // reserve: an item's page that others share, -1 of others
     int32_t* order;  // reserve: an item's place among the pages taken, -1: takes none
     int32_t* list;   // reserve: the free pages taken; compact: [0, num_pages / 2) where to, then where from
-    int32_t* map;    // compact: a page's new index
+    int32_t* map;    // compact: a page's new index, of those behind the pages that stay
     int4* copies;    // reserve: a sequence's copied page: from, to, tokens
     int32_t* moves;  // compact: how many pages move
     int64_t stride;
@@ -136,8 +136,15 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
         r.refs = r.page >= 0 ? p.refs[r.page] : 0;
         return r;
     };
+    // the first counts are on their way meanwhile
+    auto count_at = [&](int64_t page) { return page < p.num_pages ? p.refs[page] : 1; };
+    int early[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) early[j] = count_at(4 * tid + j);
+    const Item mine = tid < n ? item(tid) : Item{0, -1, -1, 0};  // an item that is needed again, its loads one behind another
+    auto again = [&](int i) { return i < kPlan ? mine : item(i); };
     for (int i = tid; i < n; i += kPlan) {
-        const Item it = item(i);
+        const Item it = again(i);
         items[i] = it.page >= 0 && it.refs > 1 ? it.page : -1;
     }
     __syncthreads();
@@ -147,7 +154,7 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
         const int i = i0 + tid;
         bool takes = false;
         if (i < n) {
-            const Item it = item(i);
+            const Item it = again(i);
             takes = it.slot >= 0 && it.page < 0;
             if (it.page >= 0 && it.refs > 1) {
                 int before = 0, j = 0;  // earlier items of the same page
@@ -168,15 +175,14 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
     // that many free pages, from the lowest index up
     int found = 0;
     for (int64_t p0 = 0; p0 < p.num_pages && found < need; p0 += 4 * kPlan) {
-        int v[4], mine = 0;
+        int v[4], free = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int64_t page = p0 + 4 * tid + j;
-            v[j] = page < p.num_pages && p.refs[page] <= 0;
-            mine += v[j];
+            v[j] = (p0 == 0 ? early[j] : count_at(p0 + 4 * tid + j)) <= 0;
+            free += v[j];
         }
         int total;
-        int k = found + scan_plan(mine, waves, total);
+        int k = found + scan_plan(free, waves, total);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (v[j] && k < need) p.list[k] = (int)(p0 + 4 * tid + j);
@@ -188,7 +194,7 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
     if (tid == 0) *p.out = need - found;
     __syncthreads();  // counts have been read, and the list is written
     for (int i = tid; i < n; i += kPlan) {
-        const Item it = item(i);
+        const Item it = again(i);
         const int k = p.order[i];
         const int to = k >= 0 && k < found ? p.list[k] : -1;
         const bool shared = k >= 0 && it.page >= 0;
@@ -241,44 +247,59 @@ __global__ void __launch_bounds__(256) kv_reserve_copy_kernel(const PagesParams 
     else copy_page<uint32_t, 256>(g, c.x, c.y, no, ni, blockIdx.z, gridDim.z);
 }
 
+// HELD: all counts are held in registers and the moves in LDS (up to kHeldPages pages).
+constexpr int kCompactPer = 16, kHeldPages = kCompactPer * kPlan;
+
+template <bool HELD>
 __global__ void __launch_bounds__(kPlan) kv_compact_plan_kernel(const PagesParams p) {
-    constexpr int PER = 16;
+    constexpr int PER = kCompactPer;
     __shared__ int waves[kPlan / 64];
+    __shared__ int lds_to[HELD ? kHeldPages / 2 : 1], lds_from[HELD ? kHeldPages / 2 : 1], lds_refs[HELD ? kHeldPages / 2 : 1];
     const int tid = threadIdx.x, P = p.num_pages;
-    int used = 0;
-    for (int64_t p0 = 0; p0 < P; p0 += PER * kPlan) {
-        int mine = 0, total;
+    int refs[PER];
+    auto load = [&](int64_t p0) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int64_t page = p0 + PER * tid + j;
-            mine += page < P && p.refs[page] > 0;
+            refs[j] = page < P ? p.refs[page] : 0;
         }
-        scan_plan(mine, waves, total);
+    };
+    int used = 0;
+    for (int64_t p0 = 0; p0 < P; p0 += PER * kPlan) {
+        load(p0);
+        int live = 0, total;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) live += refs[j] > 0;
+        scan_plan(live, waves, total);
         used += total;
     }
     if (tid == 0) *p.out = used;
-    int* to = p.list;
-    int* from = p.list + (P + 1) / 2;
+    int* to = HELD ? lds_to : p.list;
+    int* from = HELD ? lds_from : p.list + (P + 1) / 2;
     int holes = 0, late = 0;
     for (int64_t p0 = 0; p0 < P; p0 += PER * kPlan) {
-        int v[PER], hole = 0, move = 0, total;
+        if (!HELD) load(p0);
+        int hole = 0, move = 0, total;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int64_t page = p0 + PER * tid + j;
-            const bool live = page < P && p.refs[page] > 0;
-            v[j] = page >= P ? 0 : page < used ? (live ? 0 : 1) : (live ? 2 : 0);
-            hole += v[j] == 1, move += v[j] == 2;
-            if (page < P) p.map[page] = (int)page;
+            hole += page < used && refs[j] <= 0;
+            move += page >= used && refs[j] > 0;
         }
-        int h = holes + scan_plan(hole, waves, total);
-        holes += total;
-        int m = late + scan_plan(move, waves, total);
-        late += total;
+        // both sums in one: a round has 2^14 pages
+        const int before = scan_plan(hole | move << 16, waves, total);
+        int h = holes + (before & 0xffff), m = late + (before >> 16);
+        holes += total & 0xffff, late += total >> 16;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int page = (int)(p0 + PER * tid + j);
-            if (v[j] == 1) to[h++] = page;
-            if (v[j] == 2) from[m++] = page;
+            const int64_t page = p0 + PER * tid + j;
+            if (page < used && refs[j] <= 0) to[h++] = (int)page;
+            if (page >= used && refs[j] > 0) {
+                if (HELD) lds_refs[m] = refs[j];
+                from[m++] = (int)page;
+            } else if (page >= used && page < P) {
+                p.map[page] = (int)page;
+            }
         }
     }
     if (tid == 0) *p.moves = holes;  // as many as move
@@ -286,8 +307,9 @@ __global__ void __launch_bounds__(kPlan) kv_compact_plan_kernel(const PagesParam
     for (int i = tid; i < holes; i += kPlan) {
         const int a = from[i], b = to[i];
         p.map[a] = b;
-        p.refs[b] = p.refs[a];
+        p.refs[b] = HELD ? lds_refs[i] : p.refs[a];
         p.refs[a] = 0;
+        if (HELD) p.list[i] = b, p.list[(P + 1) / 2 + i] = a;
     }
 }
 
@@ -295,10 +317,11 @@ __global__ void __launch_bounds__(kPlan) kv_compact_plan_kernel(const PagesParam
 __global__ void __launch_bounds__(256) kv_compact_move_kernel(const PagesParams p, int parts) {
     if ((int)blockIdx.y == p.n_pools) {
         const int64_t n = (int64_t)p.B * p.max_pages;
+        const int used = *p.out;
         for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
             int32_t* slot = p.table + i / p.max_pages * p.stride + i % p.max_pages;
             const int page = *slot;
-            if (page >= 0 && page < p.num_pages) *slot = p.map[page];
+            if (page >= used && page < p.num_pages) *slot = p.map[page];
         }
         return;
     }
@@ -401,7 +424,8 @@ extern "C" int dtattn_kv_pages_fork(const dtattn_kv_fork_args* a, void* stream_)
     p.table = a->block_table, p.lengths = a->lengths, p.refs = a->page_refs, p.parents = a->parents;
     p.stride = a->block_table_stride;
     p.B = (int32_t)a->B, p.max_pages = (int32_t)a->max_pages, p.num_pages = (int32_t)a->num_pages;
-    p.width = (int32_t)std::min<int64_t>(kForkCells / a->B, 64);
+    // Slices of about 1024 slots: a slice's time is its loops over the rows.  us with 8192 and with 1024: 128 rows of 36 slots 16.6 and 4.6
+    p.width = (int32_t)std::max<int64_t>(std::min<int64_t>(1024 / a->B, a->max_pages), 1);
     const int64_t grid = (a->max_pages + p.width - 1) / p.width;
     hipLaunchKernelGGL(kv_fork_kernel, dim3((unsigned)grid), dim3(256), 0, reinterpret_cast<hipStream_t>(stream_), p);
     return check_launch("kv_fork_kernel");
@@ -486,7 +510,8 @@ extern "C" int dtattn_kv_pages_compact(const dtattn_kv_compact_args* a, void* st
     p.B = (int32_t)a->B, p.max_pages = (int32_t)a->max_pages, p.num_pages = (int32_t)a->num_pages;
     p.n_pools = a->n_pools;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-    hipLaunchKernelGGL(kv_compact_plan_kernel, dim3(1), dim3(kPlan), 0, stream, p);
+    if (p.num_pages <= kHeldPages) hipLaunchKernelGGL(kv_compact_plan_kernel<true>, dim3(1), dim3(kPlan), 0, stream, p);
+    else hipLaunchKernelGGL(kv_compact_plan_kernel<false>, dim3(1), dim3(kPlan), 0, stream, p);
     st = check_launch("kv_compact_plan_kernel");
     if (st != DTATTN_OK) return st;
     int64_t most = 1;

@@ -608,7 +608,7 @@ typedef struct {
     int32_t block;
     int32_t dtype;
     float scale;             /* only its sign counts; NaN means 1/sqrt(D) */
-    void* workspace;         /* >= dtattn_select_key_blocks_workspace_size(args) bytes (it may be 0), 256-byte aligned */
+    void* workspace;         /* >= dtattn_select_key_blocks_workspace_size(args) bytes, 256-byte aligned */
     size_t workspace_bytes;
 } dtattn_select_blocks_args;
 
