@@ -51,6 +51,7 @@ struct PartsParams {
     int32_t n_list, list_units, block_shift;
     int32_t d;
     float c;  // scale * log2(e)
+    float per_inv;
     uint32_t q_and, q_xor;
 };
 
@@ -59,7 +60,7 @@ namespace {
 constexpr int kPartUnit = 32;  // tokens
 constexpr int kPartWaves = 4;
 constexpr int kPartLeast = kPartWaves + 1;  // places of a share, at least
-constexpr int kPartGroups = 2048;
+constexpr int kPartGroups = 1024;
 // What a segment costs besides its units, in units: its waves meet, and the last of them take turns that others have no unit for.
 constexpr int kPartExtra = 4;
 
@@ -95,61 +96,94 @@ __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __
 
 }  // namespace
 
-// What both parts of a shared call need to know of the lengths.
-struct PartLengths {
-    int* eff;   // LDS, paged: tokens that a group shares: whole pages that each of its sequences with tokens has
-    int* lead;  // LDS, paged: the first of those sequences
-};
-
 __device__ __forceinline__ int part_clamp(int n, int most) { return min(max(n, 0), most); }
 
-__device__ __forceinline__ void part_lengths(const PartsParams& p, const PartLengths& at) {
-    if (p.table == nullptr) return;
-    const int tid = threadIdx.x;
-    for (int g = tid; g < p.groups; g += 256) at.eff[g] = at.lead[g] = 0x7fffffff;
-    __syncthreads();
-    for (int b = tid; b < p.B; b += 256) {
-        const int n = part_clamp(p.lengths[b], p.capacity[1]);
-        if (n > 0) {
-            atomicMin(&at.eff[b / p.per], n);
-            atomicMin(&at.lead[b / p.per], b);
-        }
-    }
-    __syncthreads();
-    for (int g = tid; g < p.groups; g += 256) {
-        const int n = at.eff[g] == 0x7fffffff ? 0 : min(at.eff[g], max(p.prefix[g], 0));
-        at.eff[g] = n >> p.page_shift << p.page_shift;
-    }
-    __syncthreads();
+// The group of sequence z.  Below 2^20 the float quotient is off by less than its distance of 0.5 / per from a whole number.
+__device__ __forceinline__ int part_group(const PartsParams& p, int z) {
+    if (p.groups == 1) return 0;
+    return z < (1 << 20) ? (int)(((float)z + 0.5f) * p.per_inv) : z / p.per;
 }
 
-// Units of group or sequence z, per lane.
+// What both parts of a shared call need to know of the lengths.
+struct PartLengths {
+    // LDS, paged: of each group the least tokens of its sequences with tokens, the first of those, and what it is said to share
+    int* least;
+    int* lead;
+    int* said;
+    int own0, pre0;  // this lane's of the first 64 lengths and prefixes
+
+    // Tokens that a group of a paged cache shares: whole pages that each of its sequences with tokens has.
+    __device__ __forceinline__ int shared(const PartsParams& p, int g) const {
+        const int n = least[g] == 0x7fffffff ? 0 : min(least[g], said[g]);
+        return n >> p.page_shift << p.page_shift;
+    }
+};
+
+__device__ __forceinline__ PartLengths part_lengths(const PartsParams& p, int* least, int* lead, int* said) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    PartLengths r = {least, lead, said, 0, 0};
+    r.own0 = lane < p.B ? p.lengths[lane] : 0;
+    r.pre0 = lane < p.groups ? p.prefix[lane] : 0;
+    if (p.table != nullptr) {
+        for (int g = tid; g < p.groups; g += 256) least[g] = lead[g] = 0x7fffffff;
+        for (int g = tid; g < p.groups; g += 256) said[g] = max(g < 64 ? r.pre0 : p.prefix[g], 0);
+        __syncthreads();
+        for (int b = tid; b < p.B; b += 256) {
+            const int n = part_clamp(b < 64 ? r.own0 : p.lengths[b], p.capacity[1]);
+            if (n > 0) {
+                const int g = part_group(p, b);
+                atomicMin(&least[g], n);
+                atomicMin(&lead[g], b);
+            }
+        }
+        __syncthreads();
+    }
+    r.own0 = part_clamp(r.own0, p.capacity[1]);
+    r.pre0 = part_clamp(r.pre0, p.capacity[0]);
+    return r;
+}
+
+// Units of group or sequence z, per lane (z = lane or beyond the first 64).
 template <int KIND>
 __device__ __forceinline__ int part_units(const PartsParams& p, const PartLengths& at, int z) {
     const bool paged = p.table != nullptr;
     int n;
-    if constexpr (KIND == kPrefixPart) n = paged ? at.eff[z] : part_clamp(p.prefix[z], p.capacity[0]);
-    else n = part_clamp(p.lengths[z], p.capacity[1]) - (paged ? at.eff[z / p.per] : 0);
+    if constexpr (KIND == kPrefixPart) n = paged ? at.shared(p, z) : z < 64 ? at.pre0 : part_clamp(p.prefix[z], p.capacity[0]);
+    else n = (z < 64 ? at.own0 : part_clamp(p.lengths[z], p.capacity[1])) - (paged ? at.shared(p, part_group(p, z)) : 0);
     return (max(n, 0) + kPartUnit - 1) / kPartUnit;
 }
 
 // Places of units and of what segments cost besides.
 __device__ __forceinline__ int part_places(int units) { return units > 0 ? units + kPartExtra : 0; }
 
+// The first 64 groups or sequences, one a lane: units, and sums of places and of units up to them.
+struct PartScan {
+    int units, places, sum;
+};
+template <int KIND>
+__device__ __forceinline__ PartScan part_scan(const PartsParams& p, const PartLengths& at, int j0) {
+    const int lane = threadIdx.x & 63;
+    PartScan r;
+    r.units = j0 + lane < (KIND == kPrefixPart ? p.groups : p.B) ? part_units<KIND>(p, at, j0 + lane) : 0;
+    r.places = scan64(part_places(r.units));
+    r.sum = scan64(r.units);
+    return r;
+}
+
 // Places of all groups or sequences; the wave that `tells` leaves them for the merge.
 template <int KIND>
-__device__ __forceinline__ int part_total(const PartsParams& p, const PartLengths& at, bool tells) {
+__device__ __forceinline__ int part_total(const PartsParams& p, const PartLengths& at, bool tells, PartScan& first) {
     const int Z = KIND == kPrefixPart ? p.groups : p.B, lane = threadIdx.x & 63;
     int32_t* meta = p.meta[KIND == kPrefixPart ? 0 : 1];
     int U = 0;
     for (int j0 = 0; j0 < Z; j0 += 64) {
-        const int units = j0 + lane < Z ? part_units<KIND>(p, at, j0 + lane) : 0, own = part_places(units);
-        const int s = scan64(own);
+        const PartScan s = part_scan<KIND>(p, at, j0);
+        if (j0 == 0) first = s;
         if (tells && j0 + lane < Z) {
-            meta[2 + 2 * (j0 + lane)] = U + s - own;
-            meta[3 + 2 * (j0 + lane)] = units;
+            meta[2 + 2 * (j0 + lane)] = U + s.places - part_places(s.units);
+            meta[3 + 2 * (j0 + lane)] = s.units;
         }
-        U += __builtin_amdgcn_readlane(s, 63);
+        U += __builtin_amdgcn_readlane(s.places, 63);
     }
     return U;
 }
@@ -168,18 +202,19 @@ struct PartWalk {
     };
     const PartsParams& p;
     const PartLengths& lens;
+    const PartScan& scan0;
     const int U, Z;
     const bool paged;
 
-    __device__ __forceinline__ PartWalk(const PartsParams& p_, const PartLengths& lens_, int U_)
-        : p(p_), lens(lens_), U(U_), Z(KIND == kPrefixPart ? p_.groups : p_.B), paged(p_.table != nullptr) {}
+    __device__ __forceinline__ PartWalk(const PartsParams& p_, const PartLengths& lens_, const PartScan& scan0_, int U_)
+        : p(p_), lens(lens_), scan0(scan0_), U(U_), Z(KIND == kPrefixPart ? p_.groups : p_.B), paged(p_.table != nullptr) {}
 
     // a segment's tokens: from `start` to before `end`
     __device__ __forceinline__ int start_of(int z) const {
-        return KIND == kOwnPart && paged ? __builtin_amdgcn_readfirstlane(lens.eff[z / p.per]) : 0;
+        return KIND == kOwnPart && paged ? __builtin_amdgcn_readfirstlane(lens.shared(p, part_group(p, z))) : 0;
     }
     __device__ __forceinline__ int end_of(int z) const {
-        if constexpr (KIND == kPrefixPart) return paged ? __builtin_amdgcn_readfirstlane(lens.eff[z]) : part_clamp(((cint32*)p.prefix)[z], p.capacity[0]);
+        if constexpr (KIND == kPrefixPart) return paged ? __builtin_amdgcn_readfirstlane(lens.shared(p, z)) : part_clamp(((cint32*)p.prefix)[z], p.capacity[0]);
         else return part_clamp(((cint32*)p.lengths)[z], p.capacity[1]);
     }
     __device__ __forceinline__ void enter(At& a) const {
@@ -231,7 +266,6 @@ struct PartWalk {
     }
     // The first unit at or behind a place, and its index among all.
     __device__ __forceinline__ int locate(int place, At& a) const {
-        const int lane = threadIdx.x & 63;
         a.slot = place / U;
         int x = place - a.slot * U, before;
         if constexpr (KIND == kListPart) {
@@ -243,19 +277,18 @@ struct PartWalk {
             int total = 0, left = 0;  // units of all groups or sequences, and of those before z
             bool found = false;
             for (int j0 = 0; j0 < Z; j0 += 64) {
-                const int units = j0 + lane < Z ? part_units<KIND>(p, lens, j0 + lane) : 0, own = part_places(units);
-                const int s = scan64(own), su = scan64(units);
-                const uint64_t hit = __ballot(s > x);  // segments ending past x
+                const PartScan s = j0 == 0 ? scan0 : part_scan<KIND>(p, lens, j0);
+                const uint64_t hit = __ballot(s.places > x);  // segments ending past x
                 if (!found && hit != 0) {
                     const int l = __builtin_ctzll(hit);
                     found = true;
                     a.z = j0 + l;
-                    left = total + __builtin_amdgcn_readlane(su - units, l);
-                    x -= __builtin_amdgcn_readlane(s - own, l);
+                    left = total + __builtin_amdgcn_readlane(s.sum - s.units, l);
+                    x -= __builtin_amdgcn_readlane(s.places - part_places(s.units), l);
                 } else if (!found) {
-                    x -= __builtin_amdgcn_readlane(s, 63);
+                    x -= __builtin_amdgcn_readlane(s.places, 63);
                 }
-                total += __builtin_amdgcn_readlane(su, 63);
+                total += __builtin_amdgcn_readlane(s.sum, 63);
             }
             before = a.slot * total + left;
         }
@@ -300,24 +333,17 @@ __device__ __forceinline__ void part_query_bits(const PartsParams& p, u32x4 (&w)
     for (int k = 0; k < NK; ++k) w[k] = 16 * (4 * k + g4) < row_bytes ? q_bits(w[k], p.q_and, p.q_xor) : u32x4{0u, 0u, 0u, 0u};
 }
 
-// The running maxima of NC sets of columns rise to those of a unit's scores; what was summed on the old base is scaled to the new one.
-template <int NC, int DPL>
-__device__ __forceinline__ void part_rise(const f32x4 (&sc)[NC][2], float scale, float (&M)[NC], float (&l)[NC], f32x4 (&acc)[NC][DPL]) {
-    float Mn[NC];
-    bool grows = false;
+// The running maxima of NC sets of columns rise to those of NT tiles' scores; what was summed on the old base is scaled to the new one.
+template <int NC, int NT, int DPL>
+__device__ __forceinline__ void part_rise(const f32x4 (&sc)[NC][NT], float scale, float (&M)[NC], float (&l)[NC], f32x4 (&acc)[NC][DPL]) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         float mx = kNegInf;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) mx = fmaxf(mx, fmaxf(fmaxf(sc[c][tt][0], sc[c][tt][1]), fmaxf(sc[c][tt][2], sc[c][tt][3])));
-        Mn[c] = fmaxf(M[c], max_across_groups<16>(mx) * scale);
-        grows |= Mn[c] > M[c];
-    }
-    if (__ballot(grows) == 0) return;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const float alpha = fast_exp2(M[c] - (Mn[c] == kNegInf ? 0.f : Mn[c]));
-        M[c] = Mn[c];
+        for (int tt = 0; tt < NT; ++tt) mx = fmaxf(mx, fmaxf(fmaxf(sc[c][tt][0], sc[c][tt][1]), fmaxf(sc[c][tt][2], sc[c][tt][3])));
+        const float Mn = fmaxf(M[c], max_across_groups<16>(mx) * scale);
+        const float alpha = fast_exp2(M[c] - (Mn == kNegInf ? 0.f : Mn));
+        M[c] = Mn;
         l[c] *= alpha;
 #pragma unroll
         for (int j = 0; j < DPL; ++j) acc[c][j] *= alpha;
@@ -326,24 +352,38 @@ __device__ __forceinline__ void part_rise(const f32x4 (&sc)[NC][2], float scale,
 
 // P of a unit's scores in one set of columns, as numbers and (16 bits) as two matrix operands, and its part of the row sum.
 template <typename T>
-__device__ __forceinline__ void part_weights(const f32x4 (&sc)[2], float scale, float M, float& l, float (&pf)[8],
+__device__ __forceinline__ void part_weights(const f32x4* sc, float scale, float M, float& l, float (&pf)[8],
                                              typename PartType<T>::vec8 (&pk)[PartType<T>::parts]) {
     const float base = (M == kNegInf ? 0.f : M) - PartType<T>::offset;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         pf[i] = fast_exp2(__builtin_fmaf(sc[i >> 2][i & 3], scale, -base));
         l += pf[i];
-        if constexpr (sizeof(T) == 2) {
-            pk[0][i] = Elem<T>::from_f32(pf[i]);
-            pk[1][i] = Elem<T>::from_f32(pf[i] - Elem<T>::to_f32(pk[0][i]));
+    }
+    if constexpr (sizeof(T) == 2) {
+        // two at a time: one conversion rounds a pair
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            hi[i] = pack2<T>(pf[2 * i], pf[2 * i + 1]);
+            float a, b;
+            if constexpr (__is_same(T, bf16_t)) {
+                a = __builtin_bit_cast(float, hi[i] << 16), b = __builtin_bit_cast(float, hi[i] & 0xffff0000u);
+            } else {
+                const f16x2 h = __builtin_bit_cast(f16x2, hi[i]);
+                a = (float)h[0], b = (float)h[1];
+            }
+            lo[i] = pack2<T>(pf[2 * i] - a, pf[2 * i + 1] - b);
         }
+        pk[0] = __builtin_bit_cast(typename PartType<T>::vec8, u32x4{hi[0], hi[1], hi[2], hi[3]});
+        pk[1] = __builtin_bit_cast(typename PartType<T>::vec8, u32x4{lo[0], lo[1], lo[2], lo[3]});
     }
 }
 
 // Share r of the segments of one part, U places in each of Hkv * nsub column sets.
 // NC: sets of 16 columns.  TWO: a unit's two tiles of 16 tokens may lie apart (pages or blocks of 16 tokens).
 template <typename T, int D, int NC, int KIND, bool TWO>
-__device__ void decode_part(const PartsParams& p, const PartLengths& lens, int U, const PartShares& sh, int r, float (*red_o)[16][D + 4],
+__device__ void decode_part(const PartsParams& p, const PartLengths& lens, const PartScan& scan0, int U, const PartShares& sh, int r, float (*red_o)[16][D + 4],
                             float (*red_m)[16], float (*red_l)[16]) {
     typedef typename PartType<T>::vec8 V8;
     constexpr bool kF32 = sizeof(T) == 4;
@@ -358,7 +398,7 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, int U
     typedef typename Walk::At At;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g4 = lane >> 4;
-    const Walk walk(p, lens, U);
+    const Walk walk(p, lens, scan0, U);
     At at;
     const int n = walk.units(sh, r, at);  // units of this workgroup
     if (n == 0) return;
@@ -484,7 +524,7 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, int U
                             for (int c = 0; c < NC; ++c) sc[c][tt][i] = kNegInf;
                         }
             }
-            part_rise<NC, DPL>(sc, p.c, M, l, acc);
+            part_rise(sc, p.c, M, l, acc);
             // two tokens' values of one dim side by side
             auto pair_up = [&](int w, V8* out) {
                 uint32_t a[4], b[4];
@@ -606,45 +646,76 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, int U
 template <int D>
 __device__ __forceinline__ int part_swizzle(int r) { return D == 128 ? 2 * (r & 7) + ((r >> 3) & 1) : (r >> 1) & 7; }
 
-// Share r of the prefix for many rows (16-bit types): the four waves hold 16 NC rows each, and a unit's keys and values go through LDS once
-// for all of them, by direct loads into a ring of three stages.  A unit then costs a wave half the instructions of the form above
-// (no addresses of its own, no pairing of values, which a transposed read replaces).
+// Share r of the prefix for many rows (16-bit types): the four waves hold 16 NC rows each, and keys and values go through LDS once for all
+// of them, two units a stage, by direct loads into one of two buffers while the other is worked on.  A unit then costs a wave a third of
+// the instructions of the form above: no addresses of its own, no pairing of values, which a transposed read replaces, and one
+// rescaling for two units.
+constexpr int kStageTokens = 2 * kPartUnit;
+
 template <typename T, int D, int NC>
-__device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, int U, const PartShares& sh, int r, T (*kv)[2][kPartUnit * D]) {
+__device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, const PartScan& scan0, int U, const PartShares& sh, int r,
+                                 T (*kv)[2][kStageTokens * D]) {
     typedef typename Elem<T>::vec8 V8;
     typedef typename Elem<T>::vec4 V4;
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     typedef PartWalk<kPrefixPart, 1> Walk;
     typedef typename Walk::At At;
-    constexpr int NK = D / 32, NV = D / 16, CH = D / 8, RPL = 64 / CH, NL = 8 / RPL;  // CH: chunks of a row; a wave's loads of 8 rows: NL of RPL
+    constexpr int NK = D / 32, NV = D / 16, CH = D / 8, RPL = 64 / CH, NL = 16 / RPL;  // CH: chunks of a row; a wave's 16 rows: NL loads of RPL
+    constexpr int NT = kStageTokens / 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g4 = lane >> 4;
-    const Walk walk(p, lens, U);
+    const Walk walk(p, lens, scan0, U);
     At cur;
     const int n = walk.units(sh, r, cur);
     if (n == 0) return;
     walk.enter(cur);
 
-    // rows 8 wave .. 8 wave + 7 of a unit, which lie in its tile wave / 2
+    // each wave loads a tile of a stage
     const uint32_t kp = (uint32_t)p.k_s[0], vp = (uint32_t)p.v_s[0];
     uint32_t koff[NL], voff[NL];
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-        const int row = 8 * wave + RPL * i + lane / CH, c = (lane % CH) ^ part_swizzle<D>(row);
+        const int row = RPL * i + lane / CH, c = (lane % CH) ^ part_swizzle<D>(row);
         const bool there = 8 * c < p.d;  // chunks past the real head dim come as zeros
-        koff[i] = there ? (uint32_t)(row & 15) * kp + (uint32_t)(16 * c) : 0xc0000000u;
-        voff[i] = there ? (uint32_t)(row & 15) * vp + (uint32_t)(16 * c) : 0xc0000000u;
+        koff[i] = there ? (uint32_t)row * kp + (uint32_t)(16 * c) : 0xc0000000u;
+        voff[i] = there ? (uint32_t)row * vp + (uint32_t)(16 * c) : 0xc0000000u;
     }
-    auto issue = [&](int buf, At& a) {
-        walk.find_tile(a, 0, 16 * (wave >> 1), 16);
+    // the stage to be loaded next: its units lie in one segment
+    At nx = cur;
+    int nx_left = n;                                   // units of the share from it on
+    int nx_here = min(cur.units - cur.u, nx_left);     // of its segment
+    // 64 page ids from page `ids_from` of row `ids_row` on, one a lane: a scalar load a stage would be waited for before its first key
+    int ids = 0, ids_from = 0, ids_row = -1;
+    auto issue = [&](int buf) {
+        // a second unit that is not there is loaded as no rows
+        const int t = nx.u * kPartUnit + 16 * wave;
+        nx.rows[0] = wave < 2 || nx_here > 1 ? part_clamp(nx.end - t, 16) : 0;
+        nx.t[0] = nx.rows[0] > 0 ? t : 0;
+        nx.page[0] = nx.z;
+        if (walk.paged) {
+            const int page = nx.t[0] >> p.page_shift, first = (nx.u * kPartUnit) >> p.page_shift;  // of this wave's tile, and of the unit
+            if (nx.row != ids_row || first < ids_from || first + 4 > ids_from + 64) {
+                ids_row = nx.row, ids_from = first;
+                const int64_t at = (int64_t)(p.capacity[0] >> p.page_shift) - 1;
+                ids = p.table[nx.row * p.bt_s + min((int64_t)first + lane, at)];
+            }
+            if (nx.rows[0] > 0) nx.page[0] = __builtin_amdgcn_readlane(ids, page - ids_from);
+        }
         const uint32_t row_bytes = (uint32_t)(p.d * (int)sizeof(T));
-        const auto krs = make_rsrc(walk.base(a, 0, p.k[0], p.k_b[0], p.k_h[0], p.k_s[0]), a.rows[0] > 0 ? (uint32_t)(a.rows[0] - 1) * kp + row_bytes : 0u);
-        const auto vrs = make_rsrc(walk.base(a, 0, p.v[0], p.v_b[0], p.v_h[0], p.v_s[0]), a.rows[0] > 0 ? (uint32_t)(a.rows[0] - 1) * vp + row_bytes : 0u);
+        const auto krs = make_rsrc(walk.base(nx, 0, p.k[0], p.k_b[0], p.k_h[0], p.k_s[0]), nx.rows[0] > 0 ? (uint32_t)(nx.rows[0] - 1) * kp + row_bytes : 0u);
+        const auto vrs = make_rsrc(walk.base(nx, 0, p.v[0], p.v_b[0], p.v_h[0], p.v_s[0]), nx.rows[0] > 0 ? (uint32_t)(nx.rows[0] - 1) * vp + row_bytes : 0u);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            buf_ld16_lds_async(krs, &kv[buf][0][(8 * wave + RPL * i) * D], koff[i]);
-            buf_ld16_lds_async(vrs, &kv[buf][1][(8 * wave + RPL * i) * D], voff[i]);
+            buf_ld16_lds_async(krs, &kv[buf][0][(16 * wave + RPL * i) * D], koff[i]);
+            buf_ld16_lds_async(vrs, &kv[buf][1][(16 * wave + RPL * i) * D], voff[i]);
+        }
+        const int took = min(nx_here, 2);
+        nx_left -= took, nx_here -= took, nx.u += took;
+        if (nx_here == 0 && nx_left > 0) {
+            walk.next(nx);
+            nx.u = 0;
+            nx_here = min(nx.units, nx_left);
         }
     };
     const int R = walk.rows_of_head();
@@ -659,12 +730,7 @@ __device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, 
         }
     };
     load_q(cur);
-    At nx = cur;
-    issue(0, nx);
-    if (n > 1) {
-        walk.advance(nx, 1);
-        issue(1, nx);
-    }
+    issue(0);
     f32x4 acc[NC][NV];
     float M[NC], l[NC];
     int buf = 0;
@@ -679,26 +745,18 @@ __device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, 
             for (int j = 0; j < NV; ++j) acc[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
             part_query_bits<T, NK>(p, qf[c]);
         }
-        for (int i = 0; i < m; ++i, ++u) {
-            // this wave's loads of stage u have landed when no more are left than those of stage u + 1; then everybody's
-            if (u + 1 < n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            lds_barrier();
-            if (u + 2 < n) {  // every wave is done with stage u - 1
-                walk.advance(nx, 1);
-                issue(buf == 0 ? 2 : buf - 1, nx);
-            }
+        for (int i = 0; i < m; i += 2) {
+            wait_vmem();    // this wave's loads of the stage have landed
+            lds_barrier();  // everybody's have, and the other buffer has been read
+            if (nx_left > 0) issue(buf ^ 1);
             const T* K = kv[buf][0];
             const T* V = kv[buf][1];
-            f32x4 sc[NC][2];
+            f32x4 sc[NC][NT];
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt) {
+            for (int tt = 0; tt < NT; ++tt) {
                 V8 kf[NK];
 #pragma unroll
-                for (int k = 0; k < NK; ++k) {
-                    const int row = 16 * tt + col;
-                    kf[k] = __builtin_bit_cast(V8, ld16(K + row * D + 8 * ((4 * k + g4) ^ part_swizzle<D>(row))));
-                }
+                for (int k = 0; k < NK; ++k) kf[k] = __builtin_bit_cast(V8, ld16(K + (16 * tt + col) * D + 8 * ((4 * k + g4) ^ part_swizzle<D>(col))));
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     sc[c][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -706,10 +764,10 @@ __device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, 
                     for (int k = 0; k < NK; ++k) sc[c][tt] = mfma16(kf[k], __builtin_bit_cast(V8, qf[c][k]), sc[c][tt]);
                 }
             }
-            const int left = seg.end - seg.start - (seg.u + i) * kPartUnit;
-            if (left < kPartUnit) {
+            const int left = __builtin_amdgcn_readfirstlane(min(seg.end - seg.start - (seg.u + i) * kPartUnit, (m - i) * kPartUnit));
+            if (left < kStageTokens) {
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
+                for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (16 * tt + 4 * g4 + e >= left) {
@@ -717,30 +775,34 @@ __device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, 
                             for (int c = 0; c < NC; ++c) sc[c][tt][e] = kNegInf;
                         }
             }
-            part_rise<NC, NV>(sc, p.c, M, l, acc);
-            V8 pk[NC][2];
+            part_rise(sc, p.c, M, l, acc);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float pf[8];
-                part_weights<T>(sc[c], p.c, M[c], l[c], pf, pk[c]);
+            for (int t2 = 0; t2 < NT / 2; ++t2) {
+                V8 pk[NC][2];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    float pf[8];
+                    part_weights<T>(&sc[c][2 * t2], p.c, M[c], l[c], pf, pk[c]);
+                }
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int row = 4 * g4 + (col >> 2), ch = (2 * j + ((col & 3) >> 1)) ^ part_swizzle<D>(row);
+                    const int off = (32 * t2 + row) * D + 8 * ch + 4 * (col & 1);
+                    const V4 lo = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + off)));
+                    const V4 hi = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + off + 16 * D)));
+                    const V8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < NC; ++c) acc[c][j] = mfma16(vf, pk[c][h], acc[c][j]);
+                }
             }
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int row = 4 * g4 + (col >> 2), ch = (2 * j + ((col & 3) >> 1)) ^ part_swizzle<D>(row);
-                const int off = row * D + 8 * ch + 4 * (col & 1);
-                const V4 lo = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + off)));
-                const V4 hi = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(V + off + 16 * D)));
-                const V8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) acc[c][j] = mfma16(vf, pk[c][h], acc[c][j]);
-            }
-            buf = buf == 2 ? 0 : buf + 1;
+            buf ^= 1;
         }
+        u += m;
         if (u < n) {
-            cur.u = 0;
             walk.next(cur);
+            cur.u = 0;
             load_q(cur);
         }
 #pragma unroll

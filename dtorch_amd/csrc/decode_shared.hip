@@ -17,11 +17,11 @@ constexpr int part_columns(bool f32, int kernel_d) { return f32 && kernel_d == 1
 
 // Workgroups of the prefix, in eighths of all: as its units' cost is to that of all, with one of either kind at least where there is
 // any work for it.
-__device__ __forceinline__ int prefix_shares(int64_t cost0, int64_t cost1, int most) {
+__device__ __forceinline__ int prefix_shares(float cost0, float cost1, int most) {
     const int eighth = most / 8;
-    if (cost0 == 0) return 0;
-    if (cost1 == 0) return most;
-    return 8 * (int)min(max((cost0 * eighth + (cost0 + cost1) / 2) / (cost0 + cost1), (int64_t)1), (int64_t)(eighth - 1));
+    if (cost0 == 0.f) return 0;
+    if (cost1 == 0.f) return most;
+    return 8 * min(max((int)(cost0 / (cost0 + cost1) * (float)eighth + 0.5f), 1), eighth - 1);
 }
 
 }  // namespace
@@ -31,17 +31,17 @@ __device__ __forceinline__ int prefix_shares(int64_t cost0, int64_t cost1, int m
 // ROWS: the prefix by rows (16-bit types).
 template <typename T, int D, int NC, bool TWO, bool ROWS>
 __global__ void __launch_bounds__(64 * kPartWaves, 2) decode_shared_kernel(const PartsParams p) {
-    constexpr size_t kMeet = sizeof(float) * kPartWaves * 16 * (D + 4), kRing = ROWS ? sizeof(T) * 3 * 2 * kPartUnit * D : 0;
+    constexpr size_t kMeet = sizeof(float) * kPartWaves * 16 * (D + 4), kRing = ROWS ? sizeof(T) * 2 * 2 * kStageTokens * D : 0;
     __shared__ __attribute__((aligned(1024))) char lds[kMeet > kRing ? kMeet : kRing];
     float (*const red_o)[16][D + 4] = reinterpret_cast<float (*)[16][D + 4]>(lds);
     __shared__ float red_m[kPartWaves][16], red_l[kPartWaves][16];
-    __shared__ int eff[kPartGroups], lead[kPartGroups];
-    const PartLengths lens = {eff, lead};
-    part_lengths(p, lens);
+    __shared__ int least[kPartGroups], lead[kPartGroups], said[kPartGroups];
+    const PartLengths lens = part_lengths(p, least, lead, said);
     const bool tells = blockIdx.x == 0 && threadIdx.x < 64;
-    const int U0 = part_total<kPrefixPart>(p, lens, tells), U1 = part_total<kOwnPart>(p, lens, tells);
+    PartScan scan[2];
+    const int U0 = part_total<kPrefixPart>(p, lens, tells, scan[0]), U1 = part_total<kOwnPart>(p, lens, tells, scan[1]);
     const int V0 = U0 * p.Hkv * p.nsub[0], V1 = U1 * p.Hkv * p.nsub[1];
-    const int most0 = prefix_shares((int64_t)V0 * p.weight[0], (int64_t)V1 * p.weight[1], p.shares), most1 = p.shares - most0;
+    const int most0 = prefix_shares((float)V0 * (float)p.weight[0], (float)V1 * (float)p.weight[1], p.shares), most1 = p.shares - most0;
     if (tells && threadIdx.x == 0) {
         p.meta[0][0] = U0, p.meta[0][1] = most0;
         p.meta[1][0] = U1, p.meta[1][1] = most1;
@@ -53,11 +53,11 @@ __global__ void __launch_bounds__(64 * kPartWaves, 2) decode_shared_kernel(const
     const int r = first && p.nsub[0] > 1 ? x * per + at : at * 8 + x;
     if ((first ? V0 : V1) == 0 || at >= per || r >= sh.n) return;
     if (first) {
-        if constexpr (ROWS) decode_part_rows<T, D, NC>(p, lens, U0, sh, r, reinterpret_cast<T (*)[2][kPartUnit * D]>(lds));
-        else decode_part<T, D, NC, kPrefixPart, TWO>(p, lens, U0, sh, r, red_o, red_m, red_l);
+        if constexpr (ROWS) decode_part_rows<T, D, NC>(p, lens, scan[0], U0, sh, r, reinterpret_cast<T (*)[2][kStageTokens * D]>(lds));
+        else decode_part<T, D, NC, kPrefixPart, TWO>(p, lens, scan[0], U0, sh, r, red_o, red_m, red_l);
         return;
     }
-    decode_part<T, D, 1, kOwnPart, TWO>(p, lens, U1, sh, r, red_o, red_m, red_l);
+    decode_part<T, D, 1, kOwnPart, TWO>(p, lens, scan[1], U1, sh, r, red_o, red_m, red_l);
 }
 
 namespace {
@@ -216,6 +216,7 @@ extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* st
     p.lse_b = a->lse != nullptr ? a->lse_stride[0] : 0;
     p.B = (int32_t)a->B, p.Hq = (int32_t)a->Hq, p.Hkv = (int32_t)a->Hkv, p.group = (int32_t)(a->Hq / a->Hkv);
     p.groups = (int32_t)a->groups, p.per = (int32_t)(a->B / a->groups);
+    p.per_inv = 1.f / (float)p.per;
     p.d = (int32_t)a->D;
     p.c = sp.scale * kLog2e;
     p.q_and = sp.q_and, p.q_xor = sp.q_xor;

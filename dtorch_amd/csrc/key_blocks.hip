@@ -139,6 +139,30 @@ __global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p)
     uint32_t* order = p.order + bh * p.blocks_max;
     const int quad = tid >> 2, l = tid & 3;
     const int in_page = p.c.page_shift - p.c.block_shift;  // log2 of a page's blocks
+    u32x4 wl[W][NI], wh[W][NI];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const int j = min(j0 + quad + 64 * w, cand - 1);
+            int64_t slot = b, jb = j;
+            if (p.c.table != nullptr) {
+                slot = min(max(p.c.table[b * p.c.bt_s + (j >> in_page)], 0), p.c.num_pages - 1);
+                jb = j & ((1 << in_page) - 1);
+            }
+            const char* lo = p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s;
+            const char* hi = p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int c = l + 4 * i;
+                const bool there = E * c < p.d;
+                wl[w][i] = ld16_nt(lo + (there ? 16 * c : 0));
+                wh[w][i] = ld16_nt(hi + (there ? 16 * c : 0));
+                if (!there) wl[w][i] = wh[w][i] = u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+    };
+    // on their way while the query is laid out; two blocks a quad are more than the waves that hide each other's loads have registers for
+    if constexpr (W == 1) load(blockIdx.y * 64 * W);
     for (int g0 = 0; g0 < p.group; g0 += kScoreHeads) {
         const int heads = min(p.group - g0, kScoreHeads);
         if (g0 > 0) __syncthreads();  // the last heads have been used
@@ -163,26 +187,7 @@ __global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p)
         }
         __syncthreads();
         for (int j0 = blockIdx.y * 64 * W; j0 < cand; j0 += gridDim.y * 64 * W) {
-            u32x4 wl[W][NI], wh[W][NI];
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const int j = min(j0 + quad + 64 * w, cand - 1);
-                int64_t slot = b, jb = j;
-                if (p.c.table != nullptr) {
-                    slot = min(max(p.c.table[b * p.c.bt_s + (j >> in_page)], 0), p.c.num_pages - 1);
-                    jb = j & ((1 << in_page) - 1);
-                }
-                const char* lo = p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s;
-                const char* hi = p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s;
-#pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const int c = l + 4 * i;
-                    const bool there = E * c < p.d;
-                    wl[w][i] = ld16_nt(lo + (there ? 16 * c : 0));
-                    wh[w][i] = ld16_nt(hi + (there ? 16 * c : 0));
-                    if (!there) wl[w][i] = wh[w][i] = u32x4{0u, 0u, 0u, 0u};
-                }
-            }
+            if (W > 1 || g0 > 0 || j0 > (int)blockIdx.y * 64 * W) load(j0);
             float best[W];
 #pragma unroll
             for (int w = 0; w < W; ++w) best[w] = kNegInf;

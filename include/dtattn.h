@@ -530,7 +530,7 @@ int dtattn_kv_pages_compact(const dtattn_kv_compact_args* args, void* stream);
  * the same pages for every sequence of the group with any tokens (the slots of its first such sequence are read).  Where a sequence with
  * tokens is shorter than that, the whole group shares as many whole pages as that sequence fills, no more.
  * Lengths are clamped to their capacity, page ids into the pool.  No rows: O = 0, LSE = -inf.
- * D up to 128, a multiple of 16 bytes; up to 2048 groups.  16-bit types: scores, softmax statistics and accumulators are fp32, and P
+ * D up to 128, a multiple of 16 bytes; up to 1024 groups.  16-bit types: scores, softmax statistics and accumulators are fp32, and P
  * enters the second product as two numbers of its type (its rounding and the remainder's).  FP32: fp32 matrix instructions. */
 typedef struct {
     const void* q;           /* [B, Hq, 1, D], 16-byte aligned, strides multiples of 16 bytes */

@@ -126,7 +126,7 @@ OWN = {
     "reserve": TABLE + POOLS + [(dict(short_by=None), 1, "null"), (dict(n_new=-1), 1, "new tokens"), (dict(workspace=None), 3, "workspace"),
                                 (dict(workspace=0x10080, workspace_bytes=1 << 30), 3, "256-byte")],
     "compact": TABLE + POOLS + [(dict(used=None), 1, "null"), (dict(workspace=None), 3, "workspace"), (dict(workspace=0x10080, workspace_bytes=1 << 30), 3, "256-byte")],
-    "shared": ROWS + HEADS + CACHES + [(dict(groups=0), 1, "bad sizes"), (dict(groups=3), 1, "equal groups"), (dict(B=4098, groups=2049), 2, "groups"),
+    "shared": ROWS + HEADS + CACHES + [(dict(groups=0), 1, "bad sizes"), (dict(groups=3), 1, "equal groups"), (dict(B=4098, groups=2049), 2, "groups"), (dict(B=1025, groups=1025), 2, "groups"),
                                        (dict(prefix_lengths=None), 1, "null"), (dict(k_prefix=None), 1, "null"), (dict(S_prefix=0), 1, "capacities"),
                                        (dict(S_max=(1 << 29) + 1), 1, "capacities"), (dict(v_prefix_stride=(0, 0, 64)), 2, "row stride")],
     "bounds": ROWS + BLOCK + [(dict(n_new=-1), 1, "bad sizes"), (dict(k_min=0x880000, k_max=0x880000), 1, "share memory"), (dict(k_min=None), 1, "null"),
