@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(64 * kPartWaves, 2) decode_blocks_kernel(const
     __shared__ float red_m[kPartWaves][16], red_l[kPartWaves][16];
     const int U = p.B * part_places(p.list_units);
     const PartShares sh(U * p.Hkv * p.nsub[1], p.shares);
-    if ((int)blockIdx.x < sh.n) decode_part<T, D, 1, kListPart, TWO>(p, PartLengths{}, PartScan{}, U, sh, blockIdx.x, red_o, red_m, red_l);
+    if ((int)blockIdx.x < sh.n) decode_part<T, D, kListPart, TWO>(p, PartLengths{}, PartScan{}, U, sh, blockIdx.x, red_o, red_m, red_l);
 }
 
 namespace {

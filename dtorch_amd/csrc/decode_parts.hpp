@@ -5,7 +5,7 @@
 // end, each segment's behind places that stand for its own cost, and cut in equal shares, one per workgroup, whose four waves take its
 // units in turn and meet in LDS where a segment ends.
 // A segment's columns are query rows that read the same keys: the query heads of a kv head (a sequence's own tokens and listed blocks), or
-// those of all sequences of a group (the prefix), 16 NC of them.
+// those of all sequences of a group (the prefix), 16 of them a set, or 64 and 128 where the prefix is read by rows.
 //
 // K and V go from memory to registers to matrix operands, without LDS.  Keys are the matrix rows: a lane loads 16-byte pieces of one
 // key, in an order of the head dims that the query shares.  Scores come out with a lane's four keys of a tile in registers, which is
@@ -61,7 +61,8 @@ constexpr int kPartUnit = 32;  // tokens
 constexpr int kPartWaves = 4;
 constexpr int kPartLeast = kPartWaves + 1;  // places of a share, at least
 constexpr int kPartGroups = 1024;
-// What a segment costs besides its units, in units: its waves meet, and the last of them take turns that others have no unit for.
+// What a segment costs besides its units, in units: its waves meet, and the last of them take turns that others have no unit for.  64
+// sequences of one or two tokens behind 8192 take 62.5 us with 0 and 48.7 with 4.
 constexpr int kPartExtra = 4;
 
 // V places in `n` shares of V / n or one more (all the longer ones first); the host keeps V below 2^31.
@@ -381,8 +382,8 @@ __device__ __forceinline__ void part_weights(const f32x4* sc, float scale, float
 }
 
 // Share r of the segments of one part, U places in each of Hkv * nsub column sets.
-// NC: sets of 16 columns.  TWO: a unit's two tiles of 16 tokens may lie apart (pages or blocks of 16 tokens).
-template <typename T, int D, int NC, int KIND, bool TWO>
+// TWO: a unit's two tiles of 16 tokens may lie apart (pages or blocks of 16 tokens).
+template <typename T, int D, int KIND, bool TWO>
 __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const PartScan& scan0, int U, const PartShares& sh, int r, float (*red_o)[16][D + 4],
                             float (*red_m)[16], float (*red_l)[16]) {
     typedef typename PartType<T>::vec8 V8;
@@ -451,9 +452,9 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
         }
     };
 
-    f32x4 acc[NC][DPL];
-    float M[NC], l[NC];  // running max, and this lane's part of the row sum on that base
-    u32x4 qf[NC][NK];
+    f32x4 acc[1][DPL];
+    float M[1], l[1];  // running max, and this lane's part of the row sum on that base
+    u32x4 qf[NK];
     At cur = at, nx = at;
     if (wave < n) {
         if (wave > 0) walk.advance(nx, wave);
@@ -463,27 +464,21 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
     }
     const int R = walk.rows_of_head();
     auto load_q = [&](const At& a) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            int b, hq;
-            walk.where(a.z, a.hk, min(16 * NC * (a.slot - a.hk * p.nsub[S]) + 16 * c + col, R - 1), b, hq);
-            part_query<T, NK>(p, b, hq, qf[c]);
-        }
+        int b, hq;
+        walk.where(a.z, a.hk, min(16 * (a.slot - a.hk * p.nsub[S]) + col, R - 1), b, hq);
+        part_query<T, NK>(p, b, hq, qf);
     };
     load_q(cur);
     int s = wave;  // this wave's next unit of the share
     for (int u = 0; u < n;) {
         const int m = min(cur.units - cur.u, n - u);  // units of the segment
-        const int hk = cur.hk, z = cur.z, R0 = 16 * NC * (cur.slot - hk * p.nsub[S]);
+        const int hk = cur.hk, z = cur.z, R0 = 16 * (cur.slot - hk * p.nsub[S]);
         const bool whole = cur.u == 0 && m == cur.units;
         bool seen = false;
+        M[0] = kNegInf, l[0] = 0.f;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            M[c] = kNegInf, l[c] = 0.f;
-#pragma unroll
-            for (int j = 0; j < DPL; ++j) acc[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            part_query_bits<T, NK>(p, qf[c]);
-        }
+        for (int j = 0; j < DPL; ++j) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        part_query_bits<T, NK>(p, qf);
         for (; s < u + m; s += kPartWaves) {
             int rows[NR];
 #pragma unroll
@@ -493,23 +488,18 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
                 walk.advance(nx, kPartWaves);
                 walk.find(nx);
             }
-            f32x4 sc[NC][2];
+            f32x4 sc[1][2];
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
-#pragma unroll
-                for (int c = 0; c < NC; ++c) sc[c][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                sc[0][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < NK; ++k) {
                     if constexpr (kF32) {
-                        const f32x4 kf = __builtin_bit_cast(f32x4, kr[tt][k]);
+                        const f32x4 kf = __builtin_bit_cast(f32x4, kr[tt][k]), q = __builtin_bit_cast(f32x4, qf[k]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int c = 0; c < NC; ++c) sc[c][tt] = mfma_f32(kf[e], __builtin_bit_cast(f32x4, qf[c][k])[e], sc[c][tt]);
+                        for (int e = 0; e < 4; ++e) sc[0][tt] = mfma_f32(kf[e], q[e], sc[0][tt]);
                     } else {
-#pragma unroll
-                        for (int c = 0; c < NC; ++c)
-                            sc[c][tt] = mfma16(__builtin_bit_cast(V8, kr[tt][k]), __builtin_bit_cast(V8, qf[c][k]), sc[c][tt]);
+                        sc[0][tt] = mfma16(__builtin_bit_cast(V8, kr[tt][k]), __builtin_bit_cast(V8, qf[k]), sc[0][tt]);
                     }
                 }
             }
@@ -519,55 +509,39 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
                 for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if ((TWO ? 0 : 16 * tt) + 4 * g4 + i >= rows[TWO ? tt : 0]) {
-#pragma unroll
-                            for (int c = 0; c < NC; ++c) sc[c][tt][i] = kNegInf;
-                        }
+                        if ((TWO ? 0 : 16 * tt) + 4 * g4 + i >= rows[TWO ? tt : 0]) sc[0][tt][i] = kNegInf;
             }
             part_rise(sc, p.c, M, l, acc);
-            // two tokens' values of one dim side by side
-            auto pair_up = [&](int w, V8* out) {
-                uint32_t a[4], b[4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    a[t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x05040100u);
-                    b[t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x07060302u);
-                }
-                out[0] = __builtin_bit_cast(V8, u32x4{a[0], a[1], a[2], a[3]});
-                out[1] = __builtin_bit_cast(V8, u32x4{b[0], b[1], b[2], b[3]});
-            };
-            // one set of columns leaves room for all operands, so that the values' registers take the next unit's at once
-            constexpr bool kAhead = !kF32 && NC == 1;
-            V8 vf[kAhead ? DPL : 2];
-            if constexpr (kAhead) {
-#pragma unroll
-                for (int w = 0; w < VW; ++w) pair_up(w, &vf[2 * w]);
-                if (more) load_v(nx);
-            }
-            V8 pk[NC][PP];
-            float pf[NC][8];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) part_weights<T>(sc[c], p.c, M[c], l[c], pf[c], pk[c]);
+            V8 pk[PP];
+            float pf[8];
             if constexpr (kF32) {
+                part_weights<T>(sc[0], p.c, M[0], l[0], pf, pk);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
-                    for (int j = 0; j < DPL; ++j)
-#pragma unroll
-                        for (int c = 0; c < NC; ++c) acc[c][j] = mfma_f32(__builtin_bit_cast(float, vr[i][j]), pf[c][i], acc[c][j]);
+                    for (int j = 0; j < DPL; ++j) acc[0][j] = mfma_f32(__builtin_bit_cast(float, vr[i][j]), pf[i], acc[0][j]);
+                if (more) load_v(nx);
             } else {
+                // two tokens' values of one dim side by side, all of them, so that the values' registers take the next unit's at once
+                V8 vf[DPL];
 #pragma unroll
                 for (int w = 0; w < VW; ++w) {
-                    if constexpr (!kAhead) pair_up(w, vf);
+                    uint32_t a[4], b[4];
 #pragma unroll
-                    for (int h = 0; h < PP; ++h)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int c = 0; c < NC; ++c) acc[c][2 * w + j] = mfma16(vf[kAhead ? 2 * w + j : j], pk[c][h], acc[c][2 * w + j]);
+                    for (int t = 0; t < 4; ++t) {
+                        a[t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x05040100u);
+                        b[t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x07060302u);
+                    }
+                    vf[2 * w] = __builtin_bit_cast(V8, u32x4{a[0], a[1], a[2], a[3]});
+                    vf[2 * w + 1] = __builtin_bit_cast(V8, u32x4{b[0], b[1], b[2], b[3]});
                 }
+                if (more) load_v(nx);
+                part_weights<T>(sc[0], p.c, M[0], l[0], pf, pk);
+#pragma unroll
+                for (int h = 0; h < PP; ++h)
+#pragma unroll
+                    for (int j = 0; j < DPL; ++j) acc[0][j] = mfma16(vf[j], pk[h], acc[0][j]);
             }
-            if (!kAhead && more) load_v(nx);
         }
         // the next segment's query is on its way while this one's waves meet
         const bool cut_first = u == 0;
@@ -577,64 +551,59 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
             walk.next(cur);
             load_q(cur);
         }
-        // the waves meet, 16 columns at a time
+        // the waves meet
         const bool any = KIND != kListPart || __syncthreads_or(seen);
+        const int heads = min(R - R0, 16);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int heads = min(R - R0 - 16 * c, 16);
-            if (heads <= 0) break;
-            if (c > 0) lds_barrier();  // the last columns have been read
+        for (int i = 0; i < 4; ++i) {
+            float* at_o = &red_o[wave][col][DPL * (4 * g4 + i)];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float* at_o = &red_o[wave][col][DPL * (4 * g4 + i)];
+            for (int j = 0; j < DPL; j += 4) *reinterpret_cast<f32x4*>(at_o + j) = f32x4{acc[0][j][i], acc[0][j + 1][i], acc[0][j + 2][i], acc[0][j + 3][i]};
+        }
+        const float lw = sum_across_groups<16>(l[0]);
+        if (g4 == 0) red_m[wave][col] = M[0], red_l[wave][col] = lw;
+        lds_barrier();
+        const int g = tid >> 4;  // a column, and DPL of its dims
+        if (g < heads) {
+            float X = kNegInf, lt = 0.f, o[DPL] = {};
 #pragma unroll
-                for (int j = 0; j < DPL; j += 4) *reinterpret_cast<f32x4*>(at_o + j) = f32x4{acc[c][j][i], acc[c][j + 1][i], acc[c][j + 2][i], acc[c][j + 3][i]};
+            for (int w = 0; w < kPartWaves; ++w) X = fmaxf(X, red_m[w][g]);
+#pragma unroll
+            for (int w = 0; w < kPartWaves; ++w) {
+                const float mw = red_m[w][g];
+                const float f = mw == kNegInf ? 0.f : fast_exp2(mw - X);
+                lt = __builtin_fmaf(red_l[w][g], f, lt);
+#pragma unroll
+                for (int j = 0; j < DPL; j += 4) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(&red_o[w][g][DPL * (tid & 15) + j]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[j + i] = __builtin_fmaf(a[i], f, o[j + i]);
+                }
             }
-            const float lw = sum_across_groups<16>(l[c]);
-            if (g4 == 0) red_m[wave][col] = M[c], red_l[wave][col] = lw;
-            lds_barrier();
-            const int g = tid >> 4;  // a column, and DPL of its dims
-            if (g < heads) {
-                float X = kNegInf, lt = 0.f, o[DPL] = {};
+            int b, hq;
+            walk.where(z, hk, R0 + g, b, hq);
+            const int dim = DPL * (tid & 15);
+            const bool direct = KIND == kListPart && whole;
+            const float lse = __builtin_fmaf(X - kOff, kLn2, __log2f(lt) * kLn2);
+            // every score -inf: a record of O = 0 at the LSE of -inf, which drops it in the merge; the output itself is 0 / 0
+            const float inv = (lt == 0.f && !direct) || !any ? 0.f : 1.f / lt;
 #pragma unroll
-                for (int w = 0; w < kPartWaves; ++w) X = fmaxf(X, red_m[w][g]);
+            for (int j = 0; j < DPL; ++j) o[j] *= inv;
+            if (direct) {
+                T* op = reinterpret_cast<T*>(p.o) + b * p.o_b + hq * p.o_h + dim;
 #pragma unroll
-                for (int w = 0; w < kPartWaves; ++w) {
-                    const float mw = red_m[w][g];
-                    const float f = mw == kNegInf ? 0.f : fast_exp2(mw - X);
-                    lt = __builtin_fmaf(red_l[w][g], f, lt);
-#pragma unroll
-                    for (int j = 0; j < DPL; j += 4) {
-                        const f32x4 a = *reinterpret_cast<const f32x4*>(&red_o[w][g][DPL * (tid & 15) + j]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[j + i] = __builtin_fmaf(a[i], f, o[j + i]);
+                for (int j = 0; j < DPL; j += 4)
+                    if (dim + j < p.d) {
+                        if constexpr (kF32) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
+                        else *reinterpret_cast<u32x2*>(op + j) = u32x2{pack2<T>(o[j], o[j + 1]), pack2<T>(o[j + 2], o[j + 3])};
                     }
-                }
-                int b, hq;
-                walk.where(z, hk, R0 + 16 * c + g, b, hq);
-                const int dim = DPL * (tid & 15);
-                const bool direct = KIND == kListPart && whole;
-                const float lse = __builtin_fmaf(X - kOff, kLn2, __log2f(lt) * kLn2);
-                // every score -inf: a record of O = 0 at the LSE of -inf, which drops it in the merge; the output itself is 0 / 0
-                const float inv = (lt == 0.f && !direct) || !any ? 0.f : 1.f / lt;
+                if (p.lse != nullptr && (tid & 15) == 0) p.lse[b * p.lse_b + hq] = lse;
+            } else {
+                const int64_t rec = whole ? (int64_t)b * p.Hq + hq : (int64_t)(2 * r + (cut_first ? 0 : 1)) * 16 + g;
+                float* op = (whole ? p.whole_o[S] : p.rec_o[S]) + rec * D + dim;
 #pragma unroll
-                for (int j = 0; j < DPL; ++j) o[j] *= inv;
-                if (direct) {
-                    T* op = reinterpret_cast<T*>(p.o) + b * p.o_b + hq * p.o_h + dim;
-#pragma unroll
-                    for (int j = 0; j < DPL; j += 4)
-                        if (dim + j < p.d) {
-                            if constexpr (kF32) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
-                            else *reinterpret_cast<u32x2*>(op + j) = u32x2{pack2<T>(o[j], o[j + 1]), pack2<T>(o[j + 2], o[j + 3])};
-                        }
-                    if (p.lse != nullptr && (tid & 15) == 0) p.lse[b * p.lse_b + hq] = lse;
-                } else {
-                    const int64_t rec = whole ? (int64_t)b * p.Hq + hq : (int64_t)(2 * r + (cut_first ? 0 : 1)) * (16 * NC) + 16 * c + g;
-                    float* op = (whole ? p.whole_o[S] : p.rec_o[S]) + rec * D + dim;
-#pragma unroll
-                    for (int j = 0; j < DPL; j += 4) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
-                    if ((tid & 15) == 0) (whole ? p.whole_lse[S] : p.rec_lse[S])[rec] = lse;
-                }
+                for (int j = 0; j < DPL; j += 4) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
+                if ((tid & 15) == 0) (whole ? p.whole_lse[S] : p.rec_lse[S])[rec] = lse;
             }
         }
         if (u < n) lds_barrier();  // every wave has read the others' before they write again

@@ -1,9 +1,12 @@
 // Single-token decode of sequences that share a prefix (semantics: dtattn.h, "attention over a shared prefix"): the arithmetic of
 // SdpaOp::Compute (dtorch/core/operators/standard/scaled_dot_product_attention_op.cc:107-109) at Lq = 1.  The reference has no KV cache.
 //
-// The prefix's keys meet the query heads of all sequences of a group as one matrix product of 16, 32 or 64 columns a wave, so they are
-// read once per so many query rows instead of once per sequence; a long prefix of many sequences is bound by the matrix cores, the
-// sequences' own tokens by HBM.  Both write records, which one more launch merges by LSE.
+// The prefix's keys meet the query heads of all sequences of a group as one matrix product, so they are
+// read once per so many query rows instead of once per sequence; a long prefix of many sequences is bound by the matrix cores and the
+// instructions around them, the sequences' own tokens by HBM.  Both write records, which one more launch merges by LSE.
+// 64 sequences of 32 heads and 8 kv heads, 16 to 1500 own tokens each behind 8192 shared ones, bf16, head dim 128 (233 MB of keys and
+// values): 64 us, 3.6 TB/s.  4 samples of one prompt of 2000 tokens: 17 us, of which 11 are the first launch and 8000 cycles of those the
+// lengths, the shares and the first loads.
 #include <algorithm>
 
 #include "decode_parts.hpp"
@@ -11,9 +14,6 @@
 namespace dtattn {
 
 namespace {
-
-// Sets of 16 columns of a wave that two waves per SIMD have registers for.
-constexpr int part_columns(bool f32, int kernel_d) { return f32 && kernel_d == 128 ? 1 : 2; }
 
 // Workgroups of the prefix, in eighths of all: as its units' cost is to that of all, with one of either kind at least where there is
 // any work for it.
@@ -28,10 +28,10 @@ __device__ __forceinline__ int prefix_shares(float cost0, float cost1, int most)
 
 // One launch for both parts.  Workgroups go to the XCDs in turn; of those on an XCD the first ones take the prefix, so that a CU has some
 // of both, and consecutive shares, whose column sets read the same keys, lie on one XCD and its L2.
-// ROWS: the prefix by rows (16-bit types).
-template <typename T, int D, int NC, bool TWO, bool ROWS>
+// NC: the prefix by rows (16-bit types), 16 NC of them a wave; 0: by keys.
+template <typename T, int D, int NC, bool TWO>
 __global__ void __launch_bounds__(64 * kPartWaves, 2) decode_shared_kernel(const PartsParams p) {
-    constexpr size_t kMeet = sizeof(float) * kPartWaves * 16 * (D + 4), kRing = ROWS ? sizeof(T) * 2 * 2 * kStageTokens * D : 0;
+    constexpr size_t kMeet = sizeof(float) * kPartWaves * 16 * (D + 4), kRing = NC > 0 ? sizeof(T) * 2 * 2 * kStageTokens * D : 0;
     __shared__ __attribute__((aligned(1024))) char lds[kMeet > kRing ? kMeet : kRing];
     float (*const red_o)[16][D + 4] = reinterpret_cast<float (*)[16][D + 4]>(lds);
     __shared__ float red_m[kPartWaves][16], red_l[kPartWaves][16];
@@ -53,18 +53,17 @@ __global__ void __launch_bounds__(64 * kPartWaves, 2) decode_shared_kernel(const
     const int r = first && p.nsub[0] > 1 ? x * per + at : at * 8 + x;
     if ((first ? V0 : V1) == 0 || at >= per || r >= sh.n) return;
     if (first) {
-        if constexpr (ROWS) decode_part_rows<T, D, NC>(p, lens, scan[0], U0, sh, r, reinterpret_cast<T (*)[2][kStageTokens * D]>(lds));
-        else decode_part<T, D, NC, kPrefixPart, TWO>(p, lens, scan[0], U0, sh, r, red_o, red_m, red_l);
+        if constexpr (NC > 0) decode_part_rows<T, D, NC>(p, lens, scan[0], U0, sh, r, reinterpret_cast<T (*)[2][kStageTokens * D]>(lds));
+        else decode_part<T, D, kPrefixPart, TWO>(p, lens, scan[0], U0, sh, r, red_o, red_m, red_l);
         return;
     }
-    decode_part<T, D, 1, kOwnPart, TWO>(p, lens, scan[1], U1, sh, r, red_o, red_m, red_l);
+    decode_part<T, D, kOwnPart, TWO>(p, lens, scan[1], U1, sh, r, red_o, red_m, red_l);
 }
 
 namespace {
 
 struct SharedPlan {
-    int32_t kernel_d, nc, nsub[2], shares, columns[2];
-    bool rows;
+    int32_t kernel_d, nc, nsub[2], shares, columns[2], weight[2];
     size_t meta[2], rec_o[2], rec_lse[2], whole_o, whole_lse, bytes;
 };
 
@@ -76,9 +75,15 @@ SharedPlan plan_shared(const dtattn_decode_shared_args* a, int cus) {
     const int64_t group = a->Hq / a->Hkv, rows = a->B / a->groups * group;
     r.kernel_d = a->D <= 64 ? 64 : 128;
     const bool f32 = a->dtype == DTATTN_FP32;
-    r.rows = !f32 && rows > 32;
-    r.nc = r.rows ? (rows <= 64 ? 1 : 2) : rows <= 16 ? 1 : part_columns(f32, r.kernel_d);
-    r.columns[0] = 16 * r.nc * (r.rows ? kPartWaves : 1), r.columns[1] = 16;
+    // Many rows share a stage of keys in LDS, few divide the keys among the waves.  us with a prefix of 8192 tokens, by keys and by rows: 32
+    // rows 23.6 and 25.6, 64 28.2 and 27.8, 256 57.9 and 42.0.  16 rows a wave up to 128, which leave the waves more to hide behind, 32 beyond,
+    // where the stages count: 128 rows 29.1 and 34.0, 256 65.9 and 63.5 (with up to 1500 own tokens), 512 74.7 and 70.7 (500).
+    r.nc = f32 || rows <= 32 ? 0 : rows <= 128 ? 1 : 2;
+    r.columns[0] = r.nc > 0 ? 16 * r.nc * kPartWaves : 16, r.columns[1] = 16;
+    // What a unit of the prefix costs, and one of the own tokens, of which the workgroups' division follows.  us at these weights and at others:
+    // by keys 33.2 and (1:1) 36.1 (32 rows, 1000 to 4000 own tokens), 16 rows a wave 29.3 and (3:2) 33.1 (64 rows, up to 1500), 32 rows a wave
+    // 70.7 and (1:1) 78.7 (512 rows, up to 500).
+    r.weight[0] = r.nc == 0 ? 2 : r.nc == 1 ? 1 : 3, r.weight[1] = r.nc == 0 ? 3 : r.nc == 1 ? 1 : 2;
     r.shares = std::max(2 * cus / 8 * 8, 16);
     const int64_t cols[2] = {rows, group}, sets[2] = {a->groups, a->B};
     for (int s = 0; s < 2; ++s) {
@@ -95,21 +100,21 @@ SharedPlan plan_shared(const dtattn_decode_shared_args* a, int cus) {
     return r;
 }
 
-template <typename T, int D, int NC, bool ROWS>
+template <typename T, int D, int NC>
 void launch_parts(const PartsParams& p, hipStream_t stream) {
     const dim3 grid((unsigned)p.shares), block(64 * kPartWaves);
-    if (p.table != nullptr && p.page_shift < 5) hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, true, ROWS>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, false, ROWS>), grid, block, 0, stream, p);
+    if (p.table != nullptr && p.page_shift < 5) hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((decode_shared_kernel<T, D, NC, false>), grid, block, 0, stream, p);
 }
 
 template <typename T, int D>
-int launch_shared(const PartsParams& p, int nc, bool rows, hipStream_t stream) {
-    if (!rows) {
-        if (nc == 1) launch_parts<T, D, 1, false>(p, stream);
-        else launch_parts<T, D, part_columns(sizeof(T) == 4, D), false>(p, stream);
-    } else if constexpr (sizeof(T) == 2) {
-        if (nc == 1) launch_parts<T, D, 1, true>(p, stream);
-        else launch_parts<T, D, 2, true>(p, stream);
+int launch_shared(const PartsParams& p, int nc, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2) {
+        if (nc == 0) launch_parts<T, D, 0>(p, stream);
+        else if (nc == 1) launch_parts<T, D, 1>(p, stream);
+        else launch_parts<T, D, 2>(p, stream);
+    } else {
+        launch_parts<T, D, 0>(p, stream);
     }
     const int st = check_launch("decode_shared_kernel");
     if (st != DTATTN_OK) return st;
@@ -203,7 +208,7 @@ extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* st
         return at;
     };
     for (int s = 0; s < 2; ++s) {
-        p.nsub[s] = plan.nsub[s], p.columns[s] = plan.columns[s];
+        p.nsub[s] = plan.nsub[s], p.columns[s] = plan.columns[s], p.weight[s] = plan.weight[s];
         p.meta[s] = reinterpret_cast<int32_t*>(take(plan.meta[s]));
         p.rec_o[s] = reinterpret_cast<float*>(take(plan.rec_o[s]));
         p.rec_lse[s] = reinterpret_cast<float*>(take(plan.rec_lse[s]));
@@ -211,7 +216,6 @@ extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* st
         p.whole_lse[s] = reinterpret_cast<float*>(take(plan.whole_lse));
     }
     p.shares = plan.shares;
-    p.weight[0] = plan.rows ? 3 : 2, p.weight[1] = plan.rows ? 2 : 3;
     p.q_b = a->q_stride[0], p.q_h = a->q_stride[1], p.o_b = a->o_stride[0], p.o_h = a->o_stride[1];
     p.lse_b = a->lse != nullptr ? a->lse_stride[0] : 0;
     p.B = (int32_t)a->B, p.Hq = (int32_t)a->Hq, p.Hkv = (int32_t)a->Hkv, p.group = (int32_t)(a->Hq / a->Hkv);
@@ -222,8 +226,8 @@ extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* st
     p.q_and = sp.q_and, p.q_xor = sp.q_xor;
     const bool wide = plan.kernel_d == 128;
     switch (a->dtype) {
-        case DTATTN_BF16: return wide ? launch_shared<bf16_t, 128>(p, plan.nc, plan.rows, stream) : launch_shared<bf16_t, 64>(p, plan.nc, plan.rows, stream);
-        case DTATTN_FP16: return wide ? launch_shared<f16_t, 128>(p, plan.nc, plan.rows, stream) : launch_shared<f16_t, 64>(p, plan.nc, plan.rows, stream);
-        default: return wide ? launch_shared<float, 128>(p, plan.nc, plan.rows, stream) : launch_shared<float, 64>(p, plan.nc, plan.rows, stream);
+        case DTATTN_BF16: return wide ? launch_shared<bf16_t, 128>(p, plan.nc, stream) : launch_shared<bf16_t, 64>(p, plan.nc, stream);
+        case DTATTN_FP16: return wide ? launch_shared<f16_t, 128>(p, plan.nc, stream) : launch_shared<f16_t, 64>(p, plan.nc, stream);
+        default: return wide ? launch_shared<float, 128>(p, plan.nc, stream) : launch_shared<float, 64>(p, plan.nc, stream);
     }
 }

