@@ -68,6 +68,12 @@ def _bounds(cache: torch.Tensor, block: int):
     return low, torch.zeros_like(low)
 
 
+def _check_selection(keep: int, recent: int, block: int) -> None:
+    """The sizes that select_key_blocks takes, before anything is appended."""
+    if keep % block or recent % block or not block <= recent <= keep:
+        raise ValueError(f"decode: keep {keep} and recent {recent} must be multiples of the block of {block} tokens with block <= recent <= keep")
+
+
 class KVCache:
     """Padded cache [B, Hkv, max_len, D] plus device lengths [B] (int32).
 
@@ -149,6 +155,14 @@ class KVCache:
             raise ValueError("decode(keep=) needs a cache with bounds_block, without track_weights and prefix")
         if prefix is not None and (self.weights is not None or self.k_scale is not None or prefix.k_scale is not None):
             raise ValueError("decode(prefix=) takes caches without codes and track_weights")
+        if keep:
+            _check_selection(keep, recent or self.bounds_block, self.bounds_block)
+        if prefix is not None:
+            p, own = prefix.k, self.k
+            if own.shape[0] % p.shape[0] or (p.shape[1], p.shape[3], p.dtype, p.device) != (own.shape[1], own.shape[3], own.dtype, own.device):
+                raise ValueError("decode(prefix=) takes a cache of the same kv heads, head_dim, dtype and device whose sequences divide this one's")
+            if own.shape[3] > 128 or own.shape[3] * own.element_size() % 16:
+                raise ValueError("decode(prefix=) takes a head_dim up to 128 whose rows are multiples of 16 bytes")
         self.append(k_new, v_new)
         n = self._span()
         k, v, ks = self.k[:, :, :n], self.v[:, :, :n], None
@@ -234,6 +248,7 @@ class PagedKVCache:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.page_refs: Optional[torch.Tensor] = None
         self.prefix_lengths: Optional[torch.Tensor] = None  # of each group, where sequences share pages that are read once
+        self._shares = {}  # the same for every number of groups so far: a captured step reads its own as long as it lives
         self._host_stale = False  # a step was recorded under graph capture, or its parents were on the device: _host_len is behind
 
     def _span_pages(self) -> int:
@@ -258,6 +273,8 @@ class PagedKVCache:
 
     def _track_pages(self) -> None:
         if self.page_refs is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("PagedKVCache: call fork() or compact() once before they are captured")
             self.page_refs = torch.from_numpy(self._refs()).to(self.lengths.device)
 
     def _reserve_shared(self, rows: int, n: int) -> None:
@@ -337,6 +354,10 @@ class PagedKVCache:
         (F.select_key_blocks_paged; multiples of ``bounds_block``)."""
         if keep and self.k_min is None:
             raise ValueError("decode(keep=) needs a cache with bounds_block")
+        if keep:
+            _check_selection(keep, recent or self.bounds_block, self.bounds_block)
+        if k_new.shape[0] != len(self._host_len):
+            raise ValueError(f"PagedKVCache: decode takes a token for each of the {len(self._host_len)} sequences; got {k_new.shape[0]}")
         self.append(k_new, v_new)
         table = self.block_table[:, :self._span_pages()]
         if self.k_scale is not None:
@@ -352,8 +373,8 @@ class PagedKVCache:
     def fork(self, parents) -> None:
         """Sequence b continues what sequence parents[b] is, on the same pages (F.kv_pages_fork); a parent outside the batch, such
         as -1, frees the sequence.  parents: B whole numbers on the host, or an int32 tensor [B] on the device.  The latter does not
-        wait for the device (and may be captured): the host's lengths are then behind until sync_lengths(), and with share() in use
-        each parent must belong to its child's group.  A cache that runs out of pages meanwhile drops tokens, which
+        wait for the device (and may be captured): the host's lengths are then behind until sync_lengths(), and a group that has a
+        parent from another one, or a sequence without parent, shares nothing until the next share().  A cache that runs out of pages meanwhile drops tokens, which
         sync_lengths() reports."""
         batch = len(self._host_len)
         on_device = isinstance(parents, torch.Tensor) and parents.is_cuda
@@ -361,6 +382,8 @@ class PagedKVCache:
             parents = np.asarray(parents, dtype=np.int64).reshape(-1)
         if len(parents) != batch:
             raise ValueError(f"fork takes a parent for each of the {batch} sequences; got {len(parents)}")
+        if not on_device and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKVCache: a captured fork takes its parents on the device")
         if not on_device and self._host_stale:
             parents = torch.from_numpy(parents.clip(-1, batch).astype(np.int32)).to(self.lengths.device)
             on_device = True
@@ -368,6 +391,11 @@ class PagedKVCache:
         if on_device:
             F.kv_pages_fork(self.block_table, self.lengths, self.page_refs, parents)
             self._host_stale = True
+            for groups, shared in self._shares.items():  # a group with a parent from elsewhere, or none, has nothing in common
+                per = batch // groups
+                home = torch.arange(batch, dtype=torch.int64, device=parents.device) // per
+                stays = torch.where(parents.div(per, rounding_mode="floor") == home, 0x7fffffff, 0).to(torch.int32)
+                shared.scatter_reduce_(0, home, stays, "amin")
             return
         lives = (parents >= 0) & (parents < batch)
         source = np.where(lives, parents, 0)
@@ -377,34 +405,47 @@ class PagedKVCache:
         self._pages = np.where(lives, self._pages[source], 0)
         self._host_len = np.where(lives, self._host_len[source], 0)
         self._set_free()
-        if self.prefix_lengths is not None:
-            self.share(len(self.prefix_lengths))
+        for groups in self._shares:
+            self._set_shared(groups)
 
     def free(self, sequences) -> None:
         """Free sequences (their indices): length 0, and pages that no other one names are free again."""
         parents = np.arange(len(self._host_len))
-        parents[np.asarray(sequences, dtype=np.int64)] = -1
+        sequences = np.asarray(sequences, dtype=np.int64).reshape(-1)
+        if np.any((sequences < 0) | (sequences >= len(parents))):
+            raise ValueError(f"free takes sequences from 0 to {len(parents) - 1}; got {sequences.tolist()}")
+        parents[sequences] = -1
         self.fork(parents)
 
     def share(self, groups: int) -> None:
         """Read the pages that the sequences of a group have in common once per step: ``groups`` equal groups of consecutive
-        sequences (0: no longer).  Takes effect for the pages they share now, and stays right as sequences grow."""
+        sequences (0: no longer).  Takes effect for the pages they share now, and stays right as sequences grow; a group with
+        an empty sequence shares nothing."""
         if groups == 0:
             self.prefix_lengths = None
             return
         if groups < 0 or len(self._host_len) % groups:
             raise ValueError(f"{len(self._host_len)} sequences are not {groups} equal groups")
-        if self.k_scale is not None or self.k.shape[3] > 128:
-            raise ValueError("share takes a bf16, fp16 or fp32 cache with a head_dim up to 128")
+        if groups > 1024:
+            raise ValueError(f"share takes up to 1024 groups; got {groups}")
+        if self.k_scale is not None or self.k.shape[3] > 128 or self.k.shape[3] * self.k.element_size() % 16:
+            raise ValueError("share takes a bf16, fp16 or fp32 cache with a head_dim up to 128 whose rows are multiples of 16 bytes")
         if self._host_stale:
             raise RuntimeError("PagedKVCache: call sync_lengths() before share()")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PagedKVCache: share() cannot be captured")
+        if groups not in self._shares:
+            self._shares[groups] = torch.zeros(groups, dtype=torch.int32, device=self.lengths.device)
+        self._set_shared(groups)
+        self.prefix_lengths = self._shares[groups]
+
+    def _set_shared(self, groups: int) -> None:
         common = []
         for table, lengths in zip(np.split(self._table, groups), np.split(self._host_len, groups)):
-            table, lengths = table[lengths > 0], lengths[lengths > 0]
-            whole = int(lengths.min(initial=self._table.shape[1] * self.page_size)) // self.page_size if len(lengths) else 0
+            whole = int(lengths.min()) // self.page_size
             same = (table[:, :whole] == table[:1, :whole]).all(0)
             common.append((int(same.argmin()) if not same.all() else whole) * self.page_size)
-        self.prefix_lengths = torch.tensor(common, dtype=torch.int32, device=self.lengths.device)
+        self._shares[groups].copy_(torch.tensor(common, dtype=torch.int32))
 
     def compact(self) -> torch.Tensor:
         """Move the pages in use to the front of the pools (F.kv_pages_compact).  Returns their number, int32 [1] on the device."""

@@ -258,3 +258,122 @@ def test_class_refusals():
             _paged(**kw)
     with pytest.raises(ValueError):
         KVCache(B, HKV, 64, 256, bounds_block=16)
+
+
+def _same_as_lone(cache, history, step):
+    from dtorch_amd.nn import functional as F
+    out = cache.decode(*step)
+    for b in range(B):
+        history[b].append((step[1][b].clone(), step[2][b].clone()))
+    lone = _lone(cache, history)
+    _near(out, F.decode_attention_paged(step[0], lone.k, lone.v, lone.block_table, lone.lengths)[0])
+
+
+@pytest.mark.parametrize("device", [False, True])
+def test_share_with_a_freed_sequence(device):
+    """A freed sequence grows again, on pages of its own, past what its group shared."""
+    g = _gen(9)
+    cache = _paged()
+    q, k, v = _qkv(2, 50, g)
+    cache.prefill(q, k, v)
+    cache.fork([0, 0, 0, 1, 1, 1])
+    cache.share(2)
+    held = cache.prefix_lengths
+    history = [[(k[i // 3], v[i // 3])] for i in range(B)]
+    parents = [0, -1, 2, 4, 4, 4]
+    cache.fork(torch.tensor(parents, dtype=torch.int32, device="cuda") if device else parents)
+    assert held.tolist() == [0, 48]
+    history = [list(history[p]) if p >= 0 else [] for p in parents]
+    for i in range(60):
+        step = _qkv(B, 1, g)
+        if i % 7 == 3 or i > 45:
+            _same_as_lone(cache, history, step)
+        else:
+            cache.decode(*step)
+            for b in range(B):
+                history[b].append((step[1][b], step[2][b]))
+    cache.sync_lengths()
+    cache.share(2)
+    assert cache.prefix_lengths is held and held.tolist() == [0, 48]
+
+
+def test_share_across_groups():
+    """Parents on the device from another group: the groups that take them share nothing, the others as before."""
+    g = _gen(10)
+    cache = _paged()
+    q, k, v = _qkv(2, 50, g)
+    cache.prefill(q, k, v)
+    cache.fork([0, 0, 0, 1, 1, 1])
+    cache.share(2)
+    parents = [0, 5, 2, 3, 3, 4]
+    cache.fork(torch.tensor(parents, dtype=torch.int32, device="cuda"))
+    assert cache.prefix_lengths.tolist() == [0, 48]
+    _same_as_lone(cache, [[(k[p // 3], v[p // 3])] for p in parents], _qkv(B, 1, g))
+
+
+def test_captured_step_outlives_share():
+    """A step captured under share(2) replays rightly after eager forks and another share."""
+    g = _gen(11)
+    cache = _paged()
+    q, k, v = _qkv(2, 40, g)
+    cache.prefill(q, k, v)
+    cache.fork([0, 0, 0, 1, 1, 1])
+    cache.share(2)
+    history = [[(k[i // 3], v[i // 3])] for i in range(B)]
+    step = _qkv(B, 1, g)
+    _same_as_lone(cache, history, step)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.decode(*step)
+    from dtorch_amd.nn import functional as F
+    for i in range(6):
+        for x in step:
+            x.normal_()
+        graph.replay()
+        for b in range(B):
+            history[b].append((step[1][b].clone(), step[2][b].clone()))
+        lone = _lone(cache, history)
+        _near(out, F.decode_attention_paged(step[0], lone.k, lone.v, lone.block_table, lone.lengths)[0])
+        cache.sync_lengths()
+        parents = [3, 3, 3, 0, 0, 1] if i % 2 else [2, 1, 0, 5, 0, 4]
+        cache.fork(parents)
+        history = [list(history[p]) for p in parents]
+        cache.share(3 if i % 2 else 1)
+
+
+def test_refusals_leave_the_cache_alone():
+    """What decode refuses it refuses before the append."""
+    from dtorch_amd.nn.kv_cache import KVCache
+    g = _gen(12)
+    paged, padded = _paged(bounds_block=16), KVCache(B, HKV, 64, D, bounds_block=16)
+    for c in (paged, padded):
+        c.prefill(*_qkv(B, 20, g))
+        for kw in (dict(keep=24), dict(keep=16, recent=32), dict(keep=32, recent=8), dict(keep=-16), dict(keep=32, recent=-16)):
+            with pytest.raises(ValueError):
+                c.decode(*_qkv(B, 1, g), **kw)
+    for other in (KVCache(4, HKV, 64, D), KVCache(2, 2 * HKV, 64, D), KVCache(2, HKV, 64, 32), KVCache(2, HKV, 64, D, dtype=torch.float16),
+                  KVCache(2, HKV, 64, D, device="cpu")):
+        with pytest.raises(ValueError):
+            padded.decode(*_qkv(B, 1, g), prefix=other)
+    with pytest.raises(ValueError):
+        paged.decode(*_qkv(2, 1, g))
+    for bad in ([B], [-1], [0, 99]):
+        with pytest.raises(ValueError):
+            paged.free(bad)
+    for c in (paged, padded):
+        assert c._host_len.tolist() == c.lengths.tolist() == [20] * B
+
+
+def test_capture_refusals():
+    g = _gen(13)
+    cache = _paged()
+    cache.prefill(*_qkv(B, 20, g))
+    parents = torch.arange(B, dtype=torch.int32, device="cuda")
+    x = torch.zeros(1, device="cuda")
+    for attempt in (lambda: cache.fork(list(range(B))), lambda: cache.fork(parents), lambda: cache.compact(), lambda: cache.share(2)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            x.add_(1)
+            with pytest.raises(RuntimeError):
+                attempt()
+    assert cache.page_refs is None and not cache._host_stale
