@@ -146,6 +146,15 @@ def test_shared(dtype, B, G, Hq, Hkv, D, page, prefixes, owns):
     _shared(B + D, B, G, Hq, Hkv, D, dtype, page, prefixes, owns)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page,D", [(16, 128), (0, 64), (64, 96)])
+@pytest.mark.parametrize("rows", [16, 17, 32, 33, 64, 65, 128, 129, 193])
+def test_shared_row_counts(rows, page, D, dtype):
+    """Rows of a group that meet the prefix together, on either side of where its form changes."""
+    whole = max(page, 1)
+    _shared(rows, rows, 1, 2, 2, D, dtype, page, [300 // whole * whole], [1 + b * 7 % 50 for b in range(rows)])
+
+
 @pytest.mark.parametrize("page", [0, 16, 64])
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
 def test_shared_scales(page, scale):
@@ -459,3 +468,33 @@ def test_host_refusals():
         F.decode_attention_blocks_paged(q, pool, pool, t, l, ids, 32)
     e = F.decode_attention_shared(q[:0], kp, kp, pl, k[:0], k[:0], l[:0])
     assert e[0].shape == (0, 4, 1, 64)
+
+
+def test_offsets_past_32_bits():
+    """Pages past 2^31 elements of a pool (and past 2^32 bytes): the same outputs as from a small pool, bit by bit."""
+    F = _F()
+    P, H, page, D, B = 140000, 8, 16, 128, 3
+    if torch.cuda.mem_get_info()[0] < 16 * 2 ** 30:
+        pytest.skip("needs 16 GiB of device memory")
+    rng = np.random.default_rng(21)
+    ids = np.array([P - 1, 5, P - 2, 131073, 90000, P - 7, 65537, 1])
+    small = [_tensors(rng, (8, H, page, D), torch.bfloat16) for _ in range(2)]
+    k, v = (torch.empty(P, H, page, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    at = torch.from_numpy(ids).cuda()
+    k[at], v[at] = small
+    table = np.array([[0, 1, 2, 3], [0, 1, 4, 5], [0, 1, 6, 7]])
+    q, lengths, prefix = _tensors(rng, (B, 32, 1, D), torch.bfloat16), _i32([64, 50, 33]), _i32([32])
+    bounds = [[torch.empty(x.shape[0], H, 1, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)] for x in (small[0], k)]
+    outs = []
+    for (kk, vv), (lo, hi), t in ((small, bounds[0], table), ((k, v), bounds[1], ids[table])):
+        t = _i32(t)
+        F.kv_key_bounds_paged(kk, lo, hi, t, lengths, 64)
+        kept = F.select_key_blocks_paged(q, lo, hi, t, lengths, 32, 16, 16)
+        outs.append([kept, *F.decode_attention_shared_paged(q, kk, vv, t, lengths, prefix), *F.decode_attention_blocks_paged(q, kk, vv, t, lengths, kept, 16)])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    # and the pages move
+    refs, t = torch.zeros(P, dtype=torch.int32, device="cuda"), _i32(ids[table])
+    refs[at] = _i32([3, 3, 1, 1, 1, 1, 1, 1])
+    assert F.kv_pages_compact([k, v], t, refs).item() == 8 and t.max().item() == 7
+    again = F.decode_attention_shared_paged(q, k, v, t, lengths, prefix)
+    assert all(torch.equal(a, b) for a, b in zip(outs[0][1:3], again))

@@ -232,3 +232,19 @@ def test_host_refusals():
     with pytest.raises(ValueError):
         F.kv_pages_reserve([k], t, l, r, -1)
     assert t.tolist() == [[0, 1]] and r.tolist() == [1, 1, 0]
+
+
+@pytest.mark.parametrize("P", [1023, 1024, 1025, 4096, 4097, 8192, 8193, 16384, 16385, 40001])
+def test_compact_page_counts(P):
+    """Page counts on either side of where the plan changes; counts at an odd address; every page alike, so the table tells them apart."""
+    rng = np.random.default_rng(P)
+    table, lengths, refs = _state(rng, 16, 16, min(P // 24, 300), P)
+    pool = torch.arange(P, dtype=torch.int32)[:, None, None, None].repeat(1, 1, 16, 1)
+    want_p, want_t, want_r, used = orc.compact([_num(pool)], table, refs)
+    held = torch.full((P + 1,), 7, dtype=torch.int32, device="cuda")
+    dp, dt, dr = pool.cuda(), _i32(table), held[1:]
+    dr.copy_(_i32(refs))
+    assert _F().kv_pages_compact([dp], dt, dr).item() == used
+    assert np.array_equal(dt.cpu().numpy(), want_t) and np.array_equal(dr.cpu().numpy(), want_r)
+    live = want_r > 0
+    assert np.array_equal(_num(dp)[live], want_p[0][live]) and held[0].item() == 7
