@@ -40,7 +40,7 @@ struct PartsParams {
     float* rec_lse[2];
     float* whole_o[2];  // [B, Hq, kernel D]: segments inside one share
     float* whole_lse[2];
-    int32_t* meta[2];   // places of all, and shares at most; then of each group or sequence: places before it, and its units
+    int32_t* meta[2];   // places of a column set, and the shares; then of each group or sequence: places before it, and its units
     int32_t nsub[2], columns[2];  // column sets of a kv head; columns of a set
     int32_t shares;     // of both parts, or of the listed blocks, at most
     int32_t weight[2];  // what a unit of each part costs
@@ -68,15 +68,17 @@ constexpr int kPartExtra = 4;
 // V places in `n` shares of V / n or one more (all the longer ones first); the host keeps V below 2^31.
 struct PartShares {
     int n, q, rem;
+    __device__ __forceinline__ PartShares(int n_, int q_, int rem_) : n(n_), q(q_), rem(rem_) {}
     __device__ __forceinline__ PartShares(int V, int most) {
-        n = min(most, max(1, V / kPartLeast));
+        n = max(1, min(most, V / kPartLeast));
         q = V / n;
         rem = V - q * n;
     }
     __device__ __forceinline__ int start(int r) const { return r * q + min(r, rem); }
     __device__ __forceinline__ int of(int x) const {  // the share of place x
         const int big = rem * (q + 1);
-        return x < big ? x / (q + 1) : rem + (x - big) / q;
+        const bool longer = x < big;
+        return (longer ? 0 : rem) + (longer ? x : x - big) / (longer ? q + 1 : q);
     }
 };
 
@@ -181,8 +183,8 @@ __device__ __forceinline__ int part_total(const PartsParams& p, const PartLength
         const PartScan s = part_scan<KIND>(p, at, j0);
         if (j0 == 0) first = s;
         if (tells && j0 + lane < Z) {
-            meta[2 + 2 * (j0 + lane)] = U + s.places - part_places(s.units);
-            meta[3 + 2 * (j0 + lane)] = s.units;
+            meta[4 + 2 * (j0 + lane)] = U + s.places - part_places(s.units);
+            meta[5 + 2 * (j0 + lane)] = s.units;
         }
         U += __builtin_amdgcn_readlane(s.places, 63);
     }
@@ -801,9 +803,9 @@ __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsPara
     constexpr int DL = D / 64;  // dims per lane
     __shared__ float red[W > 1 ? W : 1][D + 2];
     const int lane = threadIdx.x & 63, wave = W > 1 ? threadIdx.x >> 6 : 0;
-    const int64_t pair = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (pair >= (int64_t)p.B * p.Hq) return;
-    const int b = (int)(pair / p.Hq), hq = (int)(pair % p.Hq), hk = hq / p.group, g = hq - hk * p.group;
+    const int pair = __builtin_amdgcn_readfirstlane(W > 1 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (pair >= p.B * p.Hq) return;
+    const int b = pair / p.Hq, hq = pair - b * p.Hq, hk = hq / p.group, g = hq - hk * p.group;
     struct Part {
         int n;                // records
         int64_t first, later; // that of the part's first share, and of the one behind it
@@ -812,11 +814,12 @@ __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsPara
     };
     auto part = [&](int S, int z, int row) {
         Part r = {0, 0, 0, nullptr, nullptr};
-        const int U = SHARED ? p.meta[S][0] : p.B * part_places(p.list_units), most = SHARED ? p.meta[S][1] : p.shares;
-        const int before = SHARED ? p.meta[S][2 + 2 * z] : b * part_places(p.list_units), own = SHARED ? p.meta[S][3 + 2 * z] : p.list_units;
+        const int* meta = p.meta[S];
+        const int U = SHARED ? meta[0] : p.B * part_places(p.list_units);
+        const int before = SHARED ? meta[4 + 2 * z] : b * part_places(p.list_units), own = SHARED ? meta[5 + 2 * z] : p.list_units;
         if (own == 0) return r;
         const int cols = p.columns[S], sub = row / cols;
-        const PartShares sh(U * p.Hkv * p.nsub[S], most);
+        const PartShares sh = SHARED ? PartShares(meta[1], meta[2], meta[3]) : PartShares(U * p.Hkv * p.nsub[S], p.shares);
         const int x0 = (hk * p.nsub[S] + sub) * U + before + kPartExtra, r0 = sh.of(x0), r1 = sh.of(x0 + own - 1);
         const bool whole = r0 == r1;
         r.n = r1 - r0 + 1;

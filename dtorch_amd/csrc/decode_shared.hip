@@ -5,7 +5,7 @@
 // read once per so many query rows instead of once per sequence; a long prefix of many sequences is bound by the matrix cores and the
 // instructions around them, the sequences' own tokens by HBM.  Both write records, which one more launch merges by LSE.
 // 64 sequences of 32 heads and 8 kv heads, 16 to 1500 own tokens each behind 8192 shared ones, bf16, head dim 128 (233 MB of keys and
-// values): 64 us, 3.6 TB/s.  4 samples of one prompt of 2000 tokens: 17 us, of which 11 are the first launch and 8000 cycles of those the
+// values): 62 us, 3.8 TB/s.  4 samples of one prompt of 2000 tokens: 17 us, of which 11 are the first launch and 8000 cycles of those the
 // lengths, the shares and the first loads.
 #include <algorithm>
 
@@ -43,8 +43,9 @@ __global__ void __launch_bounds__(64 * kPartWaves, 2) decode_shared_kernel(const
     const int V0 = U0 * p.Hkv * p.nsub[0], V1 = U1 * p.Hkv * p.nsub[1];
     const int most0 = prefix_shares((float)V0 * (float)p.weight[0], (float)V1 * (float)p.weight[1], p.shares), most1 = p.shares - most0;
     if (tells && threadIdx.x == 0) {
-        p.meta[0][0] = U0, p.meta[0][1] = most0;
-        p.meta[1][0] = U1, p.meta[1][1] = most1;
+        const PartShares s0(V0, most0), s1(V1, most1);
+        p.meta[0][0] = U0, p.meta[0][1] = s0.n, p.meta[0][2] = s0.q, p.meta[0][3] = s0.rem;
+        p.meta[1][0] = U1, p.meta[1][1] = s1.n, p.meta[1][2] = s1.q, p.meta[1][3] = s1.rem;
     }
     const int x = blockIdx.x & 7, y = blockIdx.x >> 3;
     const bool first = y < most0 / 8;
@@ -89,7 +90,7 @@ SharedPlan plan_shared(const dtattn_decode_shared_args* a, int cus) {
     for (int s = 0; s < 2; ++s) {
         r.nsub[s] = (int32_t)((cols[s] + r.columns[s] - 1) / r.columns[s]);
         const size_t records = (size_t)2 * r.shares * r.columns[s];
-        r.meta[s] = part_up((2 + 2 * (size_t)sets[s]) * sizeof(int32_t));
+        r.meta[s] = part_up((4 + 2 * (size_t)sets[s]) * sizeof(int32_t));
         r.rec_o[s] = part_up(records * r.kernel_d * sizeof(float));
         r.rec_lse[s] = part_up(records * sizeof(float));
     }
@@ -120,7 +121,7 @@ int launch_shared(const PartsParams& p, int nc, hipStream_t stream) {
     if (st != DTATTN_OK) return st;
     const int64_t pairs = (int64_t)p.B * p.Hq;
     // Few pairs are cut into many records each: four waves to a pair.  Up to `most` records of the prefix; us of a call with four waves and
-    // with one: 384 pairs of 10 records 32.6 and 35.8, 2048 of 9 71.9 and 70.0.
+    // with one: 256 pairs 26.2 and 29.4, 512 29.4 and 31.9, 1024 40.9 and 40.6, 2048 67.2 and 62.1.
     const int64_t most = p.shares / ((int64_t)p.Hkv * p.nsub[0] * p.groups);
     if (pairs <= 256 || (pairs <= 1024 && most > 8)) hipLaunchKernelGGL((decode_parts_merge_kernel<T, D, 4, true>), dim3((unsigned)pairs), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((decode_parts_merge_kernel<T, D, 1, true>), dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, stream, p);
