@@ -13,7 +13,7 @@ namespace core {
 struct KvPagesForkParam : KvCacheAppendParam {};
 struct KvPagesCompactParam : KvCacheAppendParam {};
 
-// KvPagesReserve, KeyBounds and KeyBoundsPaged: how many tokens.
+// KvPagesReserve and KeyBounds: how many tokens.
 struct TokenCountParam {
     int64_t tokens = 1;
 
