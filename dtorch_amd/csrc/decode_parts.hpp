@@ -227,9 +227,18 @@ struct PartWalk {
         a.units = KIND == kListPart ? p.list_units : (max(a.end - a.start, 0) + kPartUnit - 1) / kPartUnit;
         a.row = KIND == kPrefixPart && paged && a.units > 0 ? __builtin_amdgcn_readfirstlane(lens.lead[a.z]) : a.z;
     }
-    __device__ __forceinline__ void next(At& a) const {  // the next segment with units; there is one
+    // The next segment with units.  There is one, unless somebody changes the lengths meanwhile, which must cost no more than the results:
+    // behind the last segment lie units without tokens.
+    __device__ __forceinline__ void next(At& a) const {
         do {
-            if (++a.z == Z) a.z = 0, ++a.slot;
+            if (++a.z == Z) {
+                a.z = 0;
+                if (++a.slot == p.Hkv * p.nsub[S]) {
+                    --a.slot;
+                    a.start = a.end = 0, a.units = 1 << 30;
+                    return;
+                }
+            }
             enter(a);
         } while (a.units == 0);
     }
@@ -279,6 +288,7 @@ struct PartWalk {
         } else {
             int total = 0, left = 0;  // units of all groups or sequences, and of those before z
             bool found = false;
+            a.z = Z - 1;
             for (int j0 = 0; j0 < Z; j0 += 64) {
                 const PartScan s = j0 == 0 ? scan0 : part_scan<KIND>(p, lens, j0);
                 const uint64_t hit = __ballot(s.places > x);  // segments ending past x
@@ -473,7 +483,7 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
     load_q(cur);
     int s = wave;  // this wave's next unit of the share
     for (int u = 0; u < n;) {
-        const int m = min(cur.units - cur.u, n - u);  // units of the segment
+        const int m = max(min(cur.units - cur.u, n - u), 1);  // units of the segment
         const int hk = cur.hk, z = cur.z, R0 = 16 * (cur.slot - hk * p.nsub[S]);
         const bool whole = cur.u == 0 && m == cur.units;
         bool seen = false;
@@ -655,7 +665,7 @@ __device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, 
     // the stage to be loaded next: its units lie in one segment
     At nx = cur;
     int nx_left = n;                                   // units of the share from it on
-    int nx_here = min(cur.units - cur.u, nx_left);     // of its segment
+    int nx_here = max(min(cur.units - cur.u, nx_left), 1);  // of its segment
     // 64 page ids from page `ids_from` of row `ids_row` on, one a lane: a scalar load a stage would be waited for before its first key
     int ids = 0, ids_from = 0, ids_row = -1;
     auto issue = [&](int buf) {
@@ -706,7 +716,7 @@ __device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, 
     float M[NC], l[NC];
     int buf = 0;
     for (int u = 0; u < n;) {
-        const int m = min(cur.units - cur.u, n - u);
+        const int m = max(min(cur.units - cur.u, n - u), 1);
         const bool whole = cur.u == 0 && m == cur.units, cut_first = u == 0;
         const At seg = cur;
 #pragma unroll
