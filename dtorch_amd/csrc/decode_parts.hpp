@@ -217,8 +217,12 @@ struct PartWalk {
         return KIND == kOwnPart && paged ? __builtin_amdgcn_readfirstlane(lens.shared(p, part_group(p, z))) : 0;
     }
     __device__ __forceinline__ int end_of(int z) const {
-        if constexpr (KIND == kPrefixPart) return paged ? __builtin_amdgcn_readfirstlane(lens.shared(p, z)) : part_clamp(((cint32*)p.prefix)[z], p.capacity[0]);
-        else return part_clamp(((cint32*)p.lengths)[z], p.capacity[1]);
+        if constexpr (KIND == kPrefixPart) {
+            if (paged) return __builtin_amdgcn_readfirstlane(lens.shared(p, z));
+            return z < 64 ? __builtin_amdgcn_readlane(lens.pre0, z) : part_clamp(((cint32*)p.prefix)[z], p.capacity[0]);
+        } else {
+            return KIND == kOwnPart && z < 64 ? __builtin_amdgcn_readlane(lens.own0, z) : part_clamp(((cint32*)p.lengths)[z], p.capacity[1]);
+        }
     }
     __device__ __forceinline__ void enter(At& a) const {
         a.hk = p.nsub[S] == 1 ? a.slot : a.slot / p.nsub[S];
