@@ -59,7 +59,9 @@ namespace {
 
 constexpr int kPartUnit = 32;  // tokens
 constexpr int kPartWaves = 4;
-constexpr int kPartLeast = kPartWaves + 1;  // places of a share, at least
+// Places of a share, at least: a unit for each wave.  us with 4, with 5 (a second turn for one wave) and with 2: 4 samples of one prompt 16.1,
+// 16.7 and 17.9, 2048 listed tokens of one sequence (scores and choice included) 21.6, 22.9 and 22.0.
+constexpr int kPartLeast = kPartWaves;
 constexpr int kPartGroups = 1024;
 // What a segment costs besides its units, in units: its waves meet, and the last of them take turns that others have no unit for.  64
 // sequences of one or two tokens behind 8192 take 62.5 us with 0 and 48.7 with 4.
