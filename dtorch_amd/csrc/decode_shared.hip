@@ -5,7 +5,7 @@
 // read once per so many query rows instead of once per sequence; a long prefix of many sequences is bound by the matrix cores and the
 // instructions around them, the sequences' own tokens by HBM.  Both write records, which one more launch merges by LSE.
 // 64 sequences of 32 heads and 8 kv heads, 16 to 1500 own tokens each behind 8192 shared ones, bf16, head dim 128 (233 MB of keys and
-// values): 62 us, 3.8 TB/s.  4 samples of one prompt of 2000 tokens: 17 us, of which 11 are the first launch and 8000 cycles of those the
+// values): 60 us, 3.9 TB/s.  4 samples of one prompt of 2000 tokens: 16 us, of which 11 are the first launch and 8000 cycles of those the
 // lengths, the shares and the first loads.
 #include <algorithm>
 
@@ -16,12 +16,13 @@ namespace dtattn {
 namespace {
 
 // Workgroups of the prefix, in eighths of all: as its units' cost is to that of all, with one of either kind at least where there is
-// any work for it.
+// any work for it.  Rounded up, for a short part on too few workgroups is what all wait for: 96 sequences of up to 560 tokens of 20 heads
+// behind 7 to 30 shared ones take 43 us, and 69 rounded to nearest; 64 behind 8192 60 and 62.
 __device__ __forceinline__ int prefix_shares(float cost0, float cost1, int most) {
     const int eighth = most / 8;
     if (cost0 == 0.f) return 0;
     if (cost1 == 0.f) return most;
-    return 8 * min(max((int)(cost0 / (cost0 + cost1) * (float)eighth + 0.5f), 1), eighth - 1);
+    return 8 * min(max((int)(cost0 / (cost0 + cost1) * (float)eighth) + 1, 1), eighth - 1);
 }
 
 }  // namespace
