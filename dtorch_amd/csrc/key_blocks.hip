@@ -5,8 +5,8 @@
 // The bound: a token's key lies between k_min and k_max in every dimension, so q . k <= sum_d q_d x_d with x_d = k_max_d where
 // q_d > 0 and k_min_d elsewhere.  Reading 2 D values per block instead of D per token, it says which blocks can hold large scores.
 //
-// key_bounds_kernel: a workgroup per (block, sequence and kv head); every 16-byte chunk of a row belongs to one column of threads,
-// which meet by lane exchanges and then in LDS.  Bound by HBM: the rows are read once (4 x 4000 tokens of 8 heads of 128 dims, 34 MB, 8.2
+// key_bounds_kernel: a wave or a workgroup per (block, sequence and kv head); every 16-byte chunk of a row belongs to one column of
+// threads, which meet by lane exchanges and, of several waves, in LDS.  Bound by HBM: the rows are read once (4 x 4000 tokens of 8 heads of 128 dims, 34 MB, 8.0
 // us, 4.1 TB/s; the last block of 64 sequences' steps 5.0, a launch).
 // score_blocks_kernel: four lanes to a block, with the query's heads in LDS as 64-bit numbers.  Sums in 64 bits are exact for 16-bit types (products have at
 // most 22 bits), so scores next to one another are told apart alike in any order of summation, and the vector units' 64-bit rate
@@ -54,17 +54,17 @@ __device__ __forceinline__ int tokens_in(const BlockCache& c, int64_t b) { retur
 
 }  // namespace
 
-// W: chunks of a row's columns of threads, a power of two.
-template <typename T, int W>
+// W: chunks of a row's columns of threads, a power of two.  WAVES: of a block; with one, a workgroup has four blocks.
+template <typename T, int W, int WAVES>
 __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
-    constexpr int E = 16 / (int)sizeof(T), ROWS = 256 / W;
+    constexpr int E = 16 / (int)sizeof(T), ROWS = 64 * WAVES / W;
     __shared__ float red[4][2][W * E];
-    const int tid = threadIdx.x, col = tid % W, row = tid / W;
+    const int tid = threadIdx.x % (64 * WAVES), col = tid % W, row = tid / W;
     const int64_t bh = blockIdx.x, b = bh / p.Hkv;
     const int h = (int)(bh % p.Hkv);
     const int n = tokens_in(p.c, b);
     const int block = 1 << p.c.block_shift;
-    const int64_t j = (max(n - p.n_new, 0) >> p.c.block_shift) + (int64_t)blockIdx.y;  // this workgroup's block
+    const int64_t j = (max(n - p.n_new, 0) >> p.c.block_shift) + (int64_t)blockIdx.y * (4 / WAVES) + threadIdx.x / (64 * WAVES);
     const int64_t t0 = j << p.c.block_shift;
     if (t0 >= n) return;
     const int rows = (int)min((int64_t)block, n - t0);
@@ -105,14 +105,24 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
         if (W <= 16) lo[e] = -max_xor16(-lo[e]), hi[e] = max_xor16(hi[e]);
         lo[e] = -max_xor32(-lo[e]), hi[e] = max_xor32(hi[e]);
     }
+    const int64_t jb = r0 >> p.c.block_shift;
+    T* out_lo = reinterpret_cast<T*>(p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s);
+    T* out_hi = reinterpret_cast<T*>(p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s);
+    if constexpr (WAVES == 1) {
+        if (tid < p.chunks) {
+            __attribute__((aligned(16))) T x[2][E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[0][e] = Elem<T>::from_f32(lo[e]), x[1][e] = Elem<T>::from_f32(hi[e]);
+            *reinterpret_cast<u32x4*>(out_lo + col * E) = *reinterpret_cast<const u32x4*>(x[0]);
+            *reinterpret_cast<u32x4*>(out_hi + col * E) = *reinterpret_cast<const u32x4*>(x[1]);
+        }
+        return;
+    }
     if ((tid & 63) < W) {
 #pragma unroll
         for (int e = 0; e < E; ++e) red[tid >> 6][0][col * E + e] = lo[e], red[tid >> 6][1][col * E + e] = hi[e];
     }
     __syncthreads();
-    const int64_t jb = r0 >> p.c.block_shift;
-    T* out_lo = reinterpret_cast<T*>(p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s);
-    T* out_hi = reinterpret_cast<T*>(p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s);
     for (int i = tid; i < p.chunks * E; i += 256) {
         out_lo[i] = Elem<T>::from_f32(fminf(fminf(red[0][0][i], red[1][0][i]), fminf(red[2][0][i], red[3][0][i])));
         out_hi[i] = Elem<T>::from_f32(fmaxf(fmaxf(red[0][1][i], red[1][1][i]), fmaxf(red[2][1][i], red[3][1][i])));
@@ -308,11 +318,18 @@ int row_checks(int64_t D, int32_t dtype, const int64_t* strides, int n, uintptr_
     return DTATTN_OK;
 }
 
+template <typename T, int WAVES>
+void launch_bounds_waves(const BoundsParams& p, dim3 grid, hipStream_t stream) {
+    if (p.chunks <= 8) hipLaunchKernelGGL((key_bounds_kernel<T, 8, WAVES>), grid, dim3(256), 0, stream, p);
+    else if (p.chunks <= 16) hipLaunchKernelGGL((key_bounds_kernel<T, 16, WAVES>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((key_bounds_kernel<T, 32, WAVES>), grid, dim3(256), 0, stream, p);
+}
 template <typename T>
-void launch_bounds_of(const BoundsParams& p, dim3 grid, hipStream_t stream) {
-    if (p.chunks <= 8) hipLaunchKernelGGL((key_bounds_kernel<T, 8>), grid, dim3(256), 0, stream, p);
-    else if (p.chunks <= 16) hipLaunchKernelGGL((key_bounds_kernel<T, 16>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((key_bounds_kernel<T, 32>), grid, dim3(256), 0, stream, p);
+void launch_bounds_of(const BoundsParams& p, unsigned heads, unsigned blocks, hipStream_t stream) {
+    // A wave to a block of up to 64 tokens, whose waves would have a load each before they meet.  us with one wave and with four, 4 x 4000
+    // tokens: blocks of 16 8.9 and 21.2, of 32 8.3 and 12.1, of 64 8.0 and 8.6, of 256 10.7 and 8.1.
+    if (p.c.block_shift <= 6) launch_bounds_waves<T, 1>(p, dim3(heads, (blocks + 3) / 4), stream);
+    else launch_bounds_waves<T, 4>(p, dim3(heads, blocks), stream);
 }
 
 template <typename T, int D, int HB>
@@ -376,12 +393,11 @@ extern "C" int dtattn_key_bounds(const dtattn_key_bounds_args* a, void* stream_)
     p.n_new = (int32_t)n;
     const int64_t blocks = (n + a->block - 2) / a->block + 1, heads = a->B * a->Hkv;  // that n tokens touch, at most
     if (heads > 0x7fffffff || blocks > 65535) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
-    const dim3 grid((unsigned)heads, (unsigned)blocks);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     switch (a->dtype) {
-        case DTATTN_BF16: launch_bounds_of<bf16_t>(p, grid, stream); break;
-        case DTATTN_FP16: launch_bounds_of<f16_t>(p, grid, stream); break;
-        default: launch_bounds_of<float>(p, grid, stream);
+        case DTATTN_BF16: launch_bounds_of<bf16_t>(p, (unsigned)heads, (unsigned)blocks, stream); break;
+        case DTATTN_FP16: launch_bounds_of<f16_t>(p, (unsigned)heads, (unsigned)blocks, stream); break;
+        default: launch_bounds_of<float>(p, (unsigned)heads, (unsigned)blocks, stream);
     }
     return check_launch("key_bounds_kernel");
 }
