@@ -8,7 +8,7 @@
 // key_bounds_kernel: a wave or a workgroup per (block, sequence and kv head); every 16-byte chunk of a row belongs to one column of
 // threads, which meet by lane exchanges and, of several waves, in LDS.  Bound by HBM: the rows are read once (4 x 4000 tokens of 8 heads of 128 dims, 34 MB, 8.0
 // us, 4.1 TB/s; the last block of 64 sequences' steps 5.0, a launch).
-// score_blocks_kernel: four lanes to a block, with the query's heads in LDS as 64-bit numbers.  Sums in 64 bits are exact for 16-bit types (products have at
+// score_blocks_kernel: eight lanes to a block, with the query's heads in LDS as 64-bit numbers.  Sums in 64 bits are exact for 16-bit types (products have at
 // most 22 bits), so scores next to one another are told apart alike in any order of summation, and the vector units' 64-bit rate
 // is that of 32 bits.
 // select_blocks_kernel: one workgroup per (sequence, kv head) takes the largest scores by a radix select.
@@ -129,15 +129,18 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
     }
 }
 
-// A workgroup scores blocks 64 W blockIdx.y, ... of one (sequence, kv head), four lanes to W blocks; HB: heads at a time.
+// A workgroup scores kScoreBlocks blocks of one (sequence, kv head) at a time, kScoreLanes lanes to a block; HB: heads at a time.
 // What costs is the vector units: a value's choice by a mask (for 16-bit types two values at once), its conversion and the product, for
-// every head, and the reads of the query from LDS, which two blocks of a quad share.  The 64-bit matrix cores, at the vector units' rate
-// with 16 columns for a group's 4 heads, take 29 us where this takes 18 (32 sequences of 3000 to 32000 tokens in blocks of 64).
+// every head.  The 64-bit matrix cores, at the vector units' rate with 16 columns for a group's 4 heads, take 29 us where this takes 17
+// (32 sequences of 3000 to 32000 tokens in blocks of 64).  us with 4, 8 and 16 lanes (selection and attention included): one sequence
+// of 30000 22.2, 20.9 and 20.6, eight 34.1, 33.0 and 36.0; two blocks to four lanes, which read the query from LDS half as often, 108.4 instead
+// of 107.3 for those 32, and 40.4 instead of 32.0 for 64 sequences of 32 heads of up to 104 tokens.
 constexpr int kScoreHeads = 16;
+constexpr int kScoreLanes = 8, kScoreBlocks = 256 / kScoreLanes;
 
-template <typename T, int D, int HB, int W>
+template <typename T, int D, int HB>
 __global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p) {
-    constexpr int E = 16 / (int)sizeof(T), NI = D / E / 4;  // chunks of a row per lane
+    constexpr int E = 16 / (int)sizeof(T), NI = D / E / kScoreLanes;  // chunks of a row per lane
     __shared__ __attribute__((aligned(16))) double qd[kScoreHeads][D];
     __shared__ __attribute__((aligned(16))) uint32_t qm[kScoreHeads][D * sizeof(T) / 4];  // all ones where q > 0
     const int tid = threadIdx.x;
@@ -145,35 +148,31 @@ __global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p)
     const int h = (int)(bh % p.Hkv);
     const int n = tokens_in(p.c, b);
     const int blocks = (n + (1 << p.c.block_shift) - 1) >> p.c.block_shift;
-    const int cand = blocks - p.recent;
-    if (blocks <= p.keep || (int)blockIdx.y * 64 * W >= cand) return;
+    const int cand = blocks - p.recent, first = blockIdx.y * kScoreBlocks;
+    if (blocks <= p.keep || first >= cand) return;
     uint32_t* order = p.order + bh * p.blocks_max;
-    const int quad = tid >> 2, l = tid & 3;
+    const int mine = tid / kScoreLanes, l = tid % kScoreLanes;
     const int in_page = p.c.page_shift - p.c.block_shift;  // log2 of a page's blocks
-    u32x4 wl[W][NI], wh[W][NI];
+    u32x4 wl[NI], wh[NI];
     auto load = [&](int j0) {
+        const int j = min(j0 + mine, cand - 1);
+        int64_t slot = b, jb = j;
+        if (p.c.table != nullptr) {
+            slot = min(max(p.c.table[b * p.c.bt_s + (j >> in_page)], 0), p.c.num_pages - 1);
+            jb = j & ((1 << in_page) - 1);
+        }
+        const char* lo = p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s;
+        const char* hi = p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const int j = min(j0 + quad + 64 * w, cand - 1);
-            int64_t slot = b, jb = j;
-            if (p.c.table != nullptr) {
-                slot = min(max(p.c.table[b * p.c.bt_s + (j >> in_page)], 0), p.c.num_pages - 1);
-                jb = j & ((1 << in_page) - 1);
-            }
-            const char* lo = p.lo + slot * p.lo_b + h * p.lo_h + jb * p.lo_s;
-            const char* hi = p.hi + slot * p.hi_b + h * p.hi_h + jb * p.hi_s;
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int c = l + 4 * i;
-                const bool there = E * c < p.d;
-                wl[w][i] = ld16_nt(lo + (there ? 16 * c : 0));
-                wh[w][i] = ld16_nt(hi + (there ? 16 * c : 0));
-                if (!there) wl[w][i] = wh[w][i] = u32x4{0u, 0u, 0u, 0u};
-            }
+        for (int i = 0; i < NI; ++i) {
+            const int c = l + kScoreLanes * i;
+            const bool there = E * c < p.d;
+            wl[i] = ld16_nt(lo + (there ? 16 * c : 0));
+            wh[i] = ld16_nt(hi + (there ? 16 * c : 0));
+            if (!there) wl[i] = wh[i] = u32x4{0u, 0u, 0u, 0u};
         }
     };
-    // on their way while the query is laid out; two blocks a quad are more than the waves that hide each other's loads have registers for
-    if constexpr (W == 1) load(blockIdx.y * 64 * W);
+    load(first);  // on their way while the query is laid out
     for (int g0 = 0; g0 < p.group; g0 += kScoreHeads) {
         const int heads = min(p.group - g0, kScoreHeads);
         if (g0 > 0) __syncthreads();  // the last heads have been used
@@ -197,58 +196,43 @@ __global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p)
             *reinterpret_cast<u32x4*>(&qm[g][dim * (int)sizeof(T) / 4]) = mask;
         }
         __syncthreads();
-        for (int j0 = blockIdx.y * 64 * W; j0 < cand; j0 += gridDim.y * 64 * W) {
-            if (W > 1 || g0 > 0 || j0 > (int)blockIdx.y * 64 * W) load(j0);
-            float best[W];
-#pragma unroll
-            for (int w = 0; w < W; ++w) best[w] = kNegInf;
+        for (int j0 = first; j0 < cand; j0 += gridDim.y * kScoreBlocks) {
+            if (g0 > 0 || j0 > first) load(j0);
+            float best = kNegInf;
             for (int hb = 0; hb < heads; hb += HB) {
-                double s[W][HB];
+                double s[HB];
 #pragma unroll
-                for (int w = 0; w < W; ++w)
-#pragma unroll
-                    for (int g = 0; g < HB; ++g) s[w][g] = 0.;
+                for (int g = 0; g < HB; ++g) s[g] = 0.;
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    const int dim = (l + 4 * i) * E;
+                    const int dim = (l + kScoreLanes * i) * E;
 #pragma unroll
                     for (int g = 0; g < HB; ++g) {
                         const u32x4 mask = *reinterpret_cast<const u32x4*>(&qm[hb + g][dim * (int)sizeof(T) / 4]);
-                        double q[E];
+                        const u32x4 x = (wh[i] & mask) | (wl[i] & ~mask);
+                        float f[E];
+                        if constexpr (sizeof(T) == 4) {
+                            const f32x4 v = __builtin_bit_cast(f32x4, x);
 #pragma unroll
-                        for (int e = 0; e < E; ++e) q[e] = qd[hb + g][dim + e];
-#pragma unroll
-                        for (int w = 0; w < W; ++w) {
-                            const u32x4 x = (wh[w][i] & mask) | (wl[w][i] & ~mask);
-                            float f[E];
-                            if constexpr (sizeof(T) == 4) {
-                                const f32x4 v = __builtin_bit_cast(f32x4, x);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) f[e] = v[e];
-                            } else {
-                                unpack8<T>(x, f);
-                            }
-#pragma unroll
-                            for (int e = 0; e < E; ++e) s[w][g] = __builtin_fma(q[e], (double)f[e], s[w][g]);
+                            for (int e = 0; e < 4; ++e) f[e] = v[e];
+                        } else {
+                            unpack8<T>(x, f);
                         }
+#pragma unroll
+                        for (int e = 0; e < E; ++e) s[g] = __builtin_fma(qd[hb + g][dim + e], (double)f[e], s[g]);
                     }
                 }
 #pragma unroll
-                for (int w = 0; w < W; ++w)
+                for (int g = 0; g < HB; ++g) {
 #pragma unroll
-                    for (int g = 0; g < HB; ++g) {
-                        s[w][g] += __shfl_xor(s[w][g], 1, 64);
-                        s[w][g] += __shfl_xor(s[w][g], 2, 64);
-                        if (hb + g < heads) best[w] = fmaxf(best[w], (float)s[w][g]);  // NaN is passed over
-                    }
+                    for (int x = 1; x < kScoreLanes; x *= 2) s[g] += __shfl_xor(s[g], x, 64);
+                    if (hb + g < heads) best = fmaxf(best, (float)s[g]);  // NaN is passed over
+                }
             }
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const int j = j0 + quad + 64 * w;
-                if (l == 0 && j < cand) {
-                    const uint32_t u = ordered(best[w]);
-                    order[j] = g0 == 0 ? u : max(order[j], u);
-                }
+            const int j = j0 + mine;
+            if (l == 0 && j < cand) {
+                const uint32_t u = ordered(best);
+                order[j] = g0 == 0 ? u : max(order[j], u);
             }
         }
     }
@@ -334,15 +318,9 @@ void launch_bounds_of(const BoundsParams& p, unsigned heads, unsigned blocks, hi
 
 template <typename T, int D, int HB>
 void launch_score(const SelectParams& p, unsigned heads, int64_t cus, hipStream_t stream) {
-    // A workgroup for every 64 blocks; where that is more than two to a CU, for every 128 (the query is then read from LDS half as
-    // often), until each CU has four.  us: 8 heads of 465 blocks 6.2 with 64 and 8.6 with 128, 256 of up to 492 19.1 and 18.0.
-    const int64_t chunks = (p.blocks_max + 63) / 64;
-    if (heads * chunks <= 2 * cus) {
-        hipLaunchKernelGGL((score_blocks_kernel<T, D, HB, 1>), dim3(heads, (unsigned)chunks), dim3(256), 0, stream, p);
-    } else {
-        const int64_t most = std::max<int64_t>((4 * cus + heads - 1) / heads, 1);
-        hipLaunchKernelGGL((score_blocks_kernel<T, D, HB, 2>), dim3(heads, (unsigned)std::min<int64_t>((chunks + 1) / 2, most)), dim3(256), 0, stream, p);
-    }
+    // As many workgroups as have blocks, up to 16 to a CU.  us of those 32 sequences with 8, 16 and 64: 109.2, 107.7 and 107.6
+    const int64_t most = std::max<int64_t>((16 * cus + heads - 1) / heads, 1), parts = (p.blocks_max + kScoreBlocks - 1) / kScoreBlocks;
+    hipLaunchKernelGGL((score_blocks_kernel<T, D, HB>), dim3(heads, (unsigned)std::min(parts, most)), dim3(256), 0, stream, p);
 }
 template <typename T>
 void score(const SelectParams& p, unsigned heads, int64_t cus, hipStream_t stream) {
