@@ -23,7 +23,7 @@ namespace {
 
 struct BlocksPlan {
     int32_t kernel_d, nsub, units, shares;
-    size_t rec_o, rec_lse;
+    size_t rec_o, rec_ml;
 };
 
 BlocksPlan plan_blocks(const dtattn_decode_blocks_args* a, int cus) {
@@ -35,7 +35,7 @@ BlocksPlan plan_blocks(const dtattn_decode_blocks_args* a, int cus) {
     r.shares = (int32_t)std::max<int64_t>(1, std::min<int64_t>((int64_t)2 * cus, places / kPartLeast));
     const size_t records = (size_t)2 * r.shares * 16;
     r.rec_o = part_up(records * r.kernel_d * sizeof(float));
-    r.rec_lse = part_up(records * sizeof(float));
+    r.rec_ml = part_up(records * sizeof(float2));
     return r;
 }
 
@@ -62,7 +62,7 @@ extern "C" size_t dtattn_decode_blocks_workspace_size(const dtattn_decode_blocks
     if (a == nullptr || a->B <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->D <= 0 || a->n_blocks <= 0 || a->block <= 0) return 0;
     const int cus = stream_cus(reinterpret_cast<hipStream_t>(stream));
     const BlocksPlan plan = plan_blocks(a, cus > 0 ? cus : 256);
-    return plan.rec_o + plan.rec_lse;
+    return plan.rec_o + plan.rec_ml;
 }
 
 extern "C" int dtattn_decode_blocks(const dtattn_decode_blocks_args* a, void* stream_) {
@@ -102,7 +102,7 @@ extern "C" int dtattn_decode_blocks(const dtattn_decode_blocks_args* a, void* st
     const BlocksPlan plan = plan_blocks(a, cus);
     if (a->B * a->Hkv * plan.nsub * (int64_t)(plan.units + kPartExtra) >= ((int64_t)1 << 31) || a->B * a->Hq > 0x7fffffff)
         return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many blocks", who);
-    const size_t need = plan.rec_o + plan.rec_lse;
+    const size_t need = plan.rec_o + plan.rec_ml;
     if (a->workspace == nullptr || a->workspace_bytes < need)
         return fail(DTATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, a->workspace_bytes);
     if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0)
@@ -124,7 +124,7 @@ extern "C" int dtattn_decode_blocks(const dtattn_decode_blocks_args* a, void* st
     p.n_list = (int32_t)a->n_blocks, p.list_units = plan.units, p.block_shift = __builtin_ctz((unsigned)a->block);
     p.nsub[1] = plan.nsub, p.shares = plan.shares, p.columns[1] = 16;
     p.rec_o[1] = reinterpret_cast<float*>(a->workspace);
-    p.rec_lse[1] = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + plan.rec_o);
+    p.rec_ml[1] = reinterpret_cast<float2*>(reinterpret_cast<char*>(a->workspace) + plan.rec_o);
     p.q_b = a->q_stride[0], p.q_h = a->q_stride[1], p.o_b = a->o_stride[0], p.o_h = a->o_stride[1];
     p.lse_b = a->lse != nullptr ? a->lse_stride[0] : 0;
     p.B = (int32_t)a->B, p.Hq = (int32_t)a->Hq, p.Hkv = (int32_t)a->Hkv, p.group = (int32_t)(a->Hq / a->Hkv);

@@ -37,9 +37,9 @@ struct PartsParams {
     const int32_t* list;
     // [0]: prefix, [1]: own tokens or listed blocks
     float* rec_o[2];    // [2 * shares, columns, kernel D]: segments that a share cuts (its first and its last)
-    float* rec_lse[2];
+    float2* rec_ml[2];
     float* whole_o[2];  // [B, Hq, kernel D]: segments inside one share
-    float* whole_lse[2];
+    float2* whole_ml[2];
     int32_t* meta[2];   // places of a column set, and the shares; then of each group or sequence: places before it, and its units
     int32_t nsub[2], columns[2];  // column sets of a kv head; columns of a set
     int32_t shares;     // of both parts, or of the listed blocks, at most
@@ -601,13 +601,10 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
             int b, hq;
             walk.where(z, hk, R0 + g, b, hq);
             const int dim = DPL * (tid & 15);
-            const bool direct = KIND == kListPart && whole;
-            const float lse = __builtin_fmaf(X - kOff, kLn2, __log2f(lt) * kLn2);
-            // every score -inf: a record of O = 0 at the LSE of -inf, which drops it in the merge; the output itself is 0 / 0
-            const float inv = (lt == 0.f && !direct) || !any ? 0.f : 1.f / lt;
+            if (KIND == kListPart && whole) {
+                const float inv = any ? 1.f / lt : 0.f;
 #pragma unroll
-            for (int j = 0; j < DPL; ++j) o[j] *= inv;
-            if (direct) {
+                for (int j = 0; j < DPL; ++j) o[j] *= inv;
                 T* op = reinterpret_cast<T*>(p.o) + b * p.o_b + hq * p.o_h + dim;
 #pragma unroll
                 for (int j = 0; j < DPL; j += 4)
@@ -615,13 +612,13 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
                         if constexpr (kF32) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
                         else *reinterpret_cast<u32x2*>(op + j) = u32x2{pack2<T>(o[j], o[j + 1]), pack2<T>(o[j + 2], o[j + 3])};
                     }
-                if (p.lse != nullptr && (tid & 15) == 0) p.lse[b * p.lse_b + hq] = lse;
+                if (p.lse != nullptr && (tid & 15) == 0) p.lse[b * p.lse_b + hq] = __builtin_fmaf(X - kOff, kLn2, __log2f(lt) * kLn2);
             } else {
                 const int64_t rec = whole ? (int64_t)b * p.Hq + hq : (int64_t)(2 * r + (cut_first ? 0 : 1)) * 16 + g;
                 float* op = (whole ? p.whole_o[S] : p.rec_o[S]) + rec * D + dim;
 #pragma unroll
                 for (int j = 0; j < DPL; j += 4) *reinterpret_cast<f32x4*>(op + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
-                if ((tid & 15) == 0) (whole ? p.whole_lse[S] : p.rec_lse[S])[rec] = lse;
+                if ((tid & 15) == 0) (whole ? p.whole_ml[S] : p.rec_ml[S])[rec] = make_float2(X - kOff, lt);
             }
         }
         if (u < n) lds_barrier();  // every wave has read the others' before they write again
@@ -799,21 +796,20 @@ __device__ void decode_part_rows(const PartsParams& p, const PartLengths& lens, 
             if (row < R) {
                 int b, hq;
                 walk.where(seg.z, seg.hk, row, b, hq);
-                const float lse = __builtin_fmaf(M[c] - PartType<T>::offset, kLn2, __log2f(lt) * kLn2);
-                const float inv = lt == 0.f ? 0.f : 1.f / lt;  // every score -inf: a record of O = 0 that its LSE drops
                 const int in_set = 16 * NC * wave + 16 * c + col;
                 const int64_t rec = whole ? (int64_t)b * p.Hq + hq : (int64_t)(2 * r + (cut_first ? 0 : 1)) * (16 * NC * kPartWaves) + in_set;
                 float* op = (whole ? p.whole_o[0] : p.rec_o[0]) + rec * D + 4 * g4;
 #pragma unroll
-                for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4*>(op + 16 * j) = acc[c][j] * inv;
-                if (g4 == 0) (whole ? p.whole_lse[0] : p.rec_lse[0])[rec] = lse;
+                for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4*>(op + 16 * j) = acc[c][j];
+                if (g4 == 0) (whole ? p.whole_ml[0] : p.rec_ml[0])[rec] = make_float2(M[c] - PartType<T>::offset, lt);
             }
         }
     }
 }
 
 // Merges a query head's records: of the prefix and of its own tokens (SHARED), or of listed blocks that several shares hold.  W waves
-// to a (sequence, query head).
+// to a (sequence, query head).  A record holds the sum of P V, the maximum that P is based on (times log2 e) and the row sum: an LSE in fp32
+// would be off by half a step of its own value, 5e-7 of a weight between 8 and 16.
 template <typename T, int D, int W, bool SHARED>
 __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsParams p) {
     constexpr int DL = D / 64;  // dims per lane
@@ -826,7 +822,7 @@ __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsPara
         int n;                // records
         int64_t first, later; // that of the part's first share, and of the one behind it
         const float* o;
-        const float* lse;
+        const float2* ml;
     };
     auto part = [&](int S, int z, int row) {
         Part r = {0, 0, 0, nullptr, nullptr};
@@ -843,7 +839,7 @@ __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsPara
         r.first = whole ? pair : (int64_t)(2 * r0 + (sh.start(r0) < x0 - kPartExtra ? 1 : 0)) * cols + row - sub * cols;
         r.later = (int64_t)2 * (r0 + 1) * cols + row - sub * cols;
         r.o = whole ? p.whole_o[S] : p.rec_o[S];
-        r.lse = whole ? p.whole_lse[S] : p.rec_lse[S];
+        r.ml = whole ? p.whole_ml[S] : p.rec_ml[S];
         return r;
     };
     Part pre = {0, 0, 0, nullptr, nullptr}, own = part(1, b, g);
@@ -859,32 +855,33 @@ __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsPara
     float M = kNegInf, sum = 0.f, acc[DL] = {};
     constexpr int MB = 8;  // records in flight
     for (int j0 = wave; j0 < n; j0 += W * MB) {
-        float lw[MB], v[MB][DL], top = M;
+        float2 ml[MB];
+        float v[MB][DL], top = M;
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
             const int i = min(j0 + W * j, n - 1);
             const bool is_own = !SHARED || i >= pre.n;
             const int k = i - (SHARED && is_own ? pre.n : 0);
             const int64_t q = k == 0 ? (is_own ? own.first : pre.first) : (is_own ? own.later : pre.later) + (int64_t)(k - 1) * 2 * p.columns[is_own ? 1 : 0];
-            lw[j] = (is_own ? own.lse : pre.lse)[q];
+            ml[j] = (is_own ? own.ml : pre.ml)[q];
             const float* o = (is_own ? own.o : pre.o) + q * D + DL * lane;
 #pragma unroll
             for (int e = 0; e < DL; ++e) v[j][e] = o[e];
         }
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
-            if (j0 + W * j >= n) lw[j] = kNegInf;
-            top = fmaxf(top, lw[j]);
+            if (j0 + W * j >= n) ml[j].x = kNegInf;
+            top = fmaxf(top, ml[j].x);
         }
-        const float base = top == kNegInf ? 0.f : top, alpha = __expf(M - base);
+        const float base = top == kNegInf ? 0.f : top, alpha = fast_exp2(M - base);
         M = top;
         sum *= alpha;
 #pragma unroll
         for (int e = 0; e < DL; ++e) acc[e] *= alpha;
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
-            const float w = __expf(lw[j] - base);
-            sum += w;
+            const float w = fast_exp2(ml[j].x - base);
+            sum = __builtin_fmaf(w, ml[j].y, sum);
 #pragma unroll
             for (int e = 0; e < DL; ++e) acc[e] = __builtin_fmaf(w, v[j][e], acc[e]);
         }
@@ -904,7 +901,7 @@ __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsPara
         for (int e = 0; e < DL; ++e) acc[e] = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const float f = __expf(red[w][D] - base);
+            const float f = fast_exp2(red[w][D] - base);
             sum = __builtin_fmaf(red[w][D + 1], f, sum);
 #pragma unroll
             for (int e = 0; e < DL; ++e) acc[e] = __builtin_fmaf(red[w][DL * lane + e], f, acc[e]);
@@ -922,7 +919,7 @@ __global__ void __launch_bounds__(256) decode_parts_merge_kernel(const PartsPara
 #pragma unroll
     for (int e = 0; e < DL; ++e)
         if (DL * lane + e < p.d) op[DL * lane + e] = Elem<T>::from_f32(nothing ? 0.f : acc[e] * inv);
-    if (p.lse != nullptr && lane == 0) p.lse[b * p.lse_b + hq] = M + __logf(sum);
+    if (p.lse != nullptr && lane == 0) p.lse[b * p.lse_b + hq] = __builtin_fmaf(M, kLn2, __log2f(sum) * kLn2);
 }
 
 namespace {

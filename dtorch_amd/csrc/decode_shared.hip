@@ -66,7 +66,7 @@ namespace {
 
 struct SharedPlan {
     int32_t kernel_d, nc, nsub[2], shares, columns[2], weight[2];
-    size_t meta[2], rec_o[2], rec_lse[2], whole_o, whole_lse, bytes;
+    size_t meta[2], rec_o[2], rec_ml[2], whole_o, whole_ml, bytes;
 };
 
 // Places of a segment of so many tokens.
@@ -93,12 +93,12 @@ SharedPlan plan_shared(const dtattn_decode_shared_args* a, int cus) {
         const size_t records = (size_t)2 * r.shares * r.columns[s];
         r.meta[s] = part_up((4 + 2 * (size_t)sets[s]) * sizeof(int32_t));
         r.rec_o[s] = part_up(records * r.kernel_d * sizeof(float));
-        r.rec_lse[s] = part_up(records * sizeof(float));
+        r.rec_ml[s] = part_up(records * sizeof(float2));
     }
     r.whole_o = part_up((size_t)a->B * a->Hq * r.kernel_d * sizeof(float));
-    r.whole_lse = part_up((size_t)a->B * a->Hq * sizeof(float));
-    r.bytes = 2 * (r.whole_o + r.whole_lse);
-    for (int s = 0; s < 2; ++s) r.bytes += r.meta[s] + r.rec_o[s] + r.rec_lse[s];
+    r.whole_ml = part_up((size_t)a->B * a->Hq * sizeof(float2));
+    r.bytes = 2 * (r.whole_o + r.whole_ml);
+    for (int s = 0; s < 2; ++s) r.bytes += r.meta[s] + r.rec_o[s] + r.rec_ml[s];
     return r;
 }
 
@@ -213,9 +213,9 @@ extern "C" int dtattn_decode_shared(const dtattn_decode_shared_args* a, void* st
         p.nsub[s] = plan.nsub[s], p.columns[s] = plan.columns[s], p.weight[s] = plan.weight[s];
         p.meta[s] = reinterpret_cast<int32_t*>(take(plan.meta[s]));
         p.rec_o[s] = reinterpret_cast<float*>(take(plan.rec_o[s]));
-        p.rec_lse[s] = reinterpret_cast<float*>(take(plan.rec_lse[s]));
+        p.rec_ml[s] = reinterpret_cast<float2*>(take(plan.rec_ml[s]));
         p.whole_o[s] = reinterpret_cast<float*>(take(plan.whole_o));
-        p.whole_lse[s] = reinterpret_cast<float*>(take(plan.whole_lse));
+        p.whole_ml[s] = reinterpret_cast<float2*>(take(plan.whole_ml));
     }
     p.shares = plan.shares;
     p.q_b = a->q_stride[0], p.q_h = a->q_stride[1], p.o_b = a->o_stride[0], p.o_h = a->o_stride[1];
