@@ -412,6 +412,9 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
     constexpr int VW = DPL * (int)sizeof(T) / 4; // words of them
     constexpr int NR = TWO ? 2 : 1;              // buffer resources of a unit
     constexpr int PP = PartType<T>::parts;
+    // Sums of an fp32 score, as many as there are registers for: one chain of D products is off by more (O against 64 bits 5.4e-7 of its size
+    // with one sum, 2.8e-7 with four, D = 64).
+    constexpr int SUMS = D == 64 ? 4 : 2;
     constexpr float kOff = PartType<T>::offset;
     typedef PartWalk<KIND, NR> Walk;
     typedef typename Walk::At At;
@@ -510,15 +513,20 @@ __device__ void decode_part(const PartsParams& p, const PartLengths& lens, const
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
                 sc[0][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                f32x4 part[SUMS] = {};
 #pragma unroll
                 for (int k = 0; k < NK; ++k) {
                     if constexpr (kF32) {
                         const f32x4 kf = __builtin_bit_cast(f32x4, kr[tt][k]), q = __builtin_bit_cast(f32x4, qf[k]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[0][tt] = mfma_f32(kf[e], q[e], sc[0][tt]);
+                        for (int e = 0; e < 4; ++e) part[e % SUMS] = mfma_f32(kf[e], q[e], part[e % SUMS]);
                     } else {
                         sc[0][tt] = mfma16(__builtin_bit_cast(V8, kr[tt][k]), __builtin_bit_cast(V8, qf[k]), sc[0][tt]);
                     }
+                }
+                if constexpr (kF32) {
+#pragma unroll
+                    for (int e = 0; e < SUMS; ++e) sc[0][tt] += part[e];
                 }
             }
             if (more) load_k(nx);  // the keys are used up
