@@ -249,6 +249,7 @@ class PagedKVCache:
         self.page_refs: Optional[torch.Tensor] = None
         self.prefix_lengths: Optional[torch.Tensor] = None  # of each group, where sequences share pages that are read once
         self._shares = {}  # the same for every number of groups so far: a captured step reads its own as long as it lives
+        self._fork_captured = False  # a captured fork updates the _shares that were there, and may be replayed at any time
         self._host_stale = False  # a step was recorded under graph capture, or its parents were on the device: _host_len is behind
 
     def _span_pages(self) -> int:
@@ -374,8 +375,9 @@ class PagedKVCache:
         """Sequence b continues what sequence parents[b] is, on the same pages (F.kv_pages_fork); a parent outside the batch, such
         as -1, frees the sequence.  parents: B whole numbers on the host, or an int32 tensor [B] on the device.  The latter does not
         wait for the device (and may be captured): the host's lengths are then behind until sync_lengths(), and a group that has a
-        parent from another one, or a sequence without parent, shares nothing until the next share().  A cache that runs out of pages meanwhile drops tokens, which
-        sync_lengths() reports."""
+        parent from another one, or a sequence without parent, shares nothing until the next share().  A captured fork does so for the
+        numbers of groups that share() has had before the capture; others are refused from then on.  A cache that runs out of pages
+        meanwhile drops tokens, which sync_lengths() reports."""
         batch = len(self._host_len)
         on_device = isinstance(parents, torch.Tensor) and parents.is_cuda
         if not on_device:
@@ -391,6 +393,7 @@ class PagedKVCache:
         if on_device:
             F.kv_pages_fork(self.block_table, self.lengths, self.page_refs, parents)
             self._host_stale = True
+            self._fork_captured |= torch.cuda.is_current_stream_capturing()
             for groups, shared in self._shares.items():  # a group with a parent from elsewhere, or none, has nothing in common
                 per = batch // groups
                 home = torch.arange(batch, dtype=torch.int64, device=parents.device) // per
@@ -420,7 +423,8 @@ class PagedKVCache:
     def share(self, groups: int) -> None:
         """Read the pages that the sequences of a group have in common once per step: ``groups`` equal groups of consecutive
         sequences (0: no longer).  Takes effect for the pages they share now, and stays right as sequences grow; a group with
-        an empty sequence shares nothing."""
+        an empty sequence shares nothing.  Call it once with each number of groups that will be wanted before a fork is captured:
+        the fork's replays keep those right and know no others, which are refused."""
         if groups == 0:
             self.prefix_lengths = None
             return
@@ -435,16 +439,22 @@ class PagedKVCache:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("PagedKVCache: share() cannot be captured")
         if groups not in self._shares:
+            if self._fork_captured:
+                raise RuntimeError(f"PagedKVCache: a fork was captured before the first share({groups}), and its replays would not keep the "
+                                   f"prefixes right; call share({groups}) once before the capture")
             self._shares[groups] = torch.zeros(groups, dtype=torch.int32, device=self.lengths.device)
         self._set_shared(groups)
         self.prefix_lengths = self._shares[groups]
 
-    def _set_shared(self, groups: int) -> None:
+    def _set_shared(self, groups: int, most=None) -> None:
+        """The tokens on pages that all of a group have; no more than ``most``, where that is given for each group."""
         common = []
         for table, lengths in zip(np.split(self._table, groups), np.split(self._host_len, groups)):
             whole = int(lengths.min()) // self.page_size
             same = (table[:, :whole] == table[:1, :whole]).all(0)
             common.append((int(same.argmin()) if not same.all() else whole) * self.page_size)
+        if most is not None:
+            common = np.minimum(common, most).tolist()
         self._shares[groups].copy_(torch.tensor(common, dtype=torch.int32))
 
     def compact(self) -> torch.Tensor:
@@ -464,7 +474,7 @@ class PagedKVCache:
 
     def sync_lengths(self) -> np.ndarray:
         """Refresh the host copy of the lengths from the device after HIP-graph replays (and, once pages are shared, the table
-        too).
+        too; what share() reads once comes down to what the groups still have in common).
 
         Without shared pages replays assign none: the block-table slots past a sequence's assigned pages hold -1, so the
         caller bounds the replays by the tokens left on the pages already assigned.  Raises if a replay
@@ -480,4 +490,6 @@ class PagedKVCache:
             raise RuntimeError("PagedKVCache: graph replays appended past the assigned pages")
         self._host_len = dev
         self._host_stale = False
+        for groups, shared in self._shares.items():
+            self._set_shared(groups, most=shared.tolist())
         return dev.copy()
