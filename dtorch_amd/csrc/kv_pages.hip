@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
     int* items = in_lds ? held : p.items;
     struct Item {
         int b, slot, page, refs;  // slot: -1 outside what is written; page: -1 empty
+        bool lost;                // empty though the sequence has tokens in it: they found no page
     };
     auto item = [&](int i) {
         Item r;
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
         r.page = r.slot >= 0 ? p.table[r.b * p.stride + r.slot] : -1;
         if (r.page >= p.num_pages) r.page = -1;
         r.refs = r.page >= 0 ? p.refs[r.page] : 0;
+        r.lost = r.slot >= 0 && r.page < 0 && i % p.slots == 0 && (t & ((1 << p.page_shift) - 1)) != 0;
         return r;
     };
     // the first counts are on their way meanwhile
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
     int early[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) early[j] = count_at(4 * tid + j);
-    const Item mine = tid < n ? item(tid) : Item{0, -1, -1, 0};  // an item that is needed again, its loads one behind another
+    const Item mine = tid < n ? item(tid) : Item{0, -1, -1, 0, false};  // an item that is needed again, its loads one behind another
     auto again = [&](int i) { return i < kPlan ? mine : item(i); };
     for (int i = tid; i < n; i += kPlan) {
         const Item it = again(i);
@@ -150,13 +152,14 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
     }
     __syncthreads();
     // who needs a page, and which one in turn
-    int need = 0;
+    int need = 0, lost = 0;
     for (int i0 = 0; i0 < n; i0 += kPlan) {
         const int i = i0 + tid;
-        bool takes = false;
+        bool takes = false, gone = false;
         if (i < n) {
             const Item it = again(i);
-            takes = it.slot >= 0 && it.page < 0;
+            takes = it.slot >= 0 && it.page < 0 && !it.lost;
+            gone = it.lost;
             if (it.page >= 0 && it.refs > 1) {
                 int before = 0, j = 0;  // earlier items of the same page
                 if (in_lds)
@@ -169,9 +172,9 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
             }
         }
         int total;
-        const int k = scan_plan(takes, waves, total);
+        const int k = scan_plan((int)takes | (int)gone << 16, waves, total) & 0xffff;
         if (i < n) p.order[i] = takes ? need + k : -1;
-        need += total;
+        need += total & 0xffff, lost += total >> 16;
     }
     // that many free pages, from the lowest index up
     int found = 0;
@@ -192,7 +195,7 @@ __global__ void __launch_bounds__(kPlan) kv_reserve_plan_kernel(const PagesParam
         found += total;
     }
     found = min(found, need);
-    if (tid == 0) *p.out = need - found;
+    if (tid == 0) *p.out = need - found + lost;
     __syncthreads();  // counts have been read, and the list is written
     for (int i = tid; i < n; i += kPlan) {
         const Item it = again(i);

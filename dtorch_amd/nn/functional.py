@@ -254,7 +254,8 @@ def kv_pages_reserve(pools: Sequence[torch.Tensor], block_table: torch.Tensor, l
     [num_pages, Hkv, page_size / block, D]; up to 8.  Empty slots take free pages (page_refs 0), the lowest first, sequence by
     sequence; a sequence whose next token falls into a page that others share takes a copy of its rows (of sequences that
     all write a page the last one keeps it).  Returns int32 [1] on the device: the pages that were lacking (0: none); slots
-    that got none hold -1, and what was cached in them is lost to the sequence.  lengths stay as they are.
+    that got none hold -1, and what was cached in them is lost to the sequence: they count as lacking in later calls too, until
+    the sequence has gone on to its next page or has been freed.  lengths stay as they are.
     """
     return _h.KvPagesReserveOp(_h.TokenCountParam(int(n_new))).compute([block_table, lengths, page_refs, *pools])[0]
 

@@ -247,6 +247,7 @@ class PagedKVCache:
         self.block_table = torch.from_numpy(self._table.copy()).to(device)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.page_refs: Optional[torch.Tensor] = None
+        self._lacking: Optional[torch.Tensor] = None  # pages that steps lacked on the device since the last sync_lengths()
         self.prefix_lengths: Optional[torch.Tensor] = None  # of each group, where sequences share pages that are read once
         self._shares = {}  # the same for every number of groups so far: a captured step reads its own as long as it lives
         self._fork_captured = False  # a captured fork updates the _shares that were there, and may be replayed at any time
@@ -277,6 +278,7 @@ class PagedKVCache:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("PagedKVCache: call fork() or compact() once before they are captured")
             self.page_refs = torch.from_numpy(self._refs()).to(self.lengths.device)
+            self._lacking = torch.zeros(1, dtype=torch.int32, device=self.lengths.device)
 
     def _reserve_shared(self, rows: int, n: int) -> None:
         """Pages for the next n tokens of the first sequences, on the device; the host's table follows by the same rule."""
@@ -294,8 +296,10 @@ class PagedKVCache:
                 if not free:
                     raise ValueError("PagedKVCache: out of pages")
                 table[b, s] = free.pop()
-        F.kv_pages_reserve(self._pools(), self.block_table[:rows], self.lengths[:rows], self.page_refs, n)
-        if table is not None:
+        lacking = F.kv_pages_reserve(self._pools(), self.block_table[:rows], self.lengths[:rows], self.page_refs, n)
+        if table is None:
+            self._lacking += lacking
+        else:
             self._table = table
             self._pages = (table >= 0).sum(1)
             self._set_free()
@@ -377,7 +381,7 @@ class PagedKVCache:
         wait for the device (and may be captured): the host's lengths are then behind until sync_lengths(), and a group that has a
         parent from another one, or a sequence without parent, shares nothing until the next share().  A captured fork does so for the
         numbers of groups that share() has had before the capture; others are refused from then on.  A cache that runs out of pages
-        meanwhile drops tokens, which sync_lengths() reports."""
+        meanwhile drops tokens, which sync_lengths() reports; until then what the sequences without pages attend to says nothing."""
         batch = len(self._host_len)
         on_device = isinstance(parents, torch.Tensor) and parents.is_cuda
         if not on_device:
@@ -479,13 +483,18 @@ class PagedKVCache:
         Without shared pages replays assign none: the block-table slots past a sequence's assigned pages hold -1, so the
         caller bounds the replays by the tokens left on the pages already assigned.  Raises if a replay
         went past them, or found no free page: those tokens were dropped (no page was written) and the sequence's cache is
-        incomplete.
+        incomplete.  Raises until such sequences are freed, and once if they have ended meanwhile.
         """
+        self._host_stale = True  # unless all is found well
         dev = self.lengths.to("cpu", torch.int64).numpy().copy()
         if self.page_refs is not None:
             self._table = self.block_table.to("cpu").numpy().copy()
             self._pages = np.where((self._table < 0).any(1), (self._table < 0).argmax(1), self._table.shape[1])
             self._set_free()
+            lacking = self._lacking.item()
+            self._lacking.zero_()
+            if lacking:
+                raise RuntimeError(f"PagedKVCache: steps appended past the assigned pages: {lacking} times a sequence found no page, and dropped tokens")
         if np.any(dev > self._pages * self.page_size):
             raise RuntimeError("PagedKVCache: graph replays appended past the assigned pages")
         self._host_len = dev

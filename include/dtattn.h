@@ -480,7 +480,8 @@ typedef struct {
 
 /* Reserve: pages of their own for the next n_new tokens of every sequence.  The slots of positions lengths[b] to
  * lengths[b] + n_new - 1 (those inside the table; lengths clamped to [0, max_pages * page_size]) are taken in the order of b and then
- * of the slot.  An empty one takes a free page.  One whose page is shared takes a free page as well, so long as others still name
+ * of the slot.  An empty one takes a free page, unless the sequence has tokens in it already (an earlier call found no page for them): such a slot
+ * stays empty and is counted as lacking, for another sequence's rows would stand where those tokens were.  One whose page is shared takes a free page as well, so long as others still name
  * the page: of sequences that all write a page, the last one keeps it.  The rows of the tokens that the sequence has in such a page
  * are copied, in every pool.  Free pages are taken from the lowest index up; once they run out, slots that need one become -1 (tokens
  * written through them are dropped, those they held are lost to the sequence), and *short_by says how many (0 otherwise).

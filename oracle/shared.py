@@ -51,6 +51,9 @@ def reserve(pools, table, lengths, refs, n_new, page):
                 if rank >= before_r[old] - 1:
                     continue
                 refs[old] -= 1
+            elif s == t // page and t % page:  # tokens that found no page are lost
+                short += 1
+                continue
             if not free:
                 table[b, s] = -1
                 short += 1

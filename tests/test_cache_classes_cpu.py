@@ -189,3 +189,102 @@ def test_shares_through_any_order(ops, seed):
         _shares_hold(cache)
     cache.sync_lengths()
     _shares_hold(cache)
+
+
+def _shortage(ops):
+    """Three pages: two sequences share one of 8 tokens, a third holds the others; a step with its parents on the device then lacks a page."""
+    cache = _cache(pages=3, batch=3, columns=4)
+    cache.append(*[x[:1] for x in _tokens(100, 3, 8)[1:]])
+    cache.fork([0, 0, -1])
+    rows = torch.arange(24.0).add(700).view(1, 1, 24, 1).expand(1, HKV, 24, D).contiguous()
+    table, lengths = cache.block_table[2:], cache.lengths[2:]
+    ops.kv_pages_reserve(cache._pools(), table, lengths, cache.page_refs, 24)
+    ops.kv_cache_append_paged(cache.k, cache.v, table, lengths, rows, rows)
+    cache._host_stale = True
+    cache.sync_lengths()
+    assert cache.lengths.tolist() == [8, 8, 24] and cache.block_table[2].tolist() == [1, 2, -1, -1] and not cache._free
+    cache.fork(_parents([0, 1, 2]))
+    ops.short.clear()
+    cache.decode(*_tokens(800, 3))
+    assert ops.short == [1] and cache.block_table[:2, 0].tolist() == [-1, 0]
+    return cache
+
+
+def test_a_shortage_is_not_filled_by_foreign_pages(ops):
+    """A sequence whose page was lacking gets none in its middle once another ends: it would find the other's rows there."""
+    cache = _shortage(ops)
+    cache.fork(_parents([0, 1, -1]))
+    for i in range(3):
+        cache.decode(*_tokens(810 + i, 3))
+    assert cache.block_table[0, 0].item() == -1
+    for _ in range(2):  # as long as the sequence lives
+        with pytest.raises(RuntimeError, match="past the assigned pages"):
+            cache.sync_lengths()
+    cache.free([0])
+    assert cache.sync_lengths().tolist() == [0, 12, 3]
+    assert _held(cache, 1) == [100.0 + i for i in range(8)] + [801.0, 811.0, 812.0, 813.0]
+    cache.decode(*_tokens(900, 3))
+    assert cache.lengths.tolist() == [1, 13, 4]
+
+
+def test_a_shortage_is_reported_when_its_sequence_has_ended(ops):
+    """Its steps attended to rows that were not its own, so the next sync says so, once."""
+    cache = _shortage(ops)
+    cache.fork(_parents([1, 1, -1]))
+    cache.decode(*_tokens(820, 3))
+    with pytest.raises(RuntimeError, match="past the assigned pages"):
+        cache.sync_lengths()
+    assert cache.sync_lengths().tolist() == [10, 10, 1]
+    assert _held(cache, 0) == [100.0 + i for i in range(8)] + [801.0, 820.0]
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_small_pools(ops, seed):
+    """Steps with parents on the device over a pool that is too small at times: what sync_lengths lets pass is whole, token by token."""
+    rng = np.random.default_rng(seed)
+    cache = _cache(pages=14, columns=20)
+    cache.fork(list(range(B)))  # the device gives out the pages
+    texts, lost = [[] for _ in range(B)], False
+    for step in range(120):
+        parents = rng.integers(-1 if rng.random() < 0.4 else 0, B, B).tolist()
+        cache.fork(_parents(parents))
+        texts = [list(texts[p]) if p >= 0 else [] for p in parents]
+        ops.short.clear()
+        cache.decode(*_tokens(1000 * (step + 1)))
+        lost |= any(ops.short)
+        for b in range(B):
+            texts[b].append(1000.0 * (step + 1) + b)
+        if rng.random() < 0.2:
+            if lost:
+                with pytest.raises(RuntimeError, match="past the assigned pages"):
+                    cache.sync_lengths()
+            try:
+                cache.sync_lengths()
+            except RuntimeError:
+                lost = True
+                continue
+            lost = False
+            for b in range(B):
+                assert _held(cache, b) == texts[b]
+
+
+def test_a_shortage_in_replays(ops):
+    """Replays that the host does not see lack a page: until the sequence is freed the host goes by the device, not by what it knew."""
+    cache = _shortage(ops)
+    cache.fork(_parents([1, 1, 2]))
+    with pytest.raises(RuntimeError):
+        cache.sync_lengths()
+    cache.free([2])
+    assert cache.sync_lengths().tolist() == [9, 9, 0]
+    q, k, v = _tokens(830, 3, 40)
+    cache._lacking += ops.kv_pages_reserve(cache._pools(), cache.block_table, cache.lengths, cache.page_refs, 40)  # a replay
+    ops.kv_cache_append_paged(cache.k, cache.v, cache.block_table, cache.lengths, k, v)
+    with pytest.raises(RuntimeError, match="past the assigned pages"):
+        cache.sync_lengths()
+    with pytest.raises(RuntimeError, match="sync_lengths"):
+        cache.share(1)
+    cache.free([0, 2])
+    with pytest.raises(RuntimeError, match="past the assigned pages"):
+        cache.sync_lengths()
+    cache.free([1])
+    assert cache.sync_lengths().tolist() == [0, 0, 0] and len(cache._free) == 3
