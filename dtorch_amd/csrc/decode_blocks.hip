@@ -74,6 +74,8 @@ extern "C" int dtattn_decode_blocks(const dtattn_decode_blocks_args* a, void* st
     if (a->Hq % a->Hkv != 0) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: Hq is not a multiple of Hkv", who);
     if (a->block < 16 || a->block > 256 || (a->block & (a->block - 1)) != 0)
         return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: block %d must be a power of two from 16 to 256", who, a->block);
+    // a unit's place in the list is a 32-bit number of tokens
+    if (a->n_blocks * a->block > (1 << 30)) return fail(DTATTN_ERR_UNSUPPORTED, "%s: %lld listed tokens (up to 2^30)", who, (long long)(a->n_blocks * a->block));
     const bool paged = a->block_table != nullptr;
     if (paged) {
         if (a->page_size < 16 || (a->page_size & (a->page_size - 1)) != 0 || a->page_size > (1 << 20))

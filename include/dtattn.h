@@ -618,7 +618,7 @@ int dtattn_select_key_blocks(const dtattn_select_blocks_args* args, void* stream
 
 /* Single-token attention over the listed blocks of each kv head: dtattn_decode_splitkv's formula over the tokens
  * blocks[b, hk, i] * block + (0 .. block - 1) that lie before lengths[b].  An index that is negative or past the sequence's blocks
- * stands for no token; a block listed twice counts twice.  No token: O = 0, LSE = -inf.  Types as for dtattn_decode_shared. */
+ * stands for no token; a block listed twice counts twice.  Up to 2^30 listed tokens (n_blocks * block).  No token: O = 0, LSE = -inf.  Types as for dtattn_decode_shared. */
 typedef struct {
     const void* q;
     const void* k_cache;     /* [B, Hkv, S_max, D]; paged: [num_pages, Hkv, page_size, D] */
