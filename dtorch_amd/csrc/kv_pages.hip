@@ -460,10 +460,9 @@ extern "C" int dtattn_kv_pages_reserve(const dtattn_kv_reserve_args* a, void* st
     PagesParams p = {};
     st = fill_pools(a->pools, a->n_pools, a->page_size, false, who, p.pool);
     if (st != DTATTN_OK) return st;
-    if (a->short_by == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+    if (a->short_by == nullptr || a->page_refs == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
     if (a->B > 0 && a->n_new > 0) {
-        if (a->block_table == nullptr || a->lengths == nullptr || a->page_refs == nullptr)
-            return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+        if (a->block_table == nullptr || a->lengths == nullptr) return fail(DTATTN_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
         if (a->B * slots_of(a) > (1 << 28)) return fail(DTATTN_ERR_UNSUPPORTED, "%s: too many slots", who);
         const ReserveSpace r = reserve_space(a);
         const size_t need = r.items + r.order + r.list + r.copies;

@@ -491,7 +491,7 @@ typedef struct {
     int32_t n_pools;
     int32_t* block_table;    /* [B, max_pages], slot stride 1 */
     const int32_t* lengths;  /* [B] */
-    int32_t* page_refs;      /* [num_pages] */
+    int32_t* page_refs;      /* [num_pages], also where B or n_new is 0 */
     int32_t* short_by;       /* [1] */
     int64_t B, max_pages, num_pages, page_size, n_new;
     int64_t block_table_stride;

@@ -10,3 +10,10 @@ def test_listed_tokens(paged, n, block):
     """Places in a list are 32-bit numbers of tokens: a list of more than 2^30 is refused, though its entries are fewer than 2^25."""
     got = _call("blocks", _args("blocks", paged, dict(B=1, Hq=4, n_blocks=n, block=block, page_size=256)))
     assert got[0] == 2 and "listed tokens" in got[1], got
+
+
+@pytest.mark.parametrize("kw", [dict(B=0), dict(n_new=0), dict(B=0, n_new=0)])
+def test_reserve_without_counts(kw):
+    """The plan reads the counts of all pages, also where there is nothing to reserve."""
+    got = _call("reserve", _args("reserve", False, dict(page_refs=None, **kw)))
+    assert got[0] == 1 and "null" in got[1], got
