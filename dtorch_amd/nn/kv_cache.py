@@ -226,7 +226,8 @@ class PagedKVCache:
     bounds_block: tokens (at most a page) of a block of key bounds (0: none), for decode(keep=).
 
     From the first fork(), free() or compact() on, ``page_refs`` (int32 [num_pages], how many slots of the table name
-    each page) is kept on the device, and pages are given out there by the same rule as here: the lowest free one first.
+    each page) is kept on the device, and pages are given out there by the same rule as here: the lowest free one first.  Call one
+    of them before a step is captured, if sequences are to share pages later.
     """
 
     def __init__(self, batch: int, kv_heads: int, num_pages: int, page_size: int, max_pages: int, head_dim: int,
@@ -250,6 +251,7 @@ class PagedKVCache:
         self._lacking: Optional[torch.Tensor] = None  # pages that steps lacked on the device since the last sync_lengths()
         self.prefix_lengths: Optional[torch.Tensor] = None  # of each group, where sequences share pages that are read once
         self._shares = {}  # the same for every number of groups so far: a captured step reads its own as long as it lives
+        self._append_captured = False  # before page_refs were there: its replays write the pages that the table names
         self._fork_captured = False  # a captured fork updates the _shares that were there, and may be replayed at any time
         self._host_stale = False  # a step was recorded under graph capture, or its parents were on the device: _host_len is behind
 
@@ -335,6 +337,7 @@ class PagedKVCache:
                     changed = True
             if changed:
                 self.block_table.copy_(torch.from_numpy(self._table), non_blocking=False)
+            self._append_captured |= torch.cuda.is_current_stream_capturing()
         table, lengths = self.block_table[:rows], self.lengths[:rows]
         if self.k_scale is not None:
             F.kv_cache_append_fp8_paged(self.k, self.v, self.k_scale, self.v_scale, table, lengths, k_new, v_new)
@@ -380,7 +383,8 @@ class PagedKVCache:
         as -1, frees the sequence.  parents: B whole numbers on the host, or an int32 tensor [B] on the device.  The latter does not
         wait for the device (and may be captured): the host's lengths are then behind until sync_lengths(), and a group that has a
         parent from another one, or a sequence without parent, shares nothing until the next share().  A captured fork does so for the
-        numbers of groups that share() has had before the capture; others are refused from then on.  A cache that runs out of pages
+        numbers of groups that share() has had before the capture; others are refused from then on.  A step captured before the first
+        fork() or compact() does not copy what it writes, so that sequences cannot share pages behind it.  A cache that runs out of pages
         meanwhile drops tokens, which sync_lengths() reports; until then what the sequences without pages attend to says nothing."""
         batch = len(self._host_len)
         on_device = isinstance(parents, torch.Tensor) and parents.is_cuda
@@ -390,6 +394,11 @@ class PagedKVCache:
             raise ValueError(f"fork takes a parent for each of the {batch} sequences; got {len(parents)}")
         if not on_device and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("PagedKVCache: a captured fork takes its parents on the device")
+        if self._append_captured:
+            living = None if on_device else parents[(parents >= 0) & (parents < batch)]
+            if living is None or len(np.unique(living)) < len(living):
+                raise RuntimeError("PagedKVCache: a step was captured before the first fork() or compact(), and its replays would write pages that "
+                                   "sequences share; call compact() once before the capture")
         if not on_device and self._host_stale:
             parents = torch.from_numpy(parents.clip(-1, batch).astype(np.int32)).to(self.lengths.device)
             on_device = True

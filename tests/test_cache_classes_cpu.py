@@ -288,3 +288,37 @@ def test_a_shortage_in_replays(ops):
         cache.sync_lengths()
     cache.free([1])
     assert cache.sync_lengths().tolist() == [0, 0, 0] and len(cache._free) == 3
+
+
+def test_fork_behind_a_step_captured_without_counts(ops):
+    """A step captured before the first fork gives out no pages: its replays would write the pages that a fork lets sequences share."""
+    cache = _cache()
+    cache.prefill(*_tokens(0, B, 20))
+    ops.capturing = True
+    cache.decode(*_tokens(500))
+    ops.capturing = False
+    cache.sync_lengths()
+    before = cache.block_table.clone()
+    for parents in ([0, 0, 2, 3, 4, 5], [1, 2, 3, 4, 5, 5], _parents(range(B))):
+        with pytest.raises(RuntimeError, match="captured"):
+            cache.fork(parents)
+    assert cache.page_refs is None and not cache._host_stale and torch.equal(cache.block_table, before)
+    cache.fork([5, 4, 3, 2, 1, 0])  # no page in two sequences
+    cache.free([2])
+    assert cache.compact().item() == 10
+    with pytest.raises(RuntimeError, match="captured"):
+        cache.fork([0, 0, 2, 3, 4, 5])
+    assert _held(cache, 0) == [100.0 + i for i in range(20)] + [505.0] and cache.lengths.tolist() == [21, 21, 0, 21, 21, 21]
+
+
+def test_fork_behind_a_step_captured_with_counts(ops):
+    cache = _cache()
+    cache.prefill(*_tokens(0, B, 20))
+    cache.compact()
+    ops.capturing = True
+    cache.decode(*_tokens(500))
+    ops.capturing = False
+    cache.sync_lengths()
+    cache.fork([0, 0, 2, 3, 4, 5])
+    cache.decode(*_tokens(600))
+    assert _held(cache, 0)[20:] == [500.0, 600.0] and _held(cache, 1)[20:] == [500.0, 601.0]

@@ -98,3 +98,50 @@ def test_two_captured_forks_under_different_shares():
             cache.sync_lengths()
             cache.share(2)
             cache.share(3)
+
+
+def test_step_captured_before_the_first_fork():
+    """It has no copy on write, so pages cannot be shared behind it; freed and moved pages are no matter."""
+    g = _gen(23)
+    cache = _paged()
+    q, k, v = _qkv(B, 33, g)
+    cache.prefill(q, k, v)
+    history, step = [[(k[b], v[b])] for b in range(B)], _qkv(B, 1, g)
+    graph, out = _captured(cache, step)
+    keep = torch.arange(B, dtype=torch.int32, device="cuda")
+
+    def replay():
+        for x in step:
+            x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        return _follow(history, range(B), step)
+
+    for _ in range(3):
+        history = replay()
+        _check(out, step[0], history)
+    cache.sync_lengths()
+    for parents in ([0, 0, 2, 3, 4, 5], keep):
+        with pytest.raises(RuntimeError, match="captured"):
+            cache.fork(parents)
+    cache.free([0, 1])
+    assert cache.compact().item() == 3 * (B - 2)
+    history[:2] = [[], []]
+    cache.append(*_qkv(B, 1, g)[1:])  # eager, so that the freed rows have pages
+    cache.sync_lengths()
+    rows = [orc_row(cache, b) for b in range(B)]
+    history = [[r] for r in rows]
+    for _ in range(4):
+        history = replay()
+        _check(out, step[0], history)
+    cache.sync_lengths()
+    _consistent(cache)
+    with pytest.raises(RuntimeError, match="captured"):
+        cache.fork([2, 2, 2, 3, 4, 5])
+
+
+def orc_row(cache, b):
+    """(K, V) of sequence b, as the table has it."""
+    n = int(cache.lengths[b])
+    ids = cache.block_table[b, :-(-n // cache.page_size)].long()
+    return tuple(x[ids].transpose(0, 1).flatten(1, 2)[:, :n].clone() for x in (cache.k, cache.v))
