@@ -33,6 +33,7 @@ struct BoundsParams {
     char* hi;
     int64_t k_b, k_h, k_s, lo_b, lo_h, lo_s, hi_b, hi_h, hi_s;  // bytes
     int32_t Hkv, n_new, chunks;
+    int32_t first;  // of the blocks that the new tokens touch, this launch's
 };
 
 struct SelectParams {
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
     const int h = (int)(bh % p.Hkv);
     const int n = tokens_in(p.c, b);
     const int block = 1 << p.c.block_shift;
-    const int64_t j = (max(n - p.n_new, 0) >> p.c.block_shift) + (int64_t)blockIdx.y * (4 / WAVES) + threadIdx.x / (64 * WAVES);
+    const int64_t j = (max(n - p.n_new, 0) >> p.c.block_shift) + p.first + (int64_t)blockIdx.y * (4 / WAVES) + threadIdx.x / (64 * WAVES);
     const int64_t t0 = j << p.c.block_shift;
     if (t0 >= n) return;
     const int rows = (int)min((int64_t)block, n - t0);
@@ -303,17 +304,24 @@ int row_checks(int64_t D, int32_t dtype, const int64_t* strides, int n, uintptr_
 }
 
 template <typename T, int WAVES>
-void launch_bounds_waves(const BoundsParams& p, dim3 grid, hipStream_t stream) {
+void launch_bounds_waves(const BoundsParams& p, unsigned heads, unsigned groups, hipStream_t stream) {
+    const dim3 grid(heads, groups);
     if (p.chunks <= 8) hipLaunchKernelGGL((key_bounds_kernel<T, 8, WAVES>), grid, dim3(256), 0, stream, p);
     else if (p.chunks <= 16) hipLaunchKernelGGL((key_bounds_kernel<T, 16, WAVES>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((key_bounds_kernel<T, 32, WAVES>), grid, dim3(256), 0, stream, p);
 }
 template <typename T>
-void launch_bounds_of(const BoundsParams& p, unsigned heads, unsigned blocks, hipStream_t stream) {
+void launch_bounds_of(BoundsParams p, unsigned heads, int64_t blocks, hipStream_t stream) {
     // A wave to a block of up to 64 tokens, whose waves would have a load each before they meet.  us with one wave and with four, 4 x 4000
     // tokens: blocks of 16 8.9 and 21.2, of 32 8.3 and 12.1, of 64 8.0 and 8.6, of 256 10.7 and 8.1.
-    if (p.c.block_shift <= 6) launch_bounds_waves<T, 1>(p, dim3(heads, (blocks + 3) / 4), stream);
-    else launch_bounds_waves<T, 4>(p, dim3(heads, blocks), stream);
+    const bool one = p.c.block_shift <= 6;
+    const int64_t each = one ? 4 : 1, most = 65535 * each;  // blocks of a workgroup, and of a launch
+    for (int64_t b0 = 0; b0 < blocks; b0 += most) {
+        p.first = (int32_t)b0;
+        const unsigned groups = (unsigned)((std::min(most, blocks - b0) + each - 1) / each);
+        if (one) launch_bounds_waves<T, 1>(p, heads, groups, stream);
+        else launch_bounds_waves<T, 4>(p, heads, groups, stream);
+    }
 }
 
 template <typename T, int D, int HB>
@@ -370,12 +378,12 @@ extern "C" int dtattn_key_bounds(const dtattn_key_bounds_args* a, void* stream_)
     const int64_t n = std::min<int64_t>(a->n_new, p.c.capacity);
     p.n_new = (int32_t)n;
     const int64_t blocks = (n + a->block - 2) / a->block + 1, heads = a->B * a->Hkv;  // that n tokens touch, at most
-    if (heads > 0x7fffffff || blocks > 65535) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
+    if (heads > 0x7fffffff) return fail(DTATTN_ERR_UNSUPPORTED, "%s: grid too large", who);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     switch (a->dtype) {
-        case DTATTN_BF16: launch_bounds_of<bf16_t>(p, (unsigned)heads, (unsigned)blocks, stream); break;
-        case DTATTN_FP16: launch_bounds_of<f16_t>(p, (unsigned)heads, (unsigned)blocks, stream); break;
-        default: launch_bounds_of<float>(p, (unsigned)heads, (unsigned)blocks, stream);
+        case DTATTN_BF16: launch_bounds_of<bf16_t>(p, (unsigned)heads, blocks, stream); break;
+        case DTATTN_FP16: launch_bounds_of<f16_t>(p, (unsigned)heads, blocks, stream); break;
+        default: launch_bounds_of<float>(p, (unsigned)heads, blocks, stream);
     }
     return check_launch("key_bounds_kernel");
 }

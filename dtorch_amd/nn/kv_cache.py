@@ -196,7 +196,7 @@ class KVCache:
         blocks = -(-self._host_len // self.block)  # as the kernel shortens them
         self._host_len = np.where(blocks > keep // self.block, keep + self._host_len - blocks * self.block, self._host_len)
         if self.k_min is not None:  # tokens have moved
-            F.kv_key_bounds(self.k, self.k_min, self.k_max, self.lengths, self.capacity)
+            F.kv_key_bounds(self.k, self.k_min, self.k_max, self.lengths, keep)  # what any sequence has at most
         return kept
 
     def sync_lengths(self) -> np.ndarray:
