@@ -163,6 +163,8 @@ class KVCache:
                 raise ValueError("decode(prefix=) takes a cache of the same kv heads, head_dim, dtype and device whose sequences divide this one's")
             if own.shape[3] > 128 or own.shape[3] * own.element_size() % 16:
                 raise ValueError("decode(prefix=) takes a head_dim up to 128 whose rows are multiples of 16 bytes")
+            if p.shape[0] > 1024:
+                raise ValueError(f"decode(prefix=) takes up to 1024 prefixes; got {p.shape[0]}")
         self.append(k_new, v_new)
         n = self._span()
         k, v, ks = self.k[:, :, :n], self.v[:, :, :n], None

@@ -322,3 +322,11 @@ def test_fork_behind_a_step_captured_with_counts(ops):
     cache.fork([0, 0, 2, 3, 4, 5])
     cache.decode(*_tokens(600))
     assert _held(cache, 0)[20:] == [500.0, 600.0] and _held(cache, 1)[20:] == [500.0, 601.0]
+
+
+def test_prefixes_of_too_many_groups(ops):
+    """More groups than the shared decode takes are refused before the append."""
+    cache, prefix = (kv_cache.KVCache(1025, HKV, 32, D, dtype=torch.float32, device="cpu") for _ in range(2))
+    with pytest.raises(ValueError, match="1024"):
+        cache.decode(*_tokens(0, 1025), prefix=prefix)
+    assert not cache.lengths.any() and not cache._host_len.any()
