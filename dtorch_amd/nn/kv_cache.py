@@ -321,6 +321,9 @@ class PagedKVCache:
         if rows > len(self._host_len):
             raise ValueError(f"PagedKVCache: {rows} sequences in a cache of {len(self._host_len)}")
         stale = self._host_stale and self.page_refs is not None  # the device gives out the pages
+        if stale and not torch.cuda.is_current_stream_capturing() and int(self._host_len[:rows].max(initial=0)) + n > self._table.shape[1] * self.page_size:
+            self.sync_lengths()  # by what the host knows the tokens might not fit
+            stale = False
         if not stale:
             need = (self._host_len[:rows] + n + self.page_size - 1) // self.page_size
             if int(need.max(initial=0)) > self._table.shape[1]:
@@ -383,7 +386,8 @@ class PagedKVCache:
     def fork(self, parents) -> None:
         """Sequence b continues what sequence parents[b] is, on the same pages (F.kv_pages_fork); a parent outside the batch, such
         as -1, frees the sequence.  parents: B whole numbers on the host, or an int32 tensor [B] on the device.  The latter does not
-        wait for the device (and may be captured): the host's lengths are then behind until sync_lengths(), and a group that has a
+        wait for the device (and may be captured): the host's lengths are then behind until sync_lengths() (which an eager step calls
+        by itself where its token might not fit), and a group that has a
         parent from another one, or a sequence without parent, shares nothing until the next share().  A captured fork does so for the
         numbers of groups that share() has had before the capture; others are refused from then on.  A step captured before the first
         fork() or compact() does not copy what it writes, so that sequences cannot share pages behind it.  A cache that runs out of pages
@@ -408,6 +412,7 @@ class PagedKVCache:
         if on_device:
             F.kv_pages_fork(self.block_table, self.lengths, self.page_refs, parents)
             self._host_stale = True
+            self._host_len[:] = self._host_len.max(initial=0)  # no sequence is longer, until sync_lengths()
             self._fork_captured |= torch.cuda.is_current_stream_capturing()
             for groups, shared in self._shares.items():  # a group with a parent from elsewhere, or none, has nothing in common
                 per = batch // groups

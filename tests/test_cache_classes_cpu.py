@@ -330,3 +330,36 @@ def test_prefixes_of_too_many_groups(ops):
     with pytest.raises(ValueError, match="1024"):
         cache.decode(*_tokens(0, 1025), prefix=prefix)
     assert not cache.lengths.any() and not cache._host_len.any()
+
+
+def test_full_sequences_behind_device_parents(ops):
+    """With its parents on the device the host does not know the lengths; a step that might not fit asks for them before tokens are dropped."""
+    cache = _cache(columns=2)
+    _prompts(cache, 20)
+    for i in range(12):
+        cache.fork(_parents([0, 1, 1, 3, 3, 3]))
+        cache.decode(*_tokens(1000 + 10 * i))
+    with pytest.raises(ValueError, match="max_pages"):
+        cache.decode(*_tokens(2000))
+    assert cache.sync_lengths().tolist() == [32] * B
+    assert _held(cache, 5)[20:] == [1000.0 + 10 * i + (3 if i < 11 else 5) for i in range(12)]
+    cache.fork(_parents([-1, 1, 2, 3, 4, 5]))
+    with pytest.raises(ValueError, match="max_pages"):
+        cache.decode(*_tokens(2000))
+    cache.fork(_parents([-1] * 5 + [0]))  # the long ones end: the next step fits
+    cache.decode(*_tokens(3000))
+    assert cache.sync_lengths().tolist() == [1] * B and _held(cache, 5) == [3005.0]
+
+
+def test_prefill_behind_device_parents(ops):
+    """A row that was empty may have been given a parent's tokens."""
+    cache = _cache()
+    cache.prefill(*_tokens(0, 2, 20))
+    cache.fork([-1, 1, -1, -1, -1, -1])
+    cache.fork(_parents([1, 1, -1, -1, -1, -1]))
+    with pytest.raises(ValueError, match="empty"):
+        cache.prefill(*_tokens(500, 1, 8))
+    cache.fork(_parents([-1, 1, -1, -1, -1, -1]))
+    cache.sync_lengths()
+    cache.prefill(*_tokens(500, 1, 8))
+    assert _held(cache, 0) == [500.0 + i for i in range(8)] and _held(cache, 1) == [20.0 + i for i in range(20)]
