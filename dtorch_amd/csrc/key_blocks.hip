@@ -8,9 +8,9 @@
 // key_bounds_kernel: a wave or a workgroup per (block, sequence and kv head); every 16-byte chunk of a row belongs to one column of
 // threads, which meet by lane exchanges and, of several waves, in LDS.  Bound by HBM: the rows are read once (4 x 4000 tokens of 8 heads of 128 dims, 34 MB, 8.0
 // us, 4.1 TB/s; the last block of 64 sequences' steps 5.0, a launch).
-// score_blocks_kernel: eight lanes to a block, with the query's heads in LDS as 64-bit numbers.  Sums in 64 bits are exact for 16-bit types (products have at
-// most 22 bits), so scores next to one another are told apart alike in any order of summation, and the vector units' 64-bit rate
-// is that of 32 bits.
+// score_blocks_kernel: eight lanes to a block, with the query's heads in LDS as 64-bit numbers.  Sums are taken in 64 bits, so that scores next to
+// one another are told apart: exact, and alike in any order, where the products of a 16-bit type lie within 2^24 (fp16, 22 bits each) or 2^30
+// (bf16, 16 bits) of the largest one, and off by at most D 2^-53 sum |q x| elsewhere.  The vector units' 64-bit rate is that of 32 bits.
 // select_blocks_kernel: one workgroup per (sequence, kv head) takes the largest scores by a radix select.
 #include <algorithm>
 
@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
 }
 
 // A workgroup scores kScoreBlocks blocks of one (sequence, kv head) at a time, kScoreLanes lanes to a block; HB: heads at a time.
-// What costs is the vector units: a value's choice by a mask (for 16-bit types two values at once), its conversion and the product, for
-// every head.  The 64-bit matrix cores, at the vector units' rate with 16 columns for a group's 4 heads, take 29 us where this takes 17
+// For every head a value is chosen by a mask (for 16-bit types two values at once), converted and multiplied with a query value from LDS; which
+// of these it waits for has not been told apart.  The 64-bit matrix cores, at the vector units' rate with 16 columns for a group's 4 heads, take 29 us where this takes 17
 // (32 sequences of 3000 to 32000 tokens in blocks of 64).  us with 4, 8 and 16 lanes (selection and attention included): one sequence
 // of 30000 22.2, 20.9 and 20.6, eight 34.1, 33.0 and 36.0; two blocks to four lanes, which read the query from LDS half as often, 108.4 instead
 // of 107.3 for those 32, and 40.4 instead of 32.0 for 64 sequences of 32 heads of up to 104 tokens.

@@ -316,7 +316,8 @@ class PagedKVCache:
                 yield b, s
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
-        """Append [B, Hkv, n, D] keys and values after each sequence's current length; fewer than B: to the first sequences."""
+        """Append [B, Hkv, n, D] keys and values after each sequence's current length; fewer than B: to the first sequences, and
+        nothing to the others."""
         rows, n = k_new.shape[0], k_new.shape[2]
         if rows > len(self._host_len):
             raise ValueError(f"PagedKVCache: {rows} sequences in a cache of {len(self._host_len)}")
@@ -432,7 +433,10 @@ class PagedKVCache:
             self._set_shared(groups)
 
     def free(self, sequences) -> None:
-        """Free sequences (their indices): length 0, and pages that no other one names are free again."""
+        """Free sequences (their indices): length 0, and pages that no other one names are free again.  decode() appends to every row, so a
+        freed one takes a page again at the next step, and ends what its group shares; the row of a sequence that has ended can
+        follow a living one instead (fork() with a sibling as its parent).  prefill() fills the first rows: a prompt for a
+        freed row elsewhere needs a fork() that brings that row to the front."""
         parents = np.arange(len(self._host_len))
         sequences = np.asarray(sequences, dtype=np.int64).reshape(-1)
         if np.any((sequences < 0) | (sequences >= len(parents))):
@@ -443,7 +447,7 @@ class PagedKVCache:
     def share(self, groups: int) -> None:
         """Read the pages that the sequences of a group have in common once per step: ``groups`` equal groups of consecutive
         sequences (0: no longer).  Takes effect for the pages they share now, and stays right as sequences grow; a group with
-        an empty sequence shares nothing.  Call it once with each number of groups that will be wanted before a fork is captured:
+        an empty sequence shares nothing, nor once that sequence grows again.  Call it once with each number of groups that will be wanted before a fork is captured:
         the fork's replays keep those right and know no others, which are refused."""
         if groups == 0:
             self.prefix_lengths = None

@@ -523,7 +523,8 @@ int dtattn_kv_pages_compact(const dtattn_kv_compact_args* args, void* stream);
  *
  * Single-token attention (dtattn_decode_splitkv's formula) of B sequences in `groups` equal groups of consecutive ones, whose
  * sequences share their first tokens.  Those are read once for the group's query heads together, and each sequence's own tokens
- * behind them as by the decode; both parts meet by their LSE in fp32, and O is rounded once.
+ * behind them as by the decode; both parts meet in fp32 by their bases and row sums, and O is divided and rounded once (sums of P V that pass
+ * fp32's range, as of 2^10 values of 2^118, are infinite).
  *
  * Padded (block_table NULL): sequence b attends to the first prefix_lengths[g] rows of k_prefix[g], v_prefix[g] and to the first
  * lengths[b] rows of k_cache[b], v_cache[b], g = b / (B / groups).
@@ -590,7 +591,7 @@ int dtattn_key_bounds(const dtattn_key_bounds_args* args, void* stream);
 /* Selection: for each kv head of a sequence of ceil(lengths[b] / block) blocks, the indices of keep / block blocks in ascending
  * order: the last recent / block ones, and of the others those with the largest score, of equal ones the lowest index.  With no more
  * blocks than that all of them, and -1 behind.  A block's score is the largest over the kv head's query heads of
- *   sum_d s q_d x_d,   x_d = k_max_d where s q_d > 0 and k_min_d elsewhere,   s = the sign of `scale` (0: every score is 0)
+ *   sum_d s q_d x_d,   x_d = k_max_d where s q_d > 0 and k_min_d elsewhere,   s = the sign of `scale` (0: every score is 0, over finite bounds)
  * which no score q . k of its tokens exceeds (times |scale|); sums are taken in 64 bits and rounded once to fp32, and a head whose
  * sum is NaN is passed over (-inf where all are).  `keep` and `recent` are multiples of block, block <= recent <= keep. */
 typedef struct {

@@ -363,3 +363,28 @@ def test_prefill_behind_device_parents(ops):
     cache.sync_lengths()
     cache.prefill(*_tokens(500, 1, 8))
     assert _held(cache, 0) == [500.0 + i for i in range(8)] and _held(cache, 1) == [20.0 + i for i in range(20)]
+
+
+def test_ended_sequences_follow_a_sibling(ops):
+    """Samples that end at different times: a row that goes on behind a living one keeps its group's prefix."""
+    cache = _cache()
+    _prompts(cache)
+    cache.share(2)
+    for i, parents in enumerate(([0, 0, 2, 3, 4, 5], [0, 0, 0, 3, 3, 5], [0, 0, 0, 3, 3, 3])):
+        for j in range(20):
+            cache.decode(*_tokens(1000 * (i + 1) + 10 * j))
+        cache.fork(parents)
+        assert cache.prefix_lengths.min() >= 48
+        _shares_hold(cache)
+    assert _held(cache, 2)[50:] == [1000.0 * (i + 1) + 10 * j for i in range(3) for j in range(20)]
+
+
+def test_a_prompt_for_a_freed_row(ops):
+    cache = _cache()
+    cache.prefill(*_tokens(0, 3, 20))
+    cache.free([1])
+    with pytest.raises(ValueError, match="empty"):
+        cache.prefill(*_tokens(500, 2, 8))
+    cache.fork([1, 0, 2, 3, 4, 5])
+    cache.prefill(*_tokens(500, 1, 8))
+    assert [_held(cache, b)[0] for b in range(3)] == [500.0, 0.0, 40.0] and cache.lengths.tolist() == [8, 20, 20, 0, 0, 0]
