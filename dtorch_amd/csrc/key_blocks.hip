@@ -131,8 +131,9 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
 }
 
 // A workgroup scores kScoreBlocks blocks of one (sequence, kv head) at a time, kScoreLanes lanes to a block; HB: heads at a time.
-// For every head a value is chosen by a mask (for 16-bit types two values at once), converted and multiplied with a query value from LDS; which
-// of these it waits for has not been told apart.  The 64-bit matrix cores, at the vector units' rate with 16 columns for a group's 4 heads, take 29 us where this takes 17
+// For every head a value is chosen by a mask (for 16-bit types two values at once), converted and multiplied with a query value from
+// LDS; which of these it waits for has not been told apart.  The 64-bit matrix cores, at the vector units' rate with 16 columns for a
+// group's 4 heads, take 29 us where this takes 17
 // (32 sequences of 3000 to 32000 tokens in blocks of 64).  us with 4, 8 and 16 lanes (selection and attention included): one sequence
 // of 30000 22.2, 20.9 and 20.6, eight 34.1, 33.0 and 36.0; two blocks to four lanes, which read the query from LDS half as often, 108.4 instead
 // of 107.3 for those 32, and 40.4 instead of 32.0 for 64 sequences of 32 heads of up to 104 tokens.

@@ -388,8 +388,8 @@ class PagedKVCache:
         """Sequence b continues what sequence parents[b] is, on the same pages (F.kv_pages_fork); a parent outside the batch, such
         as -1, frees the sequence.  parents: B whole numbers on the host, or an int32 tensor [B] on the device.  The latter does not
         wait for the device (and may be captured): the host's lengths are then behind until sync_lengths() (which an eager step calls
-        by itself where its token might not fit), and a group that has a
-        parent from another one, or a sequence without parent, shares nothing until the next share().  A captured fork does so for the
+        by itself where its token might not fit), and a group that has a parent from another one, or a sequence without parent,
+        shares nothing until the next share().  A captured fork does so for the
         numbers of groups that share() has had before the capture; others are refused from then on.  A step captured before the first
         fork() or compact() does not copy what it writes, so that sequences cannot share pages behind it.  A cache that runs out of pages
         meanwhile drops tokens, which sync_lengths() reports; until then what the sequences without pages attend to says nothing."""
@@ -447,8 +447,8 @@ class PagedKVCache:
     def share(self, groups: int) -> None:
         """Read the pages that the sequences of a group have in common once per step: ``groups`` equal groups of consecutive
         sequences (0: no longer).  Takes effect for the pages they share now, and stays right as sequences grow; a group with
-        an empty sequence shares nothing, nor once that sequence grows again.  Call it once with each number of groups that will be wanted before a fork is captured:
-        the fork's replays keep those right and know no others, which are refused."""
+        an empty sequence shares nothing, nor once that sequence grows again.  Call it once with each number of groups that will
+        be wanted before a fork is captured: the fork's replays keep those right and know no others, which are refused."""
         if groups == 0:
             self.prefix_lengths = None
             return

@@ -480,9 +480,10 @@ typedef struct {
 
 /* Reserve: pages of their own for the next n_new tokens of every sequence.  The slots of positions lengths[b] to
  * lengths[b] + n_new - 1 (those inside the table; lengths clamped to [0, max_pages * page_size]) are taken in the order of b and then
- * of the slot.  An empty one takes a free page, unless the sequence has tokens in it already (an earlier call found no page for them): such a slot
- * stays empty and is counted as lacking, for another sequence's rows would stand where those tokens were.  One whose page is shared takes a free page as well, so long as others still name
- * the page: of sequences that all write a page, the last one keeps it.  The rows of the tokens that the sequence has in such a page
+ * of the slot.  An empty one takes a free page, unless the sequence has tokens in it already (an earlier call found no page for
+ * them): such a slot stays empty and is counted as lacking, for another sequence's rows would stand where those tokens were.  One
+ * whose page is shared takes a free page as well, so long as others still name the page: of sequences that all write a page, the
+ * last one keeps it.  The rows of the tokens that the sequence has in such a page
  * are copied, in every pool.  Free pages are taken from the lowest index up; once they run out, slots that need one become -1 (tokens
  * written through them are dropped, those they held are lost to the sequence), and *short_by says how many (0 otherwise).
  * A copied row's other bytes, and rows behind a sequence's tokens, are left as they were. */
@@ -523,8 +524,8 @@ int dtattn_kv_pages_compact(const dtattn_kv_compact_args* args, void* stream);
  *
  * Single-token attention (dtattn_decode_splitkv's formula) of B sequences in `groups` equal groups of consecutive ones, whose
  * sequences share their first tokens.  Those are read once for the group's query heads together, and each sequence's own tokens
- * behind them as by the decode; both parts meet in fp32 by their bases and row sums, and O is divided and rounded once (sums of P V that pass
- * fp32's range, as of 2^10 values of 2^118, are infinite).
+ * behind them as by the decode; both parts meet in fp32 by their bases and row sums, and O is divided and rounded once (sums
+ * of P V that pass fp32's range, as of 2^10 values of 2^118, are infinite).
  *
  * Padded (block_table NULL): sequence b attends to the first prefix_lengths[g] rows of k_prefix[g], v_prefix[g] and to the first
  * lengths[b] rows of k_cache[b], v_cache[b], g = b / (B / groups).
@@ -619,7 +620,8 @@ int dtattn_select_key_blocks(const dtattn_select_blocks_args* args, void* stream
 
 /* Single-token attention over the listed blocks of each kv head: dtattn_decode_splitkv's formula over the tokens
  * blocks[b, hk, i] * block + (0 .. block - 1) that lie before lengths[b].  An index that is negative or past the sequence's blocks
- * stands for no token; a block listed twice counts twice.  Up to 2^30 listed tokens (n_blocks * block).  No token: O = 0, LSE = -inf.  Types as for dtattn_decode_shared. */
+ * stands for no token; a block listed twice counts twice.  Up to 2^30 listed tokens (n_blocks * block).  No token: O = 0,
+ * LSE = -inf.  Types as for dtattn_decode_shared. */
 typedef struct {
     const void* q;
     const void* k_cache;     /* [B, Hkv, S_max, D]; paged: [num_pages, Hkv, page_size, D] */

@@ -128,3 +128,25 @@ def test_partial_decode_in_every_type(dtype, paged):
         rows = [[[t for j in ids[b, h] for t in range(16 * j, min(16 * j + 16, n))] for h in range(HKV)] for b in range(B)]
         ks, vs = ([[x[b, h, rows[b][h]] for h in range(HKV)] for b in range(B)] for x in (k, v))
         _against(out, step[0], ks, vs, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,heads,kv,d,prefix", [(4, 32, 8, 128, 2000), (32, 8, 2, 64, 700), (40, 16, 2, 128, 900)])
+def test_same_bits(dtype, batch, heads, kv, d, prefix):
+    """The same call gives the same bits, whatever the workspace held before."""
+    from dtorch_amd.nn import functional as F
+    g = torch.Generator(device="cuda").manual_seed(44)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+    q, kp, vp, k, v = normal(batch, heads, 1, d), normal(1, kv, prefix, d), normal(1, kv, prefix, d), normal(batch, kv, 200, d), normal(batch, kv, 200, d)
+    n, lengths = torch.tensor([prefix], dtype=torch.int32, device="cuda"), torch.randint(0, 201, (batch,), generator=g, device="cuda", dtype=torch.int32)
+    ids = torch.randint(-1, 13, (batch, kv, 9), generator=g, device="cuda", dtype=torch.int32)
+    calls = [lambda: F.decode_attention_shared(q, kp, vp, n, k, v, lengths), lambda: F.decode_attention_blocks(q, k, v, lengths, ids, 16)]
+    first = [[x.clone() for x in call()] for call in calls]
+    for i in range(12):
+        spoil = [torch.full((size,), (float("nan"), 1e30, -3.0)[i % 3], device="cuda") for size in (1 << 10, 1 << 14, 1 << 18, 1 << 20, 1 << 22)]
+        del spoil
+        for call, want in zip(calls, first):
+            assert all(torch.equal(a, b) for a, b in zip(call(), want))
